@@ -101,6 +101,25 @@ class DecodeArgs(C.Structure):
                 ("workspace", P), ("workspace_bytes", SZ), ("gate", P), ("oq", P), ("oqs", P)]
 
 
+class PagePlanArgs(C.Structure):
+    _fields_ = [(n, I32) for n in ("B", "T", "page_size", "table_rows", "table_width", "free_count", "pt_width", "whole")] + \
+               [(n, P) for n in ("cached", "new_tokens", "req", "table", "free_pages", "qsl", "seqlens", "positions",
+                                 "out_loc", "used", "page_table")]
+
+
+class AttnFrontArgs(C.Structure):
+    _fields_ = [("T", I32), ("max_pos", I32), ("axes", I32), ("q_e4m3", I32), ("qkv_ld", I64), ("pos_stride", I64),
+                ("axis_map", I64), ("num_slots", I64), ("qkv", P), ("q_norm_w", P), ("k_norm_w", P), ("cos_sin", P),
+                ("positions", P), ("q", P), ("gate", P), ("out_loc", P), ("k_cache", P), ("v_cache", P),
+                ("eps", C.c_float)]
+
+
+class ChunkArgs(C.Structure):
+    _fields_ = [("B", I32), ("T", I32), ("HQ", I32), ("HKV", I32), ("D", I32), ("page_size", I32), ("pt_stride", I32),
+                ("q_e4m3", I32), ("num_slots", I64), ("q", P), ("k_cache", P), ("v_cache", P), ("page_table", P),
+                ("seqlens", P), ("qsl", P), ("out", P), ("workspace", P), ("workspace_bytes", SZ), ("scale", C.c_float)]
+
+
 def _packer(st):
     """struct.pack of a structure's fields in order (nested arrays flattened): the bytes of the filled structure, for packed().
     Filling the ctypes structure itself took longer than the launch it describes (45 fields: 5 us against 1)."""
@@ -119,6 +138,7 @@ def _packer(st):
 pack_moe, pack_gdn, pack_ring, pack_attn = map(_packer, (MoeArgs, GdnArgs, GdnRingArgs, AttnArgs))
 pack_oproj, pack_lmhead, pack_fp8, pack_dense8 = map(_packer, (OprojArgs, LmheadArgs, Fp8LinearArgs, Dense8LinearArgs))
 pack_addnorm, pack_decode = map(_packer, (AddNormArgs, DecodeArgs))
+pack_plan, pack_front, pack_chunk = map(_packer, (PagePlanArgs, AttnFrontArgs, ChunkArgs))
 
 
 _lib = _packed = None
@@ -150,6 +170,10 @@ SYMBOLS = [
     ("q36_tile_w16", I32, [P, C.c_int64, I32, P, P]),
     ("q36_attn_decode_workspace_bytes", SZ, [I32, I32]),
     ("q36_attn_decode", I32, [C.POINTER(DecodeArgs), P]),
+    ("q36_page_plan", I32, [C.POINTER(PagePlanArgs), P]),
+    ("q36_attn_front", I32, [C.POINTER(AttnFrontArgs), P]),
+    ("q36_attn_chunk_workspace_bytes", SZ, []),
+    ("q36_attn_chunk", I32, [C.POINTER(ChunkArgs), P]),
     ("q36_lmhead_workspace_bytes", SZ, [I32]),
     ("q36_lmhead_argmax", I32, [C.POINTER(LmheadArgs), P]),
     ("q36_quant_rows_i8", I32, [P, C.c_int64, I32, P, P, P]),
@@ -163,6 +187,7 @@ SYMBOLS = [
 OPTIONAL_SYMBOLS: list = []
 ARG_POINTERS = [C.POINTER(s) for s in (MoeArgs, GdnArgs, GdnRingArgs, AttnArgs, OprojArgs, LmheadArgs, Fp8LinearArgs,
                                        AddNormArgs, Dense8LinearArgs, DecodeArgs)]
+CHUNK_POINTERS = [C.POINTER(s) for s in (PagePlanArgs, AttnFrontArgs, ChunkArgs)]  # the prompt chunk's entries
 
 
 def _load(arg0):
@@ -190,7 +215,7 @@ def packed():
     bytes into one costs 0.3 us a call.)"""
     global _packed
     if _packed is None:
-        _packed = _load(lambda a: P if a in ARG_POINTERS else a)
+        _packed = _load(lambda a: P if a in ARG_POINTERS or a in CHUNK_POINTERS else a)
     return _packed
 
 
@@ -204,6 +229,15 @@ def check(rc: int, what: str) -> None:
 def ptr(t) -> int:
     """Device (or host) address of a torch tensor, 0 for None."""
     return 0 if t is None else t.data_ptr()
+
+
+def check_tensors(what: str, **tensors) -> None:
+    """Every given tensor (None: left out) lies on the current GPU, where its call is launched."""
+    import torch
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.get_device() != dev):
+            raise ValueError(f"{what}: {name} is on {t.device}, not on the current GPU")
 
 
 def stream_handle(stream=None) -> int:

@@ -71,6 +71,11 @@ __device__ __forceinline__ uint32_t f2e4m3x2_hw(float a, float b) {
   b = fminf(fmaxf(b, -448.f), 448.f);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
 }
+// The same, with NaN kept (f2e4m3x2_hw's clamp turns it into -448).
+__device__ __forceinline__ float sat_e4m3(float a) { return fabsf(a) > 448.f ? __builtin_copysignf(448.f, a) : a; }
+__device__ __forceinline__ uint32_t f2e4m3x2_nan(float a, float b) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(sat_e4m3(a), sat_e4m3(b), 0, false) & 0xffffu;
+}
 __device__ __forceinline__ float e4m3_to_f(uint32_t b) {
   uint32_t e = (b >> 3) & 15u, m = b & 7u;
   float v;

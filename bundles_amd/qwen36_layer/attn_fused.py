@@ -1,4 +1,5 @@
-"""Fused gated full attention on libq36 (q36_attn_proj, q36_attn_decode, q36_attn_oproj).
+"""Fused gated full attention on libq36 (q36_attn_proj, q36_attn_decode, q36_attn_oproj; for prompt chunks
+q36_attn_front and q36_attn_chunk).
 
 Mirrors the reference's attention glue (R = qwen36_nodes_kb34, L = R/qwen36_layer): the fused
 qkv projection + q/k norm + partial RoPE + e4m3 KV write (L/attn_fused.py:232-273,
@@ -14,7 +15,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
-from .._lib import check, pack_attn, pack_decode, pack_oproj, ptr
+from .._lib import check, check_tensors, pack_attn, pack_chunk, pack_decode, pack_front, pack_oproj, ptr
 from .moe import quantize_blocks_e4m3
 
 N_Q_HEADS, N_KV_HEADS, HEAD_DIM, HIDDEN = 16, 2, 256, 2048
@@ -188,4 +189,125 @@ def attn_decode(q, k_cache, v_cache, page_table, seqlens, NT: int, scale: float,
                    ptr(v_new), scale, ptr(out), ptr(ws.buf), ws.buf.numel(), ptr(gate),
                    ptr(None if oq is None else oq.codes), ptr(None if oq is None else oq.scales))
     check(_lib.packed().q36_attn_decode(a, _lib.stream_handle(stream)), "q36_attn_decode")
+    return out
+
+
+# ---- prompt chunks ---------------------------------------------------------------------------------------------
+ROT_PAIRS = 32
+
+
+class RopeAxes:
+    """Which axis of the positions (time, height, width, ..) turns each of the 32 rotary pairs.  sections: pairs of
+    each axis (two to four axes, 32 in all); contiguous (axis 0's pairs first, then axis 1's, ..), or interleaved: axis
+    a > 0 has the pairs a, a + axes, a + 2 axes, .. (sections[a] of them), axis 0 the others."""
+
+    def __init__(self, sections, interleaved: bool = False):
+        s = [int(v) for v in sections]
+        n = len(s)
+        if not 2 <= n <= 4 or min(s) < 0 or sum(s) != ROT_PAIRS:
+            raise ValueError(f"RopeAxes: sections {s} must be two to four counts of pairs, {ROT_PAIRS} in all")
+        if interleaved:
+            if any(c and a + n * (c - 1) >= ROT_PAIRS for a, c in enumerate(s) if a):
+                raise ValueError(f"RopeAxes: sections {s} do not fit {ROT_PAIRS} interleaved pairs")
+            of = [i % n if i % n and i < n * s[i % n] else 0 for i in range(ROT_PAIRS)]
+        else:
+            of = [a for a, c in enumerate(s) for _ in range(c)]
+        self.axes, self.axis_of = n, of
+        bits = sum(a << (2 * i) for i, a in enumerate(of))
+        self.map = bits - (1 << 64) if bits >> 63 else bits  # int64 of the argument structure
+
+
+def attn_front(qkv, q_norm_w, k_norm_w, eps, cos_sin, positions, cache=None, axes: RopeAxes | None = None,
+               q_dtype=torch.bfloat16, q=None, gate=None, stream=None):
+    """The projected rows qkv (bf16 [T, 9216], rows may be strided) of a prompt chunk -> (q, gate): q/k norm, RoPE,
+    the query rows [T, 16, 256] (q_dtype bf16, or uint8: e4m3 codes, as attn_chunk reads them), the gate rows (bf16
+    [T, 16, 256]), and the new e4m3 K / V rows in cache = (k_cache, v_cache, out_loc) (uint8 [slots, 2, 256], int64 [T];
+    slots outside the cache are skipped).  positions int32 [T], or with axes int32 [axes, T] (an axis a row).  Formed in
+    fp32 and rounded once (attn_proj rounds to bf16 between the steps)."""
+    T = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[1] != QKV_ROWS or (T > 0 and qkv.stride(1) != 1):
+        raise ValueError(f"attn_front: qkv must be bf16 [T, {QKV_ROWS}] with contiguous rows")
+    if T > 1 and (qkv.stride(0) < QKV_ROWS or qkv.stride(0) % 8):
+        raise ValueError(f"attn_front: qkv's row stride {qkv.stride(0)} must be a multiple of 8 from {QKV_ROWS} on")
+    for name, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.numel() != HEAD_DIM:
+            raise ValueError(f"attn_front: {name} must be contiguous bf16 [{HEAD_DIM}]")
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.dim() != 2 or cos_sin.shape[1] != 2 * ROT_PAIRS:
+        raise ValueError(f"attn_front: cos_sin must be contiguous fp32 [max_pos, {2 * ROT_PAIRS}]")
+    want = (T,) if axes is None else (axes.axes, T)
+    if positions.dtype != torch.int32 or tuple(positions.shape) != want or (T > 0 and positions.stride(-1) != 1) or \
+            (axes is not None and positions.stride(0) < T):
+        raise ValueError(f"attn_front: positions must be int32 {list(want)} with contiguous rows")
+    if q_dtype not in (torch.bfloat16, torch.uint8):
+        raise ValueError("attn_front: q_dtype must be bfloat16 or uint8 (e4m3 codes)")
+    shape = (T, N_Q_HEADS, HEAD_DIM)
+    q = torch.empty(shape, dtype=q_dtype, device=qkv.device) if q is None else q
+    gate = torch.empty(shape, dtype=torch.bfloat16, device=qkv.device) if gate is None else gate
+    for name, t, dt in (("q", q, q_dtype), ("gate", gate, torch.bfloat16)):
+        if t.dtype != dt or not t.is_contiguous() or tuple(t.shape) != shape:
+            raise ValueError(f"attn_front: {name} must be a contiguous {dt} tensor {list(shape)}")
+    kc = vc = loc = None
+    slots = 0
+    if cache is not None:
+        kc, vc, loc = cache
+        for name, t in (("k_cache", kc), ("v_cache", vc)):
+            if t.dtype != torch.uint8 or not t.is_contiguous() or t.shape[1:] != (N_KV_HEADS, HEAD_DIM):
+                raise ValueError(f"attn_front: {name} must be contiguous uint8 [slots, {N_KV_HEADS}, {HEAD_DIM}]")
+        if kc.shape != vc.shape:
+            raise ValueError("attn_front: k_cache and v_cache differ in shape")
+        if loc.dtype != torch.int64 or not loc.is_contiguous() or loc.numel() < T:
+            raise ValueError(f"attn_front: out_loc must be contiguous int64 with at least {T} entries")
+        slots = kc.shape[0]
+    check_tensors("attn_front", qkv=qkv, q_norm_w=q_norm_w, k_norm_w=k_norm_w, cos_sin=cos_sin, positions=positions, q=q,
+                  gate=gate, k_cache=kc, v_cache=vc, out_loc=loc)
+    if T == 0:
+        return q, gate
+    a = pack_front(T, cos_sin.shape[0], 1 if axes is None else axes.axes, int(q_dtype == torch.uint8),
+                   qkv.stride(0) if T > 1 else QKV_ROWS, 0 if axes is None else positions.stride(0), 0 if axes is None else axes.map,
+                   slots, ptr(qkv), ptr(q_norm_w), ptr(k_norm_w), ptr(cos_sin), ptr(positions), ptr(q), ptr(gate), ptr(loc),
+                   ptr(kc), ptr(vc), eps)
+    check(_lib.packed().q36_attn_front(a, _lib.stream_handle(stream)), "q36_attn_front")
+    return q, gate
+
+
+class ChunkWorkspace:
+    """Partials of q36_attn_chunk; one size serves every call, so the layers of a step share it (calls that may run at
+    the same time need one each)."""
+
+    def __init__(self, device):
+        self.buf = torch.empty(_lib.lib().q36_attn_chunk_workspace_bytes(), dtype=torch.uint8, device=device)
+
+
+def attn_chunk(q, k_cache, v_cache, page_table, seqlens, qsl, scale: float, ws: ChunkWorkspace, page_size: int = 1,
+               out=None, stream=None):
+    """Attention of each request's new tokens over the paged e4m3 KV cache, any number of them a request.
+
+    q [T, 16, 256] bf16 (rounded to e4m3, as attn_decode does) or uint8 (e4m3 codes, attn_front's); request b's new
+    tokens are rows qsl[b] .. qsl[b + 1] - 1 (int32 [B + 1]) and its keys, the new ones included and already in the
+    cache, number seqlens[b] (int32 [B]); k_cache / v_cache e4m3 codes (uint8) [slots, 2, 256]; page_table int32
+    [B, stride]: the page (page_size slots, a power of two) of keys j * page_size .. .  Returns bf16 [T, 16, 256] =
+    softmax(scale * q k^T) V per query head, causal among the new tokens; rows outside qsl are left as they were (a
+    fresh out holds anything there), rows that see no key are zero."""
+    if q.dim() != 3 or q.shape[1:] != (N_Q_HEADS, HEAD_DIM) or q.dtype not in (torch.bfloat16, torch.uint8) or not q.is_contiguous():
+        raise ValueError(f"attn_chunk: q must be a contiguous bfloat16 or uint8 tensor [T, {N_Q_HEADS}, {HEAD_DIM}]")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.shape[1:] != (N_KV_HEADS, HEAD_DIM):
+            raise ValueError(f"attn_chunk: {name} must be contiguous uint8 [slots, {N_KV_HEADS}, {HEAD_DIM}]")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("attn_chunk: k_cache and v_cache differ in shape")
+    B = page_table.shape[0]
+    for name, t, shape in (("page_table", page_table, (B, page_table.shape[-1])), ("seqlens", seqlens, (B,)), ("qsl", qsl, (B + 1,))):
+        if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+            raise ValueError(f"attn_chunk: {name} must be a contiguous int32 tensor {list(shape)}")
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device) if out is None else out
+    if out.dtype != torch.bfloat16 or not out.is_contiguous() or out.shape != q.shape:
+        raise ValueError(f"attn_chunk: out must be a contiguous bfloat16 tensor {list(q.shape)}")
+    check_tensors("attn_chunk", q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table, seqlens=seqlens, qsl=qsl, out=out,
+                  workspace=ws.buf)
+    if q.shape[0] == 0:
+        return out
+    a = pack_chunk(B, q.shape[0], N_Q_HEADS, N_KV_HEADS, HEAD_DIM, page_size, page_table.shape[1], int(q.dtype == torch.uint8),
+                   k_cache.shape[0], ptr(q), ptr(k_cache), ptr(v_cache), ptr(page_table), ptr(seqlens), ptr(qsl), ptr(out),
+                   ptr(ws.buf), ws.buf.numel(), scale)
+    check(_lib.packed().q36_attn_chunk(a, _lib.stream_handle(stream)), "q36_attn_chunk")
     return out

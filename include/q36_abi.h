@@ -480,6 +480,102 @@ typedef struct q36_decode_args {
 size_t q36_attn_decode_workspace_bytes(int32_t B, int32_t splits);
 int q36_attn_decode(const q36_decode_args* a, q36_stream_t stream);
 
+/* ---- A step's place in the paged cache, worked out on the device from the requests' lengths (no reference
+ * counterpart: the reference reads out_cache_loc, page_table and cache_seqlens_int32 from its engine,
+ * L/attn_fused.py:70-75) ----
+ * cached, new_tokens int32 [B]: keys that a request has in the cache and tokens it gets now.  table int32
+ * [table_rows, table_width]: the pages (page_size slots each, a power of two) of request row req[b] (int32 [B],
+ * rows distinct; NULL: row b), extended in place by free_pages int32 [free_count], taken from the front in the
+ * order of the requests.  Writes
+ *   qsl int32 [B + 1]: first row of each request among the new tokens; seqlens int32 [B]: cached + new;
+ *   positions int32 [T], out_loc int64 [T]: position and cache slot of each new token, requests in order; rows behind
+ *     the last request get position 0 and slot -1 (a batch padded to T), which q36_attn_proj and q36_attn_front skip;
+ *   page_table int32 [B, pt_width] (or NULL): the slot of every key position of request b (whole) or of its new tokens
+ *     alone; what lies behind a request's keys is left as it was;
+ *   used int32 [2]: the pages taken from the list, and 0 or the OR of what did not fit: Q36_PLAN_TOKENS more new tokens
+ *     than T, Q36_PLAN_PAGES too few free pages, Q36_PLAN_TABLE a request longer than the table or a row outside it,
+ *     Q36_PLAN_PAGE_TABLE a request longer than the page table.  A token without a page (or whose page number has no
+ *     31-bit slot) gets slot -1, a key without one page-table entry 0, and qsl stops at T.
+ * Negative counts are taken as 0.  B up to 65535; all pointers naturally aligned. */
+#define Q36_PLAN_TOKENS 1
+#define Q36_PLAN_PAGES 2
+#define Q36_PLAN_TABLE 4
+#define Q36_PLAN_PAGE_TABLE 8
+typedef struct q36_page_plan_args {
+  int32_t B, T, page_size, table_rows, table_width, free_count, pt_width, whole;
+  const int32_t* cached;
+  const int32_t* new_tokens;
+  const int32_t* req;
+  int32_t* table;
+  const int32_t* free_pages;
+  int32_t* qsl;
+  int32_t* seqlens;
+  int32_t* positions;
+  int64_t* out_loc;
+  int32_t* used;
+  int32_t* page_table;
+} q36_page_plan_args;
+int q36_page_plan(const q36_page_plan_args* a, q36_stream_t stream);
+
+/* ---- The attention layer's front for a prompt chunk: what q36_attn_proj does behind its projection, on rows that are
+ * already projected (q36_fp8_linear with N = 9216), with rotary positions of several axes (the reference's
+ * attn_prefill_front, L/qk_attn_verify.cu:765-797, has one) ----
+ * qkv bf16 [T, qkv_ld] (qkv_ld >= 9216, a multiple of 8): 16 x (256 q | 256 gate), 512 k, 512 v.  Per head of q and k:
+ * y = x * rsqrt(mean x^2 + eps) * (1 + w), then neox RoPE on dims 0..63: pair i (dims i, i + 32) turns by the cos_sin row
+ * (fp32 [max_pos, 64], cos 0..31 | sin 0..31) of positions[axis][t], axis = bits 2 i, 2 i + 1 of axis_map, positions int32
+ * [axes, pos_stride], axes 1..4 (time, height, width, ..); a position outside [0, max_pos) counts as the nearest inside.
+ * All of it in fp32, rounded once: q bf16 [T, 16, 256], or with q_e4m3 e4m3 codes (satfinite) as q36_attn_chunk reads
+ * them; k, v e4m3 (satfinite) into rows out_loc[t] (int64 [T]; a slot outside [0, num_slots) is skipped) of k_cache,
+ * v_cache [num_slots, 2, 256]; gate bf16 [T, 16, 256], copied.  (q36_attn_proj rounds to bf16 behind the norm and behind
+ * the rotation: its cache rows can differ from these by one e4m3 code.)  out_loc, k_cache, v_cache may be NULL together
+ * (no cache rows), gate may be NULL.  qkv, norm weights, cos_sin, gate and bf16 q 16-byte, e4m3 q and caches 8-byte aligned. */
+typedef struct q36_attn_front_args {
+  int32_t T, max_pos, axes, q_e4m3;
+  int64_t qkv_ld, pos_stride, axis_map, num_slots;
+  const void* qkv;
+  const void* q_norm_w;
+  const void* k_norm_w;
+  const float* cos_sin;
+  const int32_t* positions;
+  void* q;
+  void* gate;
+  const int64_t* out_loc;
+  void* k_cache;
+  void* v_cache;
+  float eps;
+} q36_attn_front_args;
+int q36_attn_front(const q36_attn_front_args* a, q36_stream_t stream);
+
+/* ---- Attention of each request's new tokens (a prompt chunk, a draft, one token: any mix) over the paged e4m3 cache.
+ * (The reference re-pages the cache and calls a library there, L/attn_fused.py:127-210.) ----
+ * q [T, HQ, D] bf16 (rounded to e4m3, as q36_attn_decode does) or, with q_e4m3, e4m3 codes; request b's new tokens are
+ * rows qsl[b] .. qsl[b + 1] - 1 (int32 [B + 1]); seqlens int32 [B]: its keys, the new tokens included, all in the cache;
+ * its i-th new token sees keys 0 .. seqlens[b] - new + i.  page_table int32 [B, pt_stride]: entry j is the page of keys
+ * j page_size .. (page_size a power of two; 1: the slots themselves).  k_cache, v_cache e4m3 [num_slots, HKV, D].
+ * out bf16 [T, HQ, D] = bf16(sum_j p_j v_j / sum_j p_j), p_j = exp(scale (q . k_j) - max): scores, maxima, sums and the
+ * output in fp32, p_j rounded to f16 for the product with v.  A row that sees no key is zero; rows outside
+ * qsl[0] .. qsl[B] are left as they were.  What a row does not see, NaN included, does not reach it.
+ * Whatever the device data hold, every access stays inside the buffers: rows outside T, keys past the page table's
+ * pt_stride * page_size and slots outside the cache are clamped.
+ * HQ = 16, HKV = 2, D = 256; T <= 2^20, B <= 65535; q, out and caches 16-byte, workspace 256-byte aligned.
+ * Workspace: q36_attn_chunk_workspace_bytes(), whatever the call's sizes (partials of the cut tiles). */
+typedef struct q36_chunk_args {
+  int32_t B, T, HQ, HKV, D, page_size, pt_stride, q_e4m3;
+  int64_t num_slots;
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* page_table;
+  const int32_t* seqlens;
+  const int32_t* qsl;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+  float scale;
+} q36_chunk_args;
+size_t q36_attn_chunk_workspace_bytes(void);
+int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream);
+
 /* ---------------------------------------------------------------------------------------
  * Int8 lm_head fused with greedy argmax (H/w8a8.py:116-120 w8a8_linear + the stock argmax,
  * H/node.py:136-151).  h bf16 [R, H] (H = 2048) -> optional final Gemma RMSNorm (norm_w bf16 [H],
