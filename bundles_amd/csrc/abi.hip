@@ -2,6 +2,8 @@
 // need more than 64 KiB of dynamic LDS.
 #include <string.h>
 
+#include <atomic>
+
 #include "q36_host.h"
 
 namespace q36 {
@@ -37,6 +39,16 @@ int ensure_lds(const void* fn, size_t bytes, const char* what) {
       break;
     }
   return Q36_OK;
+}
+int device_cus() {
+  static std::atomic<int> known[64];  // per device, 0: not asked yet
+  int cus = 256, dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return cus;
+  const bool slot = dev >= 0 && dev < 64;
+  if (slot && known[dev].load(std::memory_order_relaxed)) return known[dev].load(std::memory_order_relaxed);
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && slot)
+    known[dev].store(cus, std::memory_order_relaxed);
+  return cus;
 }
 }  // namespace q36
 

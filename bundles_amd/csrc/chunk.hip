@@ -6,8 +6,11 @@
 // (The reference re-pages the cache into 128-row pages and calls a library there, L/attn_fused.py:127-210.)
 #include <math.h>
 
+#include <algorithm>
+
 #include "q36_device.h"
 #include "q36_host.h"
+#include "q36_chunk.h"
 
 namespace q36 {
 namespace {
@@ -30,21 +33,21 @@ struct ChunkDev {
   const int32_t* qsl;
   uint16_t* out;
   float scale_log2;
+  float* ws_o;   // [2 groups][8][8][4][64][4]: partial outputs of 8 waves' 32 rows, unnormalised
+  float* ws_ml;  // [2 groups][8][2][32]: their running maxima (base 2) and weight sums
+  int4* cuts;    // [groups] the tile that starts in each share and is cut: request (-1: none), 2 tile + head, last share; and
+                 // whether a value on the causal border was NaN
 };
 
-// A request's new tokens and keys, inside the buffers whatever qsl and seqlens hold.
+// A request's first row, new tokens and keys, inside the buffers whatever qsl and seqlens hold.
 struct Req {
-  int t0, n, nk;
+  int t0;
+  ChunkReq r;
 };
 __device__ __forceinline__ Req req_of(const ChunkDev& d, int b) {
   const int t0 = min(max(d.qsl[b], 0), d.T), t1 = min(max(d.qsl[b + 1], t0), d.T);
   const int64_t keys = (int64_t)d.pt_stride << d.sh;
-  return Req{t0, t1 - t0, (int)min((int64_t)max(d.seqlens[b], 0), keys)};
-}
-__device__ __forceinline__ int64_t slot_of(const ChunkDev& d, int b, int key) {
-  const int64_t p = d.pt[(size_t)b * d.pt_stride + (key >> d.sh)];
-  const int64_t s = (p << d.sh) + (key & ((1 << d.sh) - 1));
-  return s < 0 ? 0 : s >= d.num_slots ? d.num_slots - 1 : s;
+  return Req{t0, {t1 - t0, (int)min((int64_t)max(d.seqlens[b], 0), keys)}};
 }
 __device__ __forceinline__ v8h widen8(int w0, int w1) {
   const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, false);
@@ -61,34 +64,80 @@ __device__ __forceinline__ v16f mfma_qk(v8i a, v8i b, v16f c) {
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // A step on the causal border multiplies some rows' values by a weight of zero, which would hand them a NaN that they do
-// not see.  There the NaN values count as zero, and a product of two indicators (value is NaN, key is seen) finds the
-// outputs that do see one.
-//
-// One wave: 4 new tokens x 8 query heads (32 rows) of a KV head over all their keys, 32 keys a step.
+// not see.  There the NaN values count as zero, and where a call has met one the combine kernel goes over the border's keys
+// once more and puts the NaN where it is seen.
+
+constexpr int kBlk = 2 * kCST * kCD;  // 32 keys in LDS: their K rows, then their V rows
+constexpr int kStage = 4 * kBlk;
+constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a partial
+constexpr float kLazyC = 8.f;  // the outputs are rescaled when a row's maximum has grown by 2^8 (weights up to 2^8 are exact in f16)
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uni(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
+}
+__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8)); }
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// One run of a tile's steps by the 8 waves.  RG = 8 (wide): wave w has rows 32 w .. of the tile's 256 (4 tokens x 8 heads)
+// and every wave walks all keys, 64 a step.  RG = 2 (narrow): waves 2 k, 2 k + 1 have rows 0 .. 31, 32 .. 63 and walk the
+// k-th 32 keys of each step's 128; the four are merged at the end.
 // Scores S^T = K Q^T (32x32x64, e4m3): lane l holds row l % 32 and keys 8 (i / 4) + 4 (l / 32) + i % 4.  O^T += V^T P^T
 // (32x32x16, f16): the lane's own weights in the order it has them, V^T by the transpose read from LDS rows in that order.
-__global__ __launch_bounds__(64) void chunk_kernel(ChunkDev d) {
-  __shared__ __align__(16) uint8_t vs[kCST * kCD];
-  const int lane = threadIdx.x, col = lane & 31, g = lane >> 5, h = blockIdx.x & 1;
-  int tile = blockIdx.x >> 1, b = 0;
-  Req R{0, 0, 0};
-  for (;; ++b) {
-    if (b >= d.B) return;
-    R = req_of(d, b);
-    const int n = (R.n + 3) / 4;
-    if (tile < n) break;
-    tile -= n;
-  }
-  const int pre = R.nk - R.n, i0 = 4 * tile, row_t = i0 + (col >> 3), head = h * kCG + (col & 7);
-  const bool row_ok = row_t < R.n;
-  const int lim = row_ok ? pre + row_t : -1;  // the row's last key
-  const int nkeys = min(R.nk, pre + min(i0 + 4, R.n));
+// A block of 32 keys in LDS: K row r holds key r, V row r key 16 (r / 16) + 8 ((r % 8) / 4) + 4 ((r / 8) % 2) + r % 4, 16-byte
+// piece p of a row at p ^ (r % 8), so that eight lanes' reads fall on eight bank slots.
+template <int RG>
+__device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X0, uint8_t* X1, float (*mlw)[2][32], int b, int t0, ChunkReq r, int h,
+                                         int tile, ChunkRun run, int slot) {
+  constexpr int KG = 8 / RG, SUB = KG == 1 ? 2 : 1, NE = KG == 1 ? 2 : 4, STEP = KG == 1 ? kWideKeys : kNarrowKeys;
+  static_assert(STEP == 32 * (KG == 1 ? SUB : KG), "a step's blocks");
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, g = lane >> 5;
+  const int wave = uni(tid >> 6), rw = wave % RG, kg = wave / RG;
+  const int pre = r.nk - r.n, vis = ck_keys(r, tile);
+  const int tok0 = tile * (4 * RG) + 4 * rw;  // the wave's first token
+  const bool active = tok0 < r.n;
+  const int tok = tok0 + (col >> 3), head = h * kCG + (col & 7);
+  const bool row_ok = tok < r.n;
+  const int lim = row_ok ? pre + tok : -1, lim_first = pre + tok0, lim_last = pre + min(tok0 + 3, r.n - 1);
+  const int32_t* const pt = d.pt + (size_t)b * d.pt_stride;
+  const int sh = d.sh, low = (1 << sh) - 1, top = (int)d.num_slots - 1, top_page = top >> sh;
+  // this lane's part of the wave's copies: row `lane / 16` of four, 16 bytes
+  const int t4 = lane >> 4;
+  int ent[NE];
+  auto key_of = [&](int st, int e) {
+    const int vw = KG == 1 ? wave : 4 * (wave & 1) + e, blk = KG == 1 ? e : kg;
+    return min(st * STEP + 32 * blk + 16 * (vw >> 2) + 8 * (vw & 1) + 4 * ((vw >> 1) & 1) + t4, vis - 1);
+  };
+  auto entries = [&](int st) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) ent[e] = pt[key_of(st, e) >> sh];
+  };
+  auto copy = [&](int st, uint8_t* X) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int vw = KG == 1 ? wave : 4 * (wave & 1) + e, blk = KG == 1 ? e : kg;
+      const int kap = 16 * (vw >> 2) + 8 * (vw & 1) + 4 * ((vw >> 1) & 1);
+      const int pg = min(max(ent[e], 0), top_page), s = min((pg << sh) + (key_of(st, e) & low), top);
+      const size_t at = (size_t)(uint32_t)s * (kCHKV * kCD) + h * kCD;
+      const int kp = (lane & 15) ^ (4 * ((vw >> 1) & 1) + t4), vp = (lane & 15) ^ (4 * (vw & 1) + t4);
+      uint8_t* const base = X + blk * kBlk;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(d.kc + at + 16 * kp),
+                                       (__attribute__((address_space(3))) void*)(base + kap * kCD), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(d.vc + at + 16 * vp),
+                                       (__attribute__((address_space(3))) void*)(base + kCST * kCD + 4 * vw * kCD), 16, 0, 0);
+    }
+  };
+  // query fragments: column col, dims 64 kb + 32 g .. +31; rows of no token are zero
   v8i qf[4];
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb) {
     int w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (row_ok) {
-      const size_t at = ((size_t)(R.t0 + row_t) * kCHQ + head) * kCD + 64 * kb + 32 * g;
+      const size_t at = ((size_t)(t0 + tok) * kCHQ + head) * kCD + 64 * kb + 32 * g;
       if (d.q8) {
         const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(d.q) + at);
         const v4i a = src[0], e = src[1];
@@ -97,11 +146,11 @@ __global__ __launch_bounds__(64) void chunk_kernel(ChunkDev d) {
         const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.q) + at);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const v4i r = src[c];
+          const v4i x = src[c];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            w[2 * c + j] = (int)(f2e4m3x2_nan(bf_lo((uint32_t)r[2 * j]), bf_hi((uint32_t)r[2 * j])) |
-                                 (f2e4m3x2_nan(bf_lo((uint32_t)r[2 * j + 1]), bf_hi((uint32_t)r[2 * j + 1])) << 16));
+            w[2 * c + j] = (int)(f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j]), bf_hi((uint32_t)x[2 * j])) |
+                                 (f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j + 1]), bf_hi((uint32_t)x[2 * j + 1])) << 16));
         }
       }
     }
@@ -113,82 +162,414 @@ __global__ __launch_bounds__(64) void chunk_kernel(ChunkDev d) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   float m = -1e30f, l = 0.f;
-  for (int k0 = 0; k0 < nkeys; k0 += kCST) {
-    // V rows: LDS row r holds key 16 (r / 16) + 8 ((r % 8) / 4) + 4 ((r / 8) % 2) + r % 4, its 16-byte piece p at p ^ (r % 8);
-    // a key behind the range is zero
-    __syncthreads();
+  uint32_t bad = 0;  // bits of NaN values on the causal border
+  // this lane's places in a block: K row col, piece 4 kb + 2 g + e; V row 8 g + (l % 16) / 2 (+ 16 c), piece 2 dt + (l / 16) % 2
+  int ka[4], va[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 4), p = lane & 15, key = k0 + 16 * (r >> 4) + 8 * ((r & 7) >> 2) + 4 * ((r >> 3) & 1) + (r & 3);
-      v4i v = {0, 0, 0, 0};
-      if (key < nkeys) v = *reinterpret_cast<const v4i*>(d.vc + ((size_t)slot_of(d, b, key) * kCHKV + h) * kCD + 16 * p);
-      *reinterpret_cast<v4i*>(vs + r * kCD + 16 * (p ^ (r & 7))) = v;
-    }
-    __syncthreads();
+  for (int i = 0; i < 4; ++i) {
+    ka[i] = col * kCD + 16 * ((4 * (i >> 1) + 2 * g + (i & 1)) ^ (col & 7));
+    const int vr = (lane & 15) >> 1;
+    va[i] = kCST * kCD + (8 * g + vr) * kCD + 16 * ((2 * i + ((lane >> 4) & 1)) ^ vr) + 8 * (lane & 1);
+  }
+  const float sl2 = d.scale_log2;
+  auto value = [&](const uint8_t* X, int dt, int c) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (__attribute__((address_space(3))) v2i*)(X + va[dt & 3] + 128 * (dt >> 2) + 16 * kCD * c));
+  };
+  auto block = [&](const uint8_t* X, int key0) {
     v16f s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
-    const uint8_t* kr = d.kc + ((size_t)slot_of(d, b, min(k0 + col, nkeys - 1)) * kCHKV + h) * kCD + 32 * g;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      const v4i a = *reinterpret_cast<const v4i*>(kr + 64 * kb), e = *reinterpret_cast<const v4i*>(kr + 64 * kb + 16);
+      const v4i a = *reinterpret_cast<const v4i*>(X + ka[2 * (kb & 1)] + 128 * (kb >> 1));
+      const v4i e = *reinterpret_cast<const v4i*>(X + ka[2 * (kb & 1) + 1] + 128 * (kb >> 1));
       s = mfma_qk(v8i{a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w}, qf[kb], s);
     }
-    float mx = -INFINITY;
+    const bool border = key0 + 31 > lim_first;
+    if (border) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int key = k0 + 8 * (i >> 2) + 4 * g + (i & 3);
-      s[i] = key > lim ? -INFINITY : s[i] * d.scale_log2;
-      mx = fmaxf(mx, s[i]);
+      for (int i = 0; i < 16; ++i)
+        if (key0 + 8 * (i >> 2) + 4 * g + (i & 3) > lim) s[i] = -INFINITY;
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    l *= al;
+    float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[i], s[i + 1]));
+    const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    const float tmax = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1])) * sl2;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(tmax > m + kLazyC) != 0, 0)) {
+      const float mn = fmaxf(m, tmax), al = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) o[dt] *= al;
+    }
     v8h pb[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float p = __builtin_amdgcn_exp2f(s[i] - m);
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -m));
       l += p;
       pb[i >> 3][i & 7] = (_Float16)p;
     }
-    const bool border = k0 + kCST - 1 > pre + i0;
-    v8h vis[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) vis[i >> 3][i & 7] = k0 + 8 * (i >> 2) + 4 * g + (i & 3) <= lim ? (_Float16)1.f : (_Float16)0.f;
+    for (int c = 0; c < 2; ++c) {
+      v2i w[8];
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
+      for (int dt = 0; dt < 8; ++dt) w[dt] = value(X, dt, c);
+      if (border) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[dt][i] *= al;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = 16 * c + 8 * g + ((lane & 15) >> 1), p = 2 * dt + ((lane >> 4) & 1);
-        v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (__attribute__((address_space(3))) v2i*)(vs + r * kCD + 16 * (p ^ (r & 7)) + 8 * (lane & 1)));
-        const uint32_t n0 = nan_bytes(w.x) >> 7, n1 = nan_bytes(w.y) >> 7;
-        if (border && __builtin_amdgcn_ballot_w64((n0 | n1) != 0)) {
-          v16f seen;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) seen[i] = 0.f;
-          seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(n0 * 0x38, n1 * 0x38), vis[c], seen, 0, 0, 0);
-          w = v2i{(int)(w.x & ~(n0 * 0xff)), (int)(w.y & ~(n1 * 0xff))};
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[dt][i] = seen[i] > 0.f ? __builtin_nanf("") : o[dt][i];
+        for (int dt = 0; dt < 8; ++dt) {
+          const uint32_t n0 = nan_bytes(w[dt].x), n1 = nan_bytes(w[dt].y);
+          bad |= n0 | n1;
+          w[dt] = v2i{(int)(w[dt].x & ~(n0 | (n0 - (n0 >> 7)))), (int)(w[dt].y & ~(n1 | (n1 - (n1 >> 7))))};
         }
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w.x, w.y), pb[c], o[dt], 0, 0, 0);
       }
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[c], o[dt], 0, 0, 0);
+    }
+  };
+  auto step = [&](int st, const uint8_t* X) {
+    if (!active) return;
+#pragma unroll 1
+    for (int u = 0; u < SUB; ++u) {
+      const int blk = KG == 1 ? u : kg, key0 = st * STEP + 32 * blk;
+      if (key0 > lim_last) return;
+      block(X + blk * kBlk, key0);
+    }
+  };
+  const int st1 = run.st0 + run.nst;
+  if (run.nst > 0) {
+    entries(run.st0);
+    copy(run.st0, X0);
+    entries(run.st0 + 1);
+    for (int st = run.st0; st < st1; st += 2) {
+      wait_vm0();
+      barrier();  // every wave's copies of this step have landed, and every wave is done with the other stage
+      if (st + 1 < st1) copy(st + 1, X1);
+      entries(st + 2);
+      step(st, X0);
+      if (st + 1 >= st1) break;
+      wait_vm0();
+      barrier();
+      if (st + 2 < st1) copy(st + 2, X0);
+      entries(st + 3);
+      step(st + 1, X1);
     }
   }
   l += __shfl_xor(l, 32);
-  const float il = l > 0.f ? 1.f / l : l;  // (NaN stays)
-  if (!row_ok) return;
-  uint16_t* dst = d.out + ((size_t)(R.t0 + row_t) * kCHQ + head) * kCD + 4 * g;
+  barrier();  // every wave is done with both stages
+  uint16_t* const dst = d.out + ((size_t)(t0 + tok) * kCHQ + head) * kCD + 4 * g;
+  float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane * 4;
+  float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col;
+  if constexpr (KG == 1) {
+    if (active && slot < 0) {
+      const float il = l > 0.f ? 1.f / l : l;  // (no key: 0; NaN stays)
+      if (row_ok)
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt)
+        for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
-      *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * a) = make_uint2(pack_bf2(o[dt][4 * a] * il, o[dt][4 * a + 1] * il),
-                                                                    pack_bf2(o[dt][4 * a + 2] * il, o[dt][4 * a + 3] * il));
+          for (int a = 0; a < 4; ++a)
+            *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * a) = make_uint2(pack_bf2(o[dt][4 * a] * il, o[dt][4 * a + 1] * il),
+                                                                          pack_bf2(o[dt][4 * a + 2] * il, o[dt][4 * a + 3] * il));
+    } else if (active) {
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<v4f*>(wo + (dt * 4 + a) * 256) = v4f{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
+      if (g == 0) wml[0] = m, wml[32] = l;
+    }
+  } else {
+    if (g == 0) mlw[wave][0][col] = m, mlw[wave][1][col] = l;
+    barrier();
+    float M = -1e30f, L = 0.f;
+#pragma unroll
+    for (int k = 0; k < KG; ++k) M = fmaxf(M, mlw[RG * k + rw][0][col]);
+#pragma unroll
+    for (int k = 0; k < KG; ++k) L += __builtin_amdgcn_exp2f(mlw[RG * k + rw][0][col] - M) * mlw[RG * k + rw][1][col];
+    const float f = __builtin_amdgcn_exp2f(m - M), il = L > 0.f ? 1.f / L : L;
+    if (slot >= 0 && kg == 0 && g == 0) wml[0] = M, wml[32] = L;
+    // four dim tiles at a time through LDS: [wave][dt][a][lane], waves 0-3 of it in X0, 4-7 in X1
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (q) barrier();
+      uint8_t* const mine = (wave < 4 ? X0 : X1) + (wave & 3) * 16384 + lane * 16;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<v4f*>(mine + (dt * 4 + a) * 1024) = v4f{o[4 * q + dt][4 * a] * f, o[4 * q + dt][4 * a + 1] * f,
+                                                                    o[4 * q + dt][4 * a + 2] * f, o[4 * q + dt][4 * a + 3] * f};
+      barrier();
+      // this wave sums dim tile kg of row group rw
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+          const int w = RG * k + rw;
+          v += *reinterpret_cast<const v4f*>((w < 4 ? X0 : X1) + (w & 3) * 16384 + (kg * 4 + a) * 1024 + lane * 16);
+        }
+        const int dt = 4 * q + kg;
+        if (slot >= 0)
+          *reinterpret_cast<v4f*>(wo + (dt * 4 + a) * 256) = v;
+        else if (row_ok)
+          *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * a) = make_uint2(pack_bf2(v[0] * il, v[1] * il), pack_bf2(v[2] * il, v[3] * il));
+      }
+    }
+    barrier();  // the stages are free again
+  }
+  return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+}
+
+// The line of the call's tiles (q36_chunk.h), this workgroup's share of it, and its runs one after another.
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_kernel(ChunkDev d) {
+  // two objects: the compiler then sees that a copy into one stage does not touch what is read from the other
+  __shared__ __align__(1024) uint8_t X0[kStage];
+  __shared__ __align__(1024) uint8_t X1[kStage];
+  __shared__ float mlw[8][2][32];
+  __shared__ int64_t sums[8];
+  __shared__ int64_t found_at;
+  __shared__ int found_b, nan_seen;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = gridDim.x;
+  if (tid == 0) nan_seen = 0;
+  int64_t mine = 0;
+  for (int q = tid; q < d.B; q += 512) mine += ck_weight(req_of(d, q).r);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
+  if (lane == 0) sums[wave] = mine;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) total += sums[w];
+  total = uni(total);
+  const int nsh = ck_shares(total, G);
+  // neighbouring shares on one XCD (workgroup i runs on XCD i % 8): they walk the same keys, out of its L2
+  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, first = xcd * nsh / 8, count = (xcd + 1) * nsh / 8 - first;
+  const int share = G % 8 ? (int)blockIdx.x : at < count ? first + at : nsh + (xcd * (G / 8) + at) - (first + count);
+  if (share >= nsh) {
+    if (tid == 0 && share < G) d.cuts[share] = int4{-1, 0, 0, 0};
+    return;
+  }
+  const int64_t x0 = uni(ck_share_begin(total, nsh, share)), x1 = uni(ck_share_begin(total, nsh, share + 1));
+  // the request that x0 lies in
+  int64_t before = 0;
+  for (int c0 = 0; c0 < d.B; c0 += 512) {
+    const int64_t w = c0 + tid < d.B ? ck_weight(req_of(d, c0 + tid).r) : 0;
+    int64_t inc = w;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t v = __shfl_up(inc, o);
+      inc += lane >= o ? v : 0;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = inc;
+    __syncthreads();
+    int64_t off = before + inc - w;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      off += k < wave ? sums[k] : 0;
+      before += sums[k];
+    }
+    if (off <= x0 && x0 < off + w) found_b = c0 + tid, found_at = off;
+    if (before > x0) break;
+  }
+  __syncthreads();
+  int b = uni(found_b), h = 0, tile = 0;
+  int64_t off = uni(found_at);
+  Req q = req_of(d, b);
+  q = Req{uni(q.t0), {uni(q.r.n), uni(q.r.nk)}};
+  if (q.r.n > 0) {
+    const int64_t half = ck_weight(q.r) / 2;
+    h = x0 - off >= half;
+    off += h * half;
+    tile = ck_tile_at(q.r, x0 - off);
+    off += ck_before(q.r, tile);
+  }
+  int4 cut = {-1, 0, 0, 0};
+  bool nans = false;
+  while (off < x1) {
+    if (q.r.n == 0) {
+      ++off;
+    } else {
+      const int steps = ck_steps(q.r, tile);
+      const ChunkRun run = ck_run(steps, off, x0, x1);
+      if (run.nst >= 0) {
+        const bool whole = run.first && run.last;
+        const int slot = whole ? -1 : ck_slot(share, run.first);
+        if (!whole && run.first) cut = int4{b, 2 * tile + h, ck_share_of(total, nsh, off + kTileOvh / 2 + steps - 1), 0};
+        if (ck_wide(q.r.n)) nans |= tile_run<8>(d, X0, X1, mlw, b, q.t0, q.r, h, tile, run, slot);
+        else nans |= tile_run<2>(d, X0, X1, mlw, b, q.t0, q.r, h, tile, run, slot);
+      }
+      off += steps + kTileOvh;
+      if (++tile < ck_tiles(q.r.n)) continue;
+      tile = 0;
+      if (++h < 2) continue;
+    }
+    h = 0;
+    if (++b >= d.B) break;
+    q = req_of(d, b);
+    q = Req{uni(q.t0), {uni(q.r.n), uni(q.r.nk)}};
+  }
+  if (nans && lane == 0) nan_seen = 1;
+  __syncthreads();
+  if (tid == 0) {
+    cut.w = nan_seen;
+    d.cuts[share] = cut;
+  }
+}
+
+// Which of the values at dims dim .. dim + 3 (bit 7 of each byte) are NaN at a key on the border that new token tok sees.
+__device__ __forceinline__ uint32_t border_nans(const ChunkDev& d, int b, ChunkReq r, int h, int tok, int dim) {
+  const int pre = r.nk - r.n;
+  uint32_t n = 0;
+  for (int key = max(0, pre + (tok & ~3) - 31); key <= pre + tok; ++key) {
+    const int top = (int)d.num_slots - 1, pg = min(max(d.pt[(size_t)b * d.pt_stride + (key >> d.sh)], 0), top >> d.sh);
+    const int sl = min((pg << d.sh) + (key & ((1 << d.sh) - 1)), top);
+    n |= nan_bytes(*reinterpret_cast<const uint32_t*>(d.vc + ((size_t)sl * kCHKV + h) * kCD + dim));
+  }
+  return n;
+}
+__device__ __forceinline__ uint2 put_nans(uint2 v, uint32_t n) {
+  const uint32_t q = 0x7fc0;
+  return make_uint2((n & 0x80 ? (v.x & 0xffff0000u) | q : v.x) | (n & 0x8000 ? 0xffff0000u : 0), (n & 0x800000 ? (v.y & 0xffff0000u) | q : v.y) | (n & 0x80000000u ? 0xffff0000u : 0));
+}
+
+// The cut tiles: out = bf16(sum_p exp2(m_p - M) o_p / sum_p exp2(m_p - M) l_p) over a tile's partials p.  A workgroup takes one
+// (tile, 32 rows, 32 dims) at a time; few partials: wave a has the lanes' a-th four dims of all of them; more: wave w has
+// partials w, w + 4, .. and the waves' sums meet in LDS.
+__global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
+  __shared__ int list[1024];
+  __shared__ int counts[4], nan_flags[4];
+  __shared__ v4f part[4][4][64];
+  __shared__ float pml[4][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), col = lane & 31, g = lane >> 5;
+  // the shares that leave a cut tile, in order
+  int have = 0;
+  uint64_t nans = 0;
+  for (int c0 = 0; c0 < G; c0 += 256) {
+    const int4 c = c0 + tid < G ? d.cuts[c0 + tid] : int4{-1, 0, 0, 0};
+    const bool is = c.x >= 0;
+    nans |= __builtin_amdgcn_ballot_w64(c.w != 0);
+    const uint64_t bits = __builtin_amdgcn_ballot_w64(is);
+    if (lane == 0) counts[wave] = __builtin_popcountll(bits);
+    __syncthreads();
+    int at = have + __builtin_popcountll(bits & ((1ull << lane) - 1));
+    for (int w = 0; w < 4; ++w) {
+      at += w < wave ? counts[w] : 0;
+      have += counts[w];
+    }
+    if (is) list[at] = c0 + tid;
+    __syncthreads();
+  }
+  if (lane == 0) nan_flags[wave] = nans != 0;
+  __syncthreads();
+  const bool any_nan = uni(nan_flags[0] | nan_flags[1] | nan_flags[2] | nan_flags[3]) != 0;
+  for (int unit = blockIdx.x; unit < have * 64; unit += gridDim.x) {
+    const int share = uni(list[unit >> 6]), rw = (unit >> 3) & 7, dt = unit & 7;
+    const int4 c = d.cuts[share];
+    const int b = uni(c.x), tile = uni(c.y) >> 1, h = uni(c.y) & 1, n = uni(c.z) - share + 1;
+    const Req q = req_of(d, b);
+    const int tok = tile * ck_tile_tok(q.r.n) + 4 * rw + (col >> 3), head = h * kCG + (col & 7);
+    if ((!ck_wide(q.r.n) && rw >= 2) || uni(tok) >= q.r.n) continue;
+    const bool row_ok = tok < q.r.n;
+    uint16_t* const dst = d.out + ((size_t)(q.t0 + tok) * kCHQ + head) * kCD + 32 * dt + 4 * g;
+    auto ml = [&](int p, int what) { return d.ws_ml[(size_t)ck_slot(share + p, p == 0) * kSlotML + rw * 64 + 32 * what + col]; };
+    auto po = [&](int p, int a) {
+      return *reinterpret_cast<const v4f*>(d.ws_o + (size_t)ck_slot(share + p, p == 0) * kSlotF + ((rw * 8 + dt) * 4 + a) * 256 + lane * 4);
+    };
+    auto store = [&](v4f v, float il) {
+      uint2 w = make_uint2(pack_bf2(v[0] * il, v[1] * il), pack_bf2(v[2] * il, v[3] * il));
+      if (__builtin_expect(any_nan, 0)) w = put_nans(w, border_nans(d, b, q.r, h, tok, 32 * dt + 4 * g + 8 * wave));
+      *reinterpret_cast<uint2*>(dst + 8 * wave) = w;
+    };
+    if (n <= 4) {
+      float mp[4], lp[4], M = -1e30f, L = 0.f;
+      v4f v[4], s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int pc = min(p, n - 1);
+        mp[p] = ml(pc, 0), lp[p] = ml(pc, 1), v[p] = po(pc, wave);
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p) M = fmaxf(M, mp[p]);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float w = p < n ? __builtin_amdgcn_exp2f(mp[p] - M) : 0.f;
+        if (p < n) {
+          L += w * lp[p];
+          s += w * v[p];
+        }
+      }
+      const float il = L > 0.f ? 1.f / L : L;
+      if (row_ok) store(s, il);
+      continue;
+    }
+    float M = -1e30f, L = 0.f;
+    v4f s[4] = {};
+    for (int p = wave; p < n; p += 8) {
+      const int p2 = min(p + 4, n - 1);
+      const float m0 = ml(p, 0), l0 = ml(p, 1), m1 = p + 4 < n ? ml(p2, 0) : -1e30f, l1 = p + 4 < n ? ml(p2, 1) : 0.f;
+      v4f v0[4], v1[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) v0[a] = po(p, a), v1[a] = po(p2, a);
+      const float mn = fmaxf(M, fmaxf(m0, m1)), f = __builtin_amdgcn_exp2f(M - mn), w0 = __builtin_amdgcn_exp2f(m0 - mn);
+      M = mn;
+      L = L * f + w0 * l0;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) s[a] = s[a] * f + w0 * v0[a];
+      if (p + 4 < n) {
+        const float w1 = __builtin_amdgcn_exp2f(m1 - mn);
+        L += w1 * l1;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) s[a] += w1 * v1[a];
+      }
+    }
+    pml[wave][0][lane] = M, pml[wave][1][lane] = L;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) part[wave][a][lane] = s[a];
+    __syncthreads();
+    const float Ma = fmaxf(fmaxf(pml[0][0][lane], pml[1][0][lane]), fmaxf(pml[2][0][lane], pml[3][0][lane]));
+    float La = 0.f;
+    v4f t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(pml[w][0][lane] - Ma);
+      La += f * pml[w][1][lane];
+      t += f * part[w][wave][lane];
+    }
+    const float il = La > 0.f ? 1.f / La : La;
+    if (row_ok) store(t, il);
+    __syncthreads();
+  }
+  if (__builtin_expect(!any_nan, 1)) return;
+  // every new token and KV head, a thread 4 dims: the NaN that the tiles' own workgroups left out (a cut tile's are there)
+  for (int b = 0; b < d.B; ++b) {
+    const Req q = req_of(d, b);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < (int64_t)q.r.n * (2 * kCD / 4); i += (int64_t)gridDim.x * 256) {
+      const int tok = (int)(i / (2 * kCD / 4)), h = (int)(i / (kCD / 4)) & 1, dim = 4 * (int)(i % (kCD / 4));
+      const uint32_t n = border_nans(d, b, q.r, h, tok, dim);
+      if (n)
+        for (int e = 0; e < 4; ++e)
+          if (n >> (8 * e + 7) & 1)
+            for (int hd = 0; hd < kCG; ++hd) d.out[((size_t)(q.t0 + tok) * kCHQ + h * kCG + hd) * kCD + dim + e] = 0x7fc0;
+    }
+  }
+}
+
+// Workgroups: one a CU (their LDS and registers fill it).
+int chunk_groups() { return std::min(std::max(device_cus(), 1), 1024); }
+struct ChunkWs {
+  size_t o, ml, cuts, total;
+};
+ChunkWs chunk_ws(int G) {
+  ChunkWs w;
+  w.o = 0;
+  w.ml = align_up(w.o + sizeof(float) * 2 * (size_t)G * kSlotF, 256);
+  w.cuts = align_up(w.ml + sizeof(float) * 2 * (size_t)G * kSlotML, 256);
+  w.total = align_up(w.cuts + sizeof(int4) * (size_t)G, 256);
+  return w;
 }
 
 }  // namespace
@@ -196,7 +577,7 @@ __global__ __launch_bounds__(64) void chunk_kernel(ChunkDev d) {
 
 using namespace q36;
 
-extern "C" size_t q36_attn_chunk_workspace_bytes(void) { return 256; }
+extern "C" size_t q36_attn_chunk_workspace_bytes(void) { return chunk_ws(chunk_groups()).total; }
 
 extern "C" int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream) {
   Q36_REQUIRE(a != nullptr, "q36_attn_chunk: null args");
@@ -214,13 +595,19 @@ extern "C" int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream) {
   Q36_REQUIRE(aligned16(a->q) && aligned16(a->k_cache) && aligned16(a->v_cache) && aligned16(a->out) &&
                   (reinterpret_cast<uintptr_t>(a->workspace) & 255u) == 0,
               "q36_attn_chunk: q, out and the caches must be 16-byte and workspace 256-byte aligned");
-  Q36_REQUIRE(a->workspace_bytes >= q36_attn_chunk_workspace_bytes(), "q36_attn_chunk: workspace of %zu bytes < %zu required",
-              a->workspace_bytes, q36_attn_chunk_workspace_bytes());
+  Q36_REQUIRE(a->scale > 0.f && a->scale <= 1e6f, "q36_attn_chunk: scale=%g out of range", (double)a->scale);
+  const int G = chunk_groups();
+  const ChunkWs L = chunk_ws(G);
+  Q36_REQUIRE(a->workspace_bytes >= L.total, "q36_attn_chunk: workspace of %zu bytes < %zu required", a->workspace_bytes, L.total);
   int sh = 0;
   while ((1 << sh) < a->page_size) ++sh;
+  char* const ws = static_cast<char*>(a->workspace);
   const ChunkDev d{a->B, a->T, sh, a->pt_stride, a->q_e4m3, a->num_slots, a->q, static_cast<const uint8_t*>(a->k_cache),
                    static_cast<const uint8_t*>(a->v_cache), a->page_table, a->seqlens, a->qsl, static_cast<uint16_t*>(a->out),
-                   a->scale * 1.44269504088896340736f};
-  chunk_kernel<<<2 * (unsigned)(a->T / 4 + a->B), 64, 0, static_cast<hipStream_t>(stream)>>>(d);
+                   a->scale * 1.44269504088896340736f, reinterpret_cast<float*>(ws + L.o), reinterpret_cast<float*>(ws + L.ml),
+                   reinterpret_cast<int4*>(ws + L.cuts)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  chunk_kernel<<<G, 512, 0, st>>>(d);
+  chunk_combine_kernel<<<1024, 256, 0, st>>>(d, G);
   return check_launch("q36_attn_chunk");
 }

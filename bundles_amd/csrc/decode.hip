@@ -29,7 +29,6 @@
 //                   workgroup holds whole is written by the split kernel itself).
 #include <math.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "q36_device.h"
@@ -830,28 +829,18 @@ __global__ __launch_bounds__(64 * WPR) void decode_combine_kernel(DecodeDev d, i
   put_row(d, bt, head, c, a, L, gate);
 }
 
-int decode_cus() {
-  static std::atomic<int> known[64];  // per device, 0: not asked yet
-  int cus = 256, dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return cus;
-  const bool slot = dev >= 0 && dev < 64;
-  if (slot && known[dev].load(std::memory_order_relaxed)) return known[dev].load(std::memory_order_relaxed);
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && slot)
-    known[dev].store(cus, std::memory_order_relaxed);
-  return cus;
-}
 // Equal splits per request: as asked for, or (a workspace too small for the balanced form) enough to
 // give every CU a workgroup.
 int decode_splits(int B, int splits) {
   if (splits > 0) return min(splits, 64);
-  return max(1, min(64, decode_cus() / (B * kKVH)));
+  return max(1, min(64, device_cus() / (B * kKVH)));
 }
 size_t decode_slots_bytes(size_t slots) {  // slots of kDRows rows (or twice as many of half the rows)
   return align_up(sizeof(float) * slots * kDRows * kDD, 256) + align_up(sizeof(float) * slots * 2 * kDRows, 256);
 }
 size_t decode_ws_bytes(int B, int S) { return decode_slots_bytes((size_t)B * kKVH * S); }
 // Balanced: two slots a workgroup, one workgroup a CU of kDRows rows or two a CU of half the rows
-size_t decode_bal_bytes(int B) { return decode_slots_bytes(2 * (size_t)decode_cus()) + align_up(sizeof(int2) * (size_t)B, 256); }
+size_t decode_bal_bytes(int B) { return decode_slots_bytes(2 * (size_t)device_cus()) + align_up(sizeof(int2) * (size_t)B, 256); }
 
 }  // namespace
 }  // namespace q36
@@ -884,7 +873,7 @@ extern "C" int q36_attn_decode(const q36_decode_args* a, q36_stream_t stream) {
                          (reinterpret_cast<uintptr_t>(a->oq) & 3u) == 0 && (reinterpret_cast<uintptr_t>(a->oqs) & 3u) == 0),
               "q36_attn_decode: gate must be 8-byte, oq and oqs 4-byte aligned");
   const bool one = a->NT <= 2;  // one row tile, two workgroups a CU
-  const int cus = decode_cus(), resident = (one ? kDecWPE1 : 1) * cus;
+  const int cus = device_cus(), resident = (one ? kDecWPE1 : 1) * cus;
   const int max_steps = table_steps(a->pt_stride);
   // Where no length the table can hold makes the dealing good, the splits are fixed here, by the rule that the kernel
   // applies to the lengths, and neither the dealing nor a combine that may find nothing cut is paid for.  Measured, us

@@ -1,0 +1,103 @@
+// How the chunk attention deals one call's work to its workgroups: the integer arithmetic, for the kernels and a program
+// that checks it over many batches on the CPU.
+//
+// A tile is a run of new tokens of one request with one KV head's 8 query heads; it walks the keys that its last token
+// sees, in steps.  A request of more than kNarrow new tokens is cut into wide tiles (kWideTok tokens, one set of keys for
+// all eight waves, kWideKeys a step), another into narrow ones (kNarrowTok tokens, four sets of keys a step between pairs of
+// waves).  The tiles of all requests, head by head, lie on a line; a tile weighs its steps and kTileOvh (what starting
+// and ending one costs beside its steps), half before and half behind them.  The line is cut into equal shares, a share a
+// workgroup, so that a share holds the end of a tile, whole tiles and the start of another.  A step belongs to the share
+// that its place lies in; a cut tile leaves a partial in each share that has steps of it.
+#pragma once
+#include <stdint.h>
+
+namespace q36 {
+
+constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 64, kNarrowKeys = 128;
+constexpr int kTileOvh = 4;
+constexpr int kLeastShare = 4;  // a share is no shorter (but for a line shorter than this)
+
+struct ChunkReq {
+  int n, nk;  // new tokens, keys (the new ones included)
+};
+__host__ __device__ __forceinline__ bool ck_wide(int n) { return n > kNarrow; }
+__host__ __device__ __forceinline__ int ck_tile_tok(int n) { return ck_wide(n) ? kWideTok : kNarrowTok; }
+__host__ __device__ __forceinline__ int ck_tiles(int n) {
+  return ck_wide(n) ? (n + kWideTok - 1) / kWideTok : (n + kNarrowTok - 1) / kNarrowTok;
+}
+// the keys that tile i's last token sees
+__host__ __device__ __forceinline__ int ck_keys(ChunkReq r, int i) {
+  const int64_t end = (int64_t)(i + 1) * ck_tile_tok(r.n), last = end < r.n ? end : r.n, k = (int64_t)r.nk - r.n + last;
+  return k > 0 ? (int)k : 0;
+}
+__host__ __device__ __forceinline__ int ck_step_keys(int n) { return ck_wide(n) ? kWideKeys : kNarrowKeys; }
+__host__ __device__ __forceinline__ int ck_steps(ChunkReq r, int i) {
+  const int ks = ck_step_keys(r.n);
+  return (ck_keys(r, i) + ks - 1) / ks;
+}
+// sum over j < count of max(0, c + j)
+__host__ __device__ __forceinline__ int64_t ck_series(int64_t c, int64_t count) {
+  if (c < 0) {
+    count += c;
+    c = 0;
+  }
+  return count > 0 ? count * c + count * (count - 1) / 2 : 0;
+}
+__host__ __device__ __forceinline__ int64_t ck_ceil64(int64_t v) { return v >= 0 ? (v + 63) / 64 : -((-v) / 64); }
+// the weight of one head's tiles before tile i (i up to the number of tiles)
+__host__ __device__ __forceinline__ int64_t ck_before(ChunkReq r, int i) {
+  int64_t s = 0;
+  if (ck_wide(r.n)) {
+    // all but the last tile see nk - n + 32 (k + 1) keys: a series each for even and odd k
+    const int64_t pre = (int64_t)r.nk - r.n, full = i < ck_tiles(r.n) ? i : i - 1;
+    s = ck_series(ck_ceil64(pre + 32), (full + 1) / 2) + ck_series(ck_ceil64(pre + 64), full / 2);
+    if (full < i) s += ck_steps(r, i - 1);
+  } else {
+    for (int k = 0; k < i; ++k) s += ck_steps(r, k);
+  }
+  return s + (int64_t)i * kTileOvh;
+}
+// the weight of a request, both heads (an empty one weighs 1: what passing over it costs)
+__host__ __device__ __forceinline__ int64_t ck_weight(ChunkReq r) { return r.n > 0 ? 2 * ck_before(r, ck_tiles(r.n)) : 1; }
+// the tile of a head that place x of its line lies in
+__host__ __device__ __forceinline__ int ck_tile_at(ChunkReq r, int64_t x) {
+  int lo = 0, hi = ck_tiles(r.n) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (ck_before(r, mid) <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__host__ __device__ __forceinline__ int ck_shares(int64_t total, int G) {
+  const int64_t s = total / kLeastShare;
+  return s >= G ? G : s > 1 ? (int)s : 1;
+}
+__host__ __device__ __forceinline__ int64_t ck_share_begin(int64_t total, int nsh, int w) {
+  const int64_t q = total / nsh, r = total - q * nsh;
+  return q * w + r * w / nsh;
+}
+// the share that place x lies in
+__host__ __device__ __forceinline__ int ck_share_of(int64_t total, int nsh, int64_t x) {
+  const int64_t q = total / nsh;
+  int w = (int)(x / (q + 1));  // shares are q or q + 1 long
+  while (w + 1 < nsh && ck_share_begin(total, nsh, w + 1) <= x) ++w;
+  return w;
+}
+// The steps [st0, st0 + nst) of a tile at `off` on the line that the share [x0, x1) has; first, last: whether they hold the
+// tile's first and last step.  A tile without a step is its start's share's, whole.  nst < 0: the share has none.
+struct ChunkRun {
+  int st0, nst;
+  bool first, last;
+};
+__host__ __device__ __forceinline__ ChunkRun ck_run(int steps, int64_t off, int64_t x0, int64_t x1) {
+  if (steps == 0) return ChunkRun{0, off >= x0 && off < x1 ? 0 : -1, true, true};
+  const int64_t at = off + kTileOvh / 2;  // of its first step
+  const int64_t a = x0 > at ? x0 - at : 0, e = x1 - at < steps ? x1 - at : steps;
+  return ChunkRun{(int)a, e > a ? (int)(e - a) : -1, a == 0, e == steps};
+}
+// The partial of share w: one for a tile that ends here or goes on through, one for a tile that starts here.
+__host__ __device__ __forceinline__ int ck_slot(int w, bool first) { return 2 * w + (first ? 1 : 0); }
+
+}  // namespace q36

@@ -14,6 +14,9 @@ void set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 // Allow kernel fn `bytes` of dynamic LDS (above 64 KiB: raises the kernel's limit once per device).
 int ensure_lds(const void* fn, size_t bytes, const char* what);
 
+// Compute units of the current device (256 where it cannot be asked).
+int device_cus();
+
 inline bool aligned16(const void* p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
