@@ -68,7 +68,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7
 // once more and puts the NaN where it is seen.
 
 constexpr int kBlk = 2 * kCST * kCD;  // 32 keys in LDS: their K rows, then their V rows
-constexpr int kStage = 4 * kBlk;
+constexpr int kSet = 4 * kBlk;
 constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a partial
 constexpr float kLazyC = 8.f;  // the outputs are rescaled when a row's maximum has grown by 2^8 (weights up to 2^8 are exact in f16)
 
@@ -77,191 +77,234 @@ __device__ __forceinline__ int64_t uni(int64_t v) {
   return (int64_t)(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
 }
 __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8)); }
+// 16 bytes a lane from memory into LDS at byte `at` + 16 lane of the workgroup's, past the registers.  In asm, so that the
+// compiler does not hold each read of LDS back until every copy in flight has landed; the caller waits (wait_vm0).
+__device__ __forceinline__ void copy16(const uint8_t* src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) uint8_t*)p);
+}
 __device__ __forceinline__ void barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// One run of a tile's steps by the 8 waves.  RG = 8 (wide): wave w has rows 32 w .. of the tile's 256 (4 tokens x 8 heads)
-// and every wave walks all keys, 64 a step.  RG = 2 (narrow): waves 2 k, 2 k + 1 have rows 0 .. 31, 32 .. 63 and walk the
-// k-th 32 keys of each step's 128; the four are merged at the end.
+// threadIdx.x through an empty asm: what is derived from it is formed afresh where it is used, in place of holding, or
+// spilling, a register across the steps.
+__device__ __forceinline__ int fresh_tid() {
+  int t = (int)threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// One run of a tile's steps by the 8 waves, four blocks of 32 keys between two barriers, out of one of two sets of four blocks
+// while the other fills.  RG = 8 (wide): wave w has rows 32 w .. of the tile's 256 (4 tokens x 8 heads) and walks all the
+// blocks.  RG = 2 (narrow): waves 2 k, 2 k + 1 have rows 0 .. 31, 32 .. 63 and walk block k of each set; the four are merged
+// at the end.
 // Scores S^T = K Q^T (32x32x64, e4m3): lane l holds row l % 32 and keys 8 (i / 4) + 4 (l / 32) + i % 4.  O^T += V^T P^T
 // (32x32x16, f16): the lane's own weights in the order it has them, V^T by the transpose read from LDS rows in that order.
 // A block of 32 keys in LDS: K row r holds key r, V row r key 16 (r / 16) + 8 ((r % 8) / 4) + 4 ((r / 8) % 2) + r % 4, 16-byte
-// piece p of a row at p ^ (r % 8), so that eight lanes' reads fall on eight bank slots.
+// piece p of K row r at p ^ (r % 16), of V row r at p ^ 2 (r % 8): the 16 lanes' keys and the 32 lanes' values that are served
+// together fall on all 16 of the row's bank slots.
 template <int RG>
-__device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X0, uint8_t* X1, float (*mlw)[2][32], int b, int t0, ChunkReq r, int h,
+__device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X, float (*mlw)[2][32], int b, int t0, ChunkReq r, int h,
                                          int tile, ChunkRun run, int slot) {
-  constexpr int KG = 8 / RG, SUB = KG == 1 ? 2 : 1, NE = KG == 1 ? 2 : 4, STEP = KG == 1 ? kWideKeys : kNarrowKeys;
-  static_assert(STEP == 32 * (KG == 1 ? SUB : KG), "a step's blocks");
-  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, g = lane >> 5;
-  const int wave = uni(tid >> 6), rw = wave % RG, kg = wave / RG;
+  constexpr int KG = 8 / RG, NE = 4;  // a set's blocks, and a lane's copies of a set
+  static_assert(kWideKeys == 32 && (kNarrowKeys == 32 * KG || KG == 1), "a step is a block, or a set");
+  const int wave = uni(fresh_tid() >> 6), rw = wave % RG, kg = wave / RG;
   const int pre = r.nk - r.n, vis = ck_keys(r, tile);
   const int tok0 = tile * (4 * RG) + 4 * rw;  // the wave's first token
   const bool active = tok0 < r.n;
-  const int tok = tok0 + (col >> 3), head = h * kCG + (col & 7);
-  const bool row_ok = tok < r.n;
-  const int lim = row_ok ? pre + tok : -1, lim_first = pre + tok0, lim_last = pre + min(tok0 + 3, r.n - 1);
+  const int lim_first = pre + tok0, lim_last = pre + min(tok0 + 3, r.n - 1);
   const int32_t* const pt = d.pt + (size_t)b * d.pt_stride;
   const int sh = d.sh, low = (1 << sh) - 1, top = (int)d.num_slots - 1, top_page = top >> sh;
-  // this lane's part of the wave's copies: row `lane / 16` of four, 16 bytes
-  const int t4 = lane >> 4;
-  int ent[NE];
-  auto key_of = [&](int st, int e) {
-    const int vw = KG == 1 ? wave : 4 * (wave & 1) + e, blk = KG == 1 ? e : kg;
-    return min(st * STEP + 32 * blk + 16 * (vw >> 2) + 8 * (vw & 1) + 4 * ((vw >> 1) & 1) + t4, vis - 1);
+  const uint8_t* const kbase = d.kc + h * kCD;
+  const uint8_t* const vbase = d.vc + h * kCD;
+  // A lane's part of the wave's copies: row `lane / 16` of four, 16 bytes.
+  struct Ent {
+    int v[NE];
   };
-  auto entries = [&](int st) {
+  // its e-th copy: rows of eighth vw of block blk
+  auto vw_of = [&](int e) { return KG == 1 ? wave : 4 * (wave & 1) + e; };
+  auto blk_of = [&](int e) { return KG == 1 ? e : kg; };
+  auto kap_of = [&](int vw) { return 16 * (vw >> 2) + 8 * (vw & 1) + 4 * ((vw >> 1) & 1); };
+  auto key_of = [&](int key0, int e, int t4) { return min(key0 + 32 * blk_of(e) + kap_of(vw_of(e)) + t4, vis - 1); };
+  auto entries = [&](int key0) {
+    const int t4 = (fresh_tid() & 63) >> 4;
+    Ent x;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) ent[e] = pt[key_of(st, e) >> sh];
+    for (int e = 0; e < NE; ++e) x.v[e] = pt[key_of(key0, e, t4) >> sh];
+    return x;
   };
-  auto copy = [&](int st, uint8_t* X) {
+  auto copy = [&](int key0, const Ent& x, int set) {
+    const int lane = fresh_tid() & 63, t4 = lane >> 4;
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
-      const int vw = KG == 1 ? wave : 4 * (wave & 1) + e, blk = KG == 1 ? e : kg;
-      const int kap = 16 * (vw >> 2) + 8 * (vw & 1) + 4 * ((vw >> 1) & 1);
-      const int pg = min(max(ent[e], 0), top_page), s = min((pg << sh) + (key_of(st, e) & low), top);
-      const size_t at = (size_t)(uint32_t)s * (kCHKV * kCD) + h * kCD;
-      const int kp = (lane & 15) ^ (4 * ((vw >> 1) & 1) + t4), vp = (lane & 15) ^ (4 * (vw & 1) + t4);
-      uint8_t* const base = X + blk * kBlk;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(d.kc + at + 16 * kp),
-                                       (__attribute__((address_space(3))) void*)(base + kap * kCD), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(d.vc + at + 16 * vp),
-                                       (__attribute__((address_space(3))) void*)(base + kCST * kCD + 4 * vw * kCD), 16, 0, 0);
+      const int vw = vw_of(e), pg = min(max(x.v[e], 0), top_page), s = min((pg << sh) + (key_of(key0, e, t4) & low), top);
+      const size_t at = (size_t)(uint32_t)s * (kCHKV * kCD);
+      const int kp = (lane & 15) ^ ((kap_of(vw) & 15) + t4), vp = (lane & 15) ^ (2 * (4 * (vw & 1) + t4));
+      const uint32_t to = lds_at(X) + set * kSet + blk_of(e) * kBlk;
+      copy16(kbase + (at | (size_t)(16 * kp)), to + kap_of(vw) * kCD);
+      copy16(vbase + (at | (size_t)(16 * vp)), to + kCST * kCD + 4 * vw * kCD);
     }
   };
+  int lim;  // the row's last key
   // query fragments: column col, dims 64 kb + 32 g .. +31; rows of no token are zero
   v8i qf[4];
+  const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5;
+  {
+    const int tok = tok0 + (col >> 3), head = h * kCG + (col & 7);
+    const bool row_ok = tok < r.n;
+    lim = row_ok ? pre + tok : -1;
 #pragma unroll
-  for (int kb = 0; kb < 4; ++kb) {
-    int w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (row_ok) {
-      const size_t at = ((size_t)(t0 + tok) * kCHQ + head) * kCD + 64 * kb + 32 * g;
-      if (d.q8) {
-        const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(d.q) + at);
-        const v4i a = src[0], e = src[1];
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = e.x, w[5] = e.y, w[6] = e.z, w[7] = e.w;
-      } else {
-        const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.q) + at);
+    for (int kb = 0; kb < 4; ++kb) {
+      int w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (row_ok) {
+        const size_t at = ((size_t)(t0 + tok) * kCHQ + head) * kCD + 64 * kb + 32 * g;
+        if (d.q8) {
+          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(d.q) + at);
+          const v4i a = src[0], e = src[1];
+          w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = e.x, w[5] = e.y, w[6] = e.z, w[7] = e.w;
+        } else {
+          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.q) + at);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const v4i x = src[c];
+          for (int c = 0; c < 4; ++c) {
+            const v4i x = src[c];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            w[2 * c + j] = (int)(f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j]), bf_hi((uint32_t)x[2 * j])) |
-                                 (f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j + 1]), bf_hi((uint32_t)x[2 * j + 1])) << 16));
+            for (int j = 0; j < 2; ++j)
+              w[2 * c + j] = (int)(f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j]), bf_hi((uint32_t)x[2 * j])) |
+                                   (f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j + 1]), bf_hi((uint32_t)x[2 * j + 1])) << 16));
+          }
         }
       }
+      qf[kb] = v8i{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]};
     }
-    qf[kb] = v8i{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]};
   }
   v16f o[8];
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-  float m = -1e30f, l = 0.f;
+  float m = 0.f, l = 0.f;
+  bool begun = false;  // a block has been taken: m is its rows' largest, and grows
   uint32_t bad = 0;  // bits of NaN values on the causal border
-  // this lane's places in a block: K row col, piece 4 kb + 2 g + e; V row 8 g + (l % 16) / 2 (+ 16 c), piece 2 dt + (l / 16) % 2
-  int ka[4], va[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    ka[i] = col * kCD + 16 * ((4 * (i >> 1) + 2 * g + (i & 1)) ^ (col & 7));
-    const int vr = (lane & 15) >> 1;
-    va[i] = kCST * kCD + (8 * g + vr) * kCD + 16 * ((2 * i + ((lane >> 4) & 1)) ^ vr) + 8 * (lane & 1);
-  }
+  // this lane's places in a block: K row col, piece 2 g (the others: 4 kb + 2 g + e, by an xor); V row 8 g + (l % 16) / 2
+  // (+ 16 c), piece (l / 16) % 2 (the others: 2 dt more)
+  const int ka = col * kCD + 16 * ((2 * g) ^ (col & 15));
+  const int vr = (lane & 15) >> 1;
+  const int va = kCST * kCD + (8 * g + vr) * kCD + 16 * (((lane >> 4) & 1) ^ (2 * vr)) + 8 * (lane & 1);
   const float sl2 = d.scale_log2;
-  auto value = [&](const uint8_t* X, int dt, int c) {
-    return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-        (__attribute__((address_space(3))) v2i*)(X + va[dt & 3] + 128 * (dt >> 2) + 16 * kCD * c));
+  auto value = [&](uint32_t v0, int dt, int c) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)((v0 ^ (32 * dt)) + 16 * kCD * c));
   };
-  auto block = [&](const uint8_t* X, int key0) {
+  auto key = [&](uint32_t k0, int i) {
+    return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(k0 ^ (16 * i));
+  };
+  auto clean = [&](v2i w) {
+    const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y);
+    bad |= n0 | n1;
+    return v2i{(int)(w.x & ~(n0 | (n0 - (n0 >> 7)))), (int)(w.y & ~(n1 | (n1 - (n1 >> 7))))};
+  };
+  // the block at byte `at` of LDS, keys key0 ..
+  auto block = [&](uint32_t at, int key0) {
+    uint32_t k0 = at + ka, v0 = at + va;
+    asm volatile("" : "+v"(k0), "+v"(v0));  // (the xors below are formed here, not held across blocks)
     v16f s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      const v4i a = *reinterpret_cast<const v4i*>(X + ka[2 * (kb & 1)] + 128 * (kb >> 1));
-      const v4i e = *reinterpret_cast<const v4i*>(X + ka[2 * (kb & 1) + 1] + 128 * (kb >> 1));
+      const v4i a = key(k0, 4 * kb), e = key(k0, 4 * kb + 1);
       s = mfma_qk(v8i{a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w}, qf[kb], s);
     }
+    v2i w[8];
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) w[dt] = value(v0, dt, 0);
     const bool border = key0 + 31 > lim_first;
     if (border) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (key0 + 8 * (i >> 2) + 4 * g + (i & 3) > lim) s[i] = -INFINITY;
     }
-    float mx = fmaxf(s[0], s[1]);
+    // relative to the running maximum, which the first block sets; where a row grows past 2^8 times it, all moves to the new
+    // one.  (A row that sees nothing of a block sees nothing of the later ones.)
+    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 2; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[i], s[i + 1]));
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sl2, -m);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
     const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-    const float tmax = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1])) * sl2;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(tmax > m + kLazyC) != 0, 0)) {
-      const float mn = fmaxf(m, tmax), al = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
+    mx = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
+    if (__builtin_expect(!begun || __builtin_amdgcn_ballot_w64(mx > kLazyC) != 0, 0)) {
+      const float up = begun ? fmaxf(mx, 0.f) : mx > -INFINITY ? mx : 0.f, al = begun ? __builtin_amdgcn_exp2f(-up) : 1.f;
+      begun = true;
+      m += up;
       l *= al;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] -= up;
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) o[dt] *= al;
     }
     v8h pb[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -m));
+      const float p = __builtin_amdgcn_exp2f(s[i]);
       l += p;
       pb[i >> 3][i & 7] = (_Float16)p;
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if (border) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      v2i w[8];
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) w[dt] = value(X, dt, c);
-      if (border) {
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          const uint32_t n0 = nan_bytes(w[dt].x), n1 = nan_bytes(w[dt].y);
-          bad |= n0 | n1;
-          w[dt] = v2i{(int)(w[dt].x & ~(n0 | (n0 - (n0 >> 7)))), (int)(w[dt].y & ~(n1 | (n1 - (n1 >> 7))))};
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[c], o[dt], 0, 0, 0);
+      for (int dt = 0; dt < 8; ++dt) w[dt] = clean(w[dt]);
     }
-  };
-  auto step = [&](int st, const uint8_t* X) {
-    if (!active) return;
-#pragma unroll 1
-    for (int u = 0; u < SUB; ++u) {
-      const int blk = KG == 1 ? u : kg, key0 = st * STEP + 32 * blk;
-      if (key0 > lim_last) return;
-      block(X + blk * kBlk, key0);
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[0], o[dt], 0, 0, 0);
+      w[dt] = value(v0, dt, 1);
     }
+    
+    if (border) {
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) w[dt] = clean(w[dt]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[1], o[dt], 0, 0, 0);
   };
-  const int st1 = run.st0 + run.nst;
   if (run.nst > 0) {
-    entries(run.st0);
-    copy(run.st0, X0);
-    entries(run.st0 + 1);
-    for (int st = run.st0; st < st1; st += 2) {
+    constexpr int SET = 32 * NE;
+    const int k0 = run.st0 * (KG == 1 ? kWideKeys : kNarrowKeys), k1 = k0 + run.nst * (KG == 1 ? kWideKeys : kNarrowKeys);
+    auto set = [&](int at, int key0) {
+      if (!active) return;
+      const uint32_t to = lds_at(X) + at * kSet;
+      if constexpr (KG == 1) {
+        const int end = min(min(key0 + SET, k1), lim_last + 1);
+#pragma unroll 1
+        for (int i = 0; key0 + i < end; i += 32) block(to + i * (kBlk / 32), key0 + i);
+      } else if (key0 + 32 * kg <= lim_last) {
+        block(to + kg * kBlk, key0 + 32 * kg);
+      }
+    };
+    copy(k0, entries(k0), 0);
+    Ent e = entries(k0 + SET);
+#pragma unroll 1
+    for (int k = k0, at = 0; k < k1; k += SET, at ^= 1) {
       wait_vm0();
-      barrier();  // every wave's copies of this step have landed, and every wave is done with the other stage
-      if (st + 1 < st1) copy(st + 1, X1);
-      entries(st + 2);
-      step(st, X0);
-      if (st + 1 >= st1) break;
-      wait_vm0();
-      barrier();
-      if (st + 2 < st1) copy(st + 2, X0);
-      entries(st + 3);
-      step(st + 1, X1);
+      barrier();  // every wave's copies of this set have landed, and every wave is done with the other one
+      if (k + SET < k1) copy(k + SET, e, at ^ 1);
+      e = entries(k + 2 * SET);
+      set(at, k);
     }
   }
   l += __shfl_xor(l, 32);
-  barrier();  // every wave is done with both stages
-  uint16_t* const dst = d.out + ((size_t)(t0 + tok) * kCHQ + head) * kCD + 4 * g;
-  float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane * 4;
-  float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col;
+  if (l == 0.f) m = -1e30f;  // no key seen
+  barrier();  // every wave is done with both sets
+  const int lane2 = fresh_tid() & 63, col2 = lane2 & 31, g2 = lane2 >> 5, tok = tok0 + (col2 >> 3);
+  const bool row_ok = tok < r.n;
+  uint16_t* const dst = d.out + ((size_t)(t0 + tok) * kCHQ + h * kCG + (col2 & 7)) * kCD + 4 * g2;
+  float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane2 * 4;
+  float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col2;
   if constexpr (KG == 1) {
     if (active && slot < 0) {
       const float il = l > 0.f ? 1.f / l : l;  // (no key: 0; NaN stays)
@@ -278,23 +321,23 @@ __device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X0, uint8_t
 #pragma unroll
         for (int a = 0; a < 4; ++a)
           *reinterpret_cast<v4f*>(wo + (dt * 4 + a) * 256) = v4f{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
-      if (g == 0) wml[0] = m, wml[32] = l;
+      if (g2 == 0) wml[0] = m, wml[32] = l;
     }
   } else {
-    if (g == 0) mlw[wave][0][col] = m, mlw[wave][1][col] = l;
+    if (g2 == 0) mlw[wave][0][col2] = m, mlw[wave][1][col2] = l;
     barrier();
     float M = -1e30f, L = 0.f;
 #pragma unroll
-    for (int k = 0; k < KG; ++k) M = fmaxf(M, mlw[RG * k + rw][0][col]);
+    for (int k = 0; k < KG; ++k) M = fmaxf(M, mlw[RG * k + rw][0][col2]);
 #pragma unroll
-    for (int k = 0; k < KG; ++k) L += __builtin_amdgcn_exp2f(mlw[RG * k + rw][0][col] - M) * mlw[RG * k + rw][1][col];
+    for (int k = 0; k < KG; ++k) L += __builtin_amdgcn_exp2f(mlw[RG * k + rw][0][col2] - M) * mlw[RG * k + rw][1][col2];
     const float f = __builtin_amdgcn_exp2f(m - M), il = L > 0.f ? 1.f / L : L;
-    if (slot >= 0 && kg == 0 && g == 0) wml[0] = M, wml[32] = L;
-    // four dim tiles at a time through LDS: [wave][dt][a][lane], waves 0-3 of it in X0, 4-7 in X1
+    if (slot >= 0 && kg == 0 && g2 == 0) wml[0] = M, wml[32] = L;
+    // four dim tiles at a time through LDS, a wave's [dt][a][lane] in a block
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       if (q) barrier();
-      uint8_t* const mine = (wave < 4 ? X0 : X1) + (wave & 3) * 16384 + lane * 16;
+      uint8_t* const mine = X + wave * kBlk + lane2 * 16;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
@@ -308,8 +351,7 @@ __device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X0, uint8_t
         v4f v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KG; ++k) {
-          const int w = RG * k + rw;
-          v += *reinterpret_cast<const v4f*>((w < 4 ? X0 : X1) + (w & 3) * 16384 + (kg * 4 + a) * 1024 + lane * 16);
+          v += *reinterpret_cast<const v4f*>(X + (RG * k + rw) * kBlk + (kg * 4 + a) * 1024 + lane2 * 16);
         }
         const int dt = 4 * q + kg;
         if (slot >= 0)
@@ -318,16 +360,14 @@ __device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X0, uint8_t
           *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * a) = make_uint2(pack_bf2(v[0] * il, v[1] * il), pack_bf2(v[2] * il, v[3] * il));
       }
     }
-    barrier();  // the stages are free again
+    barrier();  // the blocks are free again
   }
   return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
 }
 
 // The line of the call's tiles (q36_chunk.h), this workgroup's share of it, and its runs one after another.
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_kernel(ChunkDev d) {
-  // two objects: the compiler then sees that a copy into one stage does not touch what is read from the other
-  __shared__ __align__(1024) uint8_t X0[kStage];
-  __shared__ __align__(1024) uint8_t X1[kStage];
+  __shared__ __align__(1024) uint8_t X[2 * kSet];
   __shared__ float mlw[8][2][32];
   __shared__ int64_t sums[8];
   __shared__ int64_t found_at;
@@ -399,8 +439,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const bool whole = run.first && run.last;
         const int slot = whole ? -1 : ck_slot(share, run.first);
         if (!whole && run.first) cut = int4{b, 2 * tile + h, ck_share_of(total, nsh, off + kTileOvh / 2 + steps - 1), 0};
-        if (ck_wide(q.r.n)) nans |= tile_run<8>(d, X0, X1, mlw, b, q.t0, q.r, h, tile, run, slot);
-        else nans |= tile_run<2>(d, X0, X1, mlw, b, q.t0, q.r, h, tile, run, slot);
+        if (ck_wide(q.r.n)) nans |= tile_run<8>(d, X, mlw, b, q.t0, q.r, h, tile, run, slot);
+        else nans |= tile_run<2>(d, X, mlw, b, q.t0, q.r, h, tile, run, slot);
       }
       off += steps + kTileOvh;
       if (++tile < ck_tiles(q.r.n)) continue;

@@ -13,8 +13,8 @@
 
 namespace q36 {
 
-constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 64, kNarrowKeys = 128;
-constexpr int kTileOvh = 4;
+constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 32, kNarrowKeys = 128;
+constexpr int kTileOvh = 12;
 constexpr int kLeastShare = 4;  // a share is no shorter (but for a line shorter than this)
 
 struct ChunkReq {
@@ -43,14 +43,14 @@ __host__ __device__ __forceinline__ int64_t ck_series(int64_t c, int64_t count) 
   }
   return count > 0 ? count * c + count * (count - 1) / 2 : 0;
 }
-__host__ __device__ __forceinline__ int64_t ck_ceil64(int64_t v) { return v >= 0 ? (v + 63) / 64 : -((-v) / 64); }
+__host__ __device__ __forceinline__ int64_t ck_ceil32(int64_t v) { return v >= 0 ? (v + 31) / 32 : -((-v) / 32); }
 // the weight of one head's tiles before tile i (i up to the number of tiles)
 __host__ __device__ __forceinline__ int64_t ck_before(ChunkReq r, int i) {
   int64_t s = 0;
   if (ck_wide(r.n)) {
-    // all but the last tile see nk - n + 32 (k + 1) keys: a series each for even and odd k
-    const int64_t pre = (int64_t)r.nk - r.n, full = i < ck_tiles(r.n) ? i : i - 1;
-    s = ck_series(ck_ceil64(pre + 32), (full + 1) / 2) + ck_series(ck_ceil64(pre + 64), full / 2);
+    // all but the last tile see nk - n + 32 (k + 1) keys, a step more each
+    const int64_t full = i < ck_tiles(r.n) ? i : i - 1;
+    s = ck_series(ck_ceil32((int64_t)r.nk - r.n) + 1, full);
     if (full < i) s += ck_steps(r, i - 1);
   } else {
     for (int k = 0; k < i; ++k) s += ck_steps(r, k);
