@@ -73,9 +73,6 @@ constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a
 constexpr float kLazyC = 8.f;  // the outputs are rescaled when a row's maximum has grown by 2^8 (weights up to 2^8 are exact in f16)
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uni(int64_t v) {
-  return (int64_t)(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
-}
 __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8)); }
 // 16 bytes a lane from memory into LDS at byte `at` + 16 lane of the workgroup's, past the registers.  In asm, so that the
 // compiler does not hold each read of LDS back until every copy in flight has landed; the caller waits (wait_vm0).
@@ -99,116 +96,215 @@ __device__ __forceinline__ int fresh_tid() {
   return t;
 }
 
-// One run of a tile's steps by the 8 waves, four blocks of 32 keys between two barriers, out of one of two sets of four blocks
-// while the other fills.  RG = 8 (wide): wave w has rows 32 w .. of the tile's 256 (4 tokens x 8 heads) and walks all the
-// blocks.  RG = 2 (narrow): waves 2 k, 2 k + 1 have rows 0 .. 31, 32 .. 63 and walk block k of each set; the four are merged
-// at the end.
+// Sum over the workgroup's 512 threads of values below kMostWeight, held there (a line that long is not dealt).
+__device__ __forceinline__ int held(int a, int b) { return min(a + b, kMostWeight); }
+__device__ __forceinline__ int wave_incl(int v) {  // inclusive sums over the wave
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    v = lane >= o ? held(v, u) : v;
+  }
+  return v;
+}
+
+// A run of a tile's steps: what one workgroup does at a time.
+struct Item {
+  int b, t0, n, nk;   // the request: its number, first row, new tokens, keys
+  int h, tok;         // KV head, the tile's first token
+  int last;           // the last key that the tile's last token sees (0 where there is none)
+  int key0, key1;     // the run's keys, key1 up to a step behind vis
+  int slot;           // of its partial (-1: the whole tile)
+};
+
+// The line of the call's tiles (q36_chunk.h), this workgroup's share of it, and its runs one after another, by 8 waves.
+// Keys go by sets of four blocks of 32, between two barriers a set, out of one half of LDS while the other fills.  Wide tile:
+// wave w has rows 32 w .. of the tile's 256 (4 tokens x 8 heads) and walks all the blocks.  Narrow: waves 2 k, 2 k + 1 have
+// rows 0 .. 31, 32 .. 63 and walk block k of each set; the four are merged at the end.
 // Scores S^T = K Q^T (32x32x64, e4m3): lane l holds row l % 32 and keys 8 (i / 4) + 4 (l / 32) + i % 4.  O^T += V^T P^T
 // (32x32x16, f16): the lane's own weights in the order it has them, V^T by the transpose read from LDS rows in that order.
 // A block of 32 keys in LDS: K row r holds key r, V row r key 16 (r / 16) + 8 ((r % 8) / 4) + 4 ((r / 8) % 2) + r % 4, 16-byte
 // piece p of K row r at p ^ (r % 16), of V row r at p ^ 2 (r % 8): the 16 lanes' keys and the 32 lanes' values that are served
 // together fall on all 16 of the row's bank slots.
-template <int RG>
-__device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X, float (*mlw)[2][32], int b, int t0, ChunkReq r, int h,
-                                         int tile, ChunkRun run, int slot) {
-  constexpr int KG = 8 / RG, NE = 4;  // a set's blocks, and a lane's copies of a set
-  static_assert(kWideKeys == 32 && (kNarrowKeys == 32 * KG || KG == 1), "a step is a block, or a set");
-  const int wave = uni(fresh_tid() >> 6), rw = wave % RG, kg = wave / RG;
-  const int pre = r.nk - r.n, vis = ck_keys(r, tile);
-  const int tok0 = tile * (4 * RG) + 4 * rw;  // the wave's first token
-  const bool active = tok0 < r.n;
-  const int lim_first = pre + tok0, lim_last = pre + min(tok0 + 3, r.n - 1);
-  const int32_t* const pt = d.pt + (size_t)b * d.pt_stride;
-  const int sh = d.sh, low = (1 << sh) - 1, top = (int)d.num_slots - 1, top_page = top >> sh;
-  const uint8_t* const kbase = d.kc + h * kCD;
-  const uint8_t* const vbase = d.vc + h * kCD;
-  // A lane's part of the wave's copies: row `lane / 16` of four, 16 bytes.
-  struct Ent {
-    int v[NE];
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_kernel(ChunkDev d) {
+  constexpr int NE = 4, SET = 32 * NE;  // a set's blocks, and a wave's copies of K and of V of one; its keys
+  __shared__ __align__(1024) uint8_t X[2 * kSet];
+  __shared__ float mlw[8][2][32];
+  __shared__ int sums[8];
+  __shared__ int found_at, found_b, nan_seen;
+  const int tid = threadIdx.x, wave = uni(tid >> 6), G = gridDim.x;
+  // ---- this workgroup's share
+  int total = 0, mine = 0;
+  for (int c0 = 0; c0 < d.B; c0 += 512) {
+    const int w = c0 + tid < d.B ? ck_weight(req_of(d, c0 + tid).r) : 0;
+    mine = c0 ? held(mine, w) : w;
+  }
+  if (tid == 0) nan_seen = 0;
+  int inc = wave_incl(mine);
+  if ((tid & 63) == 63) sums[wave] = inc;
+  __syncthreads();
+  int before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before = w == wave ? total : before;
+    total = held(total, sums[w]);
+  }
+  total = uni(total);
+  const int len = ck_share_len(total, G), nsh = total < kMostWeight ? ck_shares(total, len) : 0;
+  // neighbouring shares on one XCD (workgroup i runs on XCD i % 8): they walk the same keys, out of its L2
+  const int xcd = blockIdx.x & 7, at8 = blockIdx.x >> 3, first = xcd * nsh / 8, count = (xcd + 1) * nsh / 8 - first;
+  const int share = G % 8 ? (int)blockIdx.x : at8 < count ? first + at8 : nsh + (xcd * (G / 8) + at8) - (first + count);
+  if (share >= nsh) {
+    if (tid == 0 && share < G) d.cuts[share] = int4{-1, 0, 0, 0};
+    return;
+  }
+  const int x0 = share * len, x1 = min(total, x0 + len);
+  // the request that x0 lies in
+  if (d.B <= 512) {
+    const int off = before + inc - mine;
+    if (off <= x0 && x0 < off + mine) found_b = tid, found_at = off;
+    __syncthreads();
+  } else {
+    for (int c0 = 0, base = 0; base <= x0; c0 += 512) {
+      const int w = c0 + tid < d.B ? ck_weight(req_of(d, c0 + tid).r) : 0;
+      inc = wave_incl(w);
+      __syncthreads();
+      if ((tid & 63) == 63) sums[wave] = inc;
+      __syncthreads();
+      int off = base + inc - w;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        off += k < wave ? sums[k] : 0;
+        base += sums[k];
+      }
+      if (off <= x0 && x0 < off + w) found_b = c0 + tid, found_at = off;
+    }
+    __syncthreads();
+  }
+  // the place on the line: request, head, tile
+  int cb = 0, ct0 = 0, ch = 0, ctile = 0, coff = uni(found_at);
+  ChunkReq cr = {0, 0};
+  int4 cut = {-1, 0, 0, 0};
+  auto request = [&](int b) {
+    const Req q = req_of(d, b);
+    cb = b, ct0 = uni(q.t0), cr = ChunkReq{uni(q.r.n), uni(q.r.nk)}, ch = 0, ctile = 0;
   };
-  // its e-th copy: rows of eighth vw of block blk
-  auto vw_of = [&](int e) { return KG == 1 ? wave : 4 * (wave & 1) + e; };
-  auto blk_of = [&](int e) { return KG == 1 ? e : kg; };
-  auto kap_of = [&](int vw) { return 16 * (vw >> 2) + 8 * (vw & 1) + 4 * ((vw >> 1) & 1); };
-  auto key_of = [&](int key0, int e, int t4) { return min(key0 + 32 * blk_of(e) + kap_of(vw_of(e)) + t4, vis - 1); };
-  auto entries = [&](int key0) {
-    const int t4 = (fresh_tid() & 63) >> 4;
+  request(uni(found_b));
+  if (cr.n > 0) {
+    const int w = ck_weight(cr) >> 1;
+    ch = x0 - coff >= w;
+    coff += ch * w;
+    ctile = ck_tile_at(cr, x0 - coff);
+    coff += ck_before(cr, ctile);
+  }
+  // the share's next run (none: n = 0)
+  auto next = [&] {
+    Item it = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
+    while (coff < x1 && it.n == 0) {
+      if (cr.n == 0) {
+        ++coff;
+        if (coff < x1) request(cb + 1);
+        continue;
+      }
+      const int steps = ck_steps(cr, ctile), ks = ck_step_keys(cr.n);
+      const ChunkRun run = ck_run(steps, coff, x0, x1);
+      if (run.nst >= 0) {
+        it = Item{cb, ct0, cr.n, cr.nk, ch, ctile * ck_tile_tok(cr.n), max(ck_keys(cr, ctile) - 1, 0), run.st0 * ks, (run.st0 + run.nst) * ks,
+                  run.first && run.last ? -1 : ck_slot(share, run.first)};
+        if (it.slot >= 0 && run.first) cut = int4{cb, 2 * ctile + ch, ck_last_share(steps, coff, len), 0};
+      }
+      coff += steps + kTileOvh;
+      if (++ctile < ck_tiles(cr.n)) continue;
+      ctile = 0;
+      if (++ch == 2 && coff < x1) request(cb + 1);
+    }
+    // scalars: what is made from them stays in SGPRs
+    return Item{uni(it.b), uni(it.t0), uni(it.n), uni(it.nk), uni(it.h), uni(it.tok), uni(it.last), uni(it.key0), uni(it.key1), uni(it.slot)};
+  };
+  // ---- copies: wave w takes rows 4 w .. of each block's value rows and the same keys' rows; a lane has 16 bytes of row
+  // `lane / 16` of the four
+  const int top = (int)d.num_slots - 1, top_page = top >> d.sh, mask = (1 << d.sh) - 1;
+  const int kap = 16 * (wave >> 2) + 8 * (wave & 1) + 4 * ((wave >> 1) & 1);  // the wave's first key of a block
+  struct Ent {
+    uint32_t v[NE];
+  };
+  // a set of keys: of request b, KV head h, from key0 on; behind key `last` this one again
+  struct Keys {
+    int b, h, key0, last;
+  };
+  auto keys_of = [](const Item& it, int set) { return Keys{it.b, it.h, it.key0 + set * SET, it.last}; };
+  auto entries = [&](const Keys& k) {
+    const int key = k.key0 + kap + ((fresh_tid() & 63) >> 4);
+    const char* const pt = reinterpret_cast<const char*>(d.pt + (size_t)k.b * d.pt_stride);
     Ent x;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) x.v[e] = pt[key_of(key0, e, t4) >> sh];
+    for (int e = 0; e < NE; ++e) x.v[e] = *reinterpret_cast<const uint32_t*>(pt + (uint32_t)(min(key + 32 * e, k.last) >> d.sh) * 4u);
     return x;
   };
-  auto copy = [&](int key0, const Ent& x, int set) {
-    const int lane = fresh_tid() & 63, t4 = lane >> 4;
+  auto copy = [&](const Keys& k, const Ent& x, int half) {
+    const int lane = fresh_tid() & 63, t4 = lane >> 4, key = k.key0 + kap + t4;
+    const uint8_t* const kbase = d.kc + (k.h * kCD + 16 * ((lane & 15) ^ ((kap & 15) + t4)));
+    const uint8_t* const vbase = d.vc + (k.h * kCD + 16 * ((lane & 15) ^ (2 * (4 * (wave & 1) + t4))));
+    const uint32_t to = lds_at(X) + half * kSet;
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
-      const int vw = vw_of(e), pg = min(max(x.v[e], 0), top_page), s = min((pg << sh) + (key_of(key0, e, t4) & low), top);
-      const size_t at = (size_t)(uint32_t)s * (kCHKV * kCD);
-      const int kp = (lane & 15) ^ ((kap_of(vw) & 15) + t4), vp = (lane & 15) ^ (2 * (4 * (vw & 1) + t4));
-      const uint32_t to = lds_at(X) + set * kSet + blk_of(e) * kBlk;
-      copy16(kbase + (at | (size_t)(16 * kp)), to + kap_of(vw) * kCD);
-      copy16(vbase + (at | (size_t)(16 * vp)), to + kCST * kCD + 4 * vw * kCD);
+      const uint32_t pg = min(x.v[e], (uint32_t)top_page);  // (a negative number is a large one)
+      const uint32_t sl = min((pg << d.sh) + (uint32_t)(min(key + 32 * e, k.last) & mask), (uint32_t)top);
+      const uint64_t at = (uint64_t)sl << 9;
+      copy16(kbase + at, to + e * kBlk + kap * kCD);
+      copy16(vbase + at, to + e * kBlk + kCST * kCD + 4 * wave * kCD);
     }
   };
-  int lim;  // the row's last key
-  // query fragments: column col, dims 64 kb + 32 g .. +31; rows of no token are zero
-  v8i qf[4];
-  const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5;
-  {
-    const int tok = tok0 + (col >> 3), head = h * kCG + (col & 7);
-    const bool row_ok = tok < r.n;
-    lim = row_ok ? pre + tok : -1;
+  // ---- the wave's rows of an item
+  v8i qf[4];  // query fragments: column l % 32, dims 64 kb + 32 (l / 32) .. +31; rows of no token are zero
+  v16f o[8];
+  float m = 0.f, l = 0.f;
+  int lim = -1;  // the row's last key
+  uint32_t bad = 0;  // bits of NaN values on the causal border
+  auto first_tok = [&](const Item& it) { return it.tok + 4 * (ck_wide(it.n) ? wave : wave & 1); };
+  auto queries = [&](const Item& it, bool q8) {
+    const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5, tok = first_tok(it) + (col >> 3);
+    const size_t at = ((size_t)(it.t0 + tok) * kCHQ + it.h * kCG + (col & 7)) * kCD + 32 * g;
+    const bool ok = tok < it.n;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
-      int w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (row_ok) {
-        const size_t at = ((size_t)(t0 + tok) * kCHQ + head) * kCD + 64 * kb + 32 * g;
-        if (d.q8) {
-          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(d.q) + at);
-          const v4i a = src[0], e = src[1];
-          w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = e.x, w[5] = e.y, w[6] = e.z, w[7] = e.w;
+      v4i a = {0, 0, 0, 0}, e = {0, 0, 0, 0};
+      if (ok) {
+        if (q8) {
+          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(d.q) + at + 64 * kb);
+          a = src[0], e = src[1];
         } else {
-          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.q) + at);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const v4i x = src[c];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              w[2 * c + j] = (int)(f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j]), bf_hi((uint32_t)x[2 * j])) |
-                                   (f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j + 1]), bf_hi((uint32_t)x[2 * j + 1])) << 16));
-          }
+          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.q) + at + 64 * kb);
+          auto codes = [](v4i x, int j) {
+            return (int)(f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j]), bf_hi((uint32_t)x[2 * j])) |
+                         (f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j + 1]), bf_hi((uint32_t)x[2 * j + 1])) << 16));
+          };
+          const v4i x0 = src[0], x1 = src[1], x2 = src[2], x3 = src[3];
+          a = v4i{codes(x0, 0), codes(x0, 1), codes(x1, 0), codes(x1, 1)};
+          e = v4i{codes(x2, 0), codes(x2, 1), codes(x3, 0), codes(x3, 1)};
         }
       }
-      qf[kb] = v8i{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]};
+      qf[kb] = v8i{a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
     }
-  }
-  v16f o[8];
-#pragma unroll
-  for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-  float m = 0.f, l = 0.f;
-  bool begun = false;  // a block has been taken: m is its rows' largest, and grows
-  uint32_t bad = 0;  // bits of NaN values on the causal border
-  // this lane's places in a block: K row col, piece 2 g (the others: 4 kb + 2 g + e, by an xor); V row 8 g + (l % 16) / 2
-  // (+ 16 c), piece (l / 16) % 2 (the others: 2 dt more)
-  const int ka = col * kCD + 16 * ((2 * g) ^ (col & 15));
-  const int vr = (lane & 15) >> 1;
-  const int va = kCST * kCD + (8 * g + vr) * kCD + 16 * (((lane >> 4) & 1) ^ (2 * vr)) + 8 * (lane & 1);
+  };
   const float sl2 = d.scale_log2;
-  auto value = [&](uint32_t v0, int dt, int c) {
-    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)((v0 ^ (32 * dt)) + 16 * kCD * c));
+  bool begun = false;  // a block has been taken: m is its rows' largest, and grows
+  auto value = [&](uint32_t v0, int dt, int cc) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)((v0 ^ (32 * dt)) + 16 * kCD * cc));
   };
-  auto key = [&](uint32_t k0, int i) {
-    return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(k0 ^ (16 * i));
-  };
+  auto key = [&](uint32_t k0, int i) { return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(k0 ^ (16 * i)); };
   auto clean = [&](v2i w) {
     const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y);
     bad |= n0 | n1;
     return v2i{(int)(w.x & ~(n0 | (n0 - (n0 >> 7)))), (int)(w.y & ~(n1 | (n1 - (n1 >> 7))))};
   };
-  // the block at byte `at` of LDS, keys key0 ..
-  auto block = [&](uint32_t at, int key0) {
+  // this lane's places in a block: K row l % 32, piece 2 (l / 32) (the others: 4 kb + e more, by an xor); V row
+  // 8 (l / 32) + (l % 16) / 2 (+ 16 c), piece (l / 16) % 2 (the others: 2 dt more)
+  const int lane0 = tid & 63, g0 = lane0 >> 5;
+  const uint32_t ka = (lane0 & 31) * kCD + 16 * ((2 * g0) ^ (lane0 & 15));
+  const uint32_t va = kCST * kCD + (8 * g0 + ((lane0 & 15) >> 1)) * kCD + 16 * (((lane0 >> 4) & 1) ^ (lane0 & 14)) + 8 * (lane0 & 1);
+  // the block at byte `at` of LDS, keys key0 ..; border: some row does not see all of them
+  auto block = [&](uint32_t at, int key0, bool border) {
     uint32_t k0 = at + ka, v0 = at + va;
     asm volatile("" : "+v"(k0), "+v"(v0));  // (the xors below are formed here, not held across blocks)
     v16f s;
@@ -222,11 +318,10 @@ __device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X, float (*
     v2i w[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w[dt] = value(v0, dt, 0);
-    const bool border = key0 + 31 > lim_first;
     if (border) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (key0 + 8 * (i >> 2) + 4 * g + (i & 3) > lim) s[i] = -INFINITY;
+        if (key0 + 8 * (i >> 2) + 4 * g0 + (i & 3) > lim) s[i] = -INFINITY;
     }
     // relative to the running maximum, which the first block sets; where a row grows past 2^8 times it, all moves to the new
     // one.  (A row that sees nothing of a block sees nothing of the later ones.)
@@ -264,7 +359,6 @@ __device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X, float (*
       o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[0], o[dt], 0, 0, 0);
       w[dt] = value(v0, dt, 1);
     }
-    
     if (border) {
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) w[dt] = clean(w[dt]);
@@ -272,187 +366,144 @@ __device__ __forceinline__ bool tile_run(const ChunkDev& d, uint8_t* X, float (*
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[1], o[dt], 0, 0, 0);
   };
-  if (run.nst > 0) {
-    constexpr int SET = 32 * NE;
-    const int k0 = run.st0 * (KG == 1 ? kWideKeys : kNarrowKeys), k1 = k0 + run.nst * (KG == 1 ? kWideKeys : kNarrowKeys);
-    auto set = [&](int at, int key0) {
-      if (!active) return;
-      const uint32_t to = lds_at(X) + at * kSet;
-      if constexpr (KG == 1) {
-        const int end = min(min(key0 + SET, k1), lim_last + 1);
-#pragma unroll 1
-        for (int i = 0; key0 + i < end; i += 32) block(to + i * (kBlk / 32), key0 + i);
-      } else if (key0 + 32 * kg <= lim_last) {
-        block(to + kg * kBlk, key0 + 32 * kg);
-      }
-    };
-    copy(k0, entries(k0), 0);
-    Ent e = entries(k0 + SET);
-#pragma unroll 1
-    for (int k = k0, at = 0; k < k1; k += SET, at ^= 1) {
-      wait_vm0();
-      barrier();  // every wave's copies of this set have landed, and every wave is done with the other one
-      if (k + SET < k1) copy(k + SET, e, at ^ 1);
-      e = entries(k + 2 * SET);
-      set(at, k);
-    }
+  // ---- the runs, one after another; while one ends, the first set of the next is on its way
+  Item cur = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1}, nxt = next();
+  // the keys that are copied next, and their page-table entries
+  Keys ahead = keys_of(nxt, 0);
+  Ent ent = {};
+  if (nxt.n > 0) {
+    copy(ahead, entries(ahead), 0);
+    ahead.key0 += SET;
+    ent = entries(ahead);
   }
-  l += __shfl_xor(l, 32);
-  if (l == 0.f) m = -1e30f;  // no key seen
-  barrier();  // every wave is done with both sets
-  const int lane2 = fresh_tid() & 63, col2 = lane2 & 31, g2 = lane2 >> 5, tok = tok0 + (col2 >> 3);
-  const bool row_ok = tok < r.n;
-  uint16_t* const dst = d.out + ((size_t)(t0 + tok) * kCHQ + h * kCG + (col2 & 7)) * kCD + 4 * g2;
-  float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane2 * 4;
-  float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col2;
-  if constexpr (KG == 1) {
-    if (active && slot < 0) {
-      const float il = l > 0.f ? 1.f / l : l;  // (no key: 0; NaN stays)
-      if (row_ok)
+  wait_vm0();
+  for (int half = 0;;) {
+    // the next item's query rows (codes) are asked for before this one's outputs leave
+    if (d.q8) queries(nxt, true);
+    if (cur.n > 0) {
+      l += __shfl_xor(l, 32);
+      if (l == 0.f) m = -1e30f;  // no key seen
+      const bool wide = ck_wide(cur.n);
+      const int slot = cur.slot, tok0 = first_tok(cur), rw = wide ? wave : wave & 1;
+      const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5;
+      uint8_t* const mem = X + (half ^ 1) * kSet;
+      float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane * 4;
+      float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col;
+      uint16_t* const rows = d.out + ((size_t)(cur.t0 + tok0) * kCHQ + cur.h * kCG) * kCD;  // row r: token r / 8, head r % 8
+      if (!wide) {
+        if (g == 0) mlw[wave][0][col] = m, mlw[wave][1][col] = l;
+        barrier();
+        float M = -1e30f, L = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
+        for (int k = 0; k < 4; ++k) M = fmaxf(M, mlw[2 * k + rw][0][col]);
 #pragma unroll
-          for (int a = 0; a < 4; ++a)
-            *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * a) = make_uint2(pack_bf2(o[dt][4 * a] * il, o[dt][4 * a + 1] * il),
-                                                                          pack_bf2(o[dt][4 * a + 2] * il, o[dt][4 * a + 3] * il));
-    } else if (active) {
+        for (int k = 0; k < 4; ++k) L += __builtin_amdgcn_exp2f(mlw[2 * k + rw][0][col] - M) * mlw[2 * k + rw][1][col];
+        const float f = __builtin_amdgcn_exp2f(m - M), il = L > 0.f ? 1.f / L : L;
+        if (slot >= 0 && wave < 2 && g == 0) wml[0] = M, wml[32] = L;
+        // two dim tiles at a time through LDS, [wave][dt][a][lane]; wave (k, rw) sums quads 2 k, 2 k + 1 of the eight of rw
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q) barrier();
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+              *reinterpret_cast<v4f*>(mem + wave * 8192 + (dt * 4 + a) * 1024 + lane * 16) =
+                  v4f{o[2 * q + dt][4 * a] * f, o[2 * q + dt][4 * a + 1] * f, o[2 * q + dt][4 * a + 2] * f, o[2 * q + dt][4 * a + 3] * f};
+          barrier();
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int quad = 2 * (wave >> 1) + u;
+            v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v += *reinterpret_cast<const v4f*>(mem + (2 * k + rw) * 8192 + quad * 1024 + lane * 16);
+            if (slot >= 0)
+              *reinterpret_cast<v4f*>(wo + (8 * q + quad) * 256) = v;
+            else if (tok0 + (col >> 3) < cur.n)
+              *reinterpret_cast<uint2*>(rows + ((size_t)(col >> 3) * kCHQ + (col & 7)) * kCD + 64 * q + 8 * quad + 4 * g) =
+                  make_uint2(pack_bf2_hw(v[0] * il, v[1] * il), pack_bf2_hw(v[2] * il, v[3] * il));
+          }
+        }
+      } else if (tok0 < cur.n) {
+        if (slot < 0) {
+          // rounded, through the wave's 8 KB of LDS (32 rows x 128 dims, 16-byte piece p of row r at p ^ (r % 16)), out by rows
+          const float il = l > 0.f ? 1.f / l : l;  // (no key: 0; NaN stays)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint8_t* const my = mem + wave * 8192;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+              for (int a = 0; a < 4; ++a) {
+                const v16f& v = o[4 * q + dt];
+                *reinterpret_cast<uint2*>(my + col * 256 + 16 * ((4 * dt + a) ^ (col & 15)) + 8 * g) =
+                    make_uint2(pack_bf2_hw(v[4 * a] * il, v[4 * a + 1] * il), pack_bf2_hw(v[4 * a + 2] * il, v[4 * a + 3] * il));
+              }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int row = 4 * j + (lane >> 4);
+              const v4i v = *reinterpret_cast<const v4i*>(my + row * 256 + 16 * ((lane & 15) ^ (row & 15)));
+              if (tok0 + (row >> 3) < cur.n)
+                *reinterpret_cast<v4i*>(rows + ((size_t)(row >> 3) * kCHQ + (row & 7)) * kCD + 128 * q + 8 * (lane & 15)) = v;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+              *reinterpret_cast<v4f*>(wo + (dt * 4 + a) * 256) = v4f{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
+          if (g == 0) wml[0] = m, wml[32] = l;
+        }
+      }
+    }
+    if (nxt.n == 0) break;
+    if (!d.q8) queries(nxt, false);
+    cur = nxt;
+    nxt = next();
+    const bool wide = ck_wide(cur.n);
+    const int sets = max(1, (cur.key1 - cur.key0 + SET - 1) / SET), tok0 = first_tok(cur), pre = cur.nk - cur.n;
+    if (sets == 1) ahead = keys_of(nxt, 0), ent = entries(ahead);  // (those on their way are behind this item's end)
+    {
+      const int tok = tok0 + ((fresh_tid() & 31) >> 3);
+      lim = tok < cur.n ? pre + tok : -1;
+      m = 0.f, l = 0.f;
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
-          *reinterpret_cast<v4f*>(wo + (dt * 4 + a) * 256) = v4f{o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]};
-      if (g2 == 0) wml[0] = m, wml[32] = l;
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     }
-  } else {
-    if (g2 == 0) mlw[wave][0][col2] = m, mlw[wave][1][col2] = l;
-    barrier();
-    float M = -1e30f, L = 0.f;
-#pragma unroll
-    for (int k = 0; k < KG; ++k) M = fmaxf(M, mlw[RG * k + rw][0][col2]);
-#pragma unroll
-    for (int k = 0; k < KG; ++k) L += __builtin_amdgcn_exp2f(mlw[RG * k + rw][0][col2] - M) * mlw[RG * k + rw][1][col2];
-    const float f = __builtin_amdgcn_exp2f(m - M), il = L > 0.f ? 1.f / L : L;
-    if (slot >= 0 && kg == 0 && g2 == 0) wml[0] = M, wml[32] = L;
-    // four dim tiles at a time through LDS, a wave's [dt][a][lane] in a block
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q) barrier();
-      uint8_t* const mine = X + wave * kBlk + lane2 * 16;
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-          *reinterpret_cast<v4f*>(mine + (dt * 4 + a) * 1024) = v4f{o[4 * q + dt][4 * a] * f, o[4 * q + dt][4 * a + 1] * f,
-                                                                    o[4 * q + dt][4 * a + 2] * f, o[4 * q + dt][4 * a + 3] * f};
-      barrier();
-      // this wave sums dim tile kg of row group rw
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        v4f v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KG; ++k) {
-          v += *reinterpret_cast<const v4f*>(X + (RG * k + rw) * kBlk + (kg * 4 + a) * 1024 + lane2 * 16);
-        }
-        const int dt = 4 * q + kg;
-        if (slot >= 0)
-          *reinterpret_cast<v4f*>(wo + (dt * 4 + a) * 256) = v;
-        else if (row_ok)
-          *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * a) = make_uint2(pack_bf2(v[0] * il, v[1] * il), pack_bf2(v[2] * il, v[3] * il));
+    // (waited for here: the compiler would wait in each block, for the copies too)
+    asm volatile("" : "+v"(qf[0]), "+v"(qf[1]), "+v"(qf[2]), "+v"(qf[3]));
+    begun = false;
+    // the wave's keys: of the run, up to its last token's; none without a token
+    const int end = uni(tok0 < cur.n ? min(pre + min(tok0 + 4, cur.n), cur.key1) : 0);
+#pragma unroll 1
+    for (int st = 0; st < sets; ++st) {
+      if (st > 0) wait_vm0();
+      barrier();  // every wave's copies of this set have landed, and every wave is done with the other half
+      // the next set, this item's or the next one's, and the page-table entries of the one behind it
+      if (st + 1 < sets || nxt.n > 0) {
+        copy(ahead, ent, half ^ 1);
+        ahead.key0 += SET;
+        if (st + 2 == sets) ahead = keys_of(nxt, 0);
+        ahead = Keys{uni(ahead.b), uni(ahead.h), uni(ahead.key0), uni(ahead.last)};
+        ent = entries(ahead);
       }
-    }
-    barrier();  // the blocks are free again
-  }
-  return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-}
-
-// The line of the call's tiles (q36_chunk.h), this workgroup's share of it, and its runs one after another.
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void chunk_kernel(ChunkDev d) {
-  __shared__ __align__(1024) uint8_t X[2 * kSet];
-  __shared__ float mlw[8][2][32];
-  __shared__ int64_t sums[8];
-  __shared__ int64_t found_at;
-  __shared__ int found_b, nan_seen;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = gridDim.x;
-  if (tid == 0) nan_seen = 0;
-  int64_t mine = 0;
-  for (int q = tid; q < d.B; q += 512) mine += ck_weight(req_of(d, q).r);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
-  if (lane == 0) sums[wave] = mine;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) total += sums[w];
-  total = uni(total);
-  const int nsh = ck_shares(total, G);
-  // neighbouring shares on one XCD (workgroup i runs on XCD i % 8): they walk the same keys, out of its L2
-  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, first = xcd * nsh / 8, count = (xcd + 1) * nsh / 8 - first;
-  const int share = G % 8 ? (int)blockIdx.x : at < count ? first + at : nsh + (xcd * (G / 8) + at) - (first + count);
-  if (share >= nsh) {
-    if (tid == 0 && share < G) d.cuts[share] = int4{-1, 0, 0, 0};
-    return;
-  }
-  const int64_t x0 = uni(ck_share_begin(total, nsh, share)), x1 = uni(ck_share_begin(total, nsh, share + 1));
-  // the request that x0 lies in
-  int64_t before = 0;
-  for (int c0 = 0; c0 < d.B; c0 += 512) {
-    const int64_t w = c0 + tid < d.B ? ck_weight(req_of(d, c0 + tid).r) : 0;
-    int64_t inc = w;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(inc, o);
-      inc += lane >= o ? v : 0;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = inc;
-    __syncthreads();
-    int64_t off = before + inc - w;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      off += k < wave ? sums[k] : 0;
-      before += sums[k];
-    }
-    if (off <= x0 && x0 < off + w) found_b = c0 + tid, found_at = off;
-    if (before > x0) break;
-  }
-  __syncthreads();
-  int b = uni(found_b), h = 0, tile = 0;
-  int64_t off = uni(found_at);
-  Req q = req_of(d, b);
-  q = Req{uni(q.t0), {uni(q.r.n), uni(q.r.nk)}};
-  if (q.r.n > 0) {
-    const int64_t half = ck_weight(q.r) / 2;
-    h = x0 - off >= half;
-    off += h * half;
-    tile = ck_tile_at(q.r, x0 - off);
-    off += ck_before(q.r, tile);
-  }
-  int4 cut = {-1, 0, 0, 0};
-  bool nans = false;
-  while (off < x1) {
-    if (q.r.n == 0) {
-      ++off;
-    } else {
-      const int steps = ck_steps(q.r, tile);
-      const ChunkRun run = ck_run(steps, off, x0, x1);
-      if (run.nst >= 0) {
-        const bool whole = run.first && run.last;
-        const int slot = whole ? -1 : ck_slot(share, run.first);
-        if (!whole && run.first) cut = int4{b, 2 * tile + h, ck_share_of(total, nsh, off + kTileOvh / 2 + steps - 1), 0};
-        if (ck_wide(q.r.n)) nans |= tile_run<8>(d, X, mlw, b, q.t0, q.r, h, tile, run, slot);
-        else nans |= tile_run<2>(d, X, mlw, b, q.t0, q.r, h, tile, run, slot);
+      const uint32_t to = lds_at(X) + half * kSet;
+      const int i1 = wide ? NE : (wave >> 1) + 1;
+#pragma unroll 1
+      for (int i = wide ? 0 : wave >> 1; i < i1; ++i) {
+        const int k = cur.key0 + st * SET + 32 * i;
+        if (k >= end) break;
+        block(to + i * kBlk, k, k + 31 > pre + tok0);
       }
-      off += steps + kTileOvh;
-      if (++tile < ck_tiles(q.r.n)) continue;
-      tile = 0;
-      if (++h < 2) continue;
+      half ^= 1;
     }
-    h = 0;
-    if (++b >= d.B) break;
-    q = req_of(d, b);
-    q = Req{uni(q.t0), {uni(q.r.n), uni(q.r.nk)}};
+    wait_vm0();
+    barrier();  // every wave is done with this item's last set (the other half than `half`), and the next item's first has landed
   }
-  if (nans && lane == 0) nan_seen = 1;
+  if (__builtin_amdgcn_ballot_w64(bad != 0) && (tid & 63) == 0) nan_seen = 1;
   __syncthreads();
   if (tid == 0) {
     cut.w = nan_seen;
@@ -520,7 +571,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
       return *reinterpret_cast<const v4f*>(d.ws_o + (size_t)ck_slot(share + p, p == 0) * kSlotF + ((rw * 8 + dt) * 4 + a) * 256 + lane * 4);
     };
     auto store = [&](v4f v, float il) {
-      uint2 w = make_uint2(pack_bf2(v[0] * il, v[1] * il), pack_bf2(v[2] * il, v[3] * il));
+      uint2 w = make_uint2(pack_bf2_hw(v[0] * il, v[1] * il), pack_bf2_hw(v[2] * il, v[3] * il));
       if (__builtin_expect(any_nan, 0)) w = put_nans(w, border_nans(d, b, q.r, h, tok, 32 * dt + 4 * g + 8 * wave));
       *reinterpret_cast<uint2*>(dst + 8 * wave) = w;
     };

@@ -27,8 +27,8 @@ __host__ __device__ __forceinline__ int ck_tiles(int n) {
 }
 // the keys that tile i's last token sees
 __host__ __device__ __forceinline__ int ck_keys(ChunkReq r, int i) {
-  const int64_t end = (int64_t)(i + 1) * ck_tile_tok(r.n), last = end < r.n ? end : r.n, k = (int64_t)r.nk - r.n + last;
-  return k > 0 ? (int)k : 0;
+  const int end = (i + 1) * ck_tile_tok(r.n), k = r.nk - r.n + (end < r.n ? end : r.n);
+  return k > 0 ? k : 0;
 }
 __host__ __device__ __forceinline__ int ck_step_keys(int n) { return ck_wide(n) ? kWideKeys : kNarrowKeys; }
 __host__ __device__ __forceinline__ int ck_steps(ChunkReq r, int i) {
@@ -36,67 +36,63 @@ __host__ __device__ __forceinline__ int ck_steps(ChunkReq r, int i) {
   return (ck_keys(r, i) + ks - 1) / ks;
 }
 // sum over j < count of max(0, c + j)
-__host__ __device__ __forceinline__ int64_t ck_series(int64_t c, int64_t count) {
+__host__ __device__ __forceinline__ int ck_series(int c, int count) {
   if (c < 0) {
     count += c;
     c = 0;
   }
-  return count > 0 ? count * c + count * (count - 1) / 2 : 0;
+  return count > 0 ? count * c + ((count * (count - 1)) >> 1) : 0;
 }
-__host__ __device__ __forceinline__ int64_t ck_ceil32(int64_t v) { return v >= 0 ? (v + 31) / 32 : -((-v) / 32); }
 // the weight of one head's tiles before tile i (i up to the number of tiles)
-__host__ __device__ __forceinline__ int64_t ck_before(ChunkReq r, int i) {
-  int64_t s = 0;
-  if (ck_wide(r.n)) {
-    // all but the last tile see nk - n + 32 (k + 1) keys, a step more each
-    const int64_t full = i < ck_tiles(r.n) ? i : i - 1;
-    s = ck_series(ck_ceil32((int64_t)r.nk - r.n) + 1, full);
-    if (full < i) s += ck_steps(r, i - 1);
-  } else {
-    for (int k = 0; k < i; ++k) s += ck_steps(r, k);
+__host__ __device__ __forceinline__ int ck_before(ChunkReq r, int i) {
+  int s = i * kTileOvh, full = i;
+  if (i == ck_tiles(r.n) && i > 0) {  // the last tile ends with the request
+    s += ck_steps(r, i - 1);
+    --full;
   }
-  return s + (int64_t)i * kTileOvh;
+  // the others see nk - n + tokens (k + 1) keys: a step more each (wide), or there is one (narrow)
+  if (ck_wide(r.n)) return s + ck_series(((r.nk - r.n + 31) >> 5) + 1, full);
+  return s + (full > 0 ? ck_steps(r, 0) : 0);
 }
 // the weight of a request, both heads (an empty one weighs 1: what passing over it costs)
-__host__ __device__ __forceinline__ int64_t ck_weight(ChunkReq r) { return r.n > 0 ? 2 * ck_before(r, ck_tiles(r.n)) : 1; }
+__host__ __device__ __forceinline__ int ck_weight(ChunkReq r) { return r.n > 0 ? 2 * ck_before(r, ck_tiles(r.n)) : 1; }
 // the tile of a head that place x of its line lies in
-__host__ __device__ __forceinline__ int ck_tile_at(ChunkReq r, int64_t x) {
+__host__ __device__ __forceinline__ int ck_tile_at(ChunkReq r, int x) {
   int lo = 0, hi = ck_tiles(r.n) - 1;
   while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
+    const int mid = (lo + hi + 1) >> 1;
     if (ck_before(r, mid) <= x) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
+// The most that a call of T new tokens, B requests and tables of `keys` keys can weigh; a line of kMostWeight is not dealt.
+constexpr int kMostWeight = 1 << 30;
+inline bool ck_too_long(int64_t T, int64_t B, int64_t keys) {
+  return 2.0 * ((double)T / kWideTok + 2.0 * (double)B) * ((double)keys / kWideKeys + 1 + kTileOvh) + (double)B >= kMostWeight;
+}
 
-__host__ __device__ __forceinline__ int ck_shares(int64_t total, int G) {
-  const int64_t s = total / kLeastShare;
-  return s >= G ? G : s > 1 ? (int)s : 1;
+// Equal shares: their length, and how many a line has
+__host__ __device__ __forceinline__ int ck_share_len(int total, int G) {
+  const int len = (total + G - 1) / G;
+  return len > kLeastShare ? len : kLeastShare;
 }
-__host__ __device__ __forceinline__ int64_t ck_share_begin(int64_t total, int nsh, int w) {
-  const int64_t q = total / nsh, r = total - q * nsh;
-  return q * w + r * w / nsh;
-}
-// the share that place x lies in
-__host__ __device__ __forceinline__ int ck_share_of(int64_t total, int nsh, int64_t x) {
-  const int64_t q = total / nsh;
-  int w = (int)(x / (q + 1));  // shares are q or q + 1 long
-  while (w + 1 < nsh && ck_share_begin(total, nsh, w + 1) <= x) ++w;
-  return w;
-}
+__host__ __device__ __forceinline__ int ck_shares(int total, int len) { return (total + len - 1) / len; }
+
 // The steps [st0, st0 + nst) of a tile at `off` on the line that the share [x0, x1) has; first, last: whether they hold the
 // tile's first and last step.  A tile without a step is its start's share's, whole.  nst < 0: the share has none.
 struct ChunkRun {
   int st0, nst;
   bool first, last;
 };
-__host__ __device__ __forceinline__ ChunkRun ck_run(int steps, int64_t off, int64_t x0, int64_t x1) {
+__host__ __device__ __forceinline__ ChunkRun ck_run(int steps, int off, int x0, int x1) {
   if (steps == 0) return ChunkRun{0, off >= x0 && off < x1 ? 0 : -1, true, true};
-  const int64_t at = off + kTileOvh / 2;  // of its first step
-  const int64_t a = x0 > at ? x0 - at : 0, e = x1 - at < steps ? x1 - at : steps;
-  return ChunkRun{(int)a, e > a ? (int)(e - a) : -1, a == 0, e == steps};
+  const int at = off + kTileOvh / 2;  // of its first step
+  const int a = x0 > at ? x0 - at : 0, e = x1 - at < steps ? x1 - at : steps;
+  return ChunkRun{a, e > a ? e - a : -1, a == 0, e == steps};
 }
+// the share that the last step of a tile at `off` lies in
+__host__ __device__ __forceinline__ int ck_last_share(int steps, int off, int len) { return (off + kTileOvh / 2 + steps - 1) / len; }
 // The partial of share w: one for a tile that ends here or goes on through, one for a tile that starts here.
 __host__ __device__ __forceinline__ int ck_slot(int w, bool first) { return 2 * w + (first ? 1 : 0); }
 

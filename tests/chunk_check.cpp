@@ -26,7 +26,7 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
   std::vector<std::vector<int>> written(2 * B);            // outputs written: by the tile's workgroup or the combine
   for (int b = 0; b < B; ++b) {
     total += ck_weight(req[b]);
-    int64_t sum = 0;
+    int sum = 0;
     const int nt = ck_tiles(req[b].n);
     for (int i = 0; i < nt; ++i) {
       if (ck_before(req[b], i) != sum) return "a tile's place is not the weight before it";
@@ -42,21 +42,22 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
       written[2 * b + h].assign(nt, 0);
     }
   }
-  const int nsh = ck_shares(total, G);
+  if (total >= kMostWeight) return "a line that is too long";
+  const int len = ck_share_len((int)total, G), nsh = ck_shares((int)total, len);
+  if (nsh > G) return "more shares than workgroups";
   std::vector<long> owner(2 * G, -1);
   std::vector<Cut> cut(G, Cut{-1, 0, 0, 0});
   for (int w = 0; w < nsh; ++w) {
-    const int64_t x0 = ck_share_begin(total, nsh, w), x1 = ck_share_begin(total, nsh, w + 1);
+    const int x0 = w * len, x1 = std::min((int)total, x0 + len);
     if (x1 <= x0 || (w + 1 == nsh && x1 != total)) return "a share is empty, or the shares are not the line";
-    if (ck_share_of(total, nsh, x0) != w || ck_share_of(total, nsh, x1 - 1) != w) return "a place's share is not found";
     // as the kernel walks: the request that x0 lies in, its head and tile, then on
     int b = 0;
-    int64_t at = 0;
+    int at = 0;
     while (at + ck_weight(req[b]) <= x0) at += ck_weight(req[b++]);
     int h = 0, tile = 0;
-    int64_t off = at;
+    int off = at;
     if (req[b].n > 0) {
-      const int64_t head = ck_weight(req[b]) / 2;
+      const int head = ck_weight(req[b]) / 2;
       h = x0 - at >= head;
       off += h * head;
       tile = ck_tile_at(req[b], x0 - off);
@@ -77,7 +78,7 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
             const int slot = ck_slot(w, r.first);
             if (owner[slot] >= 0) return "a slot written twice";
             owner[slot] = ((long)(2 * b + h) << 32) + tile;
-            if (r.first) cut[w] = Cut{b, h, tile, ck_share_of(total, nsh, off + kTileOvh / 2 + steps - 1)};
+            if (r.first) cut[w] = Cut{b, h, tile, ck_last_share(steps, off, len)};
           }
         }
         off += steps + kTileOvh;
