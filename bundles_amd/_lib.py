@@ -231,13 +231,20 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def check_tensors(what: str, **tensors) -> None:
-    """Every given tensor (None: left out) lies on the current GPU, where its call is launched."""
+def current_gpu() -> int:
+    """The current device's number (-2 without one: no tensor's)."""
     import torch
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != dev):
-            raise ValueError(f"{what}: {name} is on {t.device}, not on the current GPU")
+    if torch.cuda.is_initialized():
+        return torch._C._cuda_getDevice()
+    return torch.cuda.current_device() if torch.cuda.is_available() else -2
+
+
+def check_tensors(what: str, names: str, *tensors) -> None:
+    """Every given tensor (None: left out) lies on the current GPU, where its call is launched."""
+    dev = current_gpu()
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: {names.split()[i]} is on {t.device}, not on the current GPU")
 
 
 def stream_handle(stream=None) -> int:

@@ -679,6 +679,9 @@ extern "C" int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream) {
               "q36_attn_chunk: page_size=%d must be a power of two up to 1024", a->page_size);
   Q36_REQUIRE(a->pt_stride >= 1 && a->pt_stride <= (1 << 27) / a->page_size, "q36_attn_chunk: pt_stride=%d of pages of %d out of range",
               a->pt_stride, a->page_size);
+  Q36_REQUIRE(!ck_too_long(a->T, a->B, (int64_t)a->pt_stride * a->page_size),
+              "q36_attn_chunk: T=%d, B=%d with tables of %d pages of %d: more steps than one call deals", a->T, a->B, a->pt_stride,
+              a->page_size);
   Q36_REQUIRE(a->num_slots >= 1 && a->num_slots < ((int64_t)1 << 31), "q36_attn_chunk: num_slots=%lld out of range",
               (long long)a->num_slots);
   Q36_REQUIRE(a->q && a->k_cache && a->v_cache && a->page_table && a->seqlens && a->qsl && a->out && a->workspace,

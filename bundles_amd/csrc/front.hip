@@ -14,7 +14,7 @@
 namespace q36 {
 namespace {
 
-constexpr int kFItems = 18;  // waves a token: 16 heads of q and gate, 2 of k and v
+constexpr int kFItems = 18;  // pieces of a token's row: 16 heads of q and gate, 2 of k and v
 struct FrontDev {
   int T, max_pos;
   int64_t ld, pos_stride;
@@ -33,28 +33,41 @@ struct FrontDev {
   float eps;
 };
 
-// Lanes 0-31 of a wave hold a head of q (or k), 8 consecutive dims a lane, lanes 32-63 its companion (the gate, or v):
-// one contiguous 1 KB load for a head of q and its gate.  MULTI: the pairs' positions differ by axis.
+// A wave takes three of a token's pieces.  Lanes 0-31 hold a head of q (or k), 8 consecutive dims a lane, lanes 32-63 its
+// companion (the gate, or v): one contiguous 1 KB load for a head of q and its gate.  MULTI: the pairs' positions differ by axis,
+// so a lane's cosines and sines come one by one, once a wave.  Pieces a wave, us a call (one / three / nine): 8192 tokens of one
+// axis 67.9 / 53.5 / 57.6, 1777 of three axes 20.4 / 17.4 / 18.7, 4000 of three axes 40.7 / 31.3 / 31.8; from 1 token to 1000
+// the call's own launch hides them all.
+constexpr int IPW = 3, WPT = kFItems / IPW;  // pieces of a wave, WPT apart; waves a token
 template <bool MULTI, bool Q8>
 __global__ __launch_bounds__(256) void front_kernel(FrontDev d) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t wv = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  if (item >= (int64_t)d.T * kFItems) return;
-  const int t = (int)(item / kFItems), h = (int)(item % kFItems);
-  const int half = lane >> 5, j = lane & 31, hh = h - 16;
-  const bool qhead = h < 16;
-  const int col = qhead ? h * 512 + half * 256 + 8 * j : (half ? 8704 : 8192) + hh * 256 + 8 * j;
-  const v4i raw = *reinterpret_cast<const v4i*>(d.qkv + (size_t)t * d.ld + col);
-  const v4i wraw = *reinterpret_cast<const v4i*>((qhead ? d.q_norm_w : d.k_norm_w) + 8 * j);
-  // lanes j < 8 turn dims 8 j .. 8 j + 7 by the pairs 8 (j & 3) + e
-  float c[8], s[8];
-  if constexpr (MULTI) {
+  if (wv >= (int64_t)d.T * WPT) return;
+  const int t = __builtin_amdgcn_readfirstlane((int)(wv / WPT)), h0 = __builtin_amdgcn_readfirstlane((int)(wv % WPT));
+  const int half = lane >> 5, j = lane & 31;
+  const uint16_t* const row = d.qkv + (size_t)t * d.ld;
+  v4i raw[IPW];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = 8 * (j & 3) + e, axis = (int)(d.axis_map >> (2 * i)) & 3;
-      const int pos = min(max(d.positions[axis * d.pos_stride + t], 0), d.max_pos - 1);
-      c[e] = d.cos_sin[(size_t)pos * 64 + i];
-      s[e] = d.cos_sin[(size_t)pos * 64 + 32 + i];
+  for (int k = 0; k < IPW; ++k) {
+    const int h = h0 + WPT * k;
+    const int col = h < 16 ? h * 512 + half * 256 + 8 * j : (half ? 8704 : 8192) + (h - 16) * 256 + 8 * j;
+    raw[k] = *reinterpret_cast<const v4i*>(row + col);
+  }
+  const v4i qw = *reinterpret_cast<const v4i*>(d.q_norm_w + 8 * j), kw = *reinterpret_cast<const v4i*>(d.k_norm_w + 8 * j);
+  const int64_t slot = d.out_loc ? d.out_loc[t] : -1;
+  // lanes j < 8 turn dims 8 j .. 8 j + 7 by the pairs 8 (j & 3) + e
+  const bool normed = half == 0, rot = normed && j < 8;
+  float c[8] = {}, s[8] = {};
+  if constexpr (MULTI) {
+    if (rot) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = 8 * (j & 3) + e, axis = (int)(d.axis_map >> (2 * i)) & 3;
+        const int pos = min(max(d.positions[axis * d.pos_stride + t], 0), d.max_pos - 1);
+        c[e] = d.cos_sin[(size_t)pos * 64 + i];
+        s[e] = d.cos_sin[(size_t)pos * 64 + 32 + i];
+      }
     }
   } else {
     const int pos = min(max(d.positions[t], 0), d.max_pos - 1);
@@ -66,55 +79,56 @@ __global__ __launch_bounds__(256) void front_kernel(FrontDev d) {
       for (int i = 0; i < 4; ++i) c[e + i] = a[i], s[e + i] = b[i];
     }
   }
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf_lo((uint32_t)raw[i]);
-    x[2 * i + 1] = bf_hi((uint32_t)raw[i]);
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-  ss += xor_swz<16>(ss);
-  ss += xor_swz<8>(ss);
-  ss += xor_swz<4>(ss);
-  ss += xor_swz<2>(ss);
-  ss += xor_swz<1>(ss);
-  const bool normed = half == 0, rot = normed && j < 8;
-  const float inv = 1.f / sqrtf(ss / 256.f + d.eps);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = (x[2 * i] * inv) * (bf_lo((uint32_t)wraw[i]) + 1.f), b = (x[2 * i + 1] * inv) * (bf_hi((uint32_t)wraw[i]) + 1.f);
-    x[2 * i] = normed ? a : x[2 * i];
-    x[2 * i + 1] = normed ? b : x[2 * i + 1];
-  }
   const float sg = j < 4 ? -1.f : 1.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float other = xor_swz<4>(x[e]);
-    const float r = __builtin_fmaf(x[e], c[e], (sg * other) * s[e]);
-    x[e] = rot ? r : x[e];
-  }
-  const auto codes = [&] {
-    return make_uint2(f2e4m3x2_nan(x[0], x[1]) | (f2e4m3x2_nan(x[2], x[3]) << 16),
-                      f2e4m3x2_nan(x[4], x[5]) | (f2e4m3x2_nan(x[6], x[7]) << 16));
-  };
-  const auto halves = [&] {
-    return make_uint4(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]), pack_bf2(x[4], x[5]), pack_bf2(x[6], x[7]));
-  };
-  if (qhead) {
-    const size_t at = ((size_t)t * 16 + h) * 256 + 8 * j;
-    if (!normed) {
-      if (d.gate) *reinterpret_cast<v4i*>(d.gate + at) = raw;
-    } else if constexpr (Q8) {
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(d.q) + at) = codes();
-    } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(d.q) + at) = halves();
+  for (int k = 0; k < IPW; ++k) {
+    const int h = h0 + WPT * k;
+    const bool qhead = h < 16;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = bf_lo((uint32_t)raw[k][i]);
+      x[2 * i + 1] = bf_hi((uint32_t)raw[k][i]);
     }
-  } else if (d.out_loc) {
-    const int64_t slot = d.out_loc[t];
-    if (slot >= 0 && slot < d.num_slots)
-      *reinterpret_cast<uint2*>((normed ? d.kc : d.vc) + ((size_t)slot * 2 + hh) * 256 + 8 * j) = codes();
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+    ss += xor_swz<16>(ss);
+    ss += xor_swz<8>(ss);
+    ss += xor_swz<4>(ss);
+    ss += xor_swz<2>(ss);
+    ss += xor_swz<1>(ss);
+    const float inv = 1.f / sqrtf(ss / 256.f + d.eps);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = (uint32_t)(qhead ? qw[i] : kw[i]);
+      const float a = (x[2 * i] * inv) * (bf_lo(w) + 1.f), b = (x[2 * i + 1] * inv) * (bf_hi(w) + 1.f);
+      x[2 * i] = normed ? a : x[2 * i];
+      x[2 * i + 1] = normed ? b : x[2 * i + 1];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float other = xor_swz<4>(x[e]);
+      const float r = __builtin_fmaf(x[e], c[e], (sg * other) * s[e]);
+      x[e] = rot ? r : x[e];
+    }
+    const auto codes = [&] {
+      return make_uint2(f2e4m3x2_nan(x[0], x[1]) | (f2e4m3x2_nan(x[2], x[3]) << 16),
+                        f2e4m3x2_nan(x[4], x[5]) | (f2e4m3x2_nan(x[6], x[7]) << 16));
+    };
+    if (qhead) {
+      const size_t at = ((size_t)t * 16 + h) * 256 + 8 * j;
+      if (!normed) {
+        if (d.gate) *reinterpret_cast<v4i*>(d.gate + at) = raw[k];
+      } else if constexpr (Q8) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(d.q) + at) = codes();
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(d.q) + at) = make_uint4(
+            pack_bf2_hw(x[0], x[1]), pack_bf2_hw(x[2], x[3]), pack_bf2_hw(x[4], x[5]), pack_bf2_hw(x[6], x[7]));
+      }
+    } else if (slot >= 0 && slot < d.num_slots) {
+      *reinterpret_cast<uint2*>((normed ? d.kc : d.vc) + ((size_t)slot * 2 + (h - 16)) * 256 + 8 * j) = codes();
+    }
   }
 }
 
@@ -151,12 +165,12 @@ extern "C" int q36_attn_front(const q36_attn_front_args* a, q36_stream_t stream)
                    static_cast<const uint16_t*>(a->k_norm_w), a->cos_sin, a->positions, a->q,
                    static_cast<uint16_t*>(a->gate), a->out_loc, static_cast<uint8_t*>(a->k_cache),
                    static_cast<uint8_t*>(a->v_cache), a->num_slots, a->eps};
-  const unsigned grid = (unsigned)(((int64_t)a->T * kFItems + 3) / 4);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool multi = a->axis_map != 0;
+  const bool multi = a->axis_map != 0, q8 = a->q_e4m3 != 0;
+  const unsigned grid = (unsigned)(((int64_t)a->T * WPT + 3) / 4);
   if (multi)
-    a->q_e4m3 ? front_kernel<true, true><<<grid, 256, 0, st>>>(d) : front_kernel<true, false><<<grid, 256, 0, st>>>(d);
+    q8 ? front_kernel<true, true><<<grid, 256, 0, st>>>(d) : front_kernel<true, false><<<grid, 256, 0, st>>>(d);
   else
-    a->q_e4m3 ? front_kernel<false, true><<<grid, 256, 0, st>>>(d) : front_kernel<false, false><<<grid, 256, 0, st>>>(d);
+    q8 ? front_kernel<false, true><<<grid, 256, 0, st>>>(d) : front_kernel<false, false><<<grid, 256, 0, st>>>(d);
   return check_launch("q36_attn_front");
 }

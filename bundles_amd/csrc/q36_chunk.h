@@ -14,7 +14,7 @@
 namespace q36 {
 
 constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 32, kNarrowKeys = 128;
-constexpr int kTileOvh = 12;
+constexpr int kTileOvh = 8;
 constexpr int kLeastShare = 4;  // a share is no shorter (but for a line shorter than this)
 
 struct ChunkReq {

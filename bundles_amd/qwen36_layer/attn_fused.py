@@ -224,50 +224,62 @@ def attn_front(qkv, q_norm_w, k_norm_w, eps, cos_sin, positions, cache=None, axe
     [T, 16, 256]), and the new e4m3 K / V rows in cache = (k_cache, v_cache, out_loc) (uint8 [slots, 2, 256], int64 [T];
     slots outside the cache are skipped).  positions int32 [T], or with axes int32 [axes, T] (an axis a row).  Formed in
     fp32 and rounded once (attn_proj rounds to bf16 between the steps)."""
+    bf16 = torch.bfloat16
+    if qkv.dim() != 2 or qkv.dtype is not bf16 or qkv.shape[1] != QKV_ROWS:
+        raise ValueError(f"attn_front: qkv must be bf16 [T, {QKV_ROWS}]")
     T = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[1] != QKV_ROWS or (T > 0 and qkv.stride(1) != 1):
-        raise ValueError(f"attn_front: qkv must be bf16 [T, {QKV_ROWS}] with contiguous rows")
-    if T > 1 and (qkv.stride(0) < QKV_ROWS or qkv.stride(0) % 8):
-        raise ValueError(f"attn_front: qkv's row stride {qkv.stride(0)} must be a multiple of 8 from {QKV_ROWS} on")
+    ld = QKV_ROWS
+    if not qkv.is_contiguous():
+        ld = qkv.stride(0) if T > 1 else QKV_ROWS
+        if qkv.stride(1) != 1 or ld < QKV_ROWS or ld % 8:
+            raise ValueError(f"attn_front: qkv's rows must be contiguous, their stride {ld} a multiple of 8 from {QKV_ROWS} on")
     for name, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.numel() != HEAD_DIM:
+        if t.dtype is not bf16 or t.shape != (HEAD_DIM,) or not t.is_contiguous():
             raise ValueError(f"attn_front: {name} must be contiguous bf16 [{HEAD_DIM}]")
-    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.dim() != 2 or cos_sin.shape[1] != 2 * ROT_PAIRS:
+    if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != 2 * ROT_PAIRS or not cos_sin.is_contiguous():
         raise ValueError(f"attn_front: cos_sin must be contiguous fp32 [max_pos, {2 * ROT_PAIRS}]")
-    want = (T,) if axes is None else (axes.axes, T)
-    if positions.dtype != torch.int32 or tuple(positions.shape) != want or (T > 0 and positions.stride(-1) != 1) or \
-            (axes is not None and positions.stride(0) < T):
-        raise ValueError(f"attn_front: positions must be int32 {list(want)} with contiguous rows")
-    if q_dtype not in (torch.bfloat16, torch.uint8):
+    n_axes, pos_ld, axis_map = 1, 0, 0
+    if axes is not None:
+        n_axes, pos_ld, axis_map = axes.axes, positions.stride(0), axes.map
+    if positions.dtype is not torch.int32 or positions.shape != ((T,) if axes is None else (n_axes, T)) or \
+            (T > 1 and positions.stride(-1) != 1) or (axes is not None and pos_ld < T):
+        raise ValueError(f"attn_front: positions must be int32 {[T] if axes is None else [n_axes, T]} with contiguous rows")
+    if q_dtype is not bf16 and q_dtype is not torch.uint8:
         raise ValueError("attn_front: q_dtype must be bfloat16 or uint8 (e4m3 codes)")
     shape = (T, N_Q_HEADS, HEAD_DIM)
-    q = torch.empty(shape, dtype=q_dtype, device=qkv.device) if q is None else q
-    gate = torch.empty(shape, dtype=torch.bfloat16, device=qkv.device) if gate is None else gate
-    for name, t, dt in (("q", q, q_dtype), ("gate", gate, torch.bfloat16)):
-        if t.dtype != dt or not t.is_contiguous() or tuple(t.shape) != shape:
-            raise ValueError(f"attn_front: {name} must be a contiguous {dt} tensor {list(shape)}")
+    if q is None:
+        q = torch.empty(shape, dtype=q_dtype, device=qkv.device)
+    elif q.dtype is not q_dtype or q.shape != shape or not q.is_contiguous():
+        raise ValueError(f"attn_front: q must be a contiguous {q_dtype} tensor {list(shape)}")
+    if gate is None:
+        gate = torch.empty(shape, dtype=bf16, device=qkv.device)
+    elif gate.dtype is not bf16 or gate.shape != shape or not gate.is_contiguous():
+        raise ValueError(f"attn_front: gate must be a contiguous bfloat16 tensor {list(shape)}")
     kc = vc = loc = None
     slots = 0
     if cache is not None:
         kc, vc, loc = cache
-        for name, t in (("k_cache", kc), ("v_cache", vc)):
-            if t.dtype != torch.uint8 or not t.is_contiguous() or t.shape[1:] != (N_KV_HEADS, HEAD_DIM):
-                raise ValueError(f"attn_front: {name} must be contiguous uint8 [slots, {N_KV_HEADS}, {HEAD_DIM}]")
-        if kc.shape != vc.shape:
-            raise ValueError("attn_front: k_cache and v_cache differ in shape")
-        if loc.dtype != torch.int64 or not loc.is_contiguous() or loc.numel() < T:
+        _check_caches("attn_front", kc, vc)
+        if loc.dtype is not torch.int64 or not loc.is_contiguous() or loc.numel() < T:
             raise ValueError(f"attn_front: out_loc must be contiguous int64 with at least {T} entries")
         slots = kc.shape[0]
-    check_tensors("attn_front", qkv=qkv, q_norm_w=q_norm_w, k_norm_w=k_norm_w, cos_sin=cos_sin, positions=positions, q=q,
-                  gate=gate, k_cache=kc, v_cache=vc, out_loc=loc)
+    check_tensors("attn_front", "qkv q_norm_w k_norm_w cos_sin positions q gate k_cache v_cache out_loc", qkv, q_norm_w, k_norm_w,
+                  cos_sin, positions, q, gate, kc, vc, loc)
     if T == 0:
         return q, gate
-    a = pack_front(T, cos_sin.shape[0], 1 if axes is None else axes.axes, int(q_dtype == torch.uint8),
-                   qkv.stride(0) if T > 1 else QKV_ROWS, 0 if axes is None else positions.stride(0), 0 if axes is None else axes.map,
-                   slots, ptr(qkv), ptr(q_norm_w), ptr(k_norm_w), ptr(cos_sin), ptr(positions), ptr(q), ptr(gate), ptr(loc),
-                   ptr(kc), ptr(vc), eps)
+    a = pack_front(T, cos_sin.shape[0], n_axes, 1 if q_dtype is torch.uint8 else 0, ld, pos_ld, axis_map, slots, qkv.data_ptr(),
+                   q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(), q.data_ptr(),
+                   gate.data_ptr(), ptr(loc), ptr(kc), ptr(vc), eps)
     check(_lib.packed().q36_attn_front(a, _lib.stream_handle(stream)), "q36_attn_front")
     return q, gate
+
+
+def _check_caches(what, k_cache, v_cache):
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dtype is not torch.uint8 or t.dim() != 3 or t.shape[1:] != (N_KV_HEADS, HEAD_DIM) or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous uint8 [slots, {N_KV_HEADS}, {HEAD_DIM}]")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"{what}: k_cache and v_cache differ in shape")
 
 
 class ChunkWorkspace:
@@ -290,24 +302,23 @@ def attn_chunk(q, k_cache, v_cache, page_table, seqlens, qsl, scale: float, ws: 
     fresh out holds anything there), rows that see no key are zero."""
     if q.dim() != 3 or q.shape[1:] != (N_Q_HEADS, HEAD_DIM) or q.dtype not in (torch.bfloat16, torch.uint8) or not q.is_contiguous():
         raise ValueError(f"attn_chunk: q must be a contiguous bfloat16 or uint8 tensor [T, {N_Q_HEADS}, {HEAD_DIM}]")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dtype != torch.uint8 or not t.is_contiguous() or t.shape[1:] != (N_KV_HEADS, HEAD_DIM):
-            raise ValueError(f"attn_chunk: {name} must be contiguous uint8 [slots, {N_KV_HEADS}, {HEAD_DIM}]")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("attn_chunk: k_cache and v_cache differ in shape")
-    B = page_table.shape[0]
-    for name, t, shape in (("page_table", page_table, (B, page_table.shape[-1])), ("seqlens", seqlens, (B,)), ("qsl", qsl, (B + 1,))):
-        if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+    _check_caches("attn_chunk", k_cache, v_cache)
+    if page_table.dim() != 2:
+        raise ValueError("attn_chunk: page_table must be [B, stride]")
+    B, width = page_table.shape
+    for name, t, shape in (("page_table", page_table, (B, width)), ("seqlens", seqlens, (B,)), ("qsl", qsl, (B + 1,))):
+        if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"attn_chunk: {name} must be a contiguous int32 tensor {list(shape)}")
-    out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device) if out is None else out
-    if out.dtype != torch.bfloat16 or not out.is_contiguous() or out.shape != q.shape:
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype is not torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
         raise ValueError(f"attn_chunk: out must be a contiguous bfloat16 tensor {list(q.shape)}")
-    check_tensors("attn_chunk", q=q, k_cache=k_cache, v_cache=v_cache, page_table=page_table, seqlens=seqlens, qsl=qsl, out=out,
-                  workspace=ws.buf)
+    check_tensors("attn_chunk", "q k_cache v_cache page_table seqlens qsl out workspace", q, k_cache, v_cache, page_table, seqlens,
+                  qsl, out, ws.buf)
     if q.shape[0] == 0:
         return out
-    a = pack_chunk(B, q.shape[0], N_Q_HEADS, N_KV_HEADS, HEAD_DIM, page_size, page_table.shape[1], int(q.dtype == torch.uint8),
-                   k_cache.shape[0], ptr(q), ptr(k_cache), ptr(v_cache), ptr(page_table), ptr(seqlens), ptr(qsl), ptr(out),
-                   ptr(ws.buf), ws.buf.numel(), scale)
+    a = pack_chunk(B, q.shape[0], N_Q_HEADS, N_KV_HEADS, HEAD_DIM, page_size, width, 1 if q.dtype is torch.uint8 else 0,
+                   k_cache.shape[0], q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+                   seqlens.data_ptr(), qsl.data_ptr(), out.data_ptr(), ws.buf.data_ptr(), ws.buf.numel(), scale)
     check(_lib.packed().q36_attn_chunk(a, _lib.stream_handle(stream)), "q36_attn_chunk")
     return out

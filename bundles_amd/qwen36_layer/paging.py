@@ -32,9 +32,8 @@ class PagePlan:
                         torch.empty(T, dtype=torch.int64, device=device), torch.empty(2, **i32))
 
 
-def _int32(name: str, t: torch.Tensor, *shape) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
-        raise ValueError(f"plan_pages: {name} must be a contiguous int32 tensor {list(shape)}")
+def _refuse(name: str, shape, dtype="int32"):
+    raise ValueError(f"plan_pages: {name} must be a contiguous {dtype} tensor {list(shape)}")
 
 
 def plan_pages(cached, new, table, free, T: int, page_size: int = 1, req=None, page_table=None, whole: bool = True,
@@ -45,31 +44,38 @@ def plan_pages(cached, new, table, free, T: int, page_size: int = 1, req=None, p
     padded batch).  page_table int32 [B, stride] (optional) receives the slot of each request's keys, as attn_decode
     reads them: all keys (whole) or the new tokens' alone; the rest of it is left as it was.  A page number outside
     the cache is the caller's to avoid; what does not fit is told in plan.used[1] and gets no slot."""
-    B = cached.shape[0] if cached.dim() == 1 else -1
-    _int32("cached", cached, B)
-    _int32("new", new, B)
+    i32 = torch.int32
+    if cached.dim() != 1:
+        raise ValueError("plan_pages: cached must be [B]")
+    B = cached.shape[0]
     if table.dim() != 2 or free.dim() != 1:
         raise ValueError("plan_pages: table must be [rows, width] and free [pages]")
-    _int32("table", table, *table.shape)
-    _int32("free", free, *free.shape)
-    if req is not None:
-        _int32("req", req, B)
+    for name, t in (("cached", cached), ("new", new), ("req", req)):
+        if t is not None and (t.dtype is not i32 or t.shape != (B,) or not t.is_contiguous()):
+            _refuse(name, (B,))
+    rows, width = table.shape
+    if table.dtype is not i32 or not table.is_contiguous():
+        _refuse("table", (rows, width))
+    if free.dtype is not i32 or not free.is_contiguous():
+        _refuse("free", free.shape)
+    pt_width = 0
     if page_table is not None:
-        _int32("page_table", page_table, B, page_table.shape[-1])
+        pt_width = page_table.shape[-1]
+        if page_table.dtype is not i32 or page_table.shape != (B, pt_width) or not page_table.is_contiguous():
+            _refuse("page_table", (B, pt_width))
     if plan is None:
         plan = PagePlan.alloc(B, T, cached.device)
     else:
-        _int32("plan.qsl", plan.qsl, B + 1)
-        _int32("plan.seqlens", plan.seqlens, B)
-        _int32("plan.positions", plan.positions, T)
-        _int32("plan.used", plan.used, 2)
-        if plan.out_loc.dtype != torch.int64 or not plan.out_loc.is_contiguous() or tuple(plan.out_loc.shape) != (T,):
-            raise ValueError(f"plan_pages: plan.out_loc must be a contiguous int64 tensor [{T}]")
-    check_tensors("plan_pages", cached=cached, new=new, table=table, free=free, req=req, page_table=page_table,
-                  qsl=plan.qsl, seqlens=plan.seqlens, positions=plan.positions, out_loc=plan.out_loc, used=plan.used)
-    a = pack_plan(B, T, page_size, table.shape[0], table.shape[1], free.shape[0],
-                  0 if page_table is None else page_table.shape[1], int(whole), ptr(cached), ptr(new), ptr(req), ptr(table),
-                  ptr(free), ptr(plan.qsl), ptr(plan.seqlens), ptr(plan.positions), ptr(plan.out_loc), ptr(plan.used),
-                  ptr(page_table))
+        for name, t, n in (("plan.qsl", plan.qsl, B + 1), ("plan.seqlens", plan.seqlens, B),
+                           ("plan.positions", plan.positions, T), ("plan.used", plan.used, 2)):
+            if t.dtype is not i32 or t.shape != (n,) or not t.is_contiguous():
+                _refuse(name, (n,))
+        if plan.out_loc.dtype is not torch.int64 or plan.out_loc.shape != (T,) or not plan.out_loc.is_contiguous():
+            _refuse("plan.out_loc", (T,), "int64")
+    check_tensors("plan_pages", "cached new table free req page_table plan.qsl plan.seqlens plan.positions plan.out_loc plan.used",
+                  cached, new, table, free, req, page_table, plan.qsl, plan.seqlens, plan.positions, plan.out_loc, plan.used)
+    a = pack_plan(B, T, page_size, rows, width, free.shape[0], pt_width, 1 if whole else 0, cached.data_ptr(), new.data_ptr(),
+                  ptr(req), table.data_ptr(), free.data_ptr(), plan.qsl.data_ptr(), plan.seqlens.data_ptr(),
+                  plan.positions.data_ptr(), plan.out_loc.data_ptr(), plan.used.data_ptr(), ptr(page_table))
     check(_lib.packed().q36_page_plan(a, _lib.stream_handle(stream)), "q36_page_plan")
     return plan
