@@ -7,6 +7,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "q36_device.h"
 #include "q36_host.h"
@@ -37,6 +38,8 @@ struct ChunkDev {
   float* ws_ml;  // [2 groups][8][2][32]: their running maxima (base 2) and weight sums
   int4* cuts;    // [groups] the tile that starts in each share and is cut: request (-1: none), 2 tile + head, last share; and
                  // whether a value on the causal border was NaN
+  uint32_t* flags;  // [groups] said when a share has written the partial that ends the tile which the share before starts
+  uint32_t* epoch;  // calls that this workspace has served
 };
 
 // A request's first row, new tokens and keys, inside the buffers whatever qsl and seqlens hold.
@@ -115,6 +118,8 @@ struct Item {
   int last;           // the last key that the tile's last token sees (0 where there is none)
   int key0, key1;     // the run's keys, key1 up to a step behind vis
   int slot;           // of its partial (-1: the whole tile)
+  int lasts;          // of a tile's start: the share that has its end (-1: no start, or the whole tile)
+  bool pair;          // the end of a tile that the share before starts
 };
 
 // The line of the call's tiles (q36_chunk.h), this workgroup's share of it, and its runs one after another, by 8 waves.
@@ -131,8 +136,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ __align__(1024) uint8_t X[2 * kSet];
   __shared__ float mlw[8][2][32];
   __shared__ int sums[8];
-  __shared__ int found_at, found_b, nan_seen;
+  __shared__ int found_at, found_b, nan_seen, joined;
   const int tid = threadIdx.x, wave = uni(tid >> 6), G = gridDim.x;
+  // what a flag of this call from this XCD says: its number among the workspace's calls, spread, and the XCD's
+  uint32_t xcc;
+  asm("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
+  const uint32_t mark = ((d.epoch[0] * 0x9e3779b1u) & ~15u) | (xcc & 15u);
   // ---- this workgroup's share
   int total = 0, mine = 0;
   for (int c0 = 0; c0 < d.B; c0 += 512) {
@@ -199,27 +208,29 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   // the share's next run (none: n = 0)
   auto next = [&] {
-    Item it = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1};
+    Item it = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1, -1, false};
     while (coff < x1 && it.n == 0) {
       if (cr.n == 0) {
         ++coff;
         if (coff < x1) request(cb + 1);
         continue;
       }
-      const int steps = ck_steps(cr, ctile), ks = ck_step_keys(cr.n);
-      const ChunkRun run = ck_run(steps, coff, x0, x1);
+      const int steps = ck_steps(cr, ctile), ks = ck_step_keys(cr.n), cost = ck_cost(cr.n);
+      const ChunkRun run = ck_run(steps, cost, coff, x0, x1);
       if (run.nst >= 0) {
+        const bool whole = run.first && run.last;
         it = Item{cb, ct0, cr.n, cr.nk, ch, ctile * ck_tile_tok(cr.n), max(ck_keys(cr, ctile) - 1, 0), run.st0 * ks, (run.st0 + run.nst) * ks,
-                  run.first && run.last ? -1 : ck_slot(share, run.first)};
-        if (it.slot >= 0 && run.first) cut = int4{cb, 2 * ctile + ch, ck_last_share(steps, coff, len), 0};
+                  whole ? -1 : ck_slot(share, run.first), run.first && !whole ? ck_last_share(steps, cost, coff, len) : -1,
+                  run.last && !whole && ck_first_share(coff, len) == share - 1};
       }
-      coff += steps + kTileOvh;
+      coff += steps * cost + kTileOvh;
       if (++ctile < ck_tiles(cr.n)) continue;
       ctile = 0;
       if (++ch == 2 && coff < x1) request(cb + 1);
     }
     // scalars: what is made from them stays in SGPRs
-    return Item{uni(it.b), uni(it.t0), uni(it.n), uni(it.nk), uni(it.h), uni(it.tok), uni(it.last), uni(it.key0), uni(it.key1), uni(it.slot)};
+    return Item{uni(it.b), uni(it.t0), uni(it.n), uni(it.nk), uni(it.h), uni(it.tok), uni(it.last), uni(it.key0), uni(it.key1), uni(it.slot), uni(it.lasts),
+                uni(it.pair) != 0};
   };
   // ---- copies: wave w takes rows 4 w .. of each block's value rows and the same keys' rows; a lane has 16 bytes of row
   // `lane / 16` of the four
@@ -245,7 +256,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int lane = fresh_tid() & 63, t4 = lane >> 4, key = k.key0 + kap + t4;
     const uint8_t* const kbase = d.kc + (k.h * kCD + 16 * ((lane & 15) ^ ((kap & 15) + t4)));
     const uint8_t* const vbase = d.vc + (k.h * kCD + 16 * ((lane & 15) ^ (2 * (4 * (wave & 1) + t4))));
-    const uint32_t to = lds_at(X) + half * kSet;
+    const uint32_t to = (uint32_t)uni((int)lds_at(X) + half * kSet);
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
       const uint32_t pg = min(x.v[e], (uint32_t)top_page);  // (a negative number is a large one)
@@ -262,47 +273,61 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int lim = -1;  // the row's last key
   uint32_t bad = 0;  // bits of NaN values on the causal border
   auto first_tok = [&](const Item& it) { return it.tok + 4 * (ck_wide(it.n) ? wave : wave & 1); };
-  auto queries = [&](const Item& it, bool q8) {
-    const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5, tok = first_tok(it) + (col >> 3);
-    const size_t at = ((size_t)(it.t0 + tok) * kCHQ + it.h * kCG + (col & 7)) * kCD + 32 * g;
-    const bool ok = tok < it.n;
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      v4i a = {0, 0, 0, 0}, e = {0, 0, 0, 0};
-      if (ok) {
-        if (q8) {
-          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(d.q) + at + 64 * kb);
-          a = src[0], e = src[1];
-        } else {
-          const v4i* src = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.q) + at + 64 * kb);
-          auto codes = [](v4i x, int j) {
-            return (int)(f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j]), bf_hi((uint32_t)x[2 * j])) |
-                         (f2e4m3x2_nan(bf_lo((uint32_t)x[2 * j + 1]), bf_hi((uint32_t)x[2 * j + 1])) << 16));
-          };
-          const v4i x0 = src[0], x1 = src[1], x2 = src[2], x3 = src[3];
-          a = v4i{codes(x0, 0), codes(x0, 1), codes(x1, 0), codes(x1, 1)};
-          e = v4i{codes(x2, 0), codes(x2, 1), codes(x3, 0), codes(x3, 1)};
-        }
-      }
-      qf[kb] = v8i{a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
-    }
-  };
-  const float sl2 = d.scale_log2;
-  bool begun = false;  // a block has been taken: m is its rows' largest, and grows
-  auto value = [&](uint32_t v0, int dt, int cc) {
-    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)((v0 ^ (32 * dt)) + 16 * kCD * cc));
-  };
-  auto key = [&](uint32_t k0, int i) { return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(k0 ^ (16 * i)); };
-  auto clean = [&](v2i w) {
-    const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y);
-    bad |= n0 | n1;
-    return v2i{(int)(w.x & ~(n0 | (n0 - (n0 >> 7)))), (int)(w.y & ~(n1 | (n1 - (n1 >> 7))))};
-  };
   // this lane's places in a block: K row l % 32, piece 2 (l / 32) (the others: 4 kb + e more, by an xor); V row
   // 8 (l / 32) + (l % 16) / 2 (+ 16 c), piece (l / 16) % 2 (the others: 2 dt more)
   const int lane0 = tid & 63, g0 = lane0 >> 5;
   const uint32_t ka = (lane0 & 31) * kCD + 16 * ((2 * g0) ^ (lane0 & 15));
   const uint32_t va = kCST * kCD + (8 * g0 + ((lane0 & 15) >> 1)) * kCD + 16 * (((lane0 >> 4) & 1) ^ (lane0 & 14)) + 8 * (lane0 & 1);
+  auto value = [&](uint32_t v0, int dt, int cc) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)((v0 ^ (32 * dt)) + 16 * kCD * cc));
+  };
+  auto key = [&](uint32_t k0, int i) { return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(k0 ^ (16 * i)); };
+  // The wave's query rows: asked for as they lie, 1 KB a load (four rows of codes, two of bf16), and handed out to the lanes
+  // through the wave's 8 KB of `mem` (16-byte piece p of row r at p ^ (r % 16), as a block's keys).
+  v4i qraw[16];
+  auto ask = [&](const Item& it, bool q8) {
+    const int lane = fresh_tid() & 63, tok = first_tok(it);
+    const char* const rows = static_cast<const char*>(d.q) + (((size_t)(it.t0 + tok) * kCHQ + it.h * kCG) * kCD << (q8 ? 0 : 1));
+#pragma unroll
+    for (int j = 0; j < (q8 ? 8 : 16); ++j) {
+      const int r = q8 ? 4 * j + (lane >> 4) : 2 * j + (lane >> 5), at = q8 ? 256 * (r & 7) + 16 * (lane & 15) : 512 * (r & 7) + 16 * (lane & 31);
+      qraw[j] = v4i{0, 0, 0, 0};
+      if (tok + (r >> 3) < it.n) qraw[j] = *reinterpret_cast<const v4i*>(rows + (((size_t)(r >> 3) * kCHQ * kCD) << (q8 ? 0 : 1)) + at);
+    }
+  };
+  auto answer = [&](uint8_t* mem) {
+    const int lane = fresh_tid() & 63;
+    uint8_t* const my = mem + wave * 8192;
+    if (d.q8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 4 * j + (lane >> 4);
+        *reinterpret_cast<v4i*>(my + 256 * r + 16 * ((lane & 15) ^ (r & 15))) = qraw[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int r = 2 * j + (lane >> 5);
+        const v4i x = qraw[j];
+        auto two = [](int w) { return f2e4m3x2_nan(bf_lo((uint32_t)w), bf_hi((uint32_t)w)); };
+        *reinterpret_cast<uint2*>(my + 256 * r + 16 * (((lane & 31) >> 1) ^ (r & 15)) + 8 * (lane & 1)) =
+            make_uint2(two(x.x) | (two(x.y) << 16), two(x.z) | (two(x.w) << 16));
+      }
+    }
+    const uint32_t k0 = lds_at(my) + ka;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const v4i a = key(k0, 4 * kb), e = key(k0, 4 * kb + 1);
+      qf[kb] = v8i{a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+    }
+  };
+  const float sl2 = d.scale_log2;
+  bool begun = false;  // a block has been taken: m is its rows' largest, and grows
+  auto clean = [&](v2i w) {
+    const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y);
+    bad |= n0 | n1;
+    return v2i{(int)(w.x & ~(n0 | (n0 - (n0 >> 7)))), (int)(w.y & ~(n1 | (n1 - (n1 >> 7))))};
+  };
   // the block at byte `at` of LDS, keys key0 ..; border: some row does not see all of them
   auto block = [&](uint32_t at, int key0, bool border) {
     uint32_t k0 = at + ka, v0 = at + va;
@@ -367,7 +392,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int dt = 0; dt < 8; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen8(w[dt].x, w[dt].y), pb[1], o[dt], 0, 0, 0);
   };
   // ---- the runs, one after another; while one ends, the first set of the next is on its way
-  Item cur = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1}, nxt = next();
+  Item cur = {0, 0, 0, 0, 0, 0, 0, 0, 0, -1, -1, false}, nxt = next();
   // the keys that are copied next, and their page-table entries
   Keys ahead = keys_of(nxt, 0);
   Ent ent = {};
@@ -378,15 +403,24 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
   wait_vm0();
   for (int half = 0;;) {
-    // the next item's query rows (codes) are asked for before this one's outputs leave
-    if (d.q8) queries(nxt, true);
+    uint8_t* const mem = X + (half ^ 1) * kSet;
     if (cur.n > 0) {
       l += __shfl_xor(l, 32);
       if (l == 0.f) m = -1e30f;  // no key seen
       const bool wide = ck_wide(cur.n);
-      const int slot = cur.slot, tok0 = first_tok(cur), rw = wide ? wave : wave & 1;
+      int slot = cur.slot;
+      const int tok0 = first_tok(cur), rw = wide ? wave : wave & 1;
       const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5;
-      uint8_t* const mem = X + (half ^ 1) * kSet;
+      // A wide tile that the next share ends, most likely long ago, with its first run: where that partial is there, in this
+      // XCD's L2, the two are joined here, by the combine kernel's arithmetic; else the combine kernel does it.
+      bool join = false;
+      if (wide && cur.lasts == share + 1) {
+        if (tid == 0) joined = __hip_atomic_load(d.flags + share + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
+        barrier();
+        join = uni(joined) != 0;
+      }
+      if (join) slot = -1;
+      else if (cur.lasts >= 0) cut = int4{cur.b, 2 * (cur.tok / ck_tile_tok(cur.n)) + cur.h, cur.lasts, 0};
       float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane * 4;
       float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col;
       uint16_t* const rows = d.out + ((size_t)(cur.t0 + tok0) * kCHQ + cur.h * kCG) * kCD;  // row r: token r / 8, head r % 8
@@ -427,26 +461,43 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       } else if (tok0 < cur.n) {
         if (slot < 0) {
           // rounded, through the wave's 8 KB of LDS (32 rows x 128 dims, 16-byte piece p of row r at p ^ (r % 16)), out by rows
-          const float il = l > 0.f ? 1.f / l : l;  // (no key: 0; NaN stays)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
+          auto leave = [&](auto joins) {
+            const float *o2 = nullptr;
+            float f = 1.f, f2 = 0.f, L = l;
+            if constexpr (decltype(joins)::value) {
+              const size_t s2 = (size_t)ck_slot(share + 1, false);
+              const float* const ml2 = d.ws_ml + s2 * kSlotML + wave * 64 + col;
+              const float m2 = ml2[0], M = fmaxf(fmaxf(-1e30f, m), m2);
+              o2 = d.ws_o + s2 * kSlotF + (size_t)wave * (8 * 4 * 256) + lane * 4;
+              f = __builtin_amdgcn_exp2f(m - M), f2 = __builtin_amdgcn_exp2f(m2 - M);
+              L = f * l + f2 * ml2[32];
+            }
+            const float il = L > 0.f ? 1.f / L : L;  // (no key: 0; NaN stays)
             uint8_t* const my = mem + wave * 8192;
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
+            for (int q = 0; q < 2; ++q) {
 #pragma unroll
-              for (int a = 0; a < 4; ++a) {
-                const v16f& v = o[4 * q + dt];
-                *reinterpret_cast<uint2*>(my + col * 256 + 16 * ((4 * dt + a) ^ (col & 15)) + 8 * g) =
-                    make_uint2(pack_bf2_hw(v[4 * a] * il, v[4 * a + 1] * il), pack_bf2_hw(v[4 * a + 2] * il, v[4 * a + 3] * il));
+              for (int dt = 0; dt < 4; ++dt) {
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                  const v16f& u = o[4 * q + dt];
+                  v4f v = {u[4 * a], u[4 * a + 1], u[4 * a + 2], u[4 * a + 3]};
+                  if constexpr (decltype(joins)::value) v = f * v + f2 * *reinterpret_cast<const v4f*>(o2 + ((4 * q + dt) * 4 + a) * 256);
+                  *reinterpret_cast<uint2*>(my + col * 256 + 16 * ((4 * dt + a) ^ (col & 15)) + 8 * g) =
+                      make_uint2(pack_bf2_hw(v[0] * il, v[1] * il), pack_bf2_hw(v[2] * il, v[3] * il));
+                }
+                if (decltype(joins)::value && (dt & 1)) __builtin_amdgcn_sched_barrier(0);  // (eight loads in flight, no more registers)
               }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int row = 4 * j + (lane >> 4);
-              const v4i v = *reinterpret_cast<const v4i*>(my + row * 256 + 16 * ((lane & 15) ^ (row & 15)));
-              if (tok0 + (row >> 3) < cur.n)
-                *reinterpret_cast<v4i*>(rows + ((size_t)(row >> 3) * kCHQ + (row & 7)) * kCD + 128 * q + 8 * (lane & 15)) = v;
+              for (int j = 0; j < 8; ++j) {
+                const int row = 4 * j + (lane >> 4);
+                const v4i v = *reinterpret_cast<const v4i*>(my + row * 256 + 16 * ((lane & 15) ^ (row & 15)));
+                if (tok0 + (row >> 3) < cur.n)
+                  *reinterpret_cast<v4i*>(rows + ((size_t)(row >> 3) * kCHQ + (row & 7)) * kCD + 128 * q + 8 * (lane & 15)) = v;
+              }
             }
-          }
+          };
+          join ? leave(std::true_type{}) : leave(std::false_type{});
         } else {
 #pragma unroll
           for (int dt = 0; dt < 8; ++dt)
@@ -456,9 +507,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           if (g == 0) wml[0] = m, wml[32] = l;
         }
       }
+      if (wide && cur.pair) {
+        wait_vm0();
+        barrier();  // the partial is in L2
+        if (tid == 0) __hip_atomic_store(d.flags + share, mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      if (!wide) barrier();  // (the waves' LDS is theirs again)
     }
     if (nxt.n == 0) break;
-    if (!d.q8) queries(nxt, false);
+    d.q8 ? ask(nxt, true) : ask(nxt, false);
+    answer(mem);
     cur = nxt;
     nxt = next();
     const bool wide = ck_wide(cur.n);
@@ -473,8 +531,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     }
-    // (waited for here: the compiler would wait in each block, for the copies too)
-    asm volatile("" : "+v"(qf[0]), "+v"(qf[1]), "+v"(qf[2]), "+v"(qf[3]));
     begun = false;
     // the wave's keys: of the run, up to its last token's; none without a token
     const int end = uni(tok0 < cur.n ? min(pre + min(tok0 + 4, cur.n), cur.key1) : 0);
@@ -554,6 +610,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
     if (is) list[at] = c0 + tid;
     __syncthreads();
   }
+  if (blockIdx.x == 0 && tid == 0) d.epoch[0] += 1;
   if (lane == 0) nan_flags[wave] = nans != 0;
   __syncthreads();
   const bool any_nan = uni(nan_flags[0] | nan_flags[1] | nan_flags[2] | nan_flags[3]) != 0;
@@ -652,14 +709,15 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
 // Workgroups: one a CU (their LDS and registers fill it).
 int chunk_groups() { return std::min(std::max(device_cus(), 1), 1024); }
 struct ChunkWs {
-  size_t o, ml, cuts, total;
+  size_t o, ml, cuts, flags, total;
 };
 ChunkWs chunk_ws(int G) {
   ChunkWs w;
   w.o = 0;
   w.ml = align_up(w.o + sizeof(float) * 2 * (size_t)G * kSlotF, 256);
   w.cuts = align_up(w.ml + sizeof(float) * 2 * (size_t)G * kSlotML, 256);
-  w.total = align_up(w.cuts + sizeof(int4) * (size_t)G, 256);
+  w.flags = align_up(w.cuts + sizeof(int4) * (size_t)G, 256);
+  w.total = align_up(w.flags + sizeof(uint32_t) * ((size_t)G + 1), 256);
   return w;
 }
 
@@ -699,7 +757,8 @@ extern "C" int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream) {
   const ChunkDev d{a->B, a->T, sh, a->pt_stride, a->q_e4m3, a->num_slots, a->q, static_cast<const uint8_t*>(a->k_cache),
                    static_cast<const uint8_t*>(a->v_cache), a->page_table, a->seqlens, a->qsl, static_cast<uint16_t*>(a->out),
                    a->scale * 1.44269504088896340736f, reinterpret_cast<float*>(ws + L.o), reinterpret_cast<float*>(ws + L.ml),
-                   reinterpret_cast<int4*>(ws + L.cuts)};
+                   reinterpret_cast<int4*>(ws + L.cuts), reinterpret_cast<uint32_t*>(ws + L.flags) + 1,
+                   reinterpret_cast<uint32_t*>(ws + L.flags)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   chunk_kernel<<<G, 512, 0, st>>>(d);
   chunk_combine_kernel<<<1024, 256, 0, st>>>(d, G);

@@ -15,6 +15,7 @@ namespace q36 {
 
 constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 32, kNarrowKeys = 128;
 constexpr int kTileOvh = 8;
+constexpr int kNarrowCost = 2;  // what a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16
 constexpr int kLeastShare = 4;  // a share is no shorter (but for a line shorter than this)
 
 struct ChunkReq {
@@ -35,6 +36,7 @@ __host__ __device__ __forceinline__ int ck_steps(ChunkReq r, int i) {
   const int ks = ck_step_keys(r.n);
   return (ck_keys(r, i) + ks - 1) / ks;
 }
+__host__ __device__ __forceinline__ int ck_cost(int n) { return ck_wide(n) ? 1 : kNarrowCost; }
 // sum over j < count of max(0, c + j)
 __host__ __device__ __forceinline__ int ck_series(int c, int count) {
   if (c < 0) {
@@ -47,12 +49,12 @@ __host__ __device__ __forceinline__ int ck_series(int c, int count) {
 __host__ __device__ __forceinline__ int ck_before(ChunkReq r, int i) {
   int s = i * kTileOvh, full = i;
   if (i == ck_tiles(r.n) && i > 0) {  // the last tile ends with the request
-    s += ck_steps(r, i - 1);
+    s += ck_steps(r, i - 1) * ck_cost(r.n);
     --full;
   }
   // the others see nk - n + tokens (k + 1) keys: a step more each (wide), or there is one (narrow)
   if (ck_wide(r.n)) return s + ck_series(((r.nk - r.n + 31) >> 5) + 1, full);
-  return s + (full > 0 ? ck_steps(r, 0) : 0);
+  return s + (full > 0 ? ck_steps(r, 0) * kNarrowCost : 0);
 }
 // the weight of a request, both heads (an empty one weighs 1: what passing over it costs)
 __host__ __device__ __forceinline__ int ck_weight(ChunkReq r) { return r.n > 0 ? 2 * ck_before(r, ck_tiles(r.n)) : 1; }
@@ -69,7 +71,7 @@ __host__ __device__ __forceinline__ int ck_tile_at(ChunkReq r, int x) {
 // The most that a call of T new tokens, B requests and tables of `keys` keys can weigh; a line of kMostWeight is not dealt.
 constexpr int kMostWeight = 1 << 30;
 inline bool ck_too_long(int64_t T, int64_t B, int64_t keys) {
-  return 2.0 * ((double)T / kWideTok + 2.0 * (double)B) * ((double)keys / kWideKeys + 1 + kTileOvh) + (double)B >= kMostWeight;
+  return 2.0 * ((double)T / kWideTok + 2.0 * (double)B) * ((double)keys / kWideKeys + kNarrowCost + kTileOvh) + (double)B >= kMostWeight;
 }
 
 // Equal shares: their length, and how many a line has
@@ -85,14 +87,17 @@ struct ChunkRun {
   int st0, nst;
   bool first, last;
 };
-__host__ __device__ __forceinline__ ChunkRun ck_run(int steps, int off, int x0, int x1) {
+__host__ __device__ __forceinline__ ChunkRun ck_run(int steps, int cost, int off, int x0, int x1) {
   if (steps == 0) return ChunkRun{0, off >= x0 && off < x1 ? 0 : -1, true, true};
   const int at = off + kTileOvh / 2;  // of its first step
-  const int a = x0 > at ? x0 - at : 0, e = x1 - at < steps ? x1 - at : steps;
+  const int a = x0 > at ? (x0 - at + cost - 1) / cost : 0, b = x1 > at ? (x1 - at + cost - 1) / cost : 0, e = b < steps ? b : steps;
   return ChunkRun{a, e > a ? e - a : -1, a == 0, e == steps};
 }
-// the share that the last step of a tile at `off` lies in
-__host__ __device__ __forceinline__ int ck_last_share(int steps, int off, int len) { return (off + kTileOvh / 2 + steps - 1) / len; }
+// the shares that the first and the last step of a tile at `off` lie in
+__host__ __device__ __forceinline__ int ck_first_share(int off, int len) { return (off + kTileOvh / 2) / len; }
+__host__ __device__ __forceinline__ int ck_last_share(int steps, int cost, int off, int len) {
+  return (off + kTileOvh / 2 + (steps - 1) * cost) / len;
+}
 // The partial of share w: one for a tile that ends here or goes on through, one for a tile that starts here.
 __host__ __device__ __forceinline__ int ck_slot(int w, bool first) { return 2 * w + (first ? 1 : 0); }
 

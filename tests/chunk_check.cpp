@@ -30,9 +30,9 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
     const int nt = ck_tiles(req[b].n);
     for (int i = 0; i < nt; ++i) {
       if (ck_before(req[b], i) != sum) return "a tile's place is not the weight before it";
-      if (ck_tile_at(req[b], sum) != i || ck_tile_at(req[b], sum + ck_steps(req[b], i) + kTileOvh - 1) != i)
+      if (ck_tile_at(req[b], sum) != i || ck_tile_at(req[b], sum + ck_steps(req[b], i) * ck_cost(req[b].n) + kTileOvh - 1) != i)
         return "a place's tile is not found";
-      sum += ck_steps(req[b], i) + kTileOvh;
+      sum += ck_steps(req[b], i) * ck_cost(req[b].n) + kTileOvh;
       if (i + 1 == nt && ck_keys(req[b], i) != std::max(0, req[b].nk)) return "the last tile does not see all keys";
     }
     if (nt && (ck_before(req[b], nt) != sum || 2 * sum != ck_weight(req[b]))) return "a request's weight is not its tiles'";
@@ -67,8 +67,8 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
       if (req[b].n == 0) {
         ++off;
       } else {
-        const int steps = ck_steps(req[b], tile);
-        const ChunkRun r = ck_run(steps, off, x0, x1);
+        const int steps = ck_steps(req[b], tile), cost = ck_cost(req[b].n);
+        const ChunkRun r = ck_run(steps, cost, off, x0, x1);
         if (r.nst >= 0) {
           if (r.st0 < 0 || r.st0 + r.nst > steps) return "a run outside its tile";
           for (int s = r.st0; s < r.st0 + r.nst; ++s) ++done[2 * b + h][tile][s];
@@ -78,10 +78,12 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
             const int slot = ck_slot(w, r.first);
             if (owner[slot] >= 0) return "a slot written twice";
             owner[slot] = ((long)(2 * b + h) << 32) + tile;
-            if (r.first) cut[w] = Cut{b, h, tile, ck_last_share(steps, off, len)};
+            if (ck_first_share(off, len) != (r.first ? w : ck_first_share(off, len)) || (!r.first && ck_first_share(off, len) >= w))
+              return "a tile's first share is not where it starts";
+            if (r.first) cut[w] = Cut{b, h, tile, ck_last_share(steps, cost, off, len)};
           }
         }
-        off += steps + kTileOvh;
+        off += steps * cost + kTileOvh;
         if (++tile < ck_tiles(req[b].n)) continue;
         tile = 0;
         if (++h < 2) continue;
