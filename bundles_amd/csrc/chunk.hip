@@ -21,6 +21,9 @@ constexpr int kCST = 32;  // keys a step
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef short v2s __attribute__((ext_vector_type(2)));
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 struct ChunkDev {
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // what a flag of this call from this XCD says: its number among the workspace's calls, spread, and the XCD's
   uint32_t xcc;
   asm("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
-  const uint32_t mark = ((d.epoch[0] * 0x9e3779b1u) & ~15u) | (xcc & 15u);
+  const uint32_t mark = ((d.epoch[0] * 0x9e3779b1u) & ~31u) | 16u | (xcc & 15u);  // (not 0, what the first call finds)
   // ---- this workgroup's share
   int total = 0, mine = 0;
   for (int c0 = 0; c0 < d.B; c0 += 512) {
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const bool whole = run.first && run.last;
         it = Item{cb, ct0, cr.n, cr.nk, ch, ctile * ck_tile_tok(cr.n), max(ck_keys(cr, ctile) - 1, 0), run.st0 * ks, (run.st0 + run.nst) * ks,
                   whole ? -1 : ck_slot(share, run.first), run.first && !whole ? ck_last_share(steps, cost, coff, len) : -1,
-                  run.last && !whole && ck_first_share(coff, len) == share - 1};
+                  run.last && !whole && ck_first_share(steps, cost, coff, len) == share - 1};
       }
       coff += steps * cost + kTileOvh;
       if (++ctile < ck_tiles(cr.n)) continue;
@@ -305,14 +308,33 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         *reinterpret_cast<v4i*>(my + 256 * r + 16 * ((lane & 15) ^ (r & 15))) = qraw[j];
       }
     } else {
+      // the conversion makes a NaN of what is past 448 (of 464, with its rounding): rows with one of those go the long way
+      v2us big = {0, 0};
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const int r = 2 * j + (lane >> 5);
         const v4i x = qraw[j];
-        auto two = [](int w) { return f2e4m3x2_nan(bf_lo((uint32_t)w), bf_hi((uint32_t)w)); };
-        *reinterpret_cast<uint2*>(my + 256 * r + 16 * (((lane & 31) >> 1) ^ (r & 15)) + 8 * (lane & 1)) =
-            make_uint2(two(x.x) | (two(x.y) << 16), two(x.z) | (two(x.w) << 16));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(v2us, x[i] & 0x7fff7fff));
       }
+      auto hand = [&](auto two) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = 2 * j + (lane >> 5);
+          const v4i x = qraw[j];
+          *reinterpret_cast<uint2*>(my + 256 * r + 16 * (((lane & 31) >> 1) ^ (r & 15)) + 8 * (lane & 1)) =
+              make_uint2(two(x.x, x.y), two(x.z, x.w));
+        }
+      };
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(max(big.x, big.y) > 0x43e0) == 0, 1))
+        hand([](int a, int b) {
+          v2s r = {0, 0};
+          r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(v2bf, a), 1.f, false);
+          return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(v2bf, b), 1.f, true));
+        });
+      else
+        hand([](int a, int b) {
+          return f2e4m3x2_nan(bf_lo((uint32_t)a), bf_hi((uint32_t)a)) | (f2e4m3x2_nan(bf_lo((uint32_t)b), bf_hi((uint32_t)b)) << 16);
+        });
     }
     const uint32_t k0 = lds_at(my) + ka;
 #pragma unroll
@@ -401,7 +423,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     ahead.key0 += SET;
     ent = entries(ahead);
   }
-  wait_vm0();
   for (int half = 0;;) {
     uint8_t* const mem = X + (half ^ 1) * kSet;
     if (cur.n > 0) {
@@ -516,6 +537,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     if (nxt.n == 0) break;
     d.q8 ? ask(nxt, true) : ask(nxt, false);
+    wait_vm0();  // (the first item's first set of keys, too)
     answer(mem);
     cur = nxt;
     nxt = next();
@@ -587,7 +609,7 @@ __device__ __forceinline__ uint2 put_nans(uint2 v, uint32_t n) {
 // (tile, 32 rows, 32 dims) at a time; few partials: wave a has the lanes' a-th four dims of all of them; more: wave w has
 // partials w, w + 4, .. and the waves' sums meet in LDS.
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
-  __shared__ int list[1024];
+  __shared__ int4 list[1024];  // request, 2 tile + head, partials, share
   __shared__ int counts[4], nan_flags[4];
   __shared__ v4f part[4][4][64];
   __shared__ float pml[4][2][64];
@@ -607,7 +629,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
       at += w < wave ? counts[w] : 0;
       have += counts[w];
     }
-    if (is) list[at] = c0 + tid;
+    if (is) list[at] = int4{c.x, c.y, c.z - (c0 + tid) + 1, c0 + tid};
     __syncthreads();
   }
   if (blockIdx.x == 0 && tid == 0) d.epoch[0] += 1;
@@ -615,9 +637,8 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
   __syncthreads();
   const bool any_nan = uni(nan_flags[0] | nan_flags[1] | nan_flags[2] | nan_flags[3]) != 0;
   for (int unit = blockIdx.x; unit < have * 64; unit += gridDim.x) {
-    const int share = uni(list[unit >> 6]), rw = (unit >> 3) & 7, dt = unit & 7;
-    const int4 c = d.cuts[share];
-    const int b = uni(c.x), tile = uni(c.y) >> 1, h = uni(c.y) & 1, n = uni(c.z) - share + 1;
+    const int4 c = list[unit >> 6];
+    const int rw = (unit >> 3) & 7, dt = unit & 7, b = uni(c.x), tile = uni(c.y) >> 1, h = uni(c.y) & 1, n = uni(c.z), share = uni(c.w);
     const Req q = req_of(d, b);
     const int tok = tile * ck_tile_tok(q.r.n) + 4 * rw + (col >> 3), head = h * kCG + (col & 7);
     if ((!ck_wide(q.r.n) && rw >= 2) || uni(tok) >= q.r.n) continue;

@@ -7,7 +7,7 @@
 // waves).  The tiles of all requests, head by head, lie on a line; a tile weighs its steps and kTileOvh (what starting
 // and ending one costs beside its steps), half before and half behind them.  The line is cut into equal shares, a share a
 // workgroup, so that a share holds the end of a tile, whole tiles and the start of another.  A step belongs to the share
-// that its place lies in; a cut tile leaves a partial in each share that has steps of it.
+// that its place lies in, cuts close to a wide tile's ends apart; a cut tile leaves a partial in each share that has steps of it.
 #pragma once
 #include <stdint.h>
 
@@ -16,7 +16,7 @@ namespace q36 {
 constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 32, kNarrowKeys = 128;
 constexpr int kTileOvh = 8;
 constexpr int kNarrowCost = 2;  // what a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16
-constexpr int kLeastShare = 4;  // a share is no shorter (but for a line shorter than this)
+constexpr int kLeastShare = 2;  // a share is no shorter than a narrow step (five tokens over 300 keys: 20.0 us; 4: 21.5, 8: 22.7, 20: 32.8)
 
 struct ChunkReq {
   int n, nk;  // new tokens, keys (the new ones included)
@@ -81,6 +81,18 @@ __host__ __device__ __forceinline__ int ck_share_len(int total, int G) {
 }
 __host__ __device__ __forceinline__ int ck_shares(int total, int len) { return (total + len - 1) / len; }
 
+// A cut of a wide tile costs some ten steps: its 256 KB leave and come back, and its queries are read twice.  So one that
+// falls within kSnap steps of the tile's end goes to that end.  (8 prompts of 120 .. 1000 tokens: 0: 60.4 us, 2: 59.6,
+// 4: 56.3, 6: 59.1; 16 of 64 .. 2000: 133, 126 at 3 .. 6, 129 at 8.  A narrow tile's cut costs little: five tokens
+// over 300 keys: 21.6 against 19.7.)  A tile's cuts lie behind step ck_lo and before ck_hi.
+constexpr int kSnap = 4;
+__host__ __device__ __forceinline__ int ck_lo(int steps, int cost) {
+  return cost > 1 ? 0 : kSnap < (steps - 1) / 2 ? kSnap : (steps - 1) / 2;
+}
+__host__ __device__ __forceinline__ int ck_hi(int steps, int cost) {
+  const int lo = ck_lo(steps, cost);
+  return cost > 1 ? steps : steps - kSnap > lo + 1 ? steps - kSnap : lo + 1;
+}
 // The steps [st0, st0 + nst) of a tile at `off` on the line that the share [x0, x1) has; first, last: whether they hold the
 // tile's first and last step.  A tile without a step is its start's share's, whole.  nst < 0: the share has none.
 struct ChunkRun {
@@ -90,13 +102,18 @@ struct ChunkRun {
 __host__ __device__ __forceinline__ ChunkRun ck_run(int steps, int cost, int off, int x0, int x1) {
   if (steps == 0) return ChunkRun{0, off >= x0 && off < x1 ? 0 : -1, true, true};
   const int at = off + kTileOvh / 2;  // of its first step
-  const int a = x0 > at ? (x0 - at + cost - 1) / cost : 0, b = x1 > at ? (x1 - at + cost - 1) / cost : 0, e = b < steps ? b : steps;
+  const int lo = ck_lo(steps, cost), hi = ck_hi(steps, cost);
+  int a = x0 > at ? (x0 - at + cost - 1) / cost : 0, e = x1 > at ? (x1 - at + cost - 1) / cost : 0;
+  a = a <= lo ? 0 : a >= hi ? steps : a;
+  e = e <= lo ? 0 : e >= hi ? steps : e;
   return ChunkRun{a, e > a ? e - a : -1, a == 0, e == steps};
 }
 // the shares that the first and the last step of a tile at `off` lie in
-__host__ __device__ __forceinline__ int ck_first_share(int off, int len) { return (off + kTileOvh / 2) / len; }
+__host__ __device__ __forceinline__ int ck_first_share(int steps, int cost, int off, int len) {
+  return (off + kTileOvh / 2 + ck_lo(steps, cost) * cost) / len;
+}
 __host__ __device__ __forceinline__ int ck_last_share(int steps, int cost, int off, int len) {
-  return (off + kTileOvh / 2 + (steps - 1) * cost) / len;
+  return (off + kTileOvh / 2 + (ck_hi(steps, cost) - 1) * cost) / len;
 }
 // The partial of share w: one for a tile that ends here or goes on through, one for a tile that starts here.
 __host__ __device__ __forceinline__ int ck_slot(int w, bool first) { return 2 * w + (first ? 1 : 0); }

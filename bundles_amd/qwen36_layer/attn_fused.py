@@ -287,7 +287,7 @@ class ChunkWorkspace:
     the same time need one each)."""
 
     def __init__(self, device):
-        self.buf = torch.empty(_lib.lib().q36_attn_chunk_workspace_bytes(), dtype=torch.uint8, device=device)
+        self.buf = torch.zeros(_lib.lib().q36_attn_chunk_workspace_bytes(), dtype=torch.uint8, device=device)
 
 
 def attn_chunk(q, k_cache, v_cache, page_table, seqlens, qsl, scale: float, ws: ChunkWorkspace, page_size: int = 1,

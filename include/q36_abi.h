@@ -557,8 +557,11 @@ int q36_attn_front(const q36_attn_front_args* a, q36_stream_t stream);
  * qsl[0] .. qsl[B] are left as they were.  What a row does not see, NaN included, does not reach it.
  * Whatever the device data hold, every access stays inside the buffers: rows outside T, keys past the page table's
  * pt_stride * page_size and slots outside the cache are clamped.
- * HQ = 16, HKV = 2, D = 256; T <= 2^20, B <= 65535; q, out and caches 16-byte, workspace 256-byte aligned.
- * Workspace: q36_attn_chunk_workspace_bytes(), whatever the call's sizes (partials of the cut tiles). */
+ * HQ = 16, HKV = 2, D = 256; T <= 2^20, B <= 65535, 0 < scale <= 1e6; q, out and caches 16-byte, workspace 256-byte
+ * aligned.  Sizes whose worst split could weigh 2^30 steps (T / 32 + 2 B tiles over the tables' keys) are refused.
+ * Workspace: q36_attn_chunk_workspace_bytes(), whatever the call's sizes (partials of the cut tiles, and a count of the
+ * calls it has served): filled with zeros once, then left to the calls, one after another; calls that may run at the same
+ * time (streams, graphs) need one each. */
 typedef struct q36_chunk_args {
   int32_t B, T, HQ, HKV, D, page_size, pt_stride, q_e4m3;
   int64_t num_slots;

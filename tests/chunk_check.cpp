@@ -78,7 +78,7 @@ static const char* walk(const std::vector<ChunkReq>& req, int G) {
             const int slot = ck_slot(w, r.first);
             if (owner[slot] >= 0) return "a slot written twice";
             owner[slot] = ((long)(2 * b + h) << 32) + tile;
-            if (ck_first_share(off, len) != (r.first ? w : ck_first_share(off, len)) || (!r.first && ck_first_share(off, len) >= w))
+            if (ck_first_share(steps, cost, off, len) != (r.first ? w : ck_first_share(steps, cost, off, len)) || (!r.first && ck_first_share(steps, cost, off, len) >= w))
               return "a tile's first share is not where it starts";
             if (r.first) cut[w] = Cut{b, h, tile, ck_last_share(steps, cost, off, len)};
           }
