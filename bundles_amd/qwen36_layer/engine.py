@@ -51,6 +51,19 @@ class KvView:
     draft: int = 4
 
 
+@dataclass
+class ChunkView:
+    """The attention layer's e4m3 KV cache for a batch of prompt chunks (q36_attn_chunk), any number of new tokens a
+    request; paging.plan_pages makes such numbers from the batch's lengths."""
+    k_cache: torch.Tensor      # uint8 (e4m3 codes) [slots, 2, 256]
+    v_cache: torch.Tensor
+    page_table: torch.Tensor   # int32 [B, stride]: the page of keys j * page_size ..
+    seqlens: torch.Tensor      # int32 [B]: key positions including the new tokens
+    qsl: torch.Tensor          # int32 [B + 1] first row of each request
+    out_loc: torch.Tensor      # int64 [rows]: the new tokens' slots (outside the cache: not written)
+    page_size: int = 1
+
+
 class EngineView:
     """The engine lookups the layer node makes; every method may return None (run stock)."""
 
@@ -58,6 +71,10 @@ class EngineView:
         return None
 
     def kv_view(self, layer_id: int, forward_batch) -> KvView | None:
+        return None
+
+    def chunk_view(self, layer_id: int, forward_batch) -> ChunkView | None:
+        """A batch that kv_view does not serve, as prompt chunks (an engine that wants its prompts here says so)."""
         return None
 
 

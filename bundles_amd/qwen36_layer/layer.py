@@ -14,7 +14,8 @@ served module and its submodule dict untouched.  This node does the same with li
                     (W8A16, L/layer.py:13-17, L/dense8_store.py:8-13), wider ones through the e4m3 copies.
   attention      <- attn_fused.install (L/attn_fused.py:213-273): the q/gate/k/v projection with the q/k
                     norm, partial RoPE and the e4m3 KV write, the verify attention over the KV cache, and
-                    the gated o_proj, on a verify batch; stock otherwise.
+                    the gated o_proj, on a verify batch; where the engine hands a prompt batch over
+                    (chunk_view), the same steps over prompt chunks; stock otherwise.
 The row-batch rule is the reference's (L/layer.py:174-189): forward_mode.is_decode() or
 is_target_verify(); every other call, including a prefill chunk whose first row sits at position 0,
 goes to stock code.  (The libq36 MoE treats position-0 rows as padding, so it must never see prefill.)
@@ -33,12 +34,13 @@ import torch
 from . import attn_fused, gdn_fused, moe
 from .engine import EngineView, SglangView
 from .formats import quant_dense8, tile_w16
-from .glue import LinearWorkspace, dense8_linear, fp8_linear, linear_rows, prepare_fp8_weight
+from .glue import Fp8Weight, LinearWorkspace, dense8_linear, fp8_linear, linear_rows, prepare_fp8_weight
 
 HIDDEN, EXPERTS, INTERMEDIATE, TOPK = 2048, 512, 512, 10
 MAX_TOKENS = moe.MAX_TOKENS
 GDN_QKV, GDN_Z, GDN_HV = gdn_fused.QKV_DIM, gdn_fused.N_V_HEADS * gdn_fused.HEAD_V, gdn_fused.N_V_HEADS
 PROJ_IN = 4096
+MAX_CHUNK_ROWS = 65535  # of a batch of prompt chunks (the projections' limit)
 DENSE8_ROWS = 32  # the reference's DENSE8 row limit for the recurrent block's projections
 
 
@@ -93,6 +95,18 @@ class _Scratch:
         self.lin4096 = LinearWorkspace(rows, PROJ_IN, device)
         self.attn = attn_fused.Workspace(rows, device)
         self.decode = attn_fused.DecodeWorkspace(rows, device)
+
+
+class _ChunkScratch(_Scratch):
+    """The same for prompt chunks."""
+
+    _by_device: dict = {}
+
+    def __init__(self, device, rows: int):
+        self.rows = rows
+        self.lin2048 = LinearWorkspace(rows, HIDDEN, device)
+        self.attn = attn_fused.Workspace(rows, device)
+        self.chunk = attn_fused.ChunkWorkspace(device)
 
 
 # ---- MoE ---------------------------------------------------------------------------------------------
@@ -284,10 +298,20 @@ def attn_layer_refusal(module) -> str | None:
     return None
 
 
+def _rope_axes(rot):
+    """The axes of a rotary embedding's positions, where it has several and these are served."""
+    sections = getattr(rot, "mrope_section", None)
+    try:
+        return attn_fused.RopeAxes(sections, bool(getattr(rot, "mrope_interleaved", False))) if sections else None
+    except ValueError:
+        return None
+
+
 class _AttnMixer:
     """The gated attention mixer's target-verify step: q36_attn_proj (q/gate/k/v, q/k norm, partial
     RoPE, the new e4m3 K/V rows written into the engine's KV cache at out_cache_loc), q36_attn_decode
-    over that cache, and q36_attn_oproj (sigmoid gate, o_proj)."""
+    over that cache, and q36_attn_oproj (sigmoid gate, o_proj).  Prompt chunks, where the engine hands them
+    over (chunk_view): the same projection by q36_fp8_linear, q36_attn_front, q36_attn_chunk, q36_attn_oproj."""
 
     def __init__(self, module, replica, engine: EngineView, max_tokens: int):
         w_qkv, w_o = module.qkv_proj.weight, module.o_proj.weight
@@ -316,6 +340,27 @@ class _AttnMixer:
             self.cos_sin = rot.cos_sin_cache.to(torch.float32).contiguous()
             qg = nq * 2 * d
             self.w = attn_fused.prepare_weights(w_qkv[:qg], w_qkv[qg:qg + nkv * d], w_qkv[qg + nkv * d:], w_o)
+        self.w_qkv = Fp8Weight(self.w.wqkv, self.w.sqkv, self.w.wqkv_p, attn_fused.QKV_ROWS)
+        # rotary positions of several axes, where the model has them: the frequencies' axes by sections
+        self.axes = _rope_axes(rot)
+
+    def _chunk(self, positions, hidden_states, forward_batch):
+        x = hidden_states
+        rows = x.shape[0] if isinstance(x, torch.Tensor) and x.dim() == 2 else 0
+        axes = self.axes if isinstance(positions, torch.Tensor) and positions.dim() == 2 else None
+        view = getattr(self.engine, "chunk_view", None)
+        ck = (view(self.layer_id, forward_batch)
+              if view is not None and self.refusal is None and 0 < rows <= MAX_CHUNK_ROWS and x.dtype == torch.bfloat16
+              and tuple(positions.shape) == ((rows,) if axes is None else (axes.axes, rows)) else None)
+        if ck is None:
+            return self.stock(self.replica, positions, hidden_states, forward_batch)
+        sc = _ChunkScratch.get(x.device, rows)
+        qkv = fp8_linear(x.contiguous(), self.w_qkv, sc.lin2048)
+        q, gate = attn_fused.attn_front(qkv, self.q_norm_w, self.k_norm_w, self.eps, self.cos_sin, positions.to(torch.int32).contiguous(),
+                                        cache=(ck.k_cache, ck.v_cache, ck.out_loc), axes=axes, q_dtype=torch.uint8)
+        o = torch.zeros(q.shape, dtype=torch.bfloat16, device=x.device)  # (rows of no request stay zero)
+        attn_fused.attn_chunk(q, ck.k_cache, ck.v_cache, ck.page_table, ck.seqlens, ck.qsl, self.scale, sc.chunk, ck.page_size, out=o)
+        return attn_fused.attn_oproj(o.view(rows, -1), gate.view(rows, -1), self.w, sc.attn)
 
     def __call__(self, positions, hidden_states, forward_batch):
         x = hidden_states
@@ -324,7 +369,7 @@ class _AttnMixer:
               if self.refusal is None and verify_batch(forward_batch) and 0 < rows <= self.max_tokens
               and x.dtype == torch.bfloat16 else None)
         if kv is None or rows % kv.draft or not 1 <= kv.draft <= 4:
-            return self.stock(self.replica, positions, hidden_states, forward_batch)
+            return self._chunk(positions, hidden_states, forward_batch)
         sc = _Scratch.get(x.device, rows)
         pos = positions.to(torch.int32).contiguous()
         p = attn_fused.attn_proj(x.contiguous(), self.w, self.q_norm_w, self.k_norm_w, self.eps, self.cos_sin, pos,

@@ -180,3 +180,49 @@ def test_axes_that_are_none(sections, woven):
     with pytest.raises(ValueError, match="RopeAxes"):
         attn_fused.RopeAxes(sections, woven)
     assert attn_fused.RopeAxes((8, 8, 8, 8), True).map < 0  # the last pair's axis sets the top bits
+
+
+@pytest.mark.parametrize("bad", [dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2e6),
+                                 dict(T=1 << 20, B=65535, pt_stride=(1 << 27) // 16)], ids=str)
+def test_the_library_refuses_scales_and_too_long_lines(L, bad):
+    from bundles_amd import _lib
+    a = _lib.ChunkArgs()
+    for k, v in {**CHUNK, **bad}.items():
+        setattr(a, k, v)
+    assert L.q36_attn_chunk(C.byref(a), None) == _lib.Q36_EINVAL
+    assert L.q36_last_error().startswith(b"q36_attn_chunk")
+
+
+def test_the_layer_node_asks_the_engine_for_prompt_batches(monkeypatch):
+    """Which batches the attention mixer hands to the chunk path: bf16 rows that its positions fit, of a layer that is
+    served, where the engine has a chunk_view that takes them; stock's are the others."""
+    import types
+    from bundles_amd.qwen36_layer import attn_fused, engine, layer
+    m = object.__new__(layer._AttnMixer)
+    asked = []
+    view = engine.EngineView()
+    view.chunk_view = lambda layer_id, fb: asked.append(layer_id)
+    m.engine, m.refusal, m.layer_id, m.replica, m.axes, m.max_tokens = view, None, 7, object(), attn_fused.RopeAxes((11, 11, 10)), 8
+    m.stock = lambda replica, positions, x, fb: "stock"
+    x, fb = z(5, 2048, dtype=BF), types.SimpleNamespace()
+    for positions, hidden, n in ((z(5), x, 1), (z(3, 5), x, 2), (z(4), x, 2), (z(2, 5), x, 2), (z(3, 4), x, 2), (z(5), x.float(), 2),
+                                 (z(0), x[:0], 2), (z(5, dtype=I64), x, 3)):
+        assert m(positions, hidden, fb) == "stock" and asked == [7] * n
+    m.axes = None
+    assert m(z(3, 5), x, fb) == "stock" and len(asked) == 3
+    m.refusal = "a logit cap"
+    assert m(z(5), x, fb) == "stock" and len(asked) == 3
+    m.refusal, m.engine = None, types.SimpleNamespace(kv_view=lambda *a: None)
+    assert m(z(5), x, fb) == "stock"
+    assert engine.EngineView().chunk_view(7, fb) is None and engine.SglangView().chunk_view(7, fb) is None
+
+
+def test_rope_axes_of_a_rotary_embedding():
+    import types
+    from bundles_amd.qwen36_layer import layer
+    assert layer._rope_axes(types.SimpleNamespace()) is None
+    assert layer._rope_axes(types.SimpleNamespace(mrope_section=None)) is None
+    assert layer._rope_axes(types.SimpleNamespace(mrope_section=[16, 24, 24])) is None  # not 32 pairs: such positions are stock's
+    r = layer._rope_axes(types.SimpleNamespace(mrope_section=[11, 11, 10], mrope_interleaved=True))
+    assert r.axes == 3 and r.axis_of[:4] == [0, 1, 2, 0]
+    assert layer._rope_axes(types.SimpleNamespace(mrope_section=[11, 11, 10])).axis_of[:4] == [0, 0, 0, 0]
