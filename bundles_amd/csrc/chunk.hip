@@ -514,7 +514,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 const int row = 4 * j + (lane >> 4);
                 const v4i v = *reinterpret_cast<const v4i*>(my + row * 256 + 16 * ((lane & 15) ^ (row & 15)));
                 if (tok0 + (row >> 3) < cur.n)
-                  *reinterpret_cast<v4i*>(rows + ((size_t)(row >> 3) * kCHQ + (row & 7)) * kCD + 128 * q + 8 * (lane & 15)) = v;
+                  __builtin_nontemporal_store(v, reinterpret_cast<v4i*>(rows + ((size_t)(row >> 3) * kCHQ + (row & 7)) * kCD + 128 * q + 8 * (lane & 15)));
               }
             }
           };
@@ -605,111 +605,122 @@ __device__ __forceinline__ uint2 put_nans(uint2 v, uint32_t n) {
   return make_uint2((n & 0x80 ? (v.x & 0xffff0000u) | q : v.x) | (n & 0x8000 ? 0xffff0000u : 0), (n & 0x800000 ? (v.y & 0xffff0000u) | q : v.y) | (n & 0x80000000u ? 0xffff0000u : 0));
 }
 
-// The cut tiles: out = bf16(sum_p exp2(m_p - M) o_p / sum_p exp2(m_p - M) l_p) over a tile's partials p.  A workgroup takes one
-// (tile, 32 rows, 32 dims) at a time; few partials: wave a has the lanes' a-th four dims of all of them; more: wave w has
-// partials w, w + 4, .. and the waves' sums meet in LDS.
+// The cut tiles: out = bf16(sum_p exp2(m_p - M) o_p / sum_p exp2(m_p - M) l_p) over a tile's partials p.  Up to four partials:
+// a workgroup takes 32 rows and 64 dims at a time, wave a the lanes' a-th four dims of each 32, every partial's loads in
+// flight together.  More: 32 rows and 8 dims, wave w has partials w, w + 4, .., eight at a time, and the waves' sums meet in LDS.
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
-  __shared__ int4 list[1024];  // request, 2 tile + head, partials, share
-  __shared__ int counts[4], nan_flags[4];
-  __shared__ v4f part[4][4][64];
+  __shared__ uint2 list[1024];  // request and partials (16 bits each), 2 tile + head (20 bits) and share: few partials from the front, many from the back
+  __shared__ int counts[4][2], nan_flags[4];
+  __shared__ v4f part[4][64];
   __shared__ float pml[4][2][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), col = lane & 31, g = lane >> 5;
   // the shares that leave a cut tile, in order
-  int have = 0;
+  int few = 0, many = 0;
   uint64_t nans = 0;
   for (int c0 = 0; c0 < G; c0 += 256) {
     const int4 c = c0 + tid < G ? d.cuts[c0 + tid] : int4{-1, 0, 0, 0};
-    const bool is = c.x >= 0;
+    const int n = c.x >= 0 ? c.z - (c0 + tid) + 1 : 0;
     nans |= __builtin_amdgcn_ballot_w64(c.w != 0);
-    const uint64_t bits = __builtin_amdgcn_ballot_w64(is);
-    if (lane == 0) counts[wave] = __builtin_popcountll(bits);
+    const uint64_t fb = __builtin_amdgcn_ballot_w64(n > 0 && n <= 4), mb = __builtin_amdgcn_ballot_w64(n > 4), below = (1ull << lane) - 1;
+    if (lane == 0) counts[wave][0] = __builtin_popcountll(fb), counts[wave][1] = __builtin_popcountll(mb);
     __syncthreads();
-    int at = have + __builtin_popcountll(bits & ((1ull << lane) - 1));
+    int fat = few + __builtin_popcountll(fb & below), mat = many + __builtin_popcountll(mb & below);
     for (int w = 0; w < 4; ++w) {
-      at += w < wave ? counts[w] : 0;
-      have += counts[w];
+      fat += w < wave ? counts[w][0] : 0, mat += w < wave ? counts[w][1] : 0;
+      few += counts[w][0], many += counts[w][1];
     }
-    if (is) list[at] = int4{c.x, c.y, c.z - (c0 + tid) + 1, c0 + tid};
+    if (n > 0) list[n <= 4 ? fat : 1023 - mat] = make_uint2((uint32_t)c.x << 16 | (uint32_t)n, (uint32_t)c.y << 12 | (uint32_t)(c0 + tid));
     __syncthreads();
   }
   if (blockIdx.x == 0 && tid == 0) d.epoch[0] += 1;
   if (lane == 0) nan_flags[wave] = nans != 0;
   __syncthreads();
   const bool any_nan = uni(nan_flags[0] | nan_flags[1] | nan_flags[2] | nan_flags[3]) != 0;
-  for (int unit = blockIdx.x; unit < have * 64; unit += gridDim.x) {
-    const int4 c = list[unit >> 6];
-    const int rw = (unit >> 3) & 7, dt = unit & 7, b = uni(c.x), tile = uni(c.y) >> 1, h = uni(c.y) & 1, n = uni(c.z), share = uni(c.w);
+  few = uni(few), many = uni(many);
+  for (int unit = blockIdx.x; unit < few * 32 + many * 256; unit += gridDim.x) {
+    const int mu = unit - few * 32;
+    const uint2 c = list[mu < 0 ? unit >> 5 : 1023 - (mu >> 8)];
+    const int rw = mu < 0 ? (unit >> 2) & 7 : (mu >> 5) & 7, b = uni((int)(c.x >> 16)), n = uni((int)(c.x & 0xffffu));
+    const int tile = uni((int)(c.y >> 13)), h = uni((int)(c.y >> 12)) & 1, share = uni((int)(c.y & 0xfffu));
     const Req q = req_of(d, b);
     const int tok = tile * ck_tile_tok(q.r.n) + 4 * rw + (col >> 3), head = h * kCG + (col & 7);
     if ((!ck_wide(q.r.n) && rw >= 2) || uni(tok) >= q.r.n) continue;
     const bool row_ok = tok < q.r.n;
-    uint16_t* const dst = d.out + ((size_t)(q.t0 + tok) * kCHQ + head) * kCD + 32 * dt + 4 * g;
     auto ml = [&](int p, int what) { return d.ws_ml[(size_t)ck_slot(share + p, p == 0) * kSlotML + rw * 64 + 32 * what + col]; };
-    auto po = [&](int p, int a) {
+    auto po = [&](int p, int dt, int a) {
       return *reinterpret_cast<const v4f*>(d.ws_o + (size_t)ck_slot(share + p, p == 0) * kSlotF + ((rw * 8 + dt) * 4 + a) * 256 + lane * 4);
     };
-    auto store = [&](v4f v, float il) {
+    auto store = [&](int dt, int a, v4f v, float L) {
+      const float il = L > 0.f ? 1.f / L : L;
+      const int dim = 32 * dt + 8 * a + 4 * g;
       uint2 w = make_uint2(pack_bf2_hw(v[0] * il, v[1] * il), pack_bf2_hw(v[2] * il, v[3] * il));
-      if (__builtin_expect(any_nan, 0)) w = put_nans(w, border_nans(d, b, q.r, h, tok, 32 * dt + 4 * g + 8 * wave));
-      *reinterpret_cast<uint2*>(dst + 8 * wave) = w;
+      if (__builtin_expect(any_nan, 0)) w = put_nans(w, border_nans(d, b, q.r, h, tok, dim));
+      *reinterpret_cast<uint2*>(d.out + ((size_t)(q.t0 + tok) * kCHQ + head) * kCD + dim) = w;
     };
-    if (n <= 4) {
+    if (mu < 0) {
+      const int dt = 2 * (unit & 3);
       float mp[4], lp[4], M = -1e30f, L = 0.f;
-      v4f v[4], s = {0.f, 0.f, 0.f, 0.f};
+      v4f v[4][2], s[2] = {};
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const int pc = min(p, n - 1);
-        mp[p] = ml(pc, 0), lp[p] = ml(pc, 1), v[p] = po(pc, wave);
+        mp[p] = -1e30f, lp[p] = 0.f;
+        if (p < n) mp[p] = ml(p, 0), lp[p] = ml(p, 1), v[p][0] = po(p, dt, wave), v[p][1] = po(p, dt + 1, wave);
       }
 #pragma unroll
       for (int p = 0; p < 4; ++p) M = fmaxf(M, mp[p]);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const float w = p < n ? __builtin_amdgcn_exp2f(mp[p] - M) : 0.f;
         if (p < n) {
+          const float w = __builtin_amdgcn_exp2f(mp[p] - M);
           L += w * lp[p];
-          s += w * v[p];
+          s[0] += w * v[p][0];
+          s[1] += w * v[p][1];
         }
       }
-      const float il = L > 0.f ? 1.f / L : L;
-      if (row_ok) store(s, il);
+      if (row_ok) store(dt, wave, s[0], L), store(dt + 1, wave, s[1], L);
       continue;
     }
+    const int dt = (mu >> 2) & 7, a = mu & 3;
     float M = -1e30f, L = 0.f;
-    v4f s[4] = {};
-    for (int p = wave; p < n; p += 8) {
-      const int p2 = min(p + 4, n - 1);
-      const float m0 = ml(p, 0), l0 = ml(p, 1), m1 = p + 4 < n ? ml(p2, 0) : -1e30f, l1 = p + 4 < n ? ml(p2, 1) : 0.f;
-      v4f v0[4], v1[4];
+    v4f s = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = wave; p0 < n; p0 += 32) {
+      float mp[8], lp[8], mn = M;
+      v4f v[8];
 #pragma unroll
-      for (int a = 0; a < 4; ++a) v0[a] = po(p, a), v1[a] = po(p2, a);
-      const float mn = fmaxf(M, fmaxf(m0, m1)), f = __builtin_amdgcn_exp2f(M - mn), w0 = __builtin_amdgcn_exp2f(m0 - mn);
-      M = mn;
-      L = L * f + w0 * l0;
+      for (int i = 0; i < 8; ++i) {
+        const int p = min(p0 + 4 * i, n - 1);
+        mp[i] = ml(p, 0), lp[i] = ml(p, 1), v[i] = po(p, dt, a);
+      }
 #pragma unroll
-      for (int a = 0; a < 4; ++a) s[a] = s[a] * f + w0 * v0[a];
-      if (p + 4 < n) {
-        const float w1 = __builtin_amdgcn_exp2f(m1 - mn);
-        L += w1 * l1;
+      for (int i = 0; i < 8; ++i) {
+        if (p0 + 4 * i >= n) mp[i] = -INFINITY;  // (taken already, or another wave's: weight 0)
+        mn = fmaxf(mn, mp[i]);
+      }
+      const float f = __builtin_amdgcn_exp2f(M - mn);
+      M = mn, L *= f, s *= f;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) s[a] += w1 * v1[a];
+      for (int i = 0; i < 8; ++i) {
+        if (p0 + 4 * i < n) {
+          const float w = __builtin_amdgcn_exp2f(mp[i] - mn);
+          L += w * lp[i], s += w * v[i];
+        }
       }
     }
     pml[wave][0][lane] = M, pml[wave][1][lane] = L;
-#pragma unroll
-    for (int a = 0; a < 4; ++a) part[wave][a][lane] = s[a];
+    part[wave][lane] = s;
     __syncthreads();
-    const float Ma = fmaxf(fmaxf(pml[0][0][lane], pml[1][0][lane]), fmaxf(pml[2][0][lane], pml[3][0][lane]));
-    float La = 0.f;
-    v4f t = {0.f, 0.f, 0.f, 0.f};
+    if (wave == 0) {
+      const float Ma = fmaxf(fmaxf(pml[0][0][lane], pml[1][0][lane]), fmaxf(pml[2][0][lane], pml[3][0][lane]));
+      float La = 0.f;
+      v4f t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(pml[w][0][lane] - Ma);
-      La += f * pml[w][1][lane];
-      t += f * part[w][wave][lane];
+      for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(pml[w][0][lane] - Ma);
+        La += f * pml[w][1][lane];
+        t += f * part[w][lane];
+      }
+      if (row_ok) store(dt, a, t, La);
     }
-    const float il = La > 0.f ? 1.f / La : La;
-    if (row_ok) store(t, il);
     __syncthreads();
   }
   if (__builtin_expect(!any_nan, 1)) return;
