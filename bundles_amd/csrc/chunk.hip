@@ -4,6 +4,23 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp2(s_j - m),  s_j = log2(e) scale (q . k_j),  m = max_j s_j
 //
 // (The reference re-pages the cache into 128-row pages and calls a library there, L/attn_fused.py:127-210.)
+//
+// Rounded: q to e4m3 (as attn_decode takes it), the weights p_j to f16 for the product with v (v is e4m3, exact in f16;
+// 2^-11 a weight, where e4m3 weights would lose 2^-4), the outputs to bf16.  Scores, maxima, weight sums and outputs: fp32.
+//
+// Bounds.  Long chunks: the matrix units, half the products at the e4m3 rate and half at the f16 one: 289 us for 8192 tokens
+// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 405 measured, 1.36 PFLOP/s.  A step of
+// 32 keys takes a workgroup 1.45 us (2.9 K cycles), of which the matrix units are busy half and the vector units (scores to
+// weights: 16 exponentials, maxima and sums a lane, and the values' widening, all beside 2 waves a SIMD) three fifths;
+// prefetched keys, wave priorities and other bank layouts moved it by under 1 %.  Short calls: the latency of one pass:
+// lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second launch 4: 19 us for five tokens over 300
+// keys.  Between: cut tiles, 256 KB a partial out of and back into the Infinity Cache (7 TB/s over the chip).
+//
+// Why so.  256 rows a workgroup: one pass over a tile's keys feeds eight waves from LDS (a wave alone would need four times
+// the L2 rate).  LDS filled by copies past the registers: o holds 128 of a lane's 256 and q 32.  V^T by the transposing LDS
+// read, P^T in the registers that S^T left it in: no shuffle between the products.  The running maximum lazily: o is scaled
+// in the rare step in which a row has grown past 2^8 times (kLazyC).  Equal shares of one line: a call of any mix of lengths
+// ends everywhere at once.
 #include <math.h>
 
 #include <algorithm>
@@ -76,7 +93,9 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7
 constexpr int kBlk = 2 * kCST * kCD;  // 32 keys in LDS: their K rows, then their V rows
 constexpr int kSet = 4 * kBlk;
 constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a partial
-constexpr float kLazyC = 8.f;  // the outputs are rescaled when a row's maximum has grown by 2^8 (weights up to 2^8 are exact in f16)
+// The outputs are rescaled when a row's maximum has grown past 2^kLazyC times the one that the weights are relative to (a
+// weight is then at most 2^8, far inside f16).  8192 tokens at 0, 4, 8, 11, 14: 479, 440, 434, 434, 434 us.
+constexpr float kLazyC = 8.f;
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8)); }
@@ -222,7 +241,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const ChunkRun run = ck_run(steps, cost, coff, x0, x1);
       if (run.nst >= 0) {
         const bool whole = run.first && run.last;
-        it = Item{cb, ct0, cr.n, cr.nk, ch, ctile * ck_tile_tok(cr.n), max(ck_keys(cr, ctile) - 1, 0), run.st0 * ks, (run.st0 + run.nst) * ks,
+        it = Item{cb, ct0, cr.n, cr.nk, ch, ctile * kWideTok, max(ck_keys(cr, ctile) - 1, 0), run.st0 * ks, (run.st0 + run.nst) * ks,
                   whole ? -1 : ck_slot(share, run.first), run.first && !whole ? ck_last_share(steps, cost, coff, len) : -1,
                   run.last && !whole && ck_first_share(steps, cost, coff, len) == share - 1};
       }
@@ -433,7 +452,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int tok0 = first_tok(cur), rw = wide ? wave : wave & 1;
       const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5;
       // A wide tile that the next share ends, most likely long ago, with its first run: where that partial is there, in this
-      // XCD's L2, the two are joined here, by the combine kernel's arithmetic; else the combine kernel does it.
+      // XCD's L2, the two are joined here, by the combine kernel's arithmetic; else the combine kernel does it.  (With and
+      // without: 8192 tokens 434, 451 us, 16 prompts of 64 .. 2000 123, 131; four chunks of 200 .. 700 52, 49.)
       bool join = false;
       if (wide && cur.lasts == share + 1) {
         if (tid == 0) joined = __hip_atomic_load(d.flags + share + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
@@ -441,7 +461,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         join = uni(joined) != 0;
       }
       if (join) slot = -1;
-      else if (cur.lasts >= 0) cut = int4{cur.b, 2 * (cur.tok / ck_tile_tok(cur.n)) + cur.h, cur.lasts, 0};
+      else if (cur.lasts >= 0) cut = int4{cur.b, 2 * (cur.tok / kWideTok) + cur.h, cur.lasts, 0};
       float* const wo = d.ws_o + (size_t)(slot < 0 ? 0 : slot) * kSlotF + (size_t)rw * (8 * 4 * 256) + lane * 4;
       float* const wml = d.ws_ml + (size_t)(slot < 0 ? 0 : slot) * kSlotML + rw * 64 + col;
       uint16_t* const rows = d.out + ((size_t)(cur.t0 + tok0) * kCHQ + cur.h * kCG) * kCD;  // row r: token r / 8, head r % 8
@@ -643,7 +663,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
     const int rw = mu < 0 ? (unit >> 2) & 7 : (mu >> 5) & 7, b = uni((int)(c.x >> 16)), n = uni((int)(c.x & 0xffffu));
     const int tile = uni((int)(c.y >> 13)), h = uni((int)(c.y >> 12)) & 1, share = uni((int)(c.y & 0xfffu));
     const Req q = req_of(d, b);
-    const int tok = tile * ck_tile_tok(q.r.n) + 4 * rw + (col >> 3), head = h * kCG + (col & 7);
+    const int tok = tile * kWideTok + 4 * rw + (col >> 3), head = h * kCG + (col & 7);
     if ((!ck_wide(q.r.n) && rw >= 2) || uni(tok) >= q.r.n) continue;
     const bool row_ok = tok < q.r.n;
     auto ml = [&](int p, int what) { return d.ws_ml[(size_t)ck_slot(share + p, p == 0) * kSlotML + rw * 64 + 32 * what + col]; };

@@ -3,8 +3,8 @@
 //
 // A tile is a run of new tokens of one request with one KV head's 8 query heads; it walks the keys that its last token
 // sees, in steps.  A request of more than kNarrow new tokens is cut into wide tiles (kWideTok tokens, one set of keys for
-// all eight waves, kWideKeys a step), another into narrow ones (kNarrowTok tokens, four sets of keys a step between pairs of
-// waves).  The tiles of all requests, head by head, lie on a line; a tile weighs its steps and kTileOvh (what starting
+// all eight waves, kWideKeys a step), another is one narrow tile (up to kNarrow tokens, four sets of keys a step between
+// pairs of waves).  The tiles of all requests, head by head, lie on a line; a tile weighs its steps and kTileOvh (what starting
 // and ending one costs beside its steps), half before and half behind them.  The line is cut into equal shares, a share a
 // workgroup, so that a share holds the end of a tile, whole tiles and the start of another.  A step belongs to the share
 // that its place lies in, cuts close to a wide tile's ends apart; a cut tile leaves a partial in each share that has steps of it.
@@ -13,22 +13,25 @@
 
 namespace q36 {
 
-constexpr int kNarrow = 16, kWideTok = 32, kNarrowTok = 8, kWideKeys = 32, kNarrowKeys = 128;
+// kNarrow, us a call: 16 requests behind 500 keys, 4 behind 8000.  8 tokens as a narrow tile 21.2, 28.4, as a wide one 21.0,
+// 31.4; 12 tokens as two narrow ones 24.8, 36.1, as a wide one 22.4, 32.8; 16 tokens 27.0, 37.0 against 24.4, 33.8.
+constexpr int kNarrow = 8, kWideTok = 32, kWideKeys = 32, kNarrowKeys = 128;
+// kTileOvh, us a call: eight prompts at 4, 6, 8, 10, 12: 54.7, 55.1, 52.7, 58.1, 57.5; one of 8192: 415, 420, 420, 422, 425;
+// 4 x 12 tokens behind 8000 keys (narrow, two tiles): 40.3, 36.7, 36.1, 36.2, 36.5.
 constexpr int kTileOvh = 8;
-constexpr int kNarrowCost = 2;  // what a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16
-constexpr int kLeastShare = 2;  // a share is no shorter than a narrow step (five tokens over 300 keys: 20.0 us; 4: 21.5, 8: 22.7, 20: 32.8)
+// What a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16.  A batch of 24, single tokens beside chunks,
+// at 1, 2, 3: 66.2, 59.9, 61.4 us.
+constexpr int kNarrowCost = 2;
+constexpr int kLeastShare = kNarrowCost;  // a share is no shorter than a narrow step (five tokens over 300 keys: 20.0 us; 4: 21.5, 8: 22.7, 20: 32.8)
 
 struct ChunkReq {
   int n, nk;  // new tokens, keys (the new ones included)
 };
 __host__ __device__ __forceinline__ bool ck_wide(int n) { return n > kNarrow; }
-__host__ __device__ __forceinline__ int ck_tile_tok(int n) { return ck_wide(n) ? kWideTok : kNarrowTok; }
-__host__ __device__ __forceinline__ int ck_tiles(int n) {
-  return ck_wide(n) ? (n + kWideTok - 1) / kWideTok : (n + kNarrowTok - 1) / kNarrowTok;
-}
+__host__ __device__ __forceinline__ int ck_tiles(int n) { return ck_wide(n) ? (n + kWideTok - 1) / kWideTok : n > 0; }
 // the keys that tile i's last token sees
 __host__ __device__ __forceinline__ int ck_keys(ChunkReq r, int i) {
-  const int end = (i + 1) * ck_tile_tok(r.n), k = r.nk - r.n + (end < r.n ? end : r.n);
+  const int end = (i + 1) * kWideTok, k = r.nk - r.n + (end < r.n ? end : r.n);
   return k > 0 ? k : 0;
 }
 __host__ __device__ __forceinline__ int ck_step_keys(int n) { return ck_wide(n) ? kWideKeys : kNarrowKeys; }
@@ -52,9 +55,8 @@ __host__ __device__ __forceinline__ int ck_before(ChunkReq r, int i) {
     s += ck_steps(r, i - 1) * ck_cost(r.n);
     --full;
   }
-  // the others see nk - n + tokens (k + 1) keys: a step more each (wide), or there is one (narrow)
-  if (ck_wide(r.n)) return s + ck_series(((r.nk - r.n + 31) >> 5) + 1, full);
-  return s + (full > 0 ? ck_steps(r, 0) * kNarrowCost : 0);
+  // the others, of a wide request, see nk - n + kWideTok (k + 1) keys: a step more each
+  return s + ck_series(((r.nk - r.n + 31) >> 5) + 1, full);
 }
 // the weight of a request, both heads (an empty one weighs 1: what passing over it costs)
 __host__ __device__ __forceinline__ int ck_weight(ChunkReq r) { return r.n > 0 ? 2 * ck_before(r, ck_tiles(r.n)) : 1; }
