@@ -625,9 +625,14 @@ __device__ __forceinline__ uint2 put_nans(uint2 v, uint32_t n) {
   return make_uint2((n & 0x80 ? (v.x & 0xffff0000u) | q : v.x) | (n & 0x8000 ? 0xffff0000u : 0), (n & 0x800000 ? (v.y & 0xffff0000u) | q : v.y) | (n & 0x80000000u ? 0xffff0000u : 0));
 }
 
-// The cut tiles: out = bf16(sum_p exp2(m_p - M) o_p / sum_p exp2(m_p - M) l_p) over a tile's partials p.  Up to four partials:
-// a workgroup takes 32 rows and 64 dims at a time, wave a the lanes' a-th four dims of each 32, every partial's loads in
-// flight together.  More: 32 rows and 8 dims, wave w has partials w, w + 4, .., eight at a time, and the waves' sums meet in LDS.
+// The cut tiles: out = bf16(sum_p exp2(m_p - M) o_p / sum_p exp2(m_p - M) l_p) over a tile's partials p.  Up to kFew partials:
+// a workgroup takes 32 rows and 64 dims at a time, wave a the lanes' a-th four dims of each 32, four partials' loads in
+// flight.  More: 32 rows and 8 dims, wave w has partials w, w + 4, .., eight at a time, and the waves' sums meet in LDS: four
+// times the workgroups for a tile, for tiles that are few.  Bound by the partials' bytes, out of the Infinity Cache: 2048
+// tokens behind 6000 (128 tiles, 3 partials each, 96 MB) in 19 us.  us a call at kFew 4, 16, 32, 256: three chunks of 130 ..
+// 300 tokens over long contexts (6 partials a tile) 274, 250, 250, -; two of 90 tokens (21) 110, 109, 104, 101; one of 32 (128)
+// 49, 49, 49, 63.
+constexpr int kFew = 32;
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
   __shared__ uint2 list[1024];  // request and partials (16 bits each), 2 tile + head (20 bits) and share: few partials from the front, many from the back
   __shared__ int counts[4][2], nan_flags[4];
@@ -641,7 +646,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
     const int4 c = c0 + tid < G ? d.cuts[c0 + tid] : int4{-1, 0, 0, 0};
     const int n = c.x >= 0 ? c.z - (c0 + tid) + 1 : 0;
     nans |= __builtin_amdgcn_ballot_w64(c.w != 0);
-    const uint64_t fb = __builtin_amdgcn_ballot_w64(n > 0 && n <= 4), mb = __builtin_amdgcn_ballot_w64(n > 4), below = (1ull << lane) - 1;
+    const uint64_t fb = __builtin_amdgcn_ballot_w64(n > 0 && n <= kFew), mb = __builtin_amdgcn_ballot_w64(n > kFew), below = (1ull << lane) - 1;
     if (lane == 0) counts[wave][0] = __builtin_popcountll(fb), counts[wave][1] = __builtin_popcountll(mb);
     __syncthreads();
     int fat = few + __builtin_popcountll(fb & below), mat = many + __builtin_popcountll(mb & below);
@@ -649,7 +654,7 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
       fat += w < wave ? counts[w][0] : 0, mat += w < wave ? counts[w][1] : 0;
       few += counts[w][0], many += counts[w][1];
     }
-    if (n > 0) list[n <= 4 ? fat : 1023 - mat] = make_uint2((uint32_t)c.x << 16 | (uint32_t)n, (uint32_t)c.y << 12 | (uint32_t)(c0 + tid));
+    if (n > 0) list[n <= kFew ? fat : 1023 - mat] = make_uint2((uint32_t)c.x << 16 | (uint32_t)n, (uint32_t)c.y << 12 | (uint32_t)(c0 + tid));
     __syncthreads();
   }
   if (blockIdx.x == 0 && tid == 0) d.epoch[0] += 1;
@@ -666,9 +671,14 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
     const int tok = tile * kWideTok + 4 * rw + (col >> 3), head = h * kCG + (col & 7);
     if ((!ck_wide(q.r.n) && rw >= 2) || uni(tok) >= q.r.n) continue;
     const bool row_ok = tok < q.r.n;
-    auto ml = [&](int p, int what) { return d.ws_ml[(size_t)ck_slot(share + p, p == 0) * kSlotML + rw * 64 + 32 * what + col]; };
+    // (bases in scalars, a lane's part a 32-bit offset)
+    auto ml = [&](int p, int what) {
+      const char* const at = reinterpret_cast<const char*>(d.ws_ml + (size_t)uni(ck_slot(share + p, p == 0)) * kSlotML + rw * 64 + 32 * what);
+      return *reinterpret_cast<const float*>(at + (uint32_t)col * 4u);
+    };
     auto po = [&](int p, int dt, int a) {
-      return *reinterpret_cast<const v4f*>(d.ws_o + (size_t)ck_slot(share + p, p == 0) * kSlotF + ((rw * 8 + dt) * 4 + a) * 256 + lane * 4);
+      const char* const at = reinterpret_cast<const char*>(d.ws_o + (size_t)uni(ck_slot(share + p, p == 0)) * kSlotF + ((rw * 8 + dt) * 4 + a) * 256);
+      return *reinterpret_cast<const v4f*>(at + (uint32_t)lane * 16u);
     };
     auto store = [&](int dt, int a, v4f v, float L) {
       const float il = L > 0.f ? 1.f / L : L;
@@ -679,22 +689,27 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
     };
     if (mu < 0) {
       const int dt = 2 * (unit & 3);
-      float mp[4], lp[4], M = -1e30f, L = 0.f;
-      v4f v[4][2], s[2] = {};
+      float M = -1e30f, L = 0.f;
+      v4f s[2] = {};
+#pragma unroll 1
+      for (int p0 = 0; p0 < n; p0 += 4) {
+        float mp[4], lp[4], mn = M;
+        v4f v[4][2];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        mp[p] = -1e30f, lp[p] = 0.f;
-        if (p < n) mp[p] = ml(p, 0), lp[p] = ml(p, 1), v[p][0] = po(p, dt, wave), v[p][1] = po(p, dt + 1, wave);
-      }
+        for (int i = 0; i < 4; ++i) {
+          mp[i] = -1e30f, lp[i] = 0.f;
+          if (p0 + i < n) mp[i] = ml(p0 + i, 0), lp[i] = ml(p0 + i, 1), v[i][0] = po(p0 + i, dt, wave), v[i][1] = po(p0 + i, dt + 1, wave);
+        }
 #pragma unroll
-      for (int p = 0; p < 4; ++p) M = fmaxf(M, mp[p]);
+        for (int i = 0; i < 4; ++i) mn = fmaxf(mn, mp[i]);
+        const float f = __builtin_amdgcn_exp2f(M - mn);
+        M = mn, L *= f, s[0] *= f, s[1] *= f;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        if (p < n) {
-          const float w = __builtin_amdgcn_exp2f(mp[p] - M);
-          L += w * lp[p];
-          s[0] += w * v[p][0];
-          s[1] += w * v[p][1];
+        for (int i = 0; i < 4; ++i) {
+          if (p0 + i < n) {
+            const float w = __builtin_amdgcn_exp2f(mp[i] - M);
+            L += w * lp[i], s[0] += w * v[i][0], s[1] += w * v[i][1];
+          }
         }
       }
       if (row_ok) store(dt, wave, s[0], L), store(dt + 1, wave, s[1], L);
@@ -708,20 +723,17 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
       v4f v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int p = min(p0 + 4 * i, n - 1);
-        mp[i] = ml(p, 0), lp[i] = ml(p, 1), v[i] = po(p, dt, a);
+        mp[i] = -1e30f, lp[i] = 0.f;
+        if (p0 + 4 * i < n) mp[i] = ml(p0 + 4 * i, 0), lp[i] = ml(p0 + 4 * i, 1), v[i] = po(p0 + 4 * i, dt, a);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (p0 + 4 * i >= n) mp[i] = -INFINITY;  // (taken already, or another wave's: weight 0)
-        mn = fmaxf(mn, mp[i]);
-      }
+      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, mp[i]);
       const float f = __builtin_amdgcn_exp2f(M - mn);
       M = mn, L *= f, s *= f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (p0 + 4 * i < n) {
-          const float w = __builtin_amdgcn_exp2f(mp[i] - mn);
+          const float w = __builtin_amdgcn_exp2f(mp[i] - M);
           L += w * lp[i], s += w * v[i];
         }
       }
