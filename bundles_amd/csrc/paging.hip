@@ -11,7 +11,7 @@
 // One launch: a workgroup takes a segment of one request and forms that request's two prefix sums from the counts of
 // the requests before it (8 bytes a request, in L2), so no workgroup waits for another.  New pages are read from the
 // free list, never from a table entry that another workgroup writes.  Bound by the launch and two loads behind one another
-// (lengths, then pages): 3.9 us on the GPU for 7 decoding requests, 5.5 for 203 of up to 8191 keys (2.9 MB), 10.5 for 256 of
+// (lengths, then pages): 3.9 us on the GPU for 7 decoding requests, 5.5 for 203 of up to 8191 keys (1.1 MB), 10.5 for 256 of
 // up to 32000 (14 MB, 1.4 TB/s); a call from Python takes 8 us at the least.
 #include <algorithm>
 
