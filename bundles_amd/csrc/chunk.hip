@@ -121,14 +121,12 @@ __device__ __forceinline__ int fresh_tid() {
   return t;
 }
 
-// Sum over the workgroup's 512 threads of values below kMostWeight, held there (a line that long is not dealt).
-__device__ __forceinline__ int held(int a, int b) { return min(a + b, kMostWeight); }
-__device__ __forceinline__ int wave_incl(int v) {  // inclusive sums over the wave
+__device__ __forceinline__ int wave_incl(int v) {  // inclusive sums over the wave, held at kMostWeight
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int u = __shfl_up(v, o);
-    v = lane >= o ? held(v, u) : v;
+    v = lane >= o ? ck_held(v, u) : v;
   }
   return v;
 }
@@ -168,7 +166,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int total = 0, mine = 0;
   for (int c0 = 0; c0 < d.B; c0 += 512) {
     const int w = c0 + tid < d.B ? ck_weight(req_of(d, c0 + tid).r) : 0;
-    mine = c0 ? held(mine, w) : w;
+    mine = c0 ? ck_held(mine, w) : w;
   }
   if (tid == 0) nan_seen = 0;
   int inc = wave_incl(mine);
@@ -178,7 +176,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
     before = w == wave ? total : before;
-    total = held(total, sums[w]);
+    total = ck_held(total, sums[w]);
   }
   total = uni(total);
   const int len = ck_share_len(total, G), nsh = total < kMostWeight ? ck_shares(total, len) : 0;

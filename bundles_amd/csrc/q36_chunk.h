@@ -72,6 +72,11 @@ __host__ __device__ __forceinline__ int ck_tile_at(ChunkReq r, int x) {
 }
 // The most that a call of T new tokens, B requests and tables of `keys` keys can weigh; a line of kMostWeight is not dealt.
 constexpr int kMostWeight = 1 << 30;
+// the sum of two weights, held there (row starts that are no row starts can count a row for many requests)
+__host__ __device__ __forceinline__ int ck_held(int a, int b) {
+  const uint32_t s = (uint32_t)a + (uint32_t)b;
+  return s < (uint32_t)kMostWeight ? (int)s : kMostWeight;
+}
 inline bool ck_too_long(int64_t T, int64_t B, int64_t keys) {
   return 2.0 * ((double)T / kWideTok + 2.0 * (double)B) * ((double)keys / kWideKeys + kNarrowCost + kTileOvh) + (double)B >= kMostWeight;
 }

@@ -124,6 +124,9 @@ int main(int argc, char** argv) {
     return std::max(lo, std::min(hi, (int)(lo * std::pow((hi + 1.0) / lo, u))));
   };
   int bad = 0;
+  for (int a : {0, 1, 5, 1 << 29, kMostWeight - 1, kMostWeight})  // weights' sums stay between 0 and kMostWeight
+    for (int b : {0, 1, 1 << 29, kMostWeight - 1, kMostWeight})
+      if (ck_held(a, b) != (int)std::min<int64_t>((int64_t)a + b, kMostWeight)) printf("held(%d, %d) = %d\n", a, b, ck_held(a, b)), ++bad;
   auto check = [&](const std::vector<ChunkReq>& r, int G) {
     const char* e = walk(r, G);
     if (!e) return;

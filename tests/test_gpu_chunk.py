@@ -320,3 +320,18 @@ def test_a_chunk_is_its_tokens_one_by_one(attn, dev):
 def test_no_tokens(attn, dev):
     h = make([(0, 5)], 1, 21, dev)
     assert run(attn, h, dev).shape == (0, HQ, D)
+
+
+def test_row_starts_that_overlap_past_what_a_call_deals(attn, dev):
+    """Row starts that count every row for every second request: their weights' sum passes 2^31 on the device, where the
+    call's sizes alone do not.  Nothing is dealt, nothing is written, and the workspace serves the next call."""
+    B, T, P, width = 64, 1 << 15, 1024, 8192
+    ws = attn.ChunkWorkspace(dev)
+    kc, vc = (torch.zeros((P, HKV, D), dtype=torch.uint8, device=dev) for _ in range(2))
+    out = torch.full((T, HQ, D), 77.0, dtype=torch.bfloat16, device=dev)
+    qsl = torch.tensor([0, T] * (B // 2) + [0], dtype=torch.int32, device=dev)
+    attn.attn_chunk(torch.zeros((T, HQ, D), dtype=torch.uint8, device=dev), kc, vc, torch.zeros((B, width), dtype=torch.int32, device=dev),
+                    torch.full((B,), P * width, dtype=torch.int32, device=dev), qsl, SCALE, ws, page_size=P, out=out)
+    torch.cuda.synchronize()
+    assert bool((out == 77).all())
+    check(attn, make([(70, 900), (3, 40)], 16, 21, dev), dev, "after it", ws)
