@@ -102,7 +102,7 @@ __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 <
 // 16 bytes a lane from memory into LDS at byte `at` + 16 lane of the workgroup's, past the registers.  In asm, so that the
 // compiler does not hold each read of LDS back until every copy in flight has landed; the caller waits (wait_vm0).
 __device__ __forceinline__ void copy16(const uint8_t* src, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory", "m0");
 }
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
   return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) uint8_t*)p);

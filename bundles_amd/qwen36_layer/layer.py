@@ -357,7 +357,7 @@ class _AttnMixer:
         sc = _ChunkScratch.get(x.device, rows)
         qkv = fp8_linear(x.contiguous(), self.w_qkv, sc.lin2048)
         q, gate = attn_fused.attn_front(qkv, self.q_norm_w, self.k_norm_w, self.eps, self.cos_sin, positions.to(torch.int32).contiguous(),
-                                        cache=(ck.k_cache, ck.v_cache, ck.out_loc), axes=axes, q_dtype=torch.uint8)
+                                        cache=(ck.k_cache, ck.v_cache, ck.out_loc.to(torch.int64).contiguous()), axes=axes, q_dtype=torch.uint8)
         o = torch.zeros(q.shape, dtype=torch.bfloat16, device=x.device)  # (rows of no request stay zero)
         attn_fused.attn_chunk(q, ck.k_cache, ck.v_cache, ck.page_table, ck.seqlens, ck.qsl, self.scale, sc.chunk, ck.page_size, out=o)
         return attn_fused.attn_oproj(o.view(rows, -1), gate.view(rows, -1), self.w, sc.attn)

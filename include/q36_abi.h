@@ -526,7 +526,8 @@ int q36_page_plan(const q36_page_plan_args* a, q36_stream_t stream);
  * [axes, pos_stride], axes 1..4 (time, height, width, ..); a position outside [0, max_pos) counts as the nearest inside.
  * All of it in fp32, rounded once: q bf16 [T, 16, 256], or with q_e4m3 e4m3 codes (satfinite) as q36_attn_chunk reads
  * them; k, v e4m3 (satfinite) into rows out_loc[t] (int64 [T]; a slot outside [0, num_slots) is skipped) of k_cache,
- * v_cache [num_slots, 2, 256]; gate bf16 [T, 16, 256], copied.  (q36_attn_proj rounds to bf16 behind the norm and behind
+ * v_cache [num_slots, 2, 256]; gate bf16 [T, 16, 256], copied.  Cache slots of one call are distinct
+ * (rows with the same one leave a mix of their codes).  (q36_attn_proj rounds to bf16 behind the norm and behind
  * the rotation: its cache rows can differ from these by one e4m3 code.)  out_loc, k_cache, v_cache may be NULL together
  * (no cache rows), gate may be NULL.  qkv, norm weights, cos_sin, gate and bf16 q 16-byte, e4m3 q and caches 8-byte aligned. */
 typedef struct q36_attn_front_args {
