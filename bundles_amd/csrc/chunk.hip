@@ -302,44 +302,41 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(uintptr_t)((v0 ^ (32 * dt)) + 16 * kCD * cc));
   };
   auto key = [&](uint32_t k0, int i) { return *(__attribute__((address_space(3))) const v4i*)(uintptr_t)(k0 ^ (16 * i)); };
-  // The wave's query rows: asked for as they lie, 1 KB a load (four rows of codes, two of bf16), and handed out to the lanes
+  // The wave's query rows: read as they lie, 1 KB a load (four rows of codes, two of bf16), and handed out to the lanes
   // through the wave's 8 KB of `mem` (16-byte piece p of row r at p ^ (r % 16), as a block's keys).
-  v4i qraw[16];
-  auto ask = [&](const Item& it, bool q8) {
+  auto queries = [&](auto is_q8, const Item& it, uint8_t* mem) {
+    constexpr bool q8 = decltype(is_q8)::value;
     const int lane = fresh_tid() & 63, tok = first_tok(it);
     const char* const rows = static_cast<const char*>(d.q) + (((size_t)(it.t0 + tok) * kCHQ + it.h * kCG) * kCD << (q8 ? 0 : 1));
+    uint8_t* const my = mem + wave * 8192;
+    v4i raw[q8 ? 8 : 16];
 #pragma unroll
     for (int j = 0; j < (q8 ? 8 : 16); ++j) {
       const int r = q8 ? 4 * j + (lane >> 4) : 2 * j + (lane >> 5), at = q8 ? 256 * (r & 7) + 16 * (lane & 15) : 512 * (r & 7) + 16 * (lane & 31);
-      qraw[j] = v4i{0, 0, 0, 0};
-      if (tok + (r >> 3) < it.n) qraw[j] = *reinterpret_cast<const v4i*>(rows + (((size_t)(r >> 3) * kCHQ * kCD) << (q8 ? 0 : 1)) + at);
+      raw[j] = v4i{0, 0, 0, 0};
+      if (tok + (r >> 3) < it.n) raw[j] = *reinterpret_cast<const v4i*>(rows + (((size_t)(r >> 3) * kCHQ * kCD) << (q8 ? 0 : 1)) + at);
     }
-  };
-  auto answer = [&](uint8_t* mem) {
-    const int lane = fresh_tid() & 63;
-    uint8_t* const my = mem + wave * 8192;
-    if (d.q8) {
+    wait_vm0();  // (and the first item's first set of keys)
+    if constexpr (q8) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = 4 * j + (lane >> 4);
-        *reinterpret_cast<v4i*>(my + 256 * r + 16 * ((lane & 15) ^ (r & 15))) = qraw[j];
+        *reinterpret_cast<v4i*>(my + 256 * r + 16 * ((lane & 15) ^ (r & 15))) = raw[j];
       }
     } else {
       // the conversion makes a NaN of what is past 448 (of 464, with its rounding): rows with one of those go the long way
       v2us big = {0, 0};
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const v4i x = qraw[j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(v2us, x[i] & 0x7fff7fff));
+        for (int i = 0; i < 4; ++i) big = __builtin_elementwise_max(big, __builtin_bit_cast(v2us, raw[j][i] & 0x7fff7fff));
       }
       auto hand = [&](auto two) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int r = 2 * j + (lane >> 5);
-          const v4i x = qraw[j];
           *reinterpret_cast<uint2*>(my + 256 * r + 16 * (((lane & 31) >> 1) ^ (r & 15)) + 8 * (lane & 1)) =
-              make_uint2(two(x.x, x.y), two(x.z, x.w));
+              make_uint2(two(raw[j].x, raw[j].y), two(raw[j].z, raw[j].w));
         }
       };
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(max(big.x, big.y) > 0x43e0) == 0, 1))
@@ -382,6 +379,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     v2i w[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w[dt] = value(v0, dt, 0);
+    // (half of the keys' reads before the first product, the others and the values' between the products)
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
     if (border) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -554,9 +561,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (!wide) barrier();  // (the waves' LDS is theirs again)
     }
     if (nxt.n == 0) break;
-    d.q8 ? ask(nxt, true) : ask(nxt, false);
-    wait_vm0();  // (the first item's first set of keys, too)
-    answer(mem);
+    d.q8 ? queries(std::true_type{}, nxt, mem) : queries(std::false_type{}, nxt, mem);
     cur = nxt;
     nxt = next();
     const bool wide = ck_wide(cur.n);
@@ -576,7 +581,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int end = uni(tok0 < cur.n ? min(pre + min(tok0 + 4, cur.n), cur.key1) : 0);
 #pragma unroll 1
     for (int st = 0; st < sets; ++st) {
-      if (st > 0) wait_vm0();
+      wait_vm0();  // (also said of an item's first set, so that no wait for the entries stands among the copies)
       barrier();  // every wave's copies of this set have landed, and every wave is done with the other half
       // the next set, this item's or the next one's, and the page-table entries of the one behind it
       if (st + 1 < sets || nxt.n > 0) {
@@ -592,6 +597,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = wide ? 0 : wave >> 1; i < i1; ++i) {
         const int k = cur.key0 + st * SET + 32 * i;
         if (k >= end) break;
+        // a SIMD's older wave wins where both could issue, and its other one would then end each set alone: they take turns
+        // (8192 tokens 416 -> 407 us)
+        if (((i >> 1) ^ (wave >> 2)) & 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
         block(to + i * kBlk, k, k + 31 > pre + tok0);
       }
       half ^= 1;
