@@ -9,11 +9,11 @@
 // 2^-11 a weight, where e4m3 weights would lose 2^-4), the outputs to bf16.  Scores, maxima, weight sums and outputs: fp32.
 //
 // Bounds.  Long chunks: the matrix units, half the products at the e4m3 rate and half at the f16 one: 289 us for 8192 tokens
-// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 405 measured, 1.36 PFLOP/s.  A step of
-// 32 keys takes a workgroup 1.45 us (2.9 K cycles), of which the matrix units are busy half and the vector units (scores to
-// weights: 16 exponentials, maxima and sums a lane, and the values' widening, all beside 2 waves a SIMD) three fifths;
-// prefetched keys, wave priorities and other bank layouts moved it by under 1 %.  Short calls: the latency of one pass:
-// lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second launch 4: 19 us for five tokens over 300
+// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 398 to 405 measured, 1.37 PFLOP/s.  A step of
+// 32 keys takes a workgroup 1.4 us (2.8 K cycles), of which the matrix units are busy 1.54 K and the vector units (scores to
+// weights: 16 exponentials, maxima and sums a lane, and the values' widening, for 2 waves a SIMD) 1.6 K; the next block's
+// scores formed beside this one's weights would overlap them better, and did not fit the registers (54 spilled).  Short calls: the latency of one pass:
+// lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second launch 4: 17 us for five tokens over 300
 // keys.  Between: cut tiles, 256 KB a partial out of and back into the Infinity Cache (7 TB/s over the chip).
 //
 // Why so.  256 rows a workgroup: one pass over a tile's keys feeds eight waves from LDS (a wave alone would need four times
@@ -102,7 +102,7 @@ __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 <
 // 16 bytes a lane from memory into LDS at byte `at` + 16 lane of the workgroup's, past the registers.  In asm, so that the
 // compiler does not hold each read of LDS back until every copy in flight has landed; the caller waits (wait_vm0).
 __device__ __forceinline__ void copy16(const uint8_t* src, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
   return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) uint8_t*)p);
