@@ -394,8 +394,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = 0; i < 16; ++i)
         if (key0 + 8 * (i >> 2) + 4 * g0 + (i & 3) > lim) s[i] = -INFINITY;
     }
-    // relative to the running maximum, which the first block sets; where a row grows past 2^8 times it, all moves to the new
-    // one.  (A row that sees nothing of a block sees nothing of the later ones.)
+    // relative to the running maximum, which the first block sets; where a row grows past 2^8 times it, the row moves to the
+    // new one.  (A row that sees nothing of a block sees nothing of the later ones.)
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sl2, -m);
@@ -404,7 +404,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
     if (__builtin_expect(!begun || __builtin_amdgcn_ballot_w64(mx > kLazyC) != 0, 0)) {
-      const float up = begun ? fmaxf(mx, 0.f) : mx > -INFINITY ? mx : 0.f, al = begun ? __builtin_amdgcn_exp2f(-up) : 1.f;
+      // (each row by its own maximum alone: its bits do not depend on its wave's other rows)
+      const float up = mx > (begun ? kLazyC : -INFINITY) ? mx : 0.f, al = begun ? __builtin_amdgcn_exp2f(-up) : 1.f;
       begun = true;
       m += up;
       l *= al;

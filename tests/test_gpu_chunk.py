@@ -335,3 +335,25 @@ def test_row_starts_that_overlap_past_what_a_call_deals(attn, dev):
     torch.cuda.synchronize()
     assert bool((out == 77).all())
     check(attn, make([(70, 900), (3, 40)], 16, 21, dev), dev, "after it", ws)
+
+
+@pytest.mark.parametrize("lens", [[(40, 300)], [(5, 900), (1, 33)]], ids=["wide", "narrow"])
+def test_queries_past_the_largest_code(attn, dev, lens):
+    """bf16 queries are rounded to e4m3 with saturation: values past 448, infinities among them, count as 448, a NaN makes its
+    row NaN, and the other rows of its wave keep their bits."""
+    h = make(lens, 16, 22, dev, q8=False)
+    plain = run(attn, h, dev).clone()
+    q = h["q"]
+    q[0, 3] = q[0, 3] * 100
+    q[1, 9, 17], q[2, 0, 255], q[3, 15, 0] = 460.0, 465.0, -3.0e38
+    q[2, 8, 100] = torch.inf
+    q[4, 11, 64] = -torch.inf
+    check(attn, h, dev, "saturated queries")
+    q[1, 4, 5] = torch.nan
+    out = run(attn, h, dev)
+    torch.cuda.synchronize()
+    assert bool(out[1, 4].isnan().all()) and int(out.isnan().any(-1).sum()) == 1
+    touched = torch.zeros(out.shape[:2], dtype=torch.bool, device=dev)
+    for t, hd in ((0, 3), (1, 9), (2, 0), (3, 15), (2, 8), (4, 11), (1, 4)):
+        touched[t, hd] = True
+    assert torch.equal(out[~touched], plain[~touched])
