@@ -173,6 +173,7 @@ SYMBOLS = [
     ("q36_page_plan", I32, [C.POINTER(PagePlanArgs), P]),
     ("q36_attn_front", I32, [C.POINTER(AttnFrontArgs), P]),
     ("q36_attn_chunk_workspace_bytes", SZ, []),
+    ("q36_attn_chunk_workspace_init", I32, [P, SZ, P]),
     ("q36_attn_chunk", I32, [C.POINTER(ChunkArgs), P]),
     ("q36_lmhead_workspace_bytes", SZ, [I32]),
     ("q36_lmhead_argmax", I32, [C.POINTER(LmheadArgs), P]),

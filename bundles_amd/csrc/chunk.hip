@@ -9,7 +9,7 @@
 // 2^-11 a weight, where e4m3 weights would lose 2^-4), the outputs to bf16.  Scores, maxima, weight sums and outputs: fp32.
 //
 // Bounds.  Long chunks: the matrix units, half the products at the e4m3 rate and half at the f16 one: 289 us for 8192 tokens
-// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 398 to 405 measured, 1.37 PFLOP/s.  A step of
+// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 391 to 405 measured, 1.36 to 1.41 PFLOP/s.  A step of
 // 32 keys takes a workgroup 1.4 us (2.8 K cycles), of which the matrix units are busy 1.54 K and the vector units (scores to
 // weights: 16 exponentials, maxima and sums a lane, and the values' widening, for 2 waves a SIMD) 1.6 K; the next block's
 // scores formed beside this one's weights would overlap them better, and did not fit the registers (54 spilled).  Short calls: the latency of one pass:
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // what a flag of this call from this XCD says: its number among the workspace's calls, spread, and the XCD's
   uint32_t xcc;
   asm("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
-  const uint32_t mark = ((d.epoch[0] * 0x9e3779b1u) & ~31u) | 16u | (xcc & 15u);  // (not 0, what the first call finds)
+  const uint32_t mark = ((d.epoch[0] * 0x9e3779b1u) & ~31u) | 16u | (xcc & 15u);  // (not 0, what a workspace starts with)
   // ---- this workgroup's share
   int total = 0, mine = 0;
   for (int c0 = 0; c0 < d.B; c0 += 512) {
@@ -778,6 +778,11 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
   }
 }
 
+// A workspace before its first call: no calls served, no partial said to be there.
+__global__ __launch_bounds__(256) void chunk_init_kernel(uint32_t* epoch, int G) {
+  for (int i = threadIdx.x; i <= G; i += 256) epoch[i] = 0;
+}
+
 // Workgroups: one a CU (their LDS and registers fill it).
 int chunk_groups() { return std::min(std::max(device_cus(), 1), 1024); }
 struct ChunkWs {
@@ -799,6 +804,15 @@ ChunkWs chunk_ws(int G) {
 using namespace q36;
 
 extern "C" size_t q36_attn_chunk_workspace_bytes(void) { return chunk_ws(chunk_groups()).total; }
+
+extern "C" int q36_attn_chunk_workspace_init(void* workspace, size_t workspace_bytes, q36_stream_t stream) {
+  const int G = chunk_groups();
+  const ChunkWs L = chunk_ws(G);
+  Q36_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "q36_attn_chunk_workspace_init: workspace must be 256-byte aligned");
+  Q36_REQUIRE(workspace_bytes >= L.total, "q36_attn_chunk_workspace_init: workspace of %zu bytes < %zu required", workspace_bytes, L.total);
+  chunk_init_kernel<<<1, 256, 0, static_cast<hipStream_t>(stream)>>>(reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + L.flags), G);
+  return check_launch("q36_attn_chunk_workspace_init");
+}
 
 extern "C" int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream) {
   Q36_REQUIRE(a != nullptr, "q36_attn_chunk: null args");

@@ -287,7 +287,10 @@ class ChunkWorkspace:
     the same time need one each)."""
 
     def __init__(self, device):
-        self.buf = torch.zeros(_lib.lib().q36_attn_chunk_workspace_bytes(), dtype=torch.uint8, device=device)
+        L = _lib.lib()
+        self.buf = torch.empty(L.q36_attn_chunk_workspace_bytes(), dtype=torch.uint8, device=device)
+        check_tensors("ChunkWorkspace", "workspace", self.buf)
+        check(L.q36_attn_chunk_workspace_init(ptr(self.buf), self.buf.numel(), _lib.stream_handle(None)), "q36_attn_chunk_workspace_init")
 
 
 def attn_chunk(q, k_cache, v_cache, page_table, seqlens, qsl, scale: float, ws: ChunkWorkspace, page_size: int = 1,

@@ -226,3 +226,11 @@ def test_rope_axes_of_a_rotary_embedding():
     r = layer._rope_axes(types.SimpleNamespace(mrope_section=[11, 11, 10], mrope_interleaved=True))
     assert r.axes == 3 and r.axis_of[:4] == [0, 1, 2, 0]
     assert layer._rope_axes(types.SimpleNamespace(mrope_section=[11, 11, 10])).axis_of[:4] == [0, 0, 0, 0]
+
+
+def test_the_workspace_entry_refuses(L):
+    from bundles_amd import _lib
+    need = L.q36_attn_chunk_workspace_bytes()
+    for at, size in ((0, need), (4096 + 16, need), (4096, need - 1), (4096, 0)):
+        assert L.q36_attn_chunk_workspace_init(at, size, None) == _lib.Q36_EINVAL
+        assert L.q36_last_error().startswith(b"q36_attn_chunk_workspace_init")

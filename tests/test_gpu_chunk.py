@@ -357,3 +357,19 @@ def test_queries_past_the_largest_code(attn, dev, lens):
     for t, hd in ((0, 3), (1, 9), (2, 0), (3, 15), (2, 8), (4, 11), (1, 4)):
         touched[t, hd] = True
     assert torch.equal(out[~touched], plain[~touched])
+
+
+def test_a_workspace_may_hold_anything(attn, dev):
+    """Memory of another use, made ready by the workspace entry, serves a call as fresh memory does; whatever is in the
+    partials' part, and however many calls have passed."""
+    from bundles_amd import _lib
+    h = make([(300, 2000), (70, 900), (1, 5000)], 16, 23, dev)
+    want = run(attn, h, dev).clone()
+    for fill in (0xff, 0x00, 0x7f):
+        ws = attn.ChunkWorkspace(dev)
+        ws.buf.fill_(fill)
+        _lib.check(_lib.lib().q36_attn_chunk_workspace_init(ws.buf.data_ptr(), ws.buf.numel(), _lib.stream_handle(None)), "init")
+        for _ in range(3):
+            out = run(attn, h, dev, ws)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
