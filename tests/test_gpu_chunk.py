@@ -373,3 +373,26 @@ def test_a_workspace_may_hold_anything(attn, dev):
             out = run(attn, h, dev, ws)
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("B,n,T", [(16384, 64, 1 << 20), (65535, 1, 65535), (65535, 3, (1 << 20) - 9)])
+def test_the_largest_batches(attn, dev, B, n, T):
+    """As many requests and rows as a call takes (outputs past 2^32 bytes): requests spread over the batch against the formula,
+    and rows behind the last one left."""
+    P, pages, width, keys = 64, 50, 2, 100
+    g = torch.Generator(device=dev).manual_seed(24)
+    kc, vc = (codes(torch.randn((pages * P, HKV, D), generator=g, device=dev)) for _ in range(2))
+    q = torch.randint(0, 0x58, (T, HQ, D), generator=g, device=dev, dtype=torch.uint8)
+    q[:, :, ::2] |= 0x80
+    pt = torch.randint(0, pages, (B, width), generator=g, device=dev, dtype=torch.int32)
+    seqlens = torch.full((B,), keys, dtype=torch.int32, device=dev)
+    qsl = torch.arange(B + 1, device=dev, dtype=torch.int32) * n
+    out = torch.full((T, HQ, D), 77.0, dtype=torch.bfloat16, device=dev)
+    attn.attn_chunk(q, kc, vc, pt, seqlens, qsl, SCALE, attn.ChunkWorkspace(dev), page_size=P, out=out)
+    torch.cuda.synchronize()
+    assert bool((out[B * n:] == 77).all())
+    for b in (0, 1, 511, 512, 513, B // 2, B - 2, B - 1):
+        h = dict(q=q[b * n:(b + 1) * n], kc=kc, vc=vc, pt=pt[b:b + 1], P=P, lens=[(n, keys)], qsl=torch.tensor([0, n]))
+        want, bar, _ = formula(h)
+        off = (out[b * n:(b + 1) * n].double() - want).abs()
+        assert bool((off <= bar).all()), f"request {b}: {float((off / bar).max())} of the bar"
