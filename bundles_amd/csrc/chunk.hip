@@ -12,8 +12,8 @@
 // from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 391 to 405 measured, 1.36 to 1.41 PFLOP/s.  A step of
 // 32 keys takes a workgroup 1.4 us (2.8 K cycles), of which the matrix units are busy 1.54 K and the vector units (scores to
 // weights: 16 exponentials, maxima and sums a lane, and the values' widening, for 2 waves a SIMD) 1.6 K; the next block's
-// scores formed beside this one's weights would overlap them better, and did not fit the registers (54 spilled).  Short calls: the latency of one pass:
-// lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second launch 4: 17 us for five tokens over 300
+// scores formed beside this one's weights would overlap them better, and did not fit the registers (54 spilled).
+// Short calls: the latency of one pass: lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second launch 4: 17 us for five tokens over 300
 // keys.  Between: cut tiles, 256 KB a partial out of and back into the Infinity Cache (7 TB/s over the chip).
 //
 // Why so.  256 rows a workgroup: one pass over a tile's keys feeds eight waves from LDS (a wave alone would need four times
@@ -648,7 +648,8 @@ __device__ __forceinline__ uint2 put_nans(uint2 v, uint32_t n) {
 // 49, 49, 49, 63.
 constexpr int kFew = 32;
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
-  __shared__ uint2 list[1024];  // request and partials (16 bits each), 2 tile + head (20 bits) and share: few partials from the front, many from the back
+  // request and partials (16 bits each), 2 tile + head (20 bits) and share: few partials from the front, many from the back
+  __shared__ uint2 list[1024];
   __shared__ int counts[4][2], nan_flags[4];
   __shared__ v4f part[4][64];
   __shared__ float pml[4][2][64];

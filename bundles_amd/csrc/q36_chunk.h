@@ -16,13 +16,14 @@ namespace q36 {
 // kNarrow, us a call: 16 requests behind 500 keys, 4 behind 8000.  8 tokens as a narrow tile 21.2, 28.4, as a wide one 21.0,
 // 31.4; 12 tokens as two narrow ones 24.8, 36.1, as a wide one 22.4, 32.8; 16 tokens 27.0, 37.0 against 24.4, 33.8.
 constexpr int kNarrow = 8, kWideTok = 32, kWideKeys = 32, kNarrowKeys = 128;
-// kTileOvh, us a call: eight prompts at 4, 6, 8, 10, 12: 54.7, 55.1, 52.7, 58.1, 57.5; one of 8192: 415, 420, 420, 422, 425;
-// 4 x 12 tokens behind 8000 keys (narrow, two tiles): 40.3, 36.7, 36.1, 36.2, 36.5.
+// kTileOvh, us a call at 6, 7, 8, 9, 10: eight prompts 51.5, 49.4, 48.6, 52.2, 53.5; 64 requests of 1 .. 200 tokens 41.9, 40.7,
+// 38.7, 39.3, 40.7; 24 requests, chunks beside single tokens, 56 to 59, and one of 8192 tokens 391 to 395 at all of them.
 constexpr int kTileOvh = 8;
-// What a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16.  A batch of 24, single tokens beside chunks,
-// at 1, 2, 3: 66.2, 59.9, 61.4 us.
+// What a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16.  us a call at 2, 3: 64 requests of 1 .. 200
+// tokens 38.7, 43.7; 12 of 1 .. 300 over up to 6000 keys 48.9, 54.5; 24, chunks beside single tokens, 59, 57 (at 1: 66).
 constexpr int kNarrowCost = 2;
-constexpr int kLeastShare = kNarrowCost;  // a share is no shorter than a narrow step (five tokens over 300 keys: 20.0 us; 4: 21.5, 8: 22.7, 20: 32.8)
+// A share is no shorter than a narrow step.  Five tokens over 300 keys at 2, 4, 8, 20: 20.0, 21.5, 22.7, 32.8 us.
+constexpr int kLeastShare = kNarrowCost;
 
 struct ChunkReq {
   int n, nk;  // new tokens, keys (the new ones included)
@@ -89,9 +90,10 @@ __host__ __device__ __forceinline__ int ck_share_len(int total, int G) {
 __host__ __device__ __forceinline__ int ck_shares(int total, int len) { return (total + len - 1) / len; }
 
 // A cut of a wide tile costs some ten steps: its 256 KB leave and come back, and its queries are read twice.  So one that
-// falls within kSnap steps of the tile's end goes to that end.  (8 prompts of 120 .. 1000 tokens: 0: 60.4 us, 2: 59.6,
-// 4: 56.3, 6: 59.1; 16 of 64 .. 2000: 133, 126 at 3 .. 6, 129 at 8.  A narrow tile's cut costs little: five tokens
-// over 300 keys: 21.6 against 19.7.)  A tile's cuts lie behind step ck_lo and before ck_hi.
+// falls within kSnap steps of the tile's end goes to that end.  us a call at 0, 3, 4, 5, 6: eight prompts 60.4 (of a slower
+// step), 48.7, 48.6, 53.8, 52.7; 64 requests of 1 .. 200 tokens at 3 .. 6: 44.4, 38.7, 37.9, 37.4; 2048 tokens behind 6000
+// 199, 199, 198, 205.  A narrow tile's cut costs little (five tokens over 300 keys: 21.6 with it moved, 19.7 without).
+// A tile's cuts lie behind step ck_lo and before ck_hi.
 constexpr int kSnap = 4;
 __host__ __device__ __forceinline__ int ck_lo(int steps, int cost) {
   return cost > 1 ? 0 : kSnap < (steps - 1) / 2 ? kSnap : (steps - 1) / 2;
