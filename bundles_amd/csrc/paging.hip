@@ -17,11 +17,10 @@
 
 #include "q36_device.h"
 #include "q36_host.h"
+#include "q36_plan.h"
 
 namespace q36 {
 namespace {
-
-constexpr int kMost = (1 << 30) - 1;  // counts are taken between 0 and this, so a sum of two fits
 
 struct PlanDev {
   int B, T, sh, rows, width, nfree, pt_width, whole, segs;
@@ -32,9 +31,6 @@ struct PlanDev {
   int64_t* out_loc;
   int32_t *used, *page_table;
 };
-
-__device__ __forceinline__ int count_of(int v) { return min(max(v, 0), kMost); }
-__device__ __forceinline__ int pages_of(int n, int sh) { return (n + (1 << sh) - 1) >> sh; }
 
 __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* sums) {
 #pragma unroll
@@ -109,7 +105,7 @@ __global__ __launch_bounds__(256) void page_plan_kernel(PlanDev d) {
       int bits = 0;
       for (int a = tid; a < d.B; a += 256) {
         const int c = count_of(d.cached[a]), n = count_of(d.fresh[a]), r = d.req ? d.req[a] : a;
-        if (r < 0 || r >= d.rows || pages_of(c + n, sh) > d.width) bits |= Q36_PLAN_TABLE;
+        if (r < 0 || r >= d.rows || pages_of(c + n, sh) > d.width || c < d.cached[a] || n < d.fresh[a]) bits |= Q36_PLAN_TABLE;
         if (d.page_table && c + n > d.pt_width) bits |= Q36_PLAN_PAGE_TABLE;
       }
       const int64_t tokens_all = first + fresh, pages_all = off + (full - have);
@@ -151,7 +147,7 @@ extern "C" int q36_page_plan(const q36_page_plan_args* a, q36_stream_t stream) {
   // times over (a segment's threads walk on through a longer request).  On the GPU, at 512 / 2048 / 8192 keys a segment: 203
   // requests of up to 8191 keys 6.6 / 5.5 / 6.7 us, 256 of up to 32000 10.7 / 10.5 / 12.5.
   const int most = std::max(a->page_table && a->whole ? a->pt_width : 0, a->T / a->B);
-  const int segs = std::max(1, std::min((most + 2047) / 2048, std::max(1, 2048 / a->B)));
+  const int segs = std::max(1, std::min((most - 1) / 2048 + 1, std::max(1, 2048 / a->B)));
   PlanDev d{a->B, a->T, sh, a->table_rows, a->table_width, a->free_count, a->pt_width, a->whole ? 1 : 0, segs,
             a->cached, a->new_tokens, a->req, a->table, a->free_pages, a->qsl, a->seqlens, a->positions, a->out_loc,
             a->used, a->page_table};

@@ -493,10 +493,10 @@ int q36_attn_decode(const q36_decode_args* a, q36_stream_t stream);
  *   page_table int32 [B, pt_width] (or NULL): the slot of every key position of request b (whole) or of its new tokens
  *     alone; what lies behind a request's keys is left as it was;
  *   used int32 [2]: the pages taken from the list, and 0 or the OR of what did not fit: Q36_PLAN_TOKENS more new tokens
- *     than T, Q36_PLAN_PAGES too few free pages, Q36_PLAN_TABLE a request longer than the table or a row outside it,
- *     Q36_PLAN_PAGE_TABLE a request longer than the page table.  A token without a page (or whose page number has no
- *     31-bit slot) gets slot -1, a key without one page-table entry 0, and qsl stops at T.
- * Negative counts are taken as 0.  B up to 65535; all pointers naturally aligned. */
+ *     than T, Q36_PLAN_PAGES too few free pages, Q36_PLAN_TABLE a request longer than the table, a row outside it or a
+ *     count past 2^30 - 2^20, Q36_PLAN_PAGE_TABLE a request longer than the page table.  A token without a page (or
+ *     whose page number has no 31-bit slot) gets slot -1, a key without one page-table entry 0, and qsl stops at T.
+ * Negative counts are taken as 0, counts past 2^30 - 2^20 as that many.  B up to 65535; all pointers naturally aligned. */
 #define Q36_PLAN_TOKENS 1
 #define Q36_PLAN_PAGES 2
 #define Q36_PLAN_TABLE 4
