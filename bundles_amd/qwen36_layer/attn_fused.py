@@ -284,13 +284,18 @@ def _check_caches(what, k_cache, v_cache):
 
 class ChunkWorkspace:
     """Partials of q36_attn_chunk; one size serves every call, so the layers of a step share it (calls that may run at
-    the same time need one each)."""
+    the same time need one each).  Made ready on the current stream, which the constructor waits for: calls on any stream
+    may follow.  It is made outside a capture, where that would only be recorded."""
 
     def __init__(self, device):
         L = _lib.lib()
         self.buf = torch.empty(L.q36_attn_chunk_workspace_bytes(), dtype=torch.uint8, device=device)
         check_tensors("ChunkWorkspace", "workspace", self.buf)
-        check(L.q36_attn_chunk_workspace_init(ptr(self.buf), self.buf.numel(), _lib.stream_handle(None)), "q36_attn_chunk_workspace_init")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("ChunkWorkspace: make the workspace before the capture that uses it")
+        stream = torch.cuda.current_stream()
+        check(L.q36_attn_chunk_workspace_init(ptr(self.buf), self.buf.numel(), _lib.stream_handle(stream)), "q36_attn_chunk_workspace_init")
+        stream.synchronize()
 
 
 def attn_chunk(q, k_cache, v_cache, page_table, seqlens, qsl, scale: float, ws: ChunkWorkspace, page_size: int = 1,
@@ -302,7 +307,8 @@ def attn_chunk(q, k_cache, v_cache, page_table, seqlens, qsl, scale: float, ws: 
     cache, number seqlens[b] (int32 [B]); k_cache / v_cache e4m3 codes (uint8) [slots, 2, 256]; page_table int32
     [B, stride]: the page (page_size slots, a power of two) of keys j * page_size .. .  Returns bf16 [T, 16, 256] =
     softmax(scale * q k^T) V per query head, causal among the new tokens; rows outside qsl are left as they were (a
-    fresh out holds anything there), rows that see no key are zero."""
+    fresh out holds anything there), rows that see no key are zero.  Calls that share ws follow one another, on one stream
+    or by events."""
     if q.dim() != 3 or q.shape[1:] != (N_Q_HEADS, HEAD_DIM) or q.dtype not in (torch.bfloat16, torch.uint8) or not q.is_contiguous():
         raise ValueError(f"attn_chunk: q must be a contiguous bfloat16 or uint8 tensor [T, {N_Q_HEADS}, {HEAD_DIM}]")
     _check_caches("attn_chunk", k_cache, v_cache)
