@@ -40,7 +40,7 @@ HIDDEN, EXPERTS, INTERMEDIATE, TOPK = 2048, 512, 512, 10
 MAX_TOKENS = moe.MAX_TOKENS
 GDN_QKV, GDN_Z, GDN_HV = gdn_fused.QKV_DIM, gdn_fused.N_V_HEADS * gdn_fused.HEAD_V, gdn_fused.N_V_HEADS
 PROJ_IN = 4096
-MAX_CHUNK_ROWS = 65535  # of a batch of prompt chunks (the projections' limit)
+MAX_ROWS = 65535  # of a batch (the projections' limit)
 DENSE8_ROWS = 32  # the reference's DENSE8 row limit for the recurrent block's projections
 
 
@@ -78,16 +78,18 @@ def _topk_ok(block, topk: int) -> bool:
 
 class _Scratch:
     """Per-device buffers shared by every layer node on the device: the calls are stream ordered, one
-    layer after another, so one set serves them all."""
+    layer after another, so one set serves them all.  A set that a longer batch outgrows is kept, since
+    captured graphs hold its addresses; the next has at least twice its rows (up to the projections'
+    limit), so that few are kept."""
 
-    _by_device: dict = {}
+    _by_device: dict = {}  # the sets of a device, the last in use
 
     @classmethod
     def get(cls, device, rows: int):
-        s = cls._by_device.get(device)
-        if s is None or s.rows < rows:
-            s = cls._by_device[device] = cls(device, max(rows, MAX_TOKENS))
-        return s
+        sets = cls._by_device.setdefault(device, [])
+        if not sets or sets[-1].rows < rows:
+            sets.append(cls(device, max(rows, min(2 * sets[-1].rows, MAX_ROWS) if sets else MAX_TOKENS)))
+        return sets[-1]
 
     def __init__(self, device, rows: int):
         self.rows = rows
@@ -98,15 +100,17 @@ class _Scratch:
 
 
 class _ChunkScratch(_Scratch):
-    """The same for prompt chunks."""
+    """The same for prompt chunks.  The chunk attention's workspace has one size for every batch: one a device."""
 
     _by_device: dict = {}
+    _chunk_by_device: dict = {}
 
     def __init__(self, device, rows: int):
-        self.rows = rows
+        if device not in self._chunk_by_device:
+            self._chunk_by_device[device] = attn_fused.ChunkWorkspace(device)
+        self.rows, self.chunk = rows, self._chunk_by_device[device]
         self.lin2048 = LinearWorkspace(rows, HIDDEN, device)
         self.attn = attn_fused.Workspace(rows, device)
-        self.chunk = attn_fused.ChunkWorkspace(device)
 
 
 # ---- MoE ---------------------------------------------------------------------------------------------
@@ -298,6 +302,12 @@ def attn_layer_refusal(module) -> str | None:
     return None
 
 
+def _gives_chunks(engine) -> bool:
+    """Whether an engine has a chunk_view of its own (EngineView's takes no batch)."""
+    view = getattr(engine, "chunk_view", None)
+    return view is not None and getattr(view, "__func__", None) is not EngineView.chunk_view
+
+
 def _rope_axes(rot):
     """The axes of a rotary embedding's positions, where it has several and these are served."""
     sections = getattr(rot, "mrope_section", None)
@@ -343,6 +353,9 @@ class _AttnMixer:
         self.w_qkv = Fp8Weight(self.w.wqkv, self.w.sqkv, self.w.wqkv_p, attn_fused.QKV_ROWS)
         # rotary positions of several axes, where the model has them: the frequencies' axes by sections
         self.axes = _rope_axes(rot)
+        # prompt batches may be captured first of all: their workspaces are there before
+        if self.refusal is None and _gives_chunks(engine):
+            _ChunkScratch.get(w_qkv.device, MAX_TOKENS)
 
     def _chunk(self, positions, hidden_states, forward_batch):
         x = hidden_states
@@ -350,7 +363,7 @@ class _AttnMixer:
         axes = self.axes if isinstance(positions, torch.Tensor) and positions.dim() == 2 else None
         view = getattr(self.engine, "chunk_view", None)
         ck = (view(self.layer_id, forward_batch)
-              if view is not None and self.refusal is None and 0 < rows <= MAX_CHUNK_ROWS and x.dtype == torch.bfloat16
+              if view is not None and self.refusal is None and 0 < rows <= MAX_ROWS and x.dtype == torch.bfloat16
               and tuple(positions.shape) == ((rows,) if axes is None else (axes.axes, rows)) else None)
         if ck is None:
             return self.stock(self.replica, positions, hidden_states, forward_batch)
@@ -396,7 +409,8 @@ def prepare(module, dtype: int = moe.Q36_MOE_FP8, topk: int = TOPK, max_tokens: 
     submodule dict are left untouched.  engine: where the mixers find the verify batch's pools
     (default: SGLang's attention backend, absent here); mixers=False installs the MoE only;
     dense8_rows: verify batches up to this many rows run the recurrent block's projections on DENSE8
-    copies (0: never)."""
+    copies (0: never).  The mixers of a device share their workspaces: their calls, replays among them,
+    follow one another, on one stream or by events."""
     _moe_block(module, topk)
     replica = copy.copy(module)
     replica._modules = dict(module._modules)
