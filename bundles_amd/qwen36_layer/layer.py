@@ -360,11 +360,12 @@ class _AttnMixer:
     def _chunk(self, positions, hidden_states, forward_batch):
         x = hidden_states
         rows = x.shape[0] if isinstance(x, torch.Tensor) and x.dim() == 2 else 0
-        axes = self.axes if isinstance(positions, torch.Tensor) and positions.dim() == 2 else None
+        shape = tuple(positions.shape) if isinstance(positions, torch.Tensor) else None
+        axes = self.axes if shape is not None and len(shape) == 2 else None
         view = getattr(self.engine, "chunk_view", None)
         ck = (view(self.layer_id, forward_batch)
               if view is not None and self.refusal is None and 0 < rows <= MAX_ROWS and x.dtype == torch.bfloat16
-              and tuple(positions.shape) == ((rows,) if axes is None else (axes.axes, rows)) else None)
+              and shape == ((rows,) if axes is None else (axes.axes, rows)) else None)
         if ck is None:
             return self.stock(self.replica, positions, hidden_states, forward_batch)
         sc = _ChunkScratch.get(x.device, rows)
