@@ -58,8 +58,8 @@ struct ChunkDev {
   float* ws_ml;  // [2 groups][8][2][32]: their running maxima (base 2) and weight sums
   int4* cuts;    // [groups] the tile that starts in each share and is cut: request (-1: none), 2 tile + head, last share; and
                  // whether a value on the causal border was NaN
-  uint32_t* flags;  // [groups] said when a share has written the partial that ends the tile which the share before starts
-  uint32_t* epoch;  // calls that this workspace has served
+  uint32_t* flags;  // [groups] said when a share has written the partial that ends the tile which the share before starts; 0
+                    // between calls (the combine kernel clears them: no call meets what another has said)
 };
 
 // A request's first row, new tokens and keys, inside the buffers whatever qsl and seqlens hold.
@@ -158,10 +158,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ int sums[8];
   __shared__ int found_at, found_b, nan_seen, joined;
   const int tid = threadIdx.x, wave = uni(tid >> 6), G = gridDim.x;
-  // what a flag of this call from this XCD says: its number among the workspace's calls, spread, and the XCD's
+  // what a flag from this XCD says: not 0, and the XCD's number
   uint32_t xcc;
   asm("s_getreg_b32 %0, hwreg(HW_REG_XCC_ID)" : "=s"(xcc));
-  const uint32_t mark = ((d.epoch[0] * 0x9e3779b1u) & ~31u) | 16u | (xcc & 15u);  // (not 0, what a workspace starts with)
+  const uint32_t mark = 16u | (xcc & 15u);
   // ---- this workgroup's share
   int total = 0, mine = 0;
   for (int c0 = 0; c0 < d.B; c0 += 512) {
@@ -672,7 +672,8 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
     if (n > 0) list[n <= kFew ? fat : 1023 - mat] = make_uint2((uint32_t)c.x << 16 | (uint32_t)n, (uint32_t)c.y << 12 | (uint32_t)(c0 + tid));
     __syncthreads();
   }
-  if (blockIdx.x == 0 && tid == 0) d.epoch[0] += 1;
+  if (blockIdx.x == 0)
+    for (int i = tid; i < G; i += 256) __hip_atomic_store(d.flags + i, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (lane == 0) nan_flags[wave] = nans != 0;
   __syncthreads();
   const bool any_nan = uni(nan_flags[0] | nan_flags[1] | nan_flags[2] | nan_flags[3]) != 0;
@@ -785,9 +786,9 @@ __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
   }
 }
 
-// A workspace before its first call: no calls served, no partial said to be there.
-__global__ __launch_bounds__(256) void chunk_init_kernel(uint32_t* epoch, int G) {
-  for (int i = threadIdx.x; i <= G; i += 256) epoch[i] = 0;
+// A workspace before its first call: no partial said to be there.
+__global__ __launch_bounds__(256) void chunk_init_kernel(uint32_t* flags, int G) {
+  for (int i = threadIdx.x; i < G; i += 256) flags[i] = 0;
 }
 
 // Workgroups: one a CU (their LDS and registers fill it).
@@ -801,7 +802,7 @@ ChunkWs chunk_ws(int G) {
   w.ml = align_up(w.o + sizeof(float) * 2 * (size_t)G * kSlotF, 256);
   w.cuts = align_up(w.ml + sizeof(float) * 2 * (size_t)G * kSlotML, 256);
   w.flags = align_up(w.cuts + sizeof(int4) * (size_t)G, 256);
-  w.total = align_up(w.flags + sizeof(uint32_t) * ((size_t)G + 1), 256);
+  w.total = align_up(w.flags + sizeof(uint32_t) * (size_t)G, 256);
   return w;
 }
 
@@ -850,8 +851,7 @@ extern "C" int q36_attn_chunk(const q36_chunk_args* a, q36_stream_t stream) {
   const ChunkDev d{a->B, a->T, sh, a->pt_stride, a->q_e4m3, a->num_slots, a->q, static_cast<const uint8_t*>(a->k_cache),
                    static_cast<const uint8_t*>(a->v_cache), a->page_table, a->seqlens, a->qsl, static_cast<uint16_t*>(a->out),
                    a->scale * 1.44269504088896340736f, reinterpret_cast<float*>(ws + L.o), reinterpret_cast<float*>(ws + L.ml),
-                   reinterpret_cast<int4*>(ws + L.cuts), reinterpret_cast<uint32_t*>(ws + L.flags) + 1,
-                   reinterpret_cast<uint32_t*>(ws + L.flags)};
+                   reinterpret_cast<int4*>(ws + L.cuts), reinterpret_cast<uint32_t*>(ws + L.flags)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   chunk_kernel<<<G, 512, 0, st>>>(d);
   chunk_combine_kernel<<<1024, 256, 0, st>>>(d, G);

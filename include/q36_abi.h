@@ -560,8 +560,8 @@ int q36_attn_front(const q36_attn_front_args* a, q36_stream_t stream);
  * pt_stride * page_size and slots outside the cache are clamped.
  * HQ = 16, HKV = 2, D = 256; T <= 2^20, B <= 65535, 0 < scale <= 1e6; q, out and caches 16-byte, workspace 256-byte
  * aligned.  Sizes whose worst split could weigh 2^30 steps (T / 32 + 2 B tiles over the tables' keys) are refused.
- * Workspace: q36_attn_chunk_workspace_bytes(), whatever the call's sizes (partials of the cut tiles, a count of the calls
- * it has served and what they said of their partials): any contents, made ready once by q36_attn_chunk_workspace_init
+ * Workspace: q36_attn_chunk_workspace_bytes(), whatever the call's sizes (partials of the cut tiles, and flags of those that
+ * are there, which every call leaves cleared): any contents, made ready once by q36_attn_chunk_workspace_init
  * (stream-ordered), then left to the calls, one after another; calls that may run at the same time (streams, graphs) need
  * one each. */
 typedef struct q36_chunk_args {

@@ -50,3 +50,19 @@ def test_not_within_a_capture(attn, dev):
         assert torch.equal(out, want)
         chunk.run(attn, h, dev, ws)
         torch.cuda.synchronize()
+
+
+def test_a_call_leaves_no_flag(attn, dev):
+    """Calls whose workgroups hand partials to one another leave the workspace's flags as the workspace entry does, at zero:
+    what an earlier call said of its partials is never there for another to take for its own."""
+    groups = torch.cuda.get_device_properties(dev).multi_processor_count
+    ws = attn.ChunkWorkspace(dev)
+    flags = ws.buf[-(-(-4 * groups // 256) * 256):].view(torch.int32)[:groups]
+    assert flags.numel() == groups and not bool(flags.any())
+    jobs = [chunk.make(lens, 16, 30 + i, dev) for i, lens in enumerate(([(2000, 2500)], [(700, 900)] * 8, [(5, 300)], [(3000, 3000), (1, 9000)]))]
+    want = [chunk.run(attn, h, dev).clone() for h in jobs]
+    for _ in range(3):
+        for h, w in zip(jobs, want):
+            out = chunk.run(attn, h, dev, ws)
+            torch.cuda.synchronize()
+            assert not bool(flags.any()) and torch.equal(out, w)
