@@ -96,6 +96,10 @@ constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a
 // The outputs are rescaled when a row's maximum has grown past 2^kLazyC times the one that the weights are relative to (a
 // weight is then at most 2^8, far inside f16).  8192 tokens at 0, 4, 8, 11, 14: 479, 440, 434, 434, 434 us.
 constexpr float kLazyC = 8.f;
+// m lies a step of its own, 2^-23 |m| to 2^-22 |m|, below the maximum, so that the maximum's weight is never lost to m's rounding.
+// Where scores can be so large that this step passes the 2^kLazyC of room (256 products of 448^2 times the scale, past 2^23),
+// weights are held at 2^kLazyC: such rows' scores are equal to within their own rounding.
+constexpr float kFarScale = 0x1p23f / (256.f * 448.f * 448.f);
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8)); }
@@ -358,6 +362,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   };
   const float sl2 = d.scale_log2;
+  const bool far = sl2 > kFarScale;
   bool begun = false;  // a block has been taken: m is its rows' largest, and grows
   auto clean = [&](v2i w) {
     const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y);
@@ -398,21 +403,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // new one.  (A row that sees nothing of a block sees nothing of the later ones.)
     float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sl2, -m);
-#pragma unroll
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
     const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
-    if (__builtin_expect(!begun || __builtin_amdgcn_ballot_w64(mx > kLazyC) != 0, 0)) {
+    const float top = __builtin_fmaf(mx, sl2, -m);
+    if (__builtin_expect(!begun || __builtin_amdgcn_ballot_w64(top > kLazyC) != 0, 0)) {
       // (each row by its own maximum alone: its bits do not depend on its wave's other rows)
-      const float up = mx > (begun ? kLazyC : -INFINITY) ? mx : 0.f, al = begun ? __builtin_amdgcn_exp2f(-up) : 1.f;
+      const float x = mx * sl2, mn = top > (begun ? kLazyC : -INFINITY) ? x - fabsf(x) * 0x1p-23f : m;
+      const float al = begun ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
       begun = true;
-      m += up;
+      m = mn;
       l *= al;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] -= up;
-#pragma unroll
       for (int dt = 0; dt < 8; ++dt) o[dt] *= al;
+    }
+    // one formula for every block: equal scores get equal weights, however coarse m is at its size
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sl2, -m);
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = s[i] > kLazyC ? kLazyC : s[i];
     }
     v8h pb[2];
 #pragma unroll
