@@ -6,7 +6,8 @@
 // (The reference re-pages the cache into 128-row pages and calls a library there, L/attn_fused.py:127-210.)
 //
 // Rounded: q to e4m3 (as attn_decode takes it), the weights p_j to f16 for the product with v (v is e4m3, exact in f16;
-// 2^-11 a weight, where e4m3 weights would lose 2^-4), the outputs to bf16.  Scores, maxima, weight sums and outputs: fp32.
+// 2^-11 a weight, where e4m3 weights would lose 2^-4; weights below 2^-21 of the row's largest by 2^-32 of it: kHead), the
+// outputs to bf16.  Scores, maxima, weight sums and outputs: fp32.
 //
 // Bounds.  Long chunks: the matrix units, half the products at the e4m3 rate and half at the f16 one: 289 us for 8192 tokens
 // from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 391 to 405 measured, 1.36 to 1.41 PFLOP/s.  A step of
@@ -55,7 +56,7 @@ struct ChunkDev {
   uint16_t* out;
   float scale_log2;
   float* ws_o;   // [2 groups][8][8][4][64][4]: partial outputs of 8 waves' 32 rows, unnormalised
-  float* ws_ml;  // [2 groups][8][2][32]: their running maxima (base 2) and weight sums
+  float* ws_ml;  // [2 groups][8][2][32]: what their weights are relative to (base 2) and the weights' sums
   int4* cuts;    // [groups] the tile that starts in each share and is cut: request (-1: none), 2 tile + head, last share; and
                  // whether a value on the causal border was NaN
   uint32_t* flags;  // [groups] said when a share has written the partial that ends the tile which the share before starts; 0
@@ -93,12 +94,15 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7
 constexpr int kBlk = 2 * kCST * kCD;  // 32 keys in LDS: their K rows, then their V rows
 constexpr int kSet = 4 * kBlk;
 constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a partial
-// The outputs are rescaled when a row's maximum has grown past 2^kLazyC times the one that the weights are relative to (a
-// weight is then at most 2^8, far inside f16).  8192 tokens at 0, 4, 8, 11, 14: 479, 440, 434, 434, 434 us.
+// Weights are relative to m, 7 binades below the row's maximum: the largest is 2^7, and the outputs are rescaled when the
+// maximum has grown past 2^kLazyC times the one that m was taken from, so a weight is at most 2^15, inside f16.  f16 ends at
+// half a step of 2^-25: 2^-32 of the largest weight, which 2^20 keys below it lose together as 2^-12 (with no head, 2^-5).
+constexpr float kHead = 7.f;
+// 8192 tokens at 0, 4, 8, 11, 14: 479, 440, 434, 434, 434 us.
 constexpr float kLazyC = 8.f;
-// m lies a step of its own, 2^-23 |m| to 2^-22 |m|, below the maximum, so that the maximum's weight is never lost to m's rounding.
-// Where scores can be so large that this step passes the 2^kLazyC of room (256 products of 448^2 times the scale, past 2^23),
-// weights are held at 2^kLazyC: such rows' scores are equal to within their own rounding.
+// m lies a step of its own, 2^-23 |m| to 2^-22 |m|, below the maximum at the least, so that the maximum's weight is never lost
+// to m's rounding.  Where scores can be so large that this step takes the room of f16 (256 products of 448^2 times the scale,
+// past 2^23), weights are held at 2^(kHead + kLazyC): such rows' scores are equal to within their own rounding.
 constexpr float kFarScale = 0x1p23f / (256.f * 448.f * 448.f);
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -363,7 +367,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   const float sl2 = d.scale_log2;
   const bool far = sl2 > kFarScale;
-  bool begun = false;  // a block has been taken: m is its rows' largest, and grows
+  bool begun = false;  // a block has been taken: m is of its rows' largest, and grows
   auto clean = [&](v2i w) {
     const uint32_t n0 = nan_bytes(w.x), n1 = nan_bytes(w.y);
     bad |= n0 | n1;
@@ -399,17 +403,17 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int i = 0; i < 16; ++i)
         if (key0 + 8 * (i >> 2) + 4 * g0 + (i & 3) > lim) s[i] = -INFINITY;
     }
-    // relative to the running maximum, which the first block sets; where a row grows past 2^8 times it, the row moves to the
-    // new one.  (A row that sees nothing of a block sees nothing of the later ones.)
+    // relative to m, which the first block sets; where a row grows past 2^8 times the maximum that m is of, the row moves to
+    // the new one.  (A row that sees nothing of a block sees nothing of the later ones.)
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[i]), s[i + 1]);
     const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
     const float top = __builtin_fmaf(mx, sl2, -m);
-    if (__builtin_expect(!begun || __builtin_amdgcn_ballot_w64(top > kLazyC) != 0, 0)) {
+    if (__builtin_expect(!begun || __builtin_amdgcn_ballot_w64(top > kHead + kLazyC) != 0, 0)) {
       // (each row by its own maximum alone: its bits do not depend on its wave's other rows)
-      const float x = mx * sl2, mn = top > (begun ? kLazyC : -INFINITY) ? x - fabsf(x) * 0x1p-23f : m;
+      const float x = mx * sl2, mn = top > (begun ? kHead + kLazyC : -INFINITY) ? x - fmaxf(kHead, fabsf(x) * 0x1p-23f) : m;
       const float al = begun ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
       begun = true;
       m = mn;
@@ -422,7 +426,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sl2, -m);
     if (far) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = s[i] > kLazyC ? kLazyC : s[i];
+      for (int i = 0; i < 16; ++i) s[i] = s[i] > kHead + kLazyC ? kHead + kLazyC : s[i];
     }
     v8h pb[2];
 #pragma unroll

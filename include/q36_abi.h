@@ -554,8 +554,9 @@ int q36_attn_front(const q36_attn_front_args* a, q36_stream_t stream);
  * its i-th new token sees keys 0 .. seqlens[b] - new + i.  page_table int32 [B, pt_stride]: entry j is the page of keys
  * j page_size .. (page_size a power of two; 1: the slots themselves).  k_cache, v_cache e4m3 [num_slots, HKV, D].
  * out bf16 [T, HQ, D] = bf16(sum_j p_j v_j / sum_j p_j), p_j = exp(scale (q . k_j) - max): scores, maxima, sums and the
- * output in fp32, p_j rounded to f16 for the product with v.  A row that sees no key is zero; rows outside
- * qsl[0] .. qsl[B] are left as they were.  What a row does not see, NaN included, does not reach it.
+ * output in fp32, p_j rounded to f16 for the product with v (by 2^-11 of itself or 2^-32 of the row's largest).  A row that
+ * sees no key is zero; rows outside qsl[0] .. qsl[B] are left as they were.  What a row does not see, NaN included, does not
+ * reach it.
  * Whatever the device data hold, every access stays inside the buffers: rows outside T, keys past the page table's
  * pt_stride * page_size and slots outside the cache are clamped.
  * HQ = 16, HKV = 2, D = 256; T <= 2^20, B <= 65535, 0 < scale <= 1e6; q, out and caches 16-byte, workspace 256-byte
