@@ -196,6 +196,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     return;
   }
   const int x0 = share * len, x1 = min(total, x0 + len);
+  const bool joins = len >= kJoinShare;
   // the request that x0 lies in
   if (d.B <= 512) {
     const int off = before + inc - mine;
@@ -472,10 +473,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int tok0 = first_tok(cur), rw = wide ? wave : wave & 1;
       const int lane = fresh_tid() & 63, col = lane & 31, g = lane >> 5;
       // A wide tile that the next share ends, most likely long ago, with its first run: where that partial is there, in this
-      // XCD's L2, the two are joined here, by the combine kernel's arithmetic; else the combine kernel does it.  (With and
-      // without: 8192 tokens 434, 451 us, 16 prompts of 64 .. 2000 123, 131; four chunks of 200 .. 700 52, 49.)
+      // XCD's L2, the two are joined here, by the combine kernel's arithmetic; else, and in calls of short shares
+      // (kJoinShare), the combine kernel does it.
       bool join = false;
-      if (wide && cur.lasts == share + 1) {
+      if (joins && wide && cur.lasts == share + 1) {
         if (tid == 0) joined = __hip_atomic_load(d.flags + share + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
         barrier();
         join = uni(joined) != 0;
@@ -574,7 +575,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           if (g == 0) wml[0] = m, wml[32] = l;
         }
       }
-      if (wide && cur.pair) {
+      if (joins && wide && cur.pair) {
         wait_vm0();
         barrier();  // the partial is in L2
         if (tid == 0) __hip_atomic_store(d.flags + share, mark, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -24,6 +24,12 @@ constexpr int kTileOvh = 8;
 constexpr int kNarrowCost = 2;
 // A share is no shorter than a narrow step.  Five tokens over 300 keys at 2, 4, 8, 20: 20.0, 21.5, 22.7, 32.8 us.
 constexpr int kLeastShare = kNarrowCost;
+// Shares of this length and longer join a tile that two of them cut, where they meet; of shorter ones the second kernel joins
+// it, in parallel, while the join, 256 KB read by one workgroup, would make up the call's end.  us a call joined by the shares,
+// by the second kernel (share): four chunks of 200 .. 700 tokens 38.6, 34.9 (6), behind 1000 keys 64.5, 59.1 (20), behind 2000
+// 83.3, 76.8 (33), behind 4000 115.8, 115.8 (59); prompts: one of 2048 62.0, 58.6 (20), 3000 92.0, 90.6 (40), 4096 131.7, 140.7
+// (72), 8192 425, 439 (257); 16 of 64 .. 1000 53.7, 54.7 (25); 8 of 120 .. 2000 77.8, 82.8 (40).
+constexpr int kJoinShare = 36;
 
 struct ChunkReq {
   int n, nk;  // new tokens, keys (the new ones included)
