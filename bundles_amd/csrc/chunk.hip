@@ -10,12 +10,14 @@
 // outputs to bf16.  Scores, maxima, weight sums and outputs: fp32.
 //
 // Bounds.  Long chunks: the matrix units, half the products at the e4m3 rate and half at the f16 one: 289 us for 8192 tokens
-// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 391 to 405 measured, 1.36 to 1.41 PFLOP/s.  A step of
-// 32 keys takes a workgroup 1.4 us (2.8 K cycles), of which the matrix units are busy 1.54 K and the vector units (scores to
-// weights: 16 exponentials, maxima and sums a lane, and the values' widening, for 2 waves a SIMD) 1.6 K; the next block's
-// scores formed beside this one's weights would overlap them better, and did not fit the registers (54 spilled).
-// Short calls: the latency of one pass: lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second launch 4: 17 us for five tokens over 300
-// keys.  Between: cut tiles, 256 KB a partial out of and back into the Infinity Cache (7 TB/s over the chip).
+// from an empty cache at the rates of large library products (3161 and 1359 TFLOP/s); 389 to 425 measured (cards differ under
+// this load), 1.29 to 1.41 PFLOP/s.  A step of 32 keys takes a workgroup 1.4 to 1.6 us (2.8 K cycles), of which the matrix
+// units are busy 1.54 K and the vector units (scores to weights: 16 exponentials, maxima and sums a lane, and the values'
+// widening, for 2 waves a SIMD) 1.6 K; the next block's scores formed beside this one's weights would overlap them better,
+// and did not fit the registers (54 spilled).
+// Short calls: the latency of one pass: lengths, shares and page tables 5 us, queries 2 to 5, a tile's end 3, the second
+// launch 4: 17 us for five tokens over 300 keys.  Between: cut tiles, 256 KB a partial out of and back into the Infinity
+// Cache (7 TB/s over the chip).
 //
 // Why so.  256 rows a workgroup: one pass over a tile's keys feeds eight waves from LDS (a wave alone would need four times
 // the L2 rate).  LDS filled by copies past the registers: o holds 128 of a lane's 256 and q 32.  V^T by the transposing LDS
@@ -98,7 +100,7 @@ constexpr int kSlotF = 8 * 8 * 4 * 64 * 4, kSlotML = 8 * 2 * 32;  // floats of a
 // maximum has grown past 2^kLazyC times the one that m was taken from, so a weight is at most 2^15, inside f16.  f16 ends at
 // half a step of 2^-25: 2^-32 of the largest weight, which 2^20 keys below it lose together as 2^-12 (with no head, 2^-5).
 constexpr float kHead = 7.f;
-// 8192 tokens at 0, 4, 8, 11, 14: 479, 440, 434, 434, 434 us.
+// 8192 tokens at 0, 4, 8: 469, 438, 425 us; 2048 behind 6000 224, 209, 201.  (Past 8 a weight would leave f16.)
 constexpr float kLazyC = 8.f;
 // m lies a step of its own, 2^-23 |m| to 2^-22 |m|, below the maximum at the least, so that the maximum's weight is never lost
 // to m's rounding.  Where scores can be so large that this step takes the room of f16 (256 products of 448^2 times the scale,
@@ -475,6 +477,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       // A wide tile that the next share ends, most likely long ago, with its first run: where that partial is there, in this
       // XCD's L2, the two are joined here, by the combine kernel's arithmetic; else, and in calls of short shares
       // (kJoinShare), the combine kernel does it.
+      // What makes this right without a release and an acquire, which would write back and empty whole caches: the flag says
+      // the writer's XCD, so writer and reader share one L2; the writer waits until its stores have reached it before it says
+      // so; the flag itself is read and written past the L1; and the reader's L1 has no line of the partial, since a launch
+      // starts with an empty one and within a launch a partial is read once, here.  A second reader of a slot in the same
+      // launch, on this CU, could meet an old line.
       bool join = false;
       if (joins && wide && cur.lasts == share + 1) {
         if (tid == 0) joined = __hip_atomic_load(d.flags + share + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
@@ -497,7 +504,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const float f = __builtin_amdgcn_exp2f(m - M), il = L > 0.f ? 1.f / L : L;
         if (slot >= 0 && wave < 2 && g == 0) wml[0] = M, wml[32] = L;
         // two dim tiles at a time through LDS, [wave][dt][a][lane]; wave (k, rw) sums quads 2 k, 2 k + 1 of the eight of rw
-        // (rows 32 .. 63 only where there are more than 4 tokens: 4 requests of one token over 32000 keys 48.1 -> 44.4 us)
+        // (rows 32 .. 63 only where there are more than 4 tokens: 4 requests of one token over 32000 keys 40.5 -> 39.5 us)
         const bool some = tok0 < cur.n;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -620,7 +627,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int k = cur.key0 + st * SET + 32 * i;
         if (k >= end) break;
         // a SIMD's older wave wins where both could issue, and its other one would then end each set alone: they take turns
-        // (8192 tokens 416 -> 407 us)
+        // (8192 tokens 434 -> 425 us, 2048 behind 6000 207 -> 201)
         if (((i >> 1) ^ (wave >> 2)) & 1) __builtin_amdgcn_s_setprio(1);
         else __builtin_amdgcn_s_setprio(0);
         block(to + i * kBlk, k, k + 31 > pre + tok0);
@@ -658,9 +665,9 @@ __device__ __forceinline__ uint2 put_nans(uint2 v, uint32_t n) {
 // a workgroup takes 32 rows and 64 dims at a time, wave a the lanes' a-th four dims of each 32, four partials' loads in
 // flight.  More: 32 rows and 8 dims, wave w has partials w, w + 4, .., eight at a time, and the waves' sums meet in LDS: four
 // times the workgroups for a tile, for tiles that are few.  Bound by the partials' bytes, out of the Infinity Cache: 2048
-// tokens behind 6000 (128 tiles, 3 partials each, 96 MB) in 19 us.  us a call at kFew 4, 16, 32, 256: three chunks of 130 ..
-// 300 tokens over long contexts (6 partials a tile) 274, 250, 250, -; two of 90 tokens (21) 110, 109, 104, 101; one of 32 (128)
-// 49, 49, 49, 63.
+// tokens behind 6000 (128 tiles, 3 partials each, 96 MB) in 20 us.  us a call at kFew 4, 16, 32, 256: three chunks of 130 ..
+// 300 tokens over long contexts (6 partials a tile) 243, 232, 232, 233; two of 90 tokens behind 30000 (21) 95, 95, 92, 92; one
+// of 32 behind 32000 (128) 46, 46, 46, 58.
 constexpr int kFew = 32;
 __global__ __launch_bounds__(256) void chunk_combine_kernel(ChunkDev d, int G) {
   // request and partials (16 bits each), 2 tile + head (20 bits) and share: few partials from the front, many from the back

@@ -11,8 +11,8 @@
 // One launch: a workgroup takes a segment of one request and forms that request's two prefix sums from the counts of
 // the requests before it (8 bytes a request, in L2), so no workgroup waits for another.  New pages are read from the
 // free list, never from a table entry that another workgroup writes.  Bound by the launch and two loads behind one another
-// (lengths, then pages): 3.9 us on the GPU for 7 decoding requests, 5.5 for 203 of up to 8191 keys (1.1 MB), 10.5 for 256 of
-// up to 32000 (14 MB, 1.4 TB/s); a call from Python takes 8 us at the least.
+// (lengths, then pages): 3.9 us on the GPU for 7 decoding requests, 5.5 for 203 of up to 8191 keys (1.1 MB), 10.6 for 256 of
+// up to 32000 (14 MB, 1.3 TB/s); a call from Python takes 8 us at the least.
 #include <algorithm>
 
 #include "q36_device.h"
@@ -145,7 +145,7 @@ extern "C" int q36_page_plan(const q36_page_plan_args* a, q36_stream_t stream) {
   while ((1 << sh) < a->page_size) ++sh;
   // Segments: 2048 keys or tokens a workgroup where the batch is small, no more workgroups than fill the chip's CUs eight
   // times over (a segment's threads walk on through a longer request).  On the GPU, at 512 / 2048 / 8192 keys a segment: 203
-  // requests of up to 8191 keys 6.6 / 5.5 / 6.7 us, 256 of up to 32000 10.7 / 10.5 / 12.5.
+  // requests of up to 8191 keys 6.5 / 5.5 / 6.8 us, 256 of up to 32000 10.6 / 10.6 / 12.5.
   const int most = std::max(a->page_table && a->whole ? a->pt_width : 0, a->T / a->B);
   const int segs = std::max(1, std::min((most - 1) / 2048 + 1, std::max(1, 2048 / a->B)));
   PlanDev d{a->B, a->T, sh, a->table_rows, a->table_width, a->free_count, a->pt_width, a->whole ? 1 : 0, segs,

@@ -13,16 +13,17 @@
 
 namespace q36 {
 
-// kNarrow, us a call: 16 requests behind 500 keys, 4 behind 8000.  8 tokens as a narrow tile 21.2, 28.4, as a wide one 21.0,
-// 31.4; 12 tokens as two narrow ones 24.8, 36.1, as a wide one 22.4, 32.8; 16 tokens 27.0, 37.0 against 24.4, 33.8.
+// kNarrow, us a call: 16 requests of 8 tokens behind 500 keys, 4 behind 8000: as narrow tiles 23.5, 28.8, as wide ones 23.0,
+// 30.5.  (A narrow tile holds 8 tokens; 12 and 16 as two of them took 10 % longer than as a wide one.)
 constexpr int kNarrow = 8, kWideTok = 32, kWideKeys = 32, kNarrowKeys = 128;
-// kTileOvh, us a call at 6, 7, 8, 9, 10: eight prompts 51.5, 49.4, 48.6, 52.2, 53.5; 64 requests of 1 .. 200 tokens 41.9, 40.7,
-// 38.7, 39.3, 40.7; 24 requests, chunks beside single tokens, 56 to 59, and one of 8192 tokens 391 to 395 at all of them.
+// kTileOvh, us a call at 6, 7, 8, 9, 10: eight prompts 45.7, 47.3, 47.2, 48.1, 50.8; 64 requests of 1 .. 200 tokens 21.9, 22.6,
+// 22.1, 22.7, 22.0; 24 requests, chunks beside single tokens, 52.9, 53.9, 55.3, 54.7, 56.6; one of 8192 tokens 390 to 393.
+// (Chosen when shares joined every cut tile: eight prompts 51.5 at 6, 48.6 at 8.)
 constexpr int kTileOvh = 8;
-// What a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16.  us a call at 2, 3: 64 requests of 1 .. 200
-// tokens 38.7, 43.7; 12 of 1 .. 300 over up to 6000 keys 48.9, 54.5; 24, chunks beside single tokens, 59, 57 (at 1: 66).
+// What a narrow step weighs: it brings 64 KB for a block a wave, a wide one 16.  us a call at 1, 2, 3: 12 requests of 1 .. 300
+// tokens over up to 6000 keys 48.5, 41.7, 42.4; 64 of 1 .. 200 21.8, 22.2, 22.2; 24, chunks beside single tokens, 56.0, 55.7, 55.9.
 constexpr int kNarrowCost = 2;
-// A share is no shorter than a narrow step.  Five tokens over 300 keys at 2, 4, 8, 20: 20.0, 21.5, 22.7, 32.8 us.
+// A share is no shorter than a narrow step.  Five tokens over 300 keys at 2, 4, 8, 20: 17.6, 19.0, 20.2, 29.4 us.
 constexpr int kLeastShare = kNarrowCost;
 // Shares of this length and longer join a tile that two of them cut, where they meet; of shorter ones the second kernel joins
 // it, in parallel, while the join, 256 KB read by one workgroup, would make up the call's end.  us a call joined by the shares,
@@ -96,9 +97,11 @@ __host__ __device__ __forceinline__ int ck_share_len(int total, int G) {
 __host__ __device__ __forceinline__ int ck_shares(int total, int len) { return (total + len - 1) / len; }
 
 // A cut of a wide tile costs some ten steps: its 256 KB leave and come back, and its queries are read twice.  So one that
-// falls within kSnap steps of the tile's end goes to that end.  us a call at 0, 3, 4, 5, 6: eight prompts 60.4 (of a slower
-// step), 48.7, 48.6, 53.8, 52.7; 64 requests of 1 .. 200 tokens at 3 .. 6: 44.4, 38.7, 37.9, 37.4; 2048 tokens behind 6000
-// 199, 199, 198, 205.  A narrow tile's cut costs little (five tokens over 300 keys: 21.6 with it moved, 19.7 without).
+// falls within kSnap steps of the tile's end goes to that end.  us a call at 0, 3, 4, 5, 6: eight prompts 49.1, 48.8, 47.6, 47.0,
+// 46.2; 64 requests of 1 .. 200 tokens 28.5, 22.1, 22.2, 22.1, 22.1; 24, chunks beside single tokens, 52.8, 53.4, 55.4, 56.4, 55.4;
+// 2048 tokens behind 6000 191, 190, 190, 189, 194.  A narrow tile's cut stays where it falls: with it moved, without, five tokens
+// over 300 keys 18.5, 17.3, four requests of 8 behind 8000 33.2, 28.3, of one over 32000 44.5, 40.0, but 70 of one over 700 24.7,
+// 34.4.
 // A tile's cuts lie behind step ck_lo and before ck_hi.
 constexpr int kSnap = 4;
 __host__ __device__ __forceinline__ int ck_lo(int steps, int cost) {
