@@ -120,6 +120,27 @@ class ChunkArgs(C.Structure):
                 ("seqlens", P), ("qsl", P), ("out", P), ("workspace", P), ("workspace_bytes", SZ), ("scale", C.c_float)]
 
 
+class GdnCommitArgs(C.Structure):
+    _fields_ = [(n, I32) for n in ("B", "T", "room", "advance", "slots", "rslots", "wslots", "idx_i64")] + \
+               [("conv_state", P), ("cs_slot", I64), ("window", P), ("win_slot", I64), ("h0", P), ("d_ring", P),
+                ("dlo_ring", P), ("d_slot", I64), ("dlo_slot", I64), ("k_ring", P), ("klo_ring", P), ("k_slot", I64),
+                ("klo_slot", I64), ("g_ring", P), ("g_slot", I64), ("state_idx", P), ("replay_idx", P), ("win_idx", P),
+                ("accepted", P), ("write_pos", P), ("cache_base", P)]
+
+
+class GdnPromptArgs(C.Structure):
+    _fields_ = [(n, I32) for n in ("B", "rows", "slots", "idx_i64", "dt_f32")] + \
+               [("eps", C.c_float), ("scale", C.c_float), ("mixed", P), ("z", P), ("a", P), ("b", P), ("conv_state", P),
+                ("cs_slot", I64), ("conv_w", P), ("A_log", P), ("dt_bias", P), ("h0", P), ("qsl", P), ("state_idx", P),
+                ("prefix", P), ("norm_w", P), ("out", P), ("oq", P), ("oqs", P), ("workspace", P), ("workspace_bytes", SZ)]
+
+
+class VerifyDraftsArgs(C.Structure):
+    _fields_ = [(n, I32) for n in ("B", "T", "V", "logits_f32")] + \
+               [("ld", I64), ("logits", P), ("temperature", P), ("drafts", P), ("uniforms", P), ("draft_probs", P),
+                ("tokens", P), ("counts", P), ("workspace", P), ("workspace_bytes", SZ)]
+
+
 def _packer(st):
     """struct.pack of a structure's fields in order (nested arrays flattened): the bytes of the filled structure, for packed().
     Filling the ctypes structure itself took longer than the launch it describes (45 fields: 5 us against 1)."""
@@ -139,6 +160,7 @@ pack_moe, pack_gdn, pack_ring, pack_attn = map(_packer, (MoeArgs, GdnArgs, GdnRi
 pack_oproj, pack_lmhead, pack_fp8, pack_dense8 = map(_packer, (OprojArgs, LmheadArgs, Fp8LinearArgs, Dense8LinearArgs))
 pack_addnorm, pack_decode = map(_packer, (AddNormArgs, DecodeArgs))
 pack_plan, pack_front, pack_chunk = map(_packer, (PagePlanArgs, AttnFrontArgs, ChunkArgs))
+pack_commit, pack_prompt, pack_drafts = map(_packer, (GdnCommitArgs, GdnPromptArgs, VerifyDraftsArgs))
 
 
 _lib = _packed = None
@@ -157,6 +179,9 @@ SYMBOLS = [
     ("q36_moe_forward_static", I32, [C.POINTER(MoeArgs), P]),
     ("q36_gdn_verify", I32, [C.POINTER(GdnArgs), P]),
     ("q36_gdn_verify_ring", I32, [C.POINTER(GdnRingArgs), P]),
+    ("q36_gdn_ring_commit", I32, [C.POINTER(GdnCommitArgs), P]),
+    ("q36_gdn_prompt_workspace_bytes", SZ, [I32, I32]),
+    ("q36_gdn_prompt", I32, [C.POINTER(GdnPromptArgs), P]),
     ("q36_attn_act_frag", I32, [I32]),
     ("q36_attn_workspace_bytes", SZ, [I32]),
     ("q36_oproj_workspace_bytes", SZ, [I32]),
@@ -177,6 +202,8 @@ SYMBOLS = [
     ("q36_attn_chunk", I32, [C.POINTER(ChunkArgs), P]),
     ("q36_lmhead_workspace_bytes", SZ, [I32]),
     ("q36_lmhead_argmax", I32, [C.POINTER(LmheadArgs), P]),
+    ("q36_verify_drafts_workspace_bytes", SZ, [I32, I32, I32]),
+    ("q36_verify_drafts", I32, [C.POINTER(VerifyDraftsArgs), P]),
     ("q36_quant_rows_i8", I32, [P, C.c_int64, I32, P, P, P]),
     ("q36_q8_block_v1_bytes", SZ, [I32, I32]),
     ("q36_quant_q8_block_v1", I32, [P, P, I32, I32, I32, I32, P, P]),
@@ -189,6 +216,7 @@ OPTIONAL_SYMBOLS: list = []
 ARG_POINTERS = [C.POINTER(s) for s in (MoeArgs, GdnArgs, GdnRingArgs, AttnArgs, OprojArgs, LmheadArgs, Fp8LinearArgs,
                                        AddNormArgs, Dense8LinearArgs, DecodeArgs)]
 CHUNK_POINTERS = [C.POINTER(s) for s in (PagePlanArgs, AttnFrontArgs, ChunkArgs)]  # the prompt chunk's entries
+STATE_POINTERS = [C.POINTER(s) for s in (GdnCommitArgs, GdnPromptArgs, VerifyDraftsArgs)]  # the recurrent state's and the drafts'
 
 
 def _load(arg0):
@@ -216,7 +244,7 @@ def packed():
     bytes into one costs 0.3 us a call.)"""
     global _packed
     if _packed is None:
-        _packed = _load(lambda a: P if a in ARG_POINTERS or a in CHUNK_POINTERS else a)
+        _packed = _load(lambda a: P if a in ARG_POINTERS or a in CHUNK_POINTERS or a in STATE_POINTERS else a)
     return _packed
 
 

@@ -1,0 +1,425 @@
+// Verification of drafted tokens against the target's logits, from given random numbers: how many of a request's drafts
+// stand, and the token that follows them.  (No reference counterpart: the reference's node ends at the logits and the
+// serving engine samples; R/qwen36_lmhead8/node.py:136-151.)
+//
+// Row t of a request's T rows holds the logits behind window token t, p = softmax(logits / temperature).  Draft t + 1 stands
+// iff the ones before it do and u_t q(d) < p(d), q = 1 at d where no draft probabilities are given.  At the first that does
+// not, the token is drawn from max(p - q, 0); behind the last draft from p: the first index whose running sum passes
+// u_last times the total.  Temperature 0 (or NaN): p is 1 at the first largest logit.
+//
+// The draw compares running sums over the whole vocabulary with one number, so weights and sums are fp64 (a weight is good
+// to 7e-12): with fp32 weights one draw in a few hundred would land on a neighbour.  fp64 costs no more than fp32 here, the
+// vector unit issues both at one rate.
+#include <type_traits>
+
+#include "q36_device.h"
+#include "q36_host.h"
+
+namespace q36 {
+namespace {
+
+constexpr int kThreads = 256, kPer = 16, kSeg = kThreads * kPer;  // logits a thread, a segment
+constexpr int kMaxT = 8;
+
+struct DraftsDev {
+  int B, T, V, segs;
+  int64_t ld;
+  const void* logits;
+  const float* temperature;
+  const int32_t* drafts;
+  const float* uniforms;
+  const float* probs;  // [B, T - 1, V] or null
+  double* psum;        // [rows, segs] sum of a segment's weights, relative to its largest logit
+  float* pmax;         // [rows, segs] that logit
+  int32_t* pidx;       // [rows, segs] its first index
+  double* rsum;        // [B, segs] a segment's residual
+  int32_t* tokens;
+  int32_t* counts;
+};
+
+// The factor of the exponent's base-2 form, 0 for a greedy request.
+__device__ __forceinline__ double heat_of(const DraftsDev& d, int b) {
+  const float t = d.temperature ? d.temperature[b] : 1.f;
+  return t > 0.f ? 1.4426950408889634074 / (double)fminf(t, 1e30f) : 0.0;
+}
+
+// 2^((x - m) s) for x <= m, 1 at x == m whatever m is (an infinite largest logit leaves weight to its equals alone): the
+// fraction's power by its series up to f^9, off by at most (ln 2 / 2)^10 / 10! = 7e-12.
+__device__ __forceinline__ double weight(float x, float m, double s) {
+  double y = ((double)x - (double)m) * s;
+  y = y > -1100.0 ? y : -1100.0;  // (also NaN: minus infinity below itself, or beside an infinite largest)
+  const double n = __builtin_rint(y), f = y - n;
+  double p = 1.0178086009239699e-07;
+  p = __builtin_fma(p, f, 1.3215486790144307e-06);
+  p = __builtin_fma(p, f, 1.5252733804059841e-05);
+  p = __builtin_fma(p, f, 1.5403530393381608e-04);
+  p = __builtin_fma(p, f, 1.3333558146428443e-03);
+  p = __builtin_fma(p, f, 9.6181291076284772e-03);
+  p = __builtin_fma(p, f, 5.5504108664821580e-02);
+  p = __builtin_fma(p, f, 2.4022650695910071e-01);
+  p = __builtin_fma(p, f, 6.9314718055994531e-01);
+  p = __builtin_fma(p, f, 1.0);
+  p = __builtin_ldexp(p, (int)n);
+  return x == m ? 1.0 : p;
+}
+
+// Logits base .. base + kPer - 1 of a row; past V and NaN: minus infinity.
+template <bool F32, bool VEC>
+__device__ __forceinline__ void load_logits(const DraftsDev& d, int64_t row, int base, float (&x)[kPer]) {
+  const float none = -__builtin_inff();
+  if (VEC && base + kPer <= d.V) {
+    if constexpr (F32) {
+      const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(d.logits) + row * d.ld + base);
+      v4f r[kPer / 4];
+#pragma unroll
+      for (int i = 0; i < kPer / 4; ++i) r[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = r[i >> 2][i & 3];
+    } else {
+      const v4i* p = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.logits) + row * d.ld + base);
+      v4i r[kPer / 8];
+#pragma unroll
+      for (int i = 0; i < kPer / 8; ++i) r[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) {
+        x[i] = bf_lo((uint32_t)r[i >> 3][(i >> 1) & 3]);
+        x[i + 1] = bf_hi((uint32_t)r[i >> 3][(i >> 1) & 3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      x[i] = none;
+      if (base + i < d.V)
+        x[i] = F32 ? static_cast<const float*>(d.logits)[row * d.ld + base + i]
+                   : bf2f(static_cast<const uint16_t*>(d.logits)[row * d.ld + base + i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) x[i] = x[i] == x[i] ? x[i] : none;
+}
+
+template <bool F32>
+__device__ __forceinline__ float logit_at(const DraftsDev& d, int64_t row, int i) {
+  const float x = F32 ? static_cast<const float*>(d.logits)[row * d.ld + i]
+                      : bf2f(static_cast<const uint16_t*>(d.logits)[row * d.ld + i]);
+  return x == x ? x : -__builtin_inff();
+}
+
+// Sum over the wave, the same in every lane.
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// A segment of a row: its largest logit, the first index of it, the sum of its weights.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
+  __shared__ float wm[4];
+  __shared__ int wi[4];
+  __shared__ double ws[4];
+  const int64_t row = blockIdx.x / (unsigned)d.segs;
+  const int seg = blockIdx.x % (unsigned)d.segs;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float x[kPer];
+  const int base = seg * kSeg + tid * kPer;
+  load_logits<F32, VEC>(d, row, base, x);
+  const double s = heat_of(d, (int)(row / d.T));
+  float m = x[0];
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
+  m = wave_max(m);
+  int first = 0x7fffffff;
+#pragma unroll
+  for (int i = kPer - 1; i >= 0; --i) first = x[i] == m ? base + i : first;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o));
+  double sum = 0.0;
+  if (s > 0.0 && m > -__builtin_inff()) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
+    sum = wave_sum_d(sum);
+  }
+  if (lane == 0) wm[wave] = m, wi[wave] = first, ws[wave] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    double S = 0.0;
+    int I = 0x7fffffff;
+    for (int w = 3; w >= 0; --w) {
+      if (wm[w] == M) I = wi[w];
+      if (s > 0.0 && wm[w] > -__builtin_inff()) S += ws[w] * weight(wm[w], M, s);
+    }
+    const int64_t o = row * d.segs + seg;
+    d.pmax[o] = M, d.psum[o] = S, d.pidx[o] = I;
+  }
+}
+
+// What a request's rows say: the accepted drafts, and the row the next token is drawn from.
+struct Chain {
+  float m[kMaxT];     // a row's largest logit
+  int idx[kMaxT];     // its first index
+  double norm[kMaxT]; // sum of the row's weights
+  float xd[kMaxT];    // the draft's logit
+  double q[kMaxT];    // its draft probability
+  int j, refused, ended;
+};
+
+// Every wave takes rows wave, wave + waves, ..; then thread 0 walks the drafts.  (Callers synchronise behind it.)
+template <bool F32>
+__device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  for (int t = wave; t < d.T; t += waves) {
+    const int64_t row = (int64_t)b * d.T + t, o = row * d.segs;
+    float m = -__builtin_inff();
+    for (int i = lane; i < d.segs; i += 64) m = fmaxf(m, d.pmax[o + i]);
+    m = wave_max(m);
+    double n = 0.0;
+    int first = 0x7fffffff;
+    for (int i = lane; i < d.segs; i += 64) {
+      const float pm = d.pmax[o + i];
+      if (pm > -__builtin_inff()) {
+        if (pm == m) first = min(first, d.pidx[o + i]);
+        if (s > 0.0) n += d.psum[o + i] * weight(pm, m, s);
+      }
+    }
+    n = wave_sum_d(n);
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) first = min(first, __shfl_xor(first, k));
+    if (lane == 0) {
+      c->m[t] = m, c->idx[t] = first, c->norm[t] = n;
+      if (t + 1 < d.T) {
+        const int tok = d.drafts[(int64_t)b * (d.T - 1) + t];
+        const bool in = tok >= 0 && tok < d.V;
+        c->xd[t] = in ? logit_at<F32>(d, row, tok) : -__builtin_inff();
+        c->q[t] = in && d.probs ? (double)d.probs[((int64_t)b * (d.T - 1) + t) * d.V + tok] : 1.0;
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int j = 0, refused = 0, ended = 0;
+    for (; j < d.T; ++j) {
+      const float m = c->m[j];
+      if (!(m > -__builtin_inff())) {  // a row that leaves no token
+        ended = 1;
+        break;
+      }
+      if (j == d.T - 1) break;
+      const int tok = d.drafts[(int64_t)b * (d.T - 1) + j];
+      if (tok < 0 || tok >= d.V) break;  // no draft: the token is drawn from p
+      const double p = s > 0.0 ? weight(c->xd[j], m, s) / c->norm[j] : (c->idx[j] == tok ? 1.0 : 0.0);
+      if (!((double)d.uniforms[(int64_t)b * d.T + j] * c->q[j] < p)) {
+        refused = 1;
+        break;
+      }
+    }
+    c->j = j, c->refused = refused, c->ended = ended;
+  }
+}
+
+// Residual sums of the row that a request's token is drawn from, where draft probabilities were given.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) {
+  __shared__ Chain c;
+  __shared__ double ws[4];
+  const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
+  const double s = heat_of(d, b);
+  walk<F32>(d, b, s, &c);
+  __syncthreads();
+  double sum = 0.0;
+  if (c.refused) {
+    const int j = c.j;
+    const int64_t row = (int64_t)b * d.T + j;
+    const float* q = d.probs + ((int64_t)b * (d.T - 1) + j) * d.V;
+    const int base = seg * kSeg + tid * kPer;
+    float x[kPer];
+    load_logits<F32, VEC>(d, row, base, x);
+    const double inv = 1.0 / c.norm[j];
+    for (int i = 0; i < kPer; ++i) {
+      if (base + i >= d.V) break;
+      const double p = s > 0.0 ? weight(x[i], c.m[j], s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
+      const double r = p - (double)q[base + i];
+      sum += r > 0.0 ? r : 0.0;
+    }
+    sum = wave_sum_d(sum);
+  }
+  if ((tid & 63) == 0) ws[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) d.rsum[(int64_t)b * d.segs + seg] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+}
+
+// One workgroup a request: the drafts' walk, the segment in which the running sum passes the threshold, the index in it.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
+  __shared__ Chain c;
+  __shared__ double total[4], rest;
+  __shared__ int pick_seg, mode;  // mode: 0 the weights p, 1 p without the draft, 2 max(p - q, 0)
+  __shared__ int found, last;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const double s = heat_of(d, b);
+  walk<F32>(d, b, s, &c);
+  __syncthreads();
+  const int j = c.j;
+  int32_t* const out = d.tokens + (int64_t)b * d.T;
+  const int32_t* const tok = d.drafts + (int64_t)b * (d.T - 1);
+  if (tid < d.T) out[tid] = tid < j ? tok[tid] : -1;
+  if (tid == 0) d.counts[b] = c.ended ? j : j + 1;
+  if (c.ended) return;
+  const int64_t row = (int64_t)b * d.T + j;
+  const int dt = c.refused ? tok[j] : -1;  // the refused draft
+  const double u = (double)d.uniforms[(int64_t)b * d.T + d.T - 1];
+  // ---- the segment.  Wave 0 walks 64 at a time; the refused draft's own weight leaves its segment's sum.
+  if (wave == 0) {
+    const int64_t o = row * d.segs;
+    const double inv = s > 0.0 ? 1.0 / c.norm[j] : 1.0;
+    auto part = [&](int i, int md) -> double {
+      if (i >= d.segs) return 0.0;
+      if (md == 2) return d.rsum[(int64_t)b * d.segs + i];
+      double w;
+      if (s > 0.0) {
+        const float pm = d.pmax[o + i];
+        w = pm > -__builtin_inff() ? d.psum[o + i] * weight(pm, c.m[j], s) * inv : 0.0;
+      } else {
+        w = c.idx[j] / kSeg == i ? 1.0 : 0.0;
+      }
+      if (md == 1 && dt / kSeg == i) {
+        w -= s > 0.0 ? weight(c.xd[j], c.m[j], s) * inv : (c.idx[j] == dt ? 1.0 : 0.0);
+        w = w > 0.0 ? w : 0.0;
+      }
+      return w;
+    };
+    int md = c.refused ? (d.probs ? 2 : 1) : 0;
+    double all = 0.0;
+    for (int pass = 0; pass < 2; ++pass) {
+      all = 0.0;
+      for (int i0 = 0; i0 < d.segs; i0 += 64) all += wave_sum_d(part(i0 + lane, md));
+      if (all > 0.0 || md == 0) break;
+      md = 0;  // nothing is left of the row beside the draft: p itself
+    }
+    const double goal = u * all;
+    double before = 0.0, base = 0.0;
+    int at = -1, tail = -1;
+    double tail_base = 0.0;
+    for (int i0 = 0; i0 < d.segs && at < 0; i0 += 64) {
+      const double w = part(i0 + lane, md);
+      double run = w;
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) {
+        const double v = __shfl_up(run, k);
+        if (lane >= k) run += v;
+      }
+      const uint64_t over = __ballot(before + run > goal && w > 0.0), some = __ballot(w > 0.0);
+      if (over) {
+        const int l = __builtin_ctzll(over);
+        at = i0 + l;
+        base = before + __shfl(run - w, l);
+      }
+      if (some) {
+        const int l = 63 - __builtin_clzll(some);
+        tail = i0 + l;
+        tail_base = before + __shfl(run - w, l);
+      }
+      before += __shfl(run, 63);
+    }
+    if (at < 0) at = tail, base = tail_base;  // (the threshold at the very end of the sum)
+    if (lane == 0) pick_seg = at, mode = md, rest = goal - base, found = 0x7fffffff, last = -1;
+  }
+  __syncthreads();
+  // ---- the index: every thread's 16 weights, their running sums over the workgroup
+  const int md = mode, base = pick_seg * kSeg + tid * kPer;
+  if (pick_seg < 0) return;  // (cannot be: the row has weight)
+  float x[kPer];
+  load_logits<F32, VEC>(d, row, base, x);
+  double w[kPer], sum = 0.0;
+  const double inv = s > 0.0 ? 1.0 / c.norm[j] : 1.0;
+  const float* q = md == 2 ? d.probs + ((int64_t)b * (d.T - 1) + j) * d.V : nullptr;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    double p = s > 0.0 ? weight(x[i], c.m[j], s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
+    if (base + i >= d.V || (md == 1 && base + i == dt)) p = 0.0;
+    if (md == 2 && base + i < d.V) {
+      p -= (double)q[base + i];
+      p = p > 0.0 ? p : 0.0;
+    }
+    w[i] = p;
+    sum += p;
+  }
+  double run = sum;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const double v = __shfl_up(run, k);
+    if (lane >= k) run += v;
+  }
+  if (lane == 63) total[wave] = run;
+  __syncthreads();
+  run -= sum;
+  for (int i = 0; i < wave; ++i) run += total[i];
+  const double goal = rest;
+  int hit = 0x7fffffff, end = -1;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    run += w[i];
+    if (w[i] > 0.0) {
+      end = base + i;
+      if (run > goal && hit == 0x7fffffff) hit = base + i;
+    }
+  }
+  if (hit != 0x7fffffff) atomicMin(&found, hit);
+  if (end >= 0) atomicMax(&last, end);
+  __syncthreads();
+  if (tid == 0) out[j] = found != 0x7fffffff ? found : last;
+}
+
+int64_t segments(int64_t V) { return (V + kSeg - 1) / kSeg; }
+
+}  // namespace
+}  // namespace q36
+
+using namespace q36;
+
+extern "C" size_t q36_verify_drafts_workspace_bytes(int32_t B, int32_t T, int32_t V) {
+  if (B < 1 || T < 1 || T > kMaxT || V < 1) return 0;
+  const size_t s = (size_t)segments(V);
+  return align_up((size_t)B * T * s * 8, 256) + 2 * align_up((size_t)B * T * s * 4, 256) + align_up((size_t)B * s * 8, 256);
+}
+
+extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t stream) {
+  Q36_REQUIRE(a != nullptr, "q36_verify_drafts: null args");
+  Q36_REQUIRE(a->B >= 0 && a->B <= 65535, "q36_verify_drafts: B=%d out of range", a->B);
+  Q36_REQUIRE(a->T >= 1 && a->T <= kMaxT, "q36_verify_drafts: T=%d must be in [1,%d]", a->T, kMaxT);
+  Q36_REQUIRE(a->V >= 1 && a->V <= (1 << 24), "q36_verify_drafts: V=%d must be in [1, 2^24]", a->V);
+  if (a->B == 0) return Q36_OK;
+  Q36_REQUIRE(a->ld >= a->V, "q36_verify_drafts: ld=%lld < V=%d", (long long)a->ld, a->V);
+  Q36_REQUIRE(a->logits && a->uniforms && a->tokens && a->counts && a->workspace && (a->T == 1 || a->drafts),
+              "q36_verify_drafts: a required pointer is null");
+  const size_t need = q36_verify_drafts_workspace_bytes(a->B, a->T, a->V);
+  Q36_REQUIRE(a->workspace_bytes >= need, "q36_verify_drafts: workspace %zu < %zu bytes", a->workspace_bytes, need);
+  Q36_REQUIRE((reinterpret_cast<uintptr_t>(a->workspace) & 255u) == 0, "q36_verify_drafts: workspace must be 256-byte aligned");
+  Q36_REQUIRE((reinterpret_cast<uintptr_t>(a->logits) & (a->logits_f32 ? 3u : 1u)) == 0, "q36_verify_drafts: logits misaligned");
+  const int64_t segs = segments(a->V);
+  Q36_REQUIRE((int64_t)a->B * a->T * segs < (1ll << 32) / kThreads, "q36_verify_drafts: B x T x V too large");  // a launch's threads
+  const size_t n = (size_t)a->B * a->T * segs;
+  char* w = static_cast<char*>(a->workspace);
+  DraftsDev d{a->B, a->T, a->V, (int)segs, a->ld, a->logits, a->temperature, a->drafts, a->uniforms,
+              a->T > 1 ? a->draft_probs : nullptr, nullptr, nullptr, nullptr, nullptr, a->tokens, a->counts};
+  d.psum = reinterpret_cast<double*>(w), w += align_up(n * 8, 256);
+  d.pmax = reinterpret_cast<float*>(w), w += align_up(n * 4, 256);
+  d.pidx = reinterpret_cast<int32_t*>(w), w += align_up(n * 4, 256);
+  d.rsum = reinterpret_cast<double*>(w);
+  // 16 bytes a lane where every row starts at such a boundary
+  const bool vec = aligned16(a->logits) && a->ld % (a->logits_f32 ? 4 : 8) == 0;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto f32, auto v) {
+    constexpr bool F = decltype(f32)::value, W = decltype(v)::value;
+    drafts_sums_kernel<F, W><<<(unsigned)n, kThreads, 0, st>>>(d);
+    if (d.probs) drafts_residual_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
+    drafts_pick_kernel<F, W><<<a->B, kThreads, 0, st>>>(d);
+  };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  if (a->logits_f32) vec ? go(yes, yes) : go(yes, no);
+  else vec ? go(no, yes) : go(no, no);
+  return check_launch("q36_verify_drafts");
+}

@@ -1,4 +1,4 @@
-"""GDN speculative verify on libq36.
+"""The recurrent (GDN) layer on libq36: speculative verify, its commit, prompts.
 
 Mirrors the reference's glue (R = qwen36_nodes_kb34, L = R/qwen36_layer): gdn_verify_fused
 (L/gdn_fused.py:37-57 -> L/qk_gdn_verify.cu:841).  Two forms:
@@ -7,13 +7,16 @@ Mirrors the reference's glue (R = qwen36_nodes_kb34, L = R/qwen36_layer): gdn_ve
   gdn_verify_ring   (q36_gdn_verify_ring) the served ReplaySSM form: a read-only checkpoint plus
                                            the 16-entry (d, k, g) ring, conv state rolled in place,
                                            with the reference kernel's argument list.
+What its engine does around them is here too:
+  gdn_ring_commit   (q36_gdn_ring_commit)  the accepted part of a ring verify moved into the state;
+  gdn_prompt        (q36_gdn_prompt)       prompts: any number of new tokens a request.
 """
 from __future__ import annotations
 
 import torch
 
 from .. import _lib
-from .._lib import check, pack_gdn, pack_ring, ptr
+from .._lib import check, check_tensors, pack_commit, pack_gdn, pack_prompt, pack_ring, ptr
 
 HEAD_K, HEAD_V, N_K_HEADS, N_V_HEADS = 128, 128, 16, 32
 QKV_DIM = 2 * N_K_HEADS * HEAD_K + N_V_HEADS * HEAD_V  # 8192
@@ -57,18 +60,18 @@ def gdn_verify_fused(mixed, z, a, b, conv_state, conv_w, A_log, dt_bias, S0, nor
 RING = 16
 
 
-def _pool(t, name, dtype, tail, inner_strides):
+def _pool(t, name, dtype, tail, inner_strides, what="gdn_verify_ring"):
     """A slot pool [slots, *tail] with the given innermost strides (the slot stride is free but a
     multiple of 8 elements), as the reference's host checks require (L/qk_gdn_verify.cu:872-904)."""
     st = t.stride()
     if t.dtype != dtype or t.shape[1:] != tail or st[1:] != inner_strides or st[0] % 8 != 0:
-        raise ValueError(f"gdn_verify_ring: {name} must be a {dtype} [slots, {', '.join(map(str, tail))}] pool with "
+        raise ValueError(f"{what}: {name} must be a {dtype} [slots, {', '.join(map(str, tail))}] pool with "
                          f"contiguous heads, got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
 
 
-def _idx(t, name, n):
+def _idx(t, name, n, what="gdn_verify_ring"):
     if t.dim() != 1 or t.numel() < n or not t.is_contiguous() or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"gdn_verify_ring: {name} must hold at least {n} int32/int64 indices")
+        raise ValueError(f"{what}: {name} must hold at least {n} int32/int64 indices")
     return 1 if t.dtype == torch.int64 else 0
 
 
@@ -141,4 +144,108 @@ def gdn_verify_ring(mixed, z, a, b, conv_state, conv_w, window, A_log, dt_bias, 
         ptr(replay_idx), ptr(win_idx), flags, ptr(write_pos), ptr(cache_base), ptr(norm_w), eps, scale, ptr(out),
         ptr(None if oq is None else oq.codes), ptr(None if oq is None else oq.scales))
     check(_lib.packed().q36_gdn_verify_ring(args, _lib.stream_handle(stream)), "q36_gdn_verify_ring")
+    return out
+
+
+def gdn_ring_commit(conv_state, window, h0, d_ring, dlo_ring, k_ring, klo_ring, g_ring, state_idx, replay_idx, win_idx, write_pos,
+                    cache_base, accepted, *, T: int = 4, room: int | None = None, advance: bool = True, stream=None):
+    """Moves what a verify batch accepted into the recurrent state, in place, behind gdn_verify_ring on the same pools.
+
+    accepted int32/int64 [B]: how many of each request's T window tokens stand, the first included
+    (lmhead8.verify_drafts' counts).  The conv state goes to the last accepted token; where the ring then has no room
+    for another `room` tokens (None: T), its entries are folded into the checkpoint h0.  advance: the cursors write_pos and
+    cache_base move too; recurrent layers that share them commit one after another, the last one with advance.
+    A request with accepted < 1 or an index outside its pool is left as it is."""
+    what = "gdn_ring_commit"
+    if not 1 <= T <= 8 or accepted.dim() != 1:
+        raise ValueError(f"{what}: accepted must be [B] and the draft window 1..8, got {tuple(accepted.shape)}, {T}")
+    B, room = accepted.shape[0], T if room is None else room
+    _pool(conv_state, "conv_state", torch.bfloat16, (QKV_DIM, 3), (3, 1), what)
+    if window.dim() == 4:  # the deduplicated [wslots, T, 8192, 3] view of [wslots, 8192, T + 2]
+        if window.dtype != torch.bfloat16 or window.shape[1:] != (T, QKV_DIM, 3) or window.stride()[1:] != (1, T + 2, 1) or \
+                window.stride(0) % 8:
+            raise ValueError(f"{what}: conv windows must be the deduplicated [slots, T, 8192, 3] view of [slots, 8192, T + 2]")
+    else:
+        _pool(window, "window", torch.bfloat16, (QKV_DIM, T + 2), (T + 2, 1), what)
+    if h0.dtype != torch.float32 or h0.shape[1:] != (N_V_HEADS, HEAD_V, HEAD_K) or not h0.is_contiguous():
+        raise ValueError(f"{what}: the checkpoint must be a contiguous fp32 [slots, 32, 128, 128] pool")
+    for t, n in ((d_ring, "d ring"), (dlo_ring, "d ring (low parts)")):
+        _pool(t, n, torch.bfloat16, (N_V_HEADS, RING, HEAD_V), (RING * HEAD_V, HEAD_V, 1), what)
+    for t, n in ((k_ring, "k ring"), (klo_ring, "k ring (low parts)")):
+        _pool(t, n, torch.bfloat16, (N_K_HEADS, RING, HEAD_K), (RING * HEAD_K, HEAD_K, 1), what)
+    if g_ring.dtype != torch.float32 or g_ring.shape[1:] != (N_V_HEADS, RING) or g_ring.stride()[1:] != (RING, 1) or \
+            g_ring.stride(0) % 4:
+        raise ValueError(f"{what}: g ring must be an fp32 [slots, 32, 16] pool")
+    flags = (_idx(state_idx, "state_idx", B, what) | _idx(replay_idx, "replay_idx", B, what) << 1 |
+             _idx(win_idx, "win_idx", B, what) << 2 | _idx(accepted, "accepted", B, what) << 3)
+    rslots = min(d_ring.shape[0], dlo_ring.shape[0], k_ring.shape[0], klo_ring.shape[0], g_ring.shape[0])
+    for t, n in ((write_pos, "write_pos"), (cache_base, "cache_base")):
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < rslots:
+            raise ValueError(f"{what}: ring cursor {n} must be contiguous int32 [ring slots]")
+    check_tensors(what, "conv_state window h0 d_ring dlo_ring k_ring klo_ring g_ring state_idx replay_idx win_idx write_pos "
+                  "cache_base accepted", conv_state, window, h0, d_ring, dlo_ring, k_ring, klo_ring, g_ring, state_idx,
+                  replay_idx, win_idx, write_pos, cache_base, accepted)
+    args = pack_commit(
+        B, T, room, int(advance), min(conv_state.shape[0], h0.shape[0]), rslots, window.shape[0], flags,
+        ptr(conv_state), conv_state.stride(0), ptr(window), window.stride(0), ptr(h0), ptr(d_ring), ptr(dlo_ring),
+        d_ring.stride(0), dlo_ring.stride(0), ptr(k_ring), ptr(klo_ring), k_ring.stride(0), klo_ring.stride(0), ptr(g_ring),
+        g_ring.stride(0), ptr(state_idx), ptr(replay_idx), ptr(win_idx), ptr(accepted), ptr(write_pos), ptr(cache_base))
+    check(_lib.packed().q36_gdn_ring_commit(args, _lib.stream_handle(stream)), "q36_gdn_ring_commit")
+
+
+class PromptWorkspace:
+    """Scratch of gdn_prompt for up to `rows` rows of up to B requests: any contents, one for calls that follow one
+    another."""
+
+    def __init__(self, rows: int, B: int, device):
+        need = _lib.lib().q36_gdn_prompt_workspace_bytes(rows, B)
+        if need == 0:
+            raise ValueError(f"PromptWorkspace: rows={rows} B={B}")
+        self.rows, self.B = rows, B
+        self.buf = torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def gdn_prompt(mixed, z, a, b, conv_state, conv_w, A_log, dt_bias, h0, qsl, state_idx, norm_w, ws: PromptWorkspace,
+               eps: float = 1e-6, scale: float = HEAD_K ** -0.5, *, prefix=None, out=None, oq=None, stream=None):
+    """out_proj's input [rows, 4096] for a batch of prompt chunks, any number of new tokens a request.
+
+    mixed bf16 [rows, 8192], z bf16 [rows, 4096] (or [rows, 32, 128]), a, b bf16 [rows, 32]: in_proj's columns; request r owns
+    rows qsl[r] .. qsl[r + 1] - 1 (int32 [B + 1]) and slot state_idx[r] (int32/int64 [B]) of conv_state bf16 [slots, 8192, 3]
+    and of the recurrent state h0 fp32 [slots, 32, 128, 128], both updated in place.  prefix int32 [B] (optional): requests
+    with 0 tokens before these begin from zero states, whatever their slots hold.  oq (glue.linear_rows(rows, 4096)): out's
+    e4m3 codes also go there.  Rows of no request are left as they were; a slot outside the pool marks a padded request, whose
+    rows are zeroed.  Requests with rows name distinct slots."""
+    what, rows = "gdn_prompt", mixed.shape[0]
+    for t, n, w in ((mixed, "mixed", QKV_DIM), (z, "z", N_V_HEADS * HEAD_V), (a, "a", N_V_HEADS), (b, "b", N_V_HEADS)):
+        if t.dtype != torch.bfloat16 or t.dim() < 2 or t.shape[0] != rows or t.numel() != rows * w or not t.is_contiguous():
+            raise ValueError(f"{what}: {n} must be contiguous bf16 [{rows}, {w}], got {t.dtype} {tuple(t.shape)}")
+    if qsl.dtype != torch.int32 or qsl.dim() != 1 or qsl.numel() < 1 or not qsl.is_contiguous():
+        raise ValueError(f"{what}: qsl must hold B + 1 int32 row starts")
+    B = qsl.numel() - 1
+    _pool(conv_state, "conv_state", torch.bfloat16, (QKV_DIM, 3), (3, 1), what)
+    for t, n, dt, shape in ((conv_w, "conv_w", torch.bfloat16, (QKV_DIM, 4)), (A_log, "A_log", torch.float32, (N_V_HEADS,)),
+                            (norm_w, "norm_w", torch.bfloat16, (HEAD_V,)), (prefix, "prefix", torch.int32, (B,))):
+        if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{what}: {n} must be contiguous {dt} {list(shape)}")
+    if dt_bias.dtype not in (torch.float32, torch.bfloat16) or dt_bias.numel() != N_V_HEADS or not dt_bias.is_contiguous():
+        raise ValueError(f"{what}: dt_bias must hold 32 fp32 or bf16 values")
+    if h0.dtype != torch.float32 or h0.shape[1:] != (N_V_HEADS, HEAD_V, HEAD_K) or not h0.is_contiguous():
+        raise ValueError(f"{what}: the state must be a contiguous fp32 [slots, 32, 128, 128] pool")
+    flag = _idx(state_idx, "state_idx", B, what)
+    out = torch.empty((rows, N_V_HEADS * HEAD_V), dtype=torch.bfloat16, device=mixed.device) if out is None else out
+    if out.dtype != torch.bfloat16 or out.shape != (rows, N_V_HEADS * HEAD_V) or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous bf16 [{rows}, 4096]")
+    if oq is not None and (oq.T != rows or oq.frag or oq.codes.shape[1] != N_V_HEADS * HEAD_V):
+        raise ValueError(f"{what}: oq must be row-major rows of this batch (glue.linear_rows)")
+    if B == 0 or rows == 0:
+        return out
+    check_tensors(what, "mixed z a b conv_state conv_w A_log dt_bias h0 qsl state_idx norm_w ws prefix out oq", mixed, z, a, b,
+                  conv_state, conv_w, A_log, dt_bias, h0, qsl, state_idx, norm_w, ws.buf, prefix, out,
+                  None if oq is None else oq.codes)
+    args = pack_prompt(
+        B, rows, min(conv_state.shape[0], h0.shape[0]), flag, int(dt_bias.dtype == torch.float32), eps, scale, ptr(mixed), ptr(z),
+        ptr(a), ptr(b), ptr(conv_state), conv_state.stride(0), ptr(conv_w), ptr(A_log), ptr(dt_bias), ptr(h0), ptr(qsl),
+        ptr(state_idx), ptr(prefix), ptr(norm_w), ptr(out), ptr(None if oq is None else oq.codes),
+        ptr(None if oq is None else oq.scales), ptr(ws.buf), ws.buf.numel())
+    check(_lib.packed().q36_gdn_prompt(args, _lib.stream_handle(stream)), "q36_gdn_prompt")
     return out

@@ -5,13 +5,15 @@ Mirrors the reference's lm_head glue (R = qwen36_nodes_kb34, H = R/qwen36_lmhead
   w8a8_lmhead_argmax  <- H/w8a8.py:116-120 w8a8_linear (one or two activation terms) and
                          H/lmhead8.py:57-91 (W8A16), with the greedy argmax of the stock sampler
                          (H/node.py:136-151) fused in; logits are returned only when asked for.
+  verify_drafts       (no reference counterpart: its engine samples) drafted tokens against the logits, from given
+                         random numbers: what stands, and the token behind it.
 """
 from __future__ import annotations
 
 import torch
 
 from .. import _lib
-from .._lib import check, pack_lmhead, ptr
+from .._lib import check, check_tensors, pack_drafts, pack_lmhead, ptr
 
 
 def quantize_rows(w: torch.Tensor, stream=None):
@@ -77,3 +79,54 @@ def w8a8_lmhead_argmax(h, q, scale, ws: Workspace, norm_w=None, eps: float = 1e-
                     int(logits is not None and logits.dtype == torch.float32), ptr(q_t))
     check(_lib.packed().q36_lmhead_argmax(a, _lib.stream_handle(stream)), "q36_lmhead_argmax")
     return (ids, logits) if (want_logits or logits is not None) else ids
+
+
+MAX_WINDOW = 8  # tokens of a verify window
+
+
+class VerifyWorkspace:
+    """Partial sums of verify_drafts for up to B requests x T tokens over V logits: any contents, one for calls that
+    follow one another."""
+
+    def __init__(self, B: int, T: int, V: int, device):
+        need = _lib.lib().q36_verify_drafts_workspace_bytes(B, T, V)
+        if need == 0:
+            raise ValueError(f"VerifyWorkspace: B={B} T={T} V={V} (1 <= T <= {MAX_WINDOW})")
+        self.buf = torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def verify_drafts(logits, drafts, uniforms, ws: VerifyWorkspace, temperature=None, draft_probs=None, tokens=None, counts=None,
+                  stream=None):
+    """Which drafted tokens stand, and the token that follows them: (tokens int32 [B, T], counts int32 [B]).
+
+    logits bf16 or fp32 [B * T, V] (rows may be strided), row b T + t behind window token t of request b; drafts int32
+    [B, T - 1] (a number outside the vocabulary: no draft from there on; None where T is 1); uniforms fp32 [B, T] in [0, 1):
+    one for each draft and the last for the drawn token; temperature fp32 [B] (None: 1; 0: greedy); draft_probs fp32 [B, T - 1,
+    V] (None: drafts chosen without chance).  tokens[b, :counts[b]] are the drafts that stand and one token drawn from what is
+    left of the target's probabilities, -1 behind them; counts is what gdn_ring_commit takes as accepted.  A row without any
+    logit above minus infinity ends its request without that token."""
+    if logits.dim() != 2 or uniforms.dim() != 2:
+        raise ValueError("verify_drafts: logits must be [B * T, V] and uniforms [B, T]")
+    B, T = uniforms.shape
+    V = logits.shape[1]
+    if not 1 <= T <= MAX_WINDOW or logits.shape[0] != B * T or V < 1:
+        raise ValueError(f"verify_drafts: logits {tuple(logits.shape)} are not [{B} * {T}, V], 1 <= T <= {MAX_WINDOW}")
+    if logits.dtype not in (torch.bfloat16, torch.float32) or (V > 1 and logits.stride(1) != 1):
+        raise ValueError("verify_drafts: logits must be bf16 or fp32 rows of unit stride")
+    for name, t, dt, shape in (("drafts", drafts, torch.int32, (B, T - 1)), ("uniforms", uniforms, torch.float32, (B, T)),
+                               ("temperature", temperature, torch.float32, (B,)),
+                               ("draft_probs", draft_probs, torch.float32, (B, T - 1, V)),
+                               ("tokens", tokens, torch.int32, (B, T)), ("counts", counts, torch.int32, (B,))):
+        if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"verify_drafts: {name} must be a contiguous {dt} tensor {list(shape)}")
+    if drafts is None and T > 1:
+        raise ValueError("verify_drafts: drafts are required where T > 1")
+    tokens = torch.empty((B, T), dtype=torch.int32, device=logits.device) if tokens is None else tokens
+    counts = torch.empty(B, dtype=torch.int32, device=logits.device) if counts is None else counts
+    check_tensors("verify_drafts", "logits drafts uniforms temperature draft_probs tokens counts ws", logits, drafts, uniforms,
+                  temperature, draft_probs, tokens, counts, ws.buf)
+    ld = logits.stride(0) if B * T > 1 else V
+    a = pack_drafts(B, T, V, int(logits.dtype == torch.float32), ld, ptr(logits), ptr(temperature), ptr(drafts), ptr(uniforms),
+                    ptr(draft_probs if T > 1 else None), ptr(tokens), ptr(counts), ptr(ws.buf), ws.buf.numel())
+    check(_lib.packed().q36_verify_drafts(a, _lib.stream_handle(stream)), "q36_verify_drafts")
+    return tokens, counts

@@ -277,6 +277,84 @@ typedef struct q36_gdn_ring_args {
 } q36_gdn_ring_args;
 int q36_gdn_verify_ring(const q36_gdn_ring_args* a, q36_stream_t stream);
 
+/* ---- The commit of a verified window to the recurrent state (the reference leaves it to its serving engine; the pools are
+ * q36_gdn_verify_ring's) ----
+ * accepted[r] (int32, or int64 with idx_i64 bit 3): how many of the window's T tokens stand, the first one included, as
+ * q36_verify_drafts counts them; more than T counts as T.  With n = min(write_pos + accepted, 16):
+ *   conv_state <- the window record's rows for draft accepted - 1 (the three inputs up to the last accepted token);
+ *   n + room > 16 (room: the next window's tokens): the ring is folded into the checkpoint,
+ *     h0 <- e^{G_n} h0 + sum_{c < n} e^{G_n - G_c} (d + dlo)_c (k + klo)_c^T, G_c = g_0 + .. + g_c, in fp32;
+ *   with advance: write_pos <- n, or 0 where folded, and cache_base <- (cache_base + n) & 15 there.
+ * Recurrent layers that share their cursors commit one after another, the last with advance.  A request with an index outside
+ * its pool or accepted < 1 is left as it is (the verify rolled its conv state over the whole window: there is no way
+ * back to before it).  Requests must name distinct slots.  B <= 65535.  Layouts, strides and alignment as q36_gdn_ring_args. */
+typedef struct q36_gdn_commit_args {
+  int32_t B, T, room, advance;
+  int32_t slots, rslots, wslots, idx_i64;
+  void* conv_state;
+  int64_t cs_slot;
+  const void* window;
+  int64_t win_slot;
+  float* h0;
+  const void* d_ring;
+  const void* dlo_ring;
+  int64_t d_slot, dlo_slot;
+  const void* k_ring;
+  const void* klo_ring;
+  int64_t k_slot, klo_slot;
+  const float* g_ring;
+  int64_t g_slot;
+  const void* state_idx;
+  const void* replay_idx;
+  const void* win_idx;
+  const void* accepted;
+  int32_t* write_pos;
+  int32_t* cache_base;
+} q36_gdn_commit_args;
+int q36_gdn_ring_commit(const q36_gdn_commit_args* a, q36_stream_t stream);
+
+/* ---- The recurrent layer's prompt: any number of new tokens a request (a prompt chunk, one token: any mix), state carried
+ * in the engine's pools.  (The reference leaves prompts to its engine's kernels; the layer is q36_gdn_verify_ring's.) ----
+ * mixed bf16 [rows, 8192], z bf16 [rows, 4096], a, b bf16 [rows, 32] as q36_gdn_args; request r's new tokens are rows qsl[r] ..
+ * qsl[r + 1] - 1 (int32 [B + 1], non-decreasing).  state_idx[r] (int32, or int64 with idx_i64): its slot in conv_state bf16
+ * [slots, 8192, 3] (slot stride cs_slot) and h0 fp32 [slots, 32, 128 (v), 128 (k)], both updated in place: the last three
+ * inputs, and the state behind the last token.  prefix int32 [B] or NULL: a request with prefix <= 0 begins from zero states,
+ * whatever its slot holds; NULL: all continue.
+ * Per token: conv of 4 taps, SiLU, unit q and k (q times scale), g = -exp(A_log) log(1 + exp(a + dt_bias)),
+ * beta = sigmoid(b), S <- e^g S, u = beta (v - S k), S <- S + u k^T, o = S q, out = bf16(o rsqrt(mean o^2 + eps) norm_w
+ * silu(z)), formed in fp32 and rounded once.  (The verify entries round the conv's tap products, its output and o
+ * to bf16.)  oq / oqs (optional): out's e4m3 codes and scales as q36_gdn_ring_args'.
+ * A request without rows is left as it is; a slot outside [0, slots) marks a padded request: zero rows, nothing else
+ * written.  Rows of no request are left as they were.  Requests with rows must name distinct slots.  Whatever the device data
+ * hold, every access stays inside the buffers.
+ * B <= 65535, rows <= 2^20; mixed, z, conv_state, conv_w, h0, out, oq 16-byte, workspace 256-byte aligned, cs_slot a multiple
+ * of 8.  Workspace: q36_gdn_prompt_workspace_bytes(rows, B), any contents, one for calls that follow one another. */
+typedef struct q36_gdn_prompt_args {
+  int32_t B, rows, slots, idx_i64, dt_f32;
+  float eps, scale;
+  const void* mixed;
+  const void* z;
+  const void* a;
+  const void* b;
+  void* conv_state;
+  int64_t cs_slot;
+  const void* conv_w;
+  const float* A_log;
+  const void* dt_bias;
+  float* h0;
+  const int32_t* qsl;
+  const void* state_idx;
+  const int32_t* prefix;
+  const void* norm_w;
+  void* out;
+  void* oq;
+  float* oqs;
+  void* workspace;
+  size_t workspace_bytes;
+} q36_gdn_prompt_args;
+size_t q36_gdn_prompt_workspace_bytes(int32_t rows, int32_t B);
+int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream);
+
 /* ---------------------------------------------------------------------------------------
  * Fused gated full-attention projections (16 q heads x 256 with an output gate per head,
  * 2 KV heads x 256, hidden 2048), e4m3 weights with fp32 128x128 block scales.
@@ -621,6 +699,36 @@ typedef struct q36_lmhead_args {
 } q36_lmhead_args;
 size_t q36_lmhead_workspace_bytes(int32_t R);
 int q36_lmhead_argmax(const q36_lmhead_args* a, q36_stream_t stream);
+
+/* ---- Verification of drafted tokens from given random numbers (the reference leaves sampling to its serving engine,
+ * H/node.py:136-151) ----
+ * logits bf16 or (logits_f32) fp32 [B * T, ld], V of them a row: row b T + t holds the target's logits behind window token t
+ * of request b.  drafts int32 [B, T - 1]: the window's tokens 1 .. T - 1 (a number outside [0, V): no draft from there on).
+ * uniforms fp32 [B, T] in [0, 1).  temperature fp32 [B] or NULL (1).  draft_probs fp32 [B, T - 1, V] or NULL: the
+ * probabilities the drafts were drawn from; NULL: drafts chosen without chance (q = 1 at the draft).
+ * p = softmax(logits / temperature), or 1 at the first largest logit where the temperature is 0 (or less, or NaN).  Draft
+ * t + 1 stands iff those before it do and uniforms[t] q(d) < p(d).  Behind them comes one token more: at the first draft
+ * refused the first index whose running sum of max(p - q, 0) (p without the draft) passes uniforms[T - 1] times the total, of
+ * p where that leaves nothing; where no draft is refused, of p.  T = 1: a token is drawn.  tokens int32 [B, T]: the drafts that stand,
+ * that token, -1 behind; counts int32 [B]: how many.
+ * NaN logits count as minus infinity; logits of plus infinity share the row.  A row of minus infinity alone leaves no token:
+ * it ends its request, count without one more.  Weights and sums in fp64 (a weight within 7e-12 of itself).
+ * 1 <= T <= 8, B <= 65535, V <= 2^24, B T ceil(V / 4096) < 2^24.  Workspace: q36_verify_drafts_workspace_bytes(B, T, V), 256-byte aligned, any contents. */
+typedef struct q36_verify_drafts_args {
+  int32_t B, T, V, logits_f32;
+  int64_t ld;
+  const void* logits;
+  const float* temperature;
+  const int32_t* drafts;
+  const float* uniforms;
+  const float* draft_probs;
+  int32_t* tokens;
+  int32_t* counts;
+  void* workspace;
+  size_t workspace_bytes;
+} q36_verify_drafts_args;
+size_t q36_verify_drafts_workspace_bytes(int32_t B, int32_t T, int32_t V);
+int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Prepare-time weight quantizers (device to device).
