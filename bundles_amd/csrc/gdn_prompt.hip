@@ -15,6 +15,23 @@ namespace {
 
 constexpr int PK = 128, PV = 128, PHK = 16, PHV = 32, PQKV = 8192, PZ = PHV * PV;
 constexpr int kGroup = 8;  // tokens whose conv, norms and gates are formed at once
+constexpr int kShort = 8;  // requests of up to so many new tokens go token by token, longer ones by chunks
+constexpr int PC = 64;     // tokens of a chunk
+
+// A chunk's operands for one key head, as the scan's lanes load them: pieces of 1 KB, lane l's 16 bytes at 16 l, element (row
+// r, depth k) of a 16 x 32 operand piece in lane r + 16 (k / 8).  Values times 2^8 in fp16, low parts times 2^11 more.
+constexpr int kPiece = 1024;
+constexpr int kUK = 0;                        // K: [plane][token tile 4][depth 4] (depth: key dims by 32)
+constexpr int kUKt = kUK + 32 * kPiece;       // K^T: [plane][dim tile 8][depth 2] (depth: tokens by 32)
+constexpr int kUQ = kUKt + 32 * kPiece;       // Q: as K
+constexpr int kUHead = kUQ + 32 * kPiece;     // then for each of the two value heads:
+constexpr int kHT = 0;                        //   T: [plane][6 pieces on and below the diagonal]
+constexpr int kHP = kHT + 12 * kPiece;        //   P: as T
+constexpr int kHGate = kHP + 12 * kPiece;     //   fp32 [64] each: e^{b_i}, e^{b_end - b_i}, beta; then e^{b_end}
+constexpr int kHeadBytes = kHGate + kPiece;
+constexpr int kUnit = kUHead + 2 * kHeadBytes;
+// piece of (token tile w, depth s) among those on and below the diagonal: tiles 0 and 1 have one, 2 and 3 two
+__device__ __forceinline__ constexpr int tri_piece(int w, int s) { return w < 2 ? w : 2 * w - 2 + s; }
 
 struct PromptDev {
   int B, rows, slots, idx_i64, dt_f32;
@@ -36,6 +53,10 @@ struct PromptDev {
   uint16_t* out;
   uint8_t* oq;
   float* oqs;
+  // the chunks' operands and the outputs' exponents (workspace)
+  uint8_t* units;
+  int8_t* exps;
+  int by_row;
 };
 
 // Request r's rows, inside the batch whatever qsl holds, and its slot (-1: none).
@@ -45,6 +66,52 @@ __device__ __forceinline__ void request_of(const PromptDev& d, int r, int& t0, i
   const int64_t s = d.idx_i64 ? static_cast<const int64_t*>(d.state_idx)[r] : (int64_t)static_cast<const int32_t*>(d.state_idx)[r];
   slot = s >= 0 && s < d.slots ? s : -1;
   old = d.prefix == nullptr || d.prefix[r] > 0;
+}
+
+// The first of a long request's chunks in the workspace.  Chunks of different long requests never meet: the next one's t0
+// is more than kShort and more than n - 64 rows on, so (by_row) t0 / 9 or (else) r grows by one beside t0 / 64.
+__device__ __forceinline__ int first_unit(const PromptDev& d, int r, int t0) {
+  return (t0 >> 6) + (d.by_row ? t0 / (kShort + 1) : r);
+}
+
+// The last r in [0, B) with at(r) <= x, at non-decreasing: 64 probes at a time, every lane the same answer.
+template <typename At>
+__device__ __forceinline__ int last_at_most(int B, int x, At at) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, size = B;
+  while (size > 1) {
+    const int step = (size + 63) >> 6, o = lane * step;
+    const int n = __builtin_popcountll(__ballot(o < size && at(lo + min(o, size - 1)) <= x));
+    const int skip = max(n - 1, 0) * step;
+    lo += skip;
+    size = min(step, size - skip);
+  }
+  return lo;
+}
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+constexpr float kLow = 2048.f, kUnlow = 1.f / 2048.f;  // a low part's own factor
+// x = hi + lo / 2^11: 22 significand bits for x in fp16's normal range.  x is kept from the compiler's eyes: where it sees a
+// product behind x, one use of hi becomes a multiply that rounds once to fp16 and another the rounding of the fp32 product,
+// and where these differ (one value in 2^12) lo belongs to another hi.
+__device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
+  asm("" : "+v"(x));
+  hi = (_Float16)x;
+  lo = (_Float16)((x - (float)hi) * kLow);
+}
+
+__device__ __forceinline__ float fast_silu(float x) {
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+  v = v + lane_xor<1>(v);
+  v = v + lane_xor<2>(v);
+  v = v + lane_xor<4>(v);
+  return v + lane_xor<8>(v);
 }
 
 __device__ __forceinline__ float silu(float x) { return x / (1.f + expf_q(-x)); }
@@ -63,7 +130,7 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
   int64_t slot;
   bool old;
   request_of(d, r, t0, n, slot, old);
-  if (n == 0) return;
+  if (n == 0 || (n > kShort && slot >= 0)) return;
   if (slot < 0) {  // a padded request: zero rows
     for (int i = tid; i < n * 64; i += 512) {
       const int64_t o = (int64_t)(t0 + (i >> 6)) * PZ + hk * 2 * PV + (i & 63) * 4;
@@ -184,6 +251,683 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
     for (int jj = 0; jj < 4; ++jj) *reinterpret_cast<v4f*>(hp + (r0 + 64 * j) * PK + 32 * jj + 4 * c8) = st[j][jj];
 }
 
+
+// ---- chunks of 64 tokens.  With b_i = g_0 + .. + g_i inside a chunk, S the state before it (as [key dim][value]):
+//   A_ij = beta_i e^{b_i - b_j} k_i . k_j (j < i), T = (I + A)^-1
+//   U = T (beta (V - e^b K S)),  O = e^b Q S + (e^{b_i - b_j} q_i . k_j, j <= i) U,  S' = e^{b_end} S + K^T (e^{b_end - b} U)
+// A first kernel forms what does not depend on S, for all chunks at once; a second walks a request's chunks with S in
+// registers, a workgroup for every 16 or 32 value columns of a head; a third applies the gated norm to whole heads.
+//
+// Products are of fp16 operands in two parts (x = hi + lo / 2^11, three products: 22 bits), in fp32 sums, so the state keeps
+// fp32's accuracy at a third of the fp16 rate, where the fp32 matrix instruction has a sixteenth.  The output, though bf16,
+// needs them too: where the state is of nearly one key, a row hangs on one q . k that may be small beside |q| |k|, or on a sum
+// of U that nearly cancels, and the norm brings the row back to size (high parts alone: rows 8 % off, 0.1 % elsewhere).
+
+// q, k of a chunk for one key head; T, P and gates of its two value heads.
+__global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
+  constexpr int RS = PK + 8, MS = PC + 4;  // padded rows, in elements
+  __shared__ __attribute__((aligned(16))) _Float16 planes[2][2][PC][RS];  // [q, k][hi, lo]; later A and P
+  __shared__ double run[2][PC];  // log2 of the decay up to a token
+  __shared__ float beta[2][PC];
+  float(*const am)[PC][MS] = reinterpret_cast<float(*)[PC][MS]>(&planes[0][0][0][0]);
+  float(*const pm)[PC][MS] = am + 2;
+  static_assert(sizeof(planes) >= 4 * PC * MS * 4, "A and P in the planes' place");
+  const int unit = blockIdx.x / PHK, hk = blockIdx.x % PHK;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = last_at_most(d.B, unit, [&](int i) { return first_unit(d, i, min(max(d.qsl[i], 0), d.rows)); });
+  int t0, n;
+  int64_t slot;
+  bool old;
+  request_of(d, r, t0, n, slot, old);
+  const int chunk = unit - first_unit(d, r, t0), c0 = chunk * PC;  // (of the request; first token in it)
+  if (n <= kShort || slot < 0 || chunk < 0 || c0 >= n) return;
+  uint8_t* const u = d.units + (int64_t)blockIdx.x * kUnit;
+  const int g = lane >> 4, c = lane & 15;
+
+  // ---- conv, SiLU, unit vectors: thread (run of 8 tokens, 8 channels of q or k)
+  {
+    const int tr = (tid >> 5) * 8, part = (tid >> 4) & 1, ch = part * (PHK * PK) + hk * PK + c * 8;
+    v4i raw[11];
+#pragma unroll
+    for (int i = 0; i < 11; ++i) {
+      const int t = c0 + tr + i - 3;
+      raw[i] = *reinterpret_cast<const v4i*>(d.mixed + (int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + ch);
+    }
+    v4i wr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wr[i] = *reinterpret_cast<const v4i*>(d.conv_w + (int64_t)ch * 4 + 8 * i);
+    if (c0 + tr == 0) {  // the three inputs before the request's first
+      v4i cs[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        cs[i] = old ? *reinterpret_cast<const v4i*>(d.conv_state + slot * d.cs_slot + (int64_t)ch * 3 + 8 * i) : v4i{0, 0, 0, 0};
+      auto at = [&](int e) { return ((uint32_t)cs[e >> 3][(e >> 1) & 3] >> (16 * (e & 1))) & 0xffffu; };
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw[i][j] = (int)(at(3 * (2 * j) + i) | (at(3 * (2 * j + 1) + i) << 16));
+    }
+    float y[8][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t wlo = (uint32_t)wr[e >> 1][2 * (e & 1)], whi = (uint32_t)wr[e >> 1][2 * (e & 1) + 1];
+      const float w0 = bf_lo(wlo), w1 = bf_hi(wlo), w2 = bf_lo(whi), w3 = bf_hi(whi);
+      float x[11];
+#pragma unroll
+      for (int i = 0; i < 11; ++i) x[i] = (e & 1) ? bf_hi((uint32_t)raw[i][e >> 1]) : bf_lo((uint32_t)raw[i][e >> 1]);
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        y[t][e] = fast_silu(__builtin_fmaf(x[t + 3], w3, __builtin_fmaf(x[t + 2], w2, __builtin_fmaf(x[t + 1], w1, x[t] * w0))));
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(y[t][e], y[t][e], ss);
+      ss = row16_sum(ss);
+      const float rr = c0 + tr + t < n ? 256.f / sqrtf(ss + 1e-6f) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[t][e] = c0 + tr + t < n ? y[t][e] * rr : 0.f;
+    }
+    v8h lo[8];  // the low parts by token
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      v8h hi;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        _Float16 a, b;
+        split(y[t][e], a, b);
+        hi[e] = a, lo[t][e] = b;
+        y[t][e] = (float)a;
+      }
+      *reinterpret_cast<v8h*>(&planes[part][0][tr + t][8 * c]) = hi;
+      *reinterpret_cast<v8h*>(&planes[part][1][tr + t][8 * c]) = lo[t];
+    }
+    if (part == 1) {  // K^T: eight tokens of a dim are a lane's 16 bytes
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int dim = 8 * c + e;
+        v8h a, b;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) a[t] = (_Float16)y[t][e], b[t] = lo[t][e];
+        uint8_t* p = u + kUKt + ((dim >> 4) * 2 + (tr >> 5)) * kPiece + 16 * ((dim & 15) + 16 * ((tr >> 3) & 3));
+        *reinterpret_cast<v8h*>(p) = a;
+        *reinterpret_cast<v8h*>(p + 16 * kPiece) = b;
+      }
+    }
+  }
+  // ---- gates: a wave a value head, a lane a token
+  if (wave < 2) {
+    const int hv = 2 * hk + wave;
+    const bool in = c0 + lane < n;
+    const int64_t o = (int64_t)(t0 + min(c0 + lane, n - 1)) * PHV + hv;
+    const float dt = d.dt_f32 ? static_cast<const float*>(d.dt_bias)[hv] : bf2f(static_cast<const uint16_t*>(d.dt_bias)[hv]);
+    double s = in ? (double)(-expf_q(d.A_log[hv]) * softplus(bf2f(d.a[o]) + dt)) * 1.4426950408889634074 : 0.0;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const double v = __shfl_up(s, k);
+      if (lane >= k) s += v;
+    }
+    const double end = __shfl(s, 63);
+    const float bt = in ? sigmoid_q(bf2f(d.b[o])) : 0.f;
+    run[wave][lane] = s;
+    beta[wave][lane] = bt;
+    float* gt = reinterpret_cast<float*>(u + kUHead + wave * kHeadBytes + kHGate);
+    gt[lane] = __builtin_amdgcn_exp2f((float)s);
+    gt[64 + lane] = __builtin_amdgcn_exp2f((float)(end - s));
+    gt[128 + lane] = bt;
+    if (lane == 0) gt[192] = __builtin_amdgcn_exp2f((float)end);
+  }
+  __syncthreads();
+  // ---- K K^T and Q K^T on and below the diagonal: wave w rows 16 w .. + 15.  The operands' pieces go to the workspace as read
+  v4f kk[4], qk[4];
+  {
+    v8h ka[2][4], qa[2][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        ka[p][s] = *reinterpret_cast<const v8h*>(&planes[1][p][16 * wave + c][32 * s + 8 * g]);
+        qa[p][s] = *reinterpret_cast<const v8h*>(&planes[0][p][16 * wave + c][32 * s + 8 * g]);
+        *reinterpret_cast<v8h*>(u + kUK + (p * 16 + wave * 4 + s) * kPiece + 16 * lane) = ka[p][s];
+        *reinterpret_cast<v8h*>(u + kUQ + (p * 16 + wave * 4 + s) * kPiece + 16 * lane) = qa[p][s];
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      kk[j] = qk[j] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (j <= wave) {
+        v4f k2 = {0.f, 0.f, 0.f, 0.f}, q2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const v8h bh = *reinterpret_cast<const v8h*>(&planes[1][0][16 * j + c][32 * s + 8 * g]);
+          const v8h bl = *reinterpret_cast<const v8h*>(&planes[1][1][16 * j + c][32 * s + 8 * g]);
+          kk[j] = mma(ka[0][s], bh, kk[j]);
+          qk[j] = mma(qa[0][s], bh, qk[j]);
+          k2 = mma(ka[1][s], bh, k2);
+          q2 = mma(qa[1][s], bh, q2);
+          k2 = mma(ka[0][s], bl, k2);
+          q2 = mma(qa[0][s], bl, q2);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          kk[j][q] = __builtin_fmaf(k2[q], kUnlow, kk[j][q]) * 0x1p-16f;
+          qk[j][q] = __builtin_fmaf(q2[q], kUnlow, qk[j][q]) * 0x1p-8f;
+        }
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    double ri[4];
+    float bt[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = 16 * wave + 4 * g + q;
+      ri[q] = run[h][i], bt[q] = beta[h][i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = 16 * j + c;
+      const double rj = run[h][col];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = 16 * wave + 4 * g + q;
+        const float fade = i >= col ? __builtin_amdgcn_exp2f((float)(ri[q] - rj)) : 0.f;
+        am[h][i][col] = i > col ? bt[q] * fade * kk[j][q] : 0.f;
+        pm[h][i][col] = fade * qk[j][q];
+      }
+    }
+  }
+  __syncthreads();
+  // ---- a matrix's pieces on and below the diagonal, three a wave
+  auto pieces = [&](const float(*m)[PC][MS], int off, float f) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int p = wave * 3 + i, h = p / 6, k = p % 6, w = k < 2 ? k : (k + 2) >> 1, s = k < 2 ? 0 : k & 1;
+      v8h hi, lo;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const v4f v = *reinterpret_cast<const v4f*>(&m[h][16 * w + c][32 * s + 8 * g + 4 * j]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          _Float16 a, b;
+          split(v[q] * f, a, b);
+          hi[4 * j + q] = a, lo[4 * j + q] = b;
+        }
+      }
+      uint8_t* o = u + kUHead + h * kHeadBytes + off + k * kPiece + 16 * lane;
+      *reinterpret_cast<v8h*>(o) = hi;
+      *reinterpret_cast<v8h*>(o + 6 * kPiece) = lo;
+    }
+  };
+  pieces(pm, kHP, 1.f);
+  // ---- T in place of A.  First the 16 x 16 blocks on the diagonal: lane (block, column), by rows
+  if (wave < 2) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float* row = &am[wave][16 * g + i][16 * g];
+      float v = i == c ? 1.f : 0.f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) v = __builtin_fmaf(-row[l], x[l], v);
+      x[i] = v;
+    }
+    // (a block's rows were read by its own 16 lanes alone, all of them before these stores)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) am[wave][16 * g + i][16 * g + c] = x[i];
+  }
+  __syncthreads();
+  // ---- blocks of 32: -D1 A10 D0, a wave each.  The fp32 instruction's depth is taken in the order 4 g + q, so that a
+  // result's registers are the next product's operand.
+  auto mm = [](float a, float b, v4f acc) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); };
+  {
+    const int h = wave >> 1, r0 = 32 * (wave & 1), r1 = r0 + 16;
+    const v4f a = *reinterpret_cast<const v4f*>(&am[h][r1 + c][r0 + 4 * g]);
+    const v4f d1 = *reinterpret_cast<const v4f*>(&am[h][r1 + c][r1 + 4 * g]);
+    v4f y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) y = mm(a[q], am[h][r0 + 4 * g + q][r0 + c], y);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) z = mm(d1[q], y[q], z);
+    // (this block is read by this wave alone)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) am[h][r1 + 4 * g + q][r0 + c] = -z[q];
+  }
+  __syncthreads();
+  // ---- the block of 32 below: two waves a head, 16 columns each
+  {
+    const int h = wave >> 1, col = 16 * (wave & 1) + c;
+    v4f y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, z[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      float b[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) b[q] = am[h][16 * kt + 4 * g + q][col];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const v4f a = *reinterpret_cast<const v4f*>(&am[h][32 + 16 * i + c][16 * kt + 4 * g]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) y[i] = mm(a[q], b[q], y[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int kt = 0; kt <= i; ++kt) {
+        const v4f a = *reinterpret_cast<const v4f*>(&am[h][32 + 16 * i + c][32 + 16 * kt + 4 * g]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[i] = mm(a[q], y[kt][q], z[i]);
+      }
+    __syncthreads();  // both waves have read the block
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) am[h][32 + 16 * i + 4 * g + q][col] = -z[i][q];
+  }
+  __syncthreads();
+  pieces(am, kHT, 256.f);
+}
+
+// Largest power of two that keeps bound x factor within 2^15.
+__device__ __forceinline__ float factor_of(float bound) {
+  int e = 0;
+  (void)__builtin_frexpf(bound, &e);  // bound < 2^e
+  return bound > 0.f ? __builtin_ldexpf(1.f, min(max(15 - e, -100), 100)) : 1.f;
+}
+
+// A request's chunks for 16 NC value columns of a head.  Wave w holds key dims 32 w .. + 31 of the state and computes token
+// tile w of each product; the state, X and U pass between the waves through LDS as fp16 parts.  They are brought into
+// fp16's range by a power of two for each column, from a bound on the column's norm that holds whatever the values:
+// |s_j| <= |s_{j-1}| + |v_j| (the step shrinks s), so |S|, |X|, |U| <= |S before the chunk| + 65 max |v|.
+template <int NC>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void prompt_scan_kernel(PromptDev d) {
+  constexpr int COLS = 16 * NC, BLOCKS = PV / COLS, SS = PK + 8, XS = PC + 8;
+  __shared__ __attribute__((aligned(16))) _Float16 sp[2][COLS][SS];  // the state's parts
+  __shared__ __attribute__((aligned(16))) _Float16 xp[2][COLS][XS];  // X's
+  __shared__ __attribute__((aligned(16))) _Float16 up[4][COLS][XS];  // U's parts; the decayed U's
+  __shared__ float most[4][COLS];
+  // the 2 BLOCKS workgroups of a (request, key head) on one XCD, which the chunks' operands came from
+  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  const int grp = (at / (2 * BLOCKS)) * 8 + xcd, in = at % (2 * BLOCKS);
+  const int r = grp / PHK, hk = grp % PHK, hh = in / BLOCKS, hv = 2 * hk + hh, col0 = (in % BLOCKS) * COLS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+  int t0, n;
+  int64_t slot;
+  bool old;
+  request_of(d, r, t0, n, slot, old);
+  if (n <= kShort || slot < 0) return;
+  const int chunks = (n + PC - 1) / PC;
+  const uint8_t* u = d.units + ((int64_t)first_unit(d, r, t0) * PHK + hk) * kUnit;  // a chunk's operands, then the next's
+  constexpr int64_t kNext = (int64_t)PHK * kUnit;
+
+  // ---- the state: dims 32 wave + 16 i + 4 g + q of column 16 j + c
+  float* const hp = d.h0 + ((slot * PHV + hv) * PV + col0 + c) * PK + 32 * wave + 4 * g;
+  v4f S[2][NC];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) S[i][j] = old ? *reinterpret_cast<const v4f*>(hp + 16 * j * PK + 16 * i) : v4f{0.f, 0.f, 0.f, 0.f};
+  // ---- values: tokens 16 wave + 4 g + q of a chunk
+  const int vch = 2 * PHK * PK + hv * PV + col0 + c;
+  float cw[NC][4];
+  uint32_t raw[NC][7];
+  float v[NC][4];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const v2i w = *reinterpret_cast<const v2i*>(d.conv_w + (int64_t)(vch + 16 * j) * 4);
+    cw[j][0] = bf_lo((uint32_t)w[0]), cw[j][1] = bf_hi((uint32_t)w[0]), cw[j][2] = bf_lo((uint32_t)w[1]), cw[j][3] = bf_hi((uint32_t)w[1]);
+  }
+  auto load_v = [&](int ch) {
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+      const int t = ch * PC + 16 * wave + 4 * g + i - 3;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) raw[j][i] = d.mixed[(int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + vch + 16 * j];
+    }
+  };
+  auto conv_v = [&](int ch) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float y = __builtin_fmaf(bf2f(raw[j][q + 3]), cw[j][3],
+                                       __builtin_fmaf(bf2f(raw[j][q + 2]), cw[j][2],
+                                                      __builtin_fmaf(bf2f(raw[j][q + 1]), cw[j][1], bf2f(raw[j][q]) * cw[j][0])));
+        v[j][q] = ch * PC + 16 * wave + 4 * g + q < n ? fast_silu(y) : 0.f;
+      }
+      float m = fmaxf(fmaxf(fabsf(v[j][0]), fabsf(v[j][1])), fmaxf(fabsf(v[j][2]), fabsf(v[j][3])));
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      if (g == 0) most[wave][16 * j + c] = m;
+    }
+  };
+  auto store_s = [&](const float* f) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        v4h hi, lo;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          _Float16 a, b;
+          split(S[i][j][q] * f[j], a, b);
+          hi[q] = a, lo[q] = b;
+        }
+        *reinterpret_cast<v4h*>(&sp[0][16 * j + c][32 * wave + 16 * i + 4 * g]) = hi;
+        *reinterpret_cast<v4h*>(&sp[1][16 * j + c][32 * wave + 16 * i + 4 * g]) = lo;
+      }
+  };
+  load_v(0);
+  if (wave == 0 && g == 0) {  // the inputs before the request's first
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) raw[j][i] = old ? d.conv_state[slot * d.cs_slot + (int64_t)(vch + 16 * j) * 3 + i] : 0;
+  }
+  // ---- operands of a chunk
+  v8h K[2][4], Kt[2][2][2], Q[2][4], T[2][2], P[2][2];
+  v4f eb, rest, bt;
+  float eend;
+  auto piece = [&](const uint8_t* p, int off) { return *reinterpret_cast<const v8h*>(p + off + 16 * lane); };
+  auto load_kq = [&](const uint8_t* p) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      K[0][s] = piece(p, kUK + (wave * 4 + s) * kPiece);
+      K[1][s] = piece(p, kUK + (16 + wave * 4 + s) * kPiece);
+      Q[0][s] = piece(p, kUQ + (wave * 4 + s) * kPiece);
+      Q[1][s] = piece(p, kUQ + (16 + wave * 4 + s) * kPiece);
+    }
+  };
+  auto load_t = [&](const uint8_t* p) {
+    const uint8_t* h = p + kUHead + hh * kHeadBytes;
+    const int last = wave < 2 ? 0 : 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      T[0][s] = piece(h, kHT + tri_piece(wave, min(s, last)) * kPiece);
+      T[1][s] = piece(h, kHT + (6 + tri_piece(wave, min(s, last))) * kPiece);
+    }
+  };
+  auto load_kt = [&](const uint8_t* p) {
+    const uint8_t* h = p + kUHead + hh * kHeadBytes;
+    const int last = wave < 2 ? 0 : 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        Kt[0][i][s] = piece(p, kUKt + ((2 * wave + i) * 2 + s) * kPiece);
+        Kt[1][i][s] = piece(p, kUKt + (16 + (2 * wave + i) * 2 + s) * kPiece);
+      }
+      P[0][s] = piece(h, kHP + tri_piece(wave, min(s, last)) * kPiece);
+      P[1][s] = piece(h, kHP + (6 + tri_piece(wave, min(s, last))) * kPiece);
+    }
+  };
+  auto load_gates = [&](const uint8_t* p) {
+    const float* gt = reinterpret_cast<const float*>(p + kUHead + hh * kHeadBytes + kHGate);
+    eb = *reinterpret_cast<const v4f*>(gt + 16 * wave + 4 * g);
+    rest = *reinterpret_cast<const v4f*>(gt + 64 + 16 * wave + 4 * g);
+    bt = *reinterpret_cast<const v4f*>(gt + 128 + 16 * wave + 4 * g);
+    eend = gt[192];
+  };
+  load_kq(u), load_t(u), load_kt(u), load_gates(u);
+  // ---- the columns' bounds: the state's norms, then the first chunk's values
+  float before[NC], vmost[NC], fac[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ss = fmaxf(ss, fabsf(S[i][j][q]));
+    ss = fmaxf(ss, __shfl_xor(ss, 16));
+    ss = fmaxf(ss, __shfl_xor(ss, 32));
+    if (g == 0) most[wave][16 * j + c] = ss;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NC; ++j)  // a norm is at most sqrt(128) times the largest value
+    before[j] = 11.32f * fmaxf(fmaxf(most[0][16 * j + c], most[1][16 * j + c]), fmaxf(most[2][16 * j + c], most[3][16 * j + c]));
+#pragma unroll
+  for (int j = 0; j < NC; ++j) vmost[j] = 0.f;
+  __syncthreads();
+  conv_v(0);
+  __syncthreads();
+  auto next_factor = [&](float e) {  // (behind a barrier since conv_v)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const float m = fmaxf(fmaxf(most[0][16 * j + c], most[1][16 * j + c]), fmaxf(most[2][16 * j + c], most[3][16 * j + c]));
+      before[j] = __builtin_fmaf(64.f, vmost[j], before[j] * e);  // (what the chunk adds is not decayed by all of e)
+      vmost[j] = m;
+      fac[j] = factor_of(__builtin_fmaf(65.f, m, before[j]) * 1.01f);
+    }
+  };
+  next_factor(1.f);
+  store_s(fac);
+  if (chunks > 1) load_v(1);
+  __syncthreads();
+  const int nks = wave < 2 ? 1 : 2;
+  uint16_t* const outp = d.out + (int64_t)(t0 + 16 * wave + 4 * g) * PZ + hv * PV + col0 + c;
+  int8_t* const expp = d.exps + (int64_t)(t0 + 16 * wave) * 256 + hv * 8 + col0 / 16;
+
+  for (int ch = 0; ch < chunks; ++ch) {
+    const bool more = ch + 1 < chunks;
+    const uint8_t* const un = u + kNext;
+    v4f o[NC];
+    float inv[NC];
+    // ---- K S and Q S
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1, q1 = a1, q2 = a1;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const v8h bh = *reinterpret_cast<const v8h*>(&sp[0][16 * j + c][32 * s + 8 * g]);
+        const v8h bl = *reinterpret_cast<const v8h*>(&sp[1][16 * j + c][32 * s + 8 * g]);
+        a1 = mma(K[0][s], bh, a1);
+        a2 = mma(K[1][s], bh, a2);
+        q1 = mma(Q[0][s], bh, q1);
+        q2 = mma(Q[1][s], bh, q2);
+        a2 = mma(K[0][s], bl, a2);
+        q2 = mma(Q[0][s], bl, q2);
+      }
+      inv[j] = 0x1p-8f / fac[j];
+      v4h hi, lo;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float ks = __builtin_fmaf(a2[q], kUnlow, a1[q]) * 0x1p-8f;
+        _Float16 a, b;
+        split(bt[q] * __builtin_fmaf(-eb[q], ks, v[j][q] * fac[j]), a, b);
+        hi[q] = a, lo[q] = b;
+        o[j][q] = eb[q] * __builtin_fmaf(q2[q], kUnlow, q1[q]);
+      }
+      *reinterpret_cast<v4h*>(&xp[0][16 * j + c][16 * wave + 4 * g]) = hi;
+      *reinterpret_cast<v4h*>(&xp[1][16 * j + c][16 * wave + 4 * g]) = lo;
+    }
+    const v4f fade = rest;
+    const float e = eend;
+    if (more) {
+      load_kq(un);
+      load_gates(un);
+      conv_v(ch + 1);
+      if (ch + 2 < chunks) load_v(ch + 2);
+    }
+    __syncthreads();
+    // ---- U = T X
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s < nks) {
+          const v8h bh = *reinterpret_cast<const v8h*>(&xp[0][16 * j + c][32 * s + 8 * g]);
+          const v8h bl = *reinterpret_cast<const v8h*>(&xp[1][16 * j + c][32 * s + 8 * g]);
+          a1 = mma(T[0][s], bh, a1);
+          a2 = mma(T[1][s], bh, a2);
+          a2 = mma(T[0][s], bl, a2);
+        }
+      }
+      v4h uh, ul, dh, dl;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float x = __builtin_fmaf(a2[q], kUnlow, a1[q]) * 0x1p-8f;
+        _Float16 a, b;
+        split(x, a, b);
+        uh[q] = a, ul[q] = b;
+        split(x * fade[q], a, b);
+        dh[q] = a, dl[q] = b;
+      }
+      *reinterpret_cast<v4h*>(&up[0][16 * j + c][16 * wave + 4 * g]) = uh;
+      *reinterpret_cast<v4h*>(&up[1][16 * j + c][16 * wave + 4 * g]) = ul;
+      *reinterpret_cast<v4h*>(&up[2][16 * j + c][16 * wave + 4 * g]) = dh;
+      *reinterpret_cast<v4h*>(&up[3][16 * j + c][16 * wave + 4 * g]) = dl;
+    }
+    if (more) {
+      load_t(un);
+      next_factor(e);
+    }
+    __syncthreads();
+    // ---- S' = e^{b_end} S + K^T U, and its parts for the next chunk
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const v8h bh = *reinterpret_cast<const v8h*>(&up[2][16 * j + c][32 * s + 8 * g]);
+          const v8h bl = *reinterpret_cast<const v8h*>(&up[3][16 * j + c][32 * s + 8 * g]);
+          a1 = mma(Kt[0][i][s], bh, a1);
+          a2 = mma(Kt[1][i][s], bh, a2);
+          a2 = mma(Kt[0][i][s], bl, a2);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          S[i][j][q] = __builtin_fmaf(__builtin_fmaf(a2[q], kUnlow, a1[q]), inv[j], e * S[i][j][q]);
+      }
+    }
+    if (more) store_s(fac);
+    // ---- O = e^b Q S + P U
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s < nks) {
+          const v8h bh = *reinterpret_cast<const v8h*>(&up[0][16 * j + c][32 * s + 8 * g]);
+          const v8h bl = *reinterpret_cast<const v8h*>(&up[1][16 * j + c][32 * s + 8 * g]);
+          a1 = mma(P[0][s], bh, a1);
+          a2 = mma(P[1][s], bh, a2);
+          a2 = mma(P[0][s], bl, a2);
+        }
+      }
+      float y[4], m = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        y[q] = (o[j][q] + __builtin_fmaf(a2[q], kUnlow, a1[q])) * (inv[j] * d.scale);
+        m = fmaxf(m, fabsf(y[q]));
+      }
+      // the tile's outputs as fp16 times a power of two, in out's place until the norm
+      m = __uint_as_float(wave_max_u32(__float_as_uint(m)));
+      int ex = 0;
+      (void)__builtin_frexpf(m, &ex);
+      ex = min(max(ex, -110), 127);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int t = ch * PC + 16 * wave + 4 * g + q;
+        if (t < n) {
+          outp[((int64_t)ch * PC + q) * PZ + 16 * j] = __builtin_bit_cast(uint16_t, (_Float16)__builtin_ldexpf(y[q], 14 - ex));
+        }
+      }
+      if (g == 0 && ch * PC + 16 * wave + c < n) expp[((int64_t)ch * PC + c) * 256 + j] = (int8_t)ex;
+    }
+    if (more) load_kt(un);
+    u = un;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) *reinterpret_cast<v4f*>(hp + 16 * j * PK + 16 * i) = S[i][j];
+  // ---- the conv state: the request's last three inputs (longer than three).  This workgroup's value channels; q and k by the
+  // first workgroup of the key head, behind the kernel that read them
+  for (int i = tid; i < COLS * 3; i += 256) {
+    const int cc = 2 * PHK * PK + hv * PV + col0 + i / 3;
+    d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
+  }
+  if (in == 0)
+    for (int i = tid; i < 2 * PK * 3; i += 256) {
+      const int cc = (i / (3 * PK)) * (PHK * PK) + hk * PK + i / 3 % PK;
+      d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
+    }
+}
+
+// The gated norm of the chunks' rows: a wave a row, 16 lanes a head.
+__global__ __launch_bounds__(256) void prompt_norm_kernel(PromptDev d) {
+  const int lane = threadIdx.x & 63;
+  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (row >= d.rows) return;
+  const int r = last_at_most(d.B, row, [&](int i) { return d.qsl[i]; });
+  int t0, n;
+  int64_t slot;
+  bool old;
+  request_of(d, r, t0, n, slot, old);
+  if (n <= kShort || slot < 0 || row < t0 || row >= t0 + n) return;
+  const int c = lane & 15;
+  const v4i wr = *reinterpret_cast<const v4i*>(d.norm_w + 8 * c);
+  v4i o[8], z[8];
+  int ex[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t at = (int64_t)row * PZ + i * 512 + lane * 8;
+    o[i] = *reinterpret_cast<const v4i*>(d.out + at);
+    z[i] = *reinterpret_cast<const v4i*>(d.z + at);
+    ex[i] = d.exps[(int64_t)row * 256 + (4 * i + (lane >> 4)) * 8 + (c >> 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t at = (int64_t)row * PZ + i * 512 + lane * 8;
+    const v8h h = __builtin_bit_cast(v8h, o[i]);
+    float x[8], ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      x[k] = __builtin_ldexpf((float)h[k], ex[i] - 14);
+      ss = __builtin_fmaf(x[k], x[k], ss);
+    }
+    const float rstd = 1.f / sqrtf(row16_sum(ss) * (1.f / PV) + d.eps);
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float zz = (k & 1) ? bf_hi((uint32_t)z[i][k >> 1]) : bf_lo((uint32_t)z[i][k >> 1]);
+      const float ww = (k & 1) ? bf_hi((uint32_t)wr[k >> 1]) : bf_lo((uint32_t)wr[k >> 1]);
+      y[k] = x[k] * rstd * ww * fast_silu(zz);
+    }
+    v4i w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (int)pack_bf2(y[2 * k], y[2 * k + 1]);
+    *reinterpret_cast<v4i*>(d.out + at) = w;
+    if (d.oq) {
+      float f[8], m = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        f[k] = (k & 1) ? bf_hi((uint32_t)w[k >> 1]) : bf_lo((uint32_t)w[k >> 1]);
+        m = fmaxf(m, fabsf(f[k]));
+      }
+      m = fmaxf(m, lane_xor<1>(m));
+      m = fmaxf(m, lane_xor<2>(m));
+      m = fmaxf(m, lane_xor<4>(m));
+      m = fmaxf(m, lane_xor<8>(m));
+      const uint2 q = e4m3_run8(f, m > 0.f ? 448.f / m : 0.f);
+      *reinterpret_cast<uint2*>(d.oq + at) = q;
+      if (c == 0) d.oqs[(int64_t)row * PHV + 4 * i + (lane >> 4)] = m / 448.f;
+    }
+  }
+}
+
+// Chunks that `rows` rows of B requests can make: one a request more than whole ones, and a long request has kShort + 1 rows.
+int64_t chunk_units(int64_t rows, int64_t B) {
+  const int64_t by = rows / (kShort + 1);
+  return rows <= kShort ? 0 : rows / PC + (B <= by ? B : by);
+}
+
 }  // namespace
 }  // namespace q36
 
@@ -191,7 +935,8 @@ using namespace q36;
 
 extern "C" size_t q36_gdn_prompt_workspace_bytes(int32_t rows, int32_t B) {
   if (rows < 1 || B < 1) return 0;
-  return 256;
+  const size_t units = (size_t)chunk_units(rows, B);
+  return units ? units * PHK * kUnit + align_up((size_t)rows * 256, 256) : 256;
 }
 
 extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream) {
@@ -218,8 +963,16 @@ extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream)
               static_cast<const uint16_t*>(a->mixed), static_cast<const uint16_t*>(a->z), static_cast<const uint16_t*>(a->a),
               static_cast<const uint16_t*>(a->b), static_cast<uint16_t*>(a->conv_state), a->cs_slot,
               static_cast<const uint16_t*>(a->conv_w), a->A_log, a->dt_bias, a->h0, a->qsl, a->state_idx, a->prefix,
-              static_cast<const uint16_t*>(a->norm_w), static_cast<uint16_t*>(a->out), static_cast<uint8_t*>(a->oq), a->oqs};
+              static_cast<const uint16_t*>(a->norm_w), static_cast<uint16_t*>(a->out), static_cast<uint8_t*>(a->oq), a->oqs,
+              static_cast<uint8_t*>(a->workspace), nullptr, a->B > a->rows / (kShort + 1)};
+  const int64_t units = chunk_units(a->rows, a->B);
+  d.exps = reinterpret_cast<int8_t*>(d.units + units * PHK * kUnit);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   prompt_steps_kernel<<<(unsigned)a->B * PHK, 512, 0, st>>>(d);
+  if (units) {
+    prompt_chunks_kernel<<<(unsigned)units * PHK, 256, 0, st>>>(d);
+    prompt_scan_kernel<1><<<(unsigned)a->B * PHK * 16, 256, 0, st>>>(d);
+    prompt_norm_kernel<<<(unsigned)(a->rows + 3) / 4, 256, 0, st>>>(d);
+  }
   return check_launch("q36_gdn_prompt");
 }
