@@ -19,7 +19,8 @@ constexpr int kShort = 8;  // requests of up to so many new tokens go token by t
 constexpr int PC = 64;     // tokens of a chunk
 
 // A chunk's operands for one key head, as the scan's lanes load them: pieces of 1 KB, lane l's 16 bytes at 16 l, element (row
-// r, depth k) of a 16 x 32 operand piece in lane r + 16 (k / 8).  Values times 2^8 in fp16, low parts times 2^11 more.
+// r, depth k) of a 16 x 32 operand piece in lane r + 16 (k / 8).  fp16 times 2^8, in a plane of high and one of low parts.
+// (The factor keeps small entries exact: T's are of the size of beta, and what they multiply can be large.)
 constexpr int kPiece = 1024;
 constexpr int kUK = 0;                        // K: [plane][token tile 4][depth 4] (depth: key dims by 32)
 constexpr int kUKt = kUK + 32 * kPiece;       // K^T: [plane][dim tile 8][depth 2] (depth: tokens by 32)
@@ -27,7 +28,7 @@ constexpr int kUQ = kUKt + 32 * kPiece;       // Q: as K
 constexpr int kUHead = kUQ + 32 * kPiece;     // then for each of the two value heads:
 constexpr int kHT = 0;                        //   T: [plane][6 pieces on and below the diagonal]
 constexpr int kHP = kHT + 12 * kPiece;        //   P: as T
-constexpr int kHGate = kHP + 12 * kPiece;     //   fp32 [64] each: e^{b_i}, e^{b_end - b_i}, beta; then e^{b_end}
+constexpr int kHGate = kHP + 12 * kPiece;     //   fp32 [64] each: e^{b_i}, 2^-8 e^{b_end - b_i}, beta, 2^-8 beta e^{b_i}
 constexpr int kHeadBytes = kHGate + kPiece;
 constexpr int kUnit = kUHead + 2 * kHeadBytes;
 // piece of (token tile w, depth s) among those on and below the diagonal: tiles 0 and 1 have one, 2 and 3 two
@@ -94,14 +95,19 @@ typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-constexpr float kLow = 2048.f, kUnlow = 1.f / 2048.f;  // a low part's own factor
-// x = hi + lo / 2^11: 22 significand bits for x in fp16's normal range.  x is kept from the compiler's eyes: where it sees a
-// product behind x, one use of hi becomes a multiply that rounds once to fp16 and another the rounding of the fp32 product,
-// and where these differ (one value in 2^12) lo belongs to another hi.
-__device__ __forceinline__ void split(float x, _Float16& hi, _Float16& lo) {
+// Four values in two parts each, x = hi + lo within 2^-22 of itself or 2^-25, whichever is more (fp16's smallest step is 2^-24;
+// the matrix instruction takes subnormal operands).  x is kept from the compiler's eyes: where it sees a product behind x,
+// it makes one use of hi a multiply that rounds once to fp16 and another the rounding of the fp32 product, and where these
+// differ (one value in 2^12) lo belongs to another hi.
+__device__ __forceinline__ void split4(v4f x, v4h& hi, v4h& lo) {
   asm("" : "+v"(x));
-  hi = (_Float16)x;
-  lo = (_Float16)((x - (float)hi) * kLow);
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const v2h h = __builtin_convertvector((q36_v2f){x[i], x[i + 1]}, v2h);
+    const v2h l = __builtin_convertvector(
+        (q36_v2f){__builtin_fmaf((float)h[0], -1.f, x[i]), __builtin_fmaf((float)h[1], -1.f, x[i + 1])}, v2h);
+    hi[i] = h[0], hi[i + 1] = h[1], lo[i] = l[0], lo[i + 1] = l[1];
+  }
 }
 
 __device__ __forceinline__ float fast_silu(float x) {
@@ -264,7 +270,7 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
 // of U that nearly cancels, and the norm brings the row back to size (high parts alone: rows 8 % off, 0.1 % elsewhere).
 
 // q, k of a chunk for one key head; T, P and gates of its two value heads.
-__global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void prompt_chunks_kernel(PromptDev d) {
   constexpr int RS = PK + 8, MS = PC + 4;  // padded rows, in elements
   __shared__ __attribute__((aligned(16))) _Float16 planes[2][2][PC][RS];  // [q, k][hi, lo]; later A and P
   __shared__ double run[2][PC];  // log2 of the decay up to a token
@@ -284,12 +290,13 @@ __global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
   uint8_t* const u = d.units + (int64_t)blockIdx.x * kUnit;
   const int g = lane >> 4, c = lane & 15;
 
-  // ---- conv, SiLU, unit vectors: thread (run of 8 tokens, 8 channels of q or k)
+  // ---- conv, SiLU, unit vectors: thread (run of 4 tokens, 8 channels of q or k)
   {
-    const int tr = (tid >> 5) * 8, part = (tid >> 4) & 1, ch = part * (PHK * PK) + hk * PK + c * 8;
-    v4i raw[11];
+    constexpr int R = 4;
+    const int tr = (tid >> 5) * R, part = (tid >> 4) & 1, ch = part * (PHK * PK) + hk * PK + c * 8;
+    v4i raw[R + 3];
 #pragma unroll
-    for (int i = 0; i < 11; ++i) {
+    for (int i = 0; i < R + 3; ++i) {
       const int t = c0 + tr + i - 3;
       raw[i] = *reinterpret_cast<const v4i*>(d.mixed + (int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + ch);
     }
@@ -307,53 +314,38 @@ __global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) raw[i][j] = (int)(at(3 * (2 * j) + i) | (at(3 * (2 * j + 1) + i) << 16));
     }
-    float y[8][8];
+    float y[R][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t wlo = (uint32_t)wr[e >> 1][2 * (e & 1)], whi = (uint32_t)wr[e >> 1][2 * (e & 1) + 1];
       const float w0 = bf_lo(wlo), w1 = bf_hi(wlo), w2 = bf_lo(whi), w3 = bf_hi(whi);
-      float x[11];
+      float x[R + 3];
 #pragma unroll
-      for (int i = 0; i < 11; ++i) x[i] = (e & 1) ? bf_hi((uint32_t)raw[i][e >> 1]) : bf_lo((uint32_t)raw[i][e >> 1]);
+      for (int i = 0; i < R + 3; ++i) x[i] = (e & 1) ? bf_hi((uint32_t)raw[i][e >> 1]) : bf_lo((uint32_t)raw[i][e >> 1]);
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
+      for (int t = 0; t < R; ++t)
         y[t][e] = fast_silu(__builtin_fmaf(x[t + 3], w3, __builtin_fmaf(x[t + 2], w2, __builtin_fmaf(x[t + 1], w1, x[t] * w0))));
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
+    for (int t = 0; t < R; ++t) {
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(y[t][e], y[t][e], ss);
-      ss = row16_sum(ss);
-      const float rr = c0 + tr + t < n ? 256.f / sqrtf(ss + 1e-6f) : 0.f;
+      const bool in = c0 + tr + t < n;
+      const float rr = in ? 256.f / sqrtf(row16_sum(ss) + 1e-6f) : 0.f;
+      v8h hi, lo;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[t][e] = c0 + tr + t < n ? y[t][e] * rr : 0.f;
-    }
-    v8h lo[8];  // the low parts by token
+      for (int e = 0; e < 8; e += 4) {
+        v4h a, b;
+        v4f x;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      v8h hi;
+        for (int k = 0; k < 4; ++k) x[k] = in ? y[t][e + k] * rr : 0.f;  // (a row behind the request's may hold anything)
+        split4(x, a, b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        _Float16 a, b;
-        split(y[t][e], a, b);
-        hi[e] = a, lo[t][e] = b;
-        y[t][e] = (float)a;
+        for (int k = 0; k < 4; ++k) hi[e + k] = a[k], lo[e + k] = b[k];
       }
       *reinterpret_cast<v8h*>(&planes[part][0][tr + t][8 * c]) = hi;
-      *reinterpret_cast<v8h*>(&planes[part][1][tr + t][8 * c]) = lo[t];
-    }
-    if (part == 1) {  // K^T: eight tokens of a dim are a lane's 16 bytes
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int dim = 8 * c + e;
-        v8h a, b;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) a[t] = (_Float16)y[t][e], b[t] = lo[t][e];
-        uint8_t* p = u + kUKt + ((dim >> 4) * 2 + (tr >> 5)) * kPiece + 16 * ((dim & 15) + 16 * ((tr >> 3) & 3));
-        *reinterpret_cast<v8h*>(p) = a;
-        *reinterpret_cast<v8h*>(p + 16 * kPiece) = b;
-      }
+      *reinterpret_cast<v8h*>(&planes[part][1][tr + t][8 * c]) = lo;
     }
   }
   // ---- gates: a wave a value head, a lane a token
@@ -373,96 +365,102 @@ __global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
     run[wave][lane] = s;
     beta[wave][lane] = bt;
     float* gt = reinterpret_cast<float*>(u + kUHead + wave * kHeadBytes + kHGate);
-    gt[lane] = __builtin_amdgcn_exp2f((float)s);
-    gt[64 + lane] = __builtin_amdgcn_exp2f((float)(end - s));
+    const float eb = __builtin_amdgcn_exp2f((float)s);
+    gt[lane] = eb;
+    gt[64 + lane] = 0x1p-8f * __builtin_amdgcn_exp2f((float)(end - s));
     gt[128 + lane] = bt;
-    if (lane == 0) gt[192] = __builtin_amdgcn_exp2f((float)end);
+    gt[192 + lane] = 0x1p-8f * bt * eb;
   }
   __syncthreads();
-  // ---- K K^T and Q K^T on and below the diagonal: wave w rows 16 w .. + 15.  The operands' pieces go to the workspace as read
-  v4f kk[4], qk[4];
+  // ---- K K^T (waves 0-3) and Q K^T (4-7) on and below the diagonal: rows 16 (w & 3) .. + 15.  The operands' pieces go to the
+  // workspace as read; then K^T's, gathered eight tokens a lane
+  const int w = wave & 3, what = wave < 4 ? 1 : 0;
+  v4f qk[4];
   {
-    v8h ka[2][4], qa[2][4];
+    v8h a[2][4];
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        ka[p][s] = *reinterpret_cast<const v8h*>(&planes[1][p][16 * wave + c][32 * s + 8 * g]);
-        qa[p][s] = *reinterpret_cast<const v8h*>(&planes[0][p][16 * wave + c][32 * s + 8 * g]);
-        *reinterpret_cast<v8h*>(u + kUK + (p * 16 + wave * 4 + s) * kPiece + 16 * lane) = ka[p][s];
-        *reinterpret_cast<v8h*>(u + kUQ + (p * 16 + wave * 4 + s) * kPiece + 16 * lane) = qa[p][s];
+        a[p][s] = *reinterpret_cast<const v8h*>(&planes[what][p][16 * w + c][32 * s + 8 * g]);
+        *reinterpret_cast<v8h*>(u + (what ? kUK : kUQ) + (p * 16 + w * 4 + s) * kPiece + 16 * lane) = a[p][s];
       }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      kk[j] = qk[j] = v4f{0.f, 0.f, 0.f, 0.f};
-      if (j <= wave) {
-        v4f k2 = {0.f, 0.f, 0.f, 0.f}, q2 = {0.f, 0.f, 0.f, 0.f};
+      qk[j] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (j <= w) {
+        v4f q2 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const v8h bh = *reinterpret_cast<const v8h*>(&planes[1][0][16 * j + c][32 * s + 8 * g]);
           const v8h bl = *reinterpret_cast<const v8h*>(&planes[1][1][16 * j + c][32 * s + 8 * g]);
-          kk[j] = mma(ka[0][s], bh, kk[j]);
-          qk[j] = mma(qa[0][s], bh, qk[j]);
-          k2 = mma(ka[1][s], bh, k2);
-          q2 = mma(qa[1][s], bh, q2);
-          k2 = mma(ka[0][s], bl, k2);
-          q2 = mma(qa[0][s], bl, q2);
+          qk[j] = mma(a[0][s], bh, qk[j]);
+          q2 = mma(a[1][s], bh, q2);
+          q2 = mma(a[0][s], bl, q2);
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          kk[j][q] = __builtin_fmaf(k2[q], kUnlow, kk[j][q]) * 0x1p-16f;
-          qk[j][q] = __builtin_fmaf(q2[q], kUnlow, qk[j][q]) * 0x1p-8f;
-        }
+        for (int q = 0; q < 4; ++q) qk[j][q] = (qk[j][q] + q2[q]) * (what ? 0x1p-16f : 0x1p-8f);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = wave * 4 + i, p = k >> 4, tile = (k >> 1) & 7, s = k & 1;
+      v8h x;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) x[t] = planes[1][p][32 * s + 8 * g + t][16 * tile + c];
+      *reinterpret_cast<v8h*>(u + kUKt + k * kPiece + 16 * lane) = x;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    float(*const m)[MS] = what ? am[h] : pm[h];
     double ri[4];
     float bt[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int i = 16 * wave + 4 * g + q;
-      ri[q] = run[h][i], bt[q] = beta[h][i];
+      const int i = 16 * w + 4 * g + q;
+      ri[q] = run[h][i], bt[q] = what ? beta[h][i] : 1.f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int col = 16 * j + c;
+      if (j > w) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m[16 * w + 4 * g + q][col] = 0.f;
+        continue;
+      }
       const double rj = run[h][col];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int i = 16 * wave + 4 * g + q;
-        const float fade = i >= col ? __builtin_amdgcn_exp2f((float)(ri[q] - rj)) : 0.f;
-        am[h][i][col] = i > col ? bt[q] * fade * kk[j][q] : 0.f;
-        pm[h][i][col] = fade * qk[j][q];
+        const int i = 16 * w + 4 * g + q;
+        const bool on = what ? i > col : i >= col;  // (above, e^{b_i - b_j} may be infinite)
+        m[i][col] = on ? bt[q] * __builtin_amdgcn_exp2f((float)(ri[q] - rj)) * qk[j][q] : 0.f;
       }
     }
   }
   __syncthreads();
-  // ---- a matrix's pieces on and below the diagonal, three a wave
-  auto pieces = [&](const float(*m)[PC][MS], int off, float f) {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int p = wave * 3 + i, h = p / 6, k = p % 6, w = k < 2 ? k : (k + 2) >> 1, s = k < 2 ? 0 : k & 1;
+  // ---- a matrix's pieces on and below the diagonal, one of twelve a wave
+  auto pieces = [&](const float(*m)[PC][MS], int first, int waves, int off, float f) {
+    for (int p = first; p < 12; p += waves) {
+      const int h = p / 6, k = p % 6, pw = k < 2 ? k : (k + 2) >> 1, s = k < 2 ? 0 : k & 1;
       v8h hi, lo;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const v4f v = *reinterpret_cast<const v4f*>(&m[h][16 * w + c][32 * s + 8 * g + 4 * j]);
+        v4h a, b;
+        v4f x = *reinterpret_cast<const v4f*>(&m[h][16 * pw + c][32 * s + 8 * g + 4 * j]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          _Float16 a, b;
-          split(v[q] * f, a, b);
-          hi[4 * j + q] = a, lo[4 * j + q] = b;
-        }
+        for (int q = 0; q < 4; ++q) x[q] *= f;
+        split4(x, a, b);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) hi[4 * j + q] = a[q], lo[4 * j + q] = b[q];
       }
       uint8_t* o = u + kUHead + h * kHeadBytes + off + k * kPiece + 16 * lane;
       *reinterpret_cast<v8h*>(o) = hi;
       *reinterpret_cast<v8h*>(o + 6 * kPiece) = lo;
     }
   };
-  pieces(pm, kHP, 1.f);
-  // ---- T in place of A.  First the 16 x 16 blocks on the diagonal: lane (block, column), by rows
+  // ---- T in place of A.  First the 16 x 16 blocks on the diagonal: lane (block, column), by rows; the others write P
   if (wave < 2) {
     float x[16];
 #pragma unroll
@@ -476,12 +474,14 @@ __global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
     // (a block's rows were read by its own 16 lanes alone, all of them before these stores)
 #pragma unroll
     for (int i = 0; i < 16; ++i) am[wave][16 * g + i][16 * g + c] = x[i];
+  } else {
+    pieces(pm, wave - 2, 6, kHP, 1.f);
   }
   __syncthreads();
   // ---- blocks of 32: -D1 A10 D0, a wave each.  The fp32 instruction's depth is taken in the order 4 g + q, so that a
   // result's registers are the next product's operand.
   auto mm = [](float a, float b, v4f acc) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); };
-  {
+  if (wave < 4) {
     const int h = wave >> 1, r0 = 32 * (wave & 1), r1 = r0 + 16;
     const v4f a = *reinterpret_cast<const v4f*>(&am[h][r1 + c][r0 + 4 * g]);
     const v4f d1 = *reinterpret_cast<const v4f*>(&am[h][r1 + c][r1 + 4 * g]);
@@ -495,369 +495,420 @@ __global__ __launch_bounds__(256) void prompt_chunks_kernel(PromptDev d) {
     for (int q = 0; q < 4; ++q) am[h][r1 + 4 * g + q][r0 + c] = -z[q];
   }
   __syncthreads();
-  // ---- the block of 32 below: two waves a head, 16 columns each
+  // ---- the block of 32 below: four waves a head, 16 rows and 16 columns each (a row tile's products twice)
   {
-    const int h = wave >> 1, col = 16 * (wave & 1) + c;
-    v4f y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, z[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const int h = wave >> 2, i = (wave >> 1) & 1, col = 16 * (wave & 1) + c;
+    v4f y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       float b[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) b[q] = am[h][16 * kt + 4 * g + q][col];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const v4f a = *reinterpret_cast<const v4f*>(&am[h][32 + 16 * i + c][16 * kt + 4 * g]);
+      for (int k = 0; k < 2; ++k) {
+        if (k <= i) {
+          const v4f a = *reinterpret_cast<const v4f*>(&am[h][32 + 16 * k + c][16 * kt + 4 * g]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[i] = mm(a[q], b[q], y[i]);
+          for (int q = 0; q < 4; ++q) y[k] = mm(a[q], b[q], y[k]);
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int kt = 0; kt <= i; ++kt) {
+    for (int kt = 0; kt < 2; ++kt) {
+      if (kt <= i) {
         const v4f a = *reinterpret_cast<const v4f*>(&am[h][32 + 16 * i + c][32 + 16 * kt + 4 * g]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) z[i] = mm(a[q], y[kt][q], z[i]);
+        for (int q = 0; q < 4; ++q) z = mm(a[q], y[kt][q], z);
       }
-    __syncthreads();  // both waves have read the block
+    }
+    __syncthreads();  // every wave has read the block
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) am[h][32 + 16 * i + 4 * g + q][col] = -z[i][q];
+    for (int q = 0; q < 4; ++q) am[h][32 + 16 * i + 4 * g + q][col] = -z[q];
   }
   __syncthreads();
-  pieces(am, kHT, 256.f);
+  pieces(am, wave, 8, kHT, 256.f);
 }
 
-// Largest power of two that keeps bound x factor within 2^15.
-__device__ __forceinline__ float factor_of(float bound) {
+// The exponent of the largest power of two that keeps bound times it within 2^15.
+__device__ __forceinline__ int factor_of(float bound) {
   int e = 0;
   (void)__builtin_frexpf(bound, &e);  // bound < 2^e
-  return bound > 0.f ? __builtin_ldexpf(1.f, min(max(15 - e, -100), 100)) : 1.f;
+  return bound > 0.f ? min(max(15 - e, -100), 100) : 0;
 }
 
-// A request's chunks for 16 NC value columns of a head.  Wave w holds key dims 32 w .. + 31 of the state and computes token
-// tile w of each product; the state, X and U pass between the waves through LDS as fp16 parts.  They are brought into
-// fp16's range by a power of two for each column, from a bound on the column's norm that holds whatever the values:
-// |s_j| <= |s_{j-1}| + |v_j| (the step shrinks s), so |S|, |X|, |U| <= |S before the chunk| + 65 max |v|.
+// A buffer of `bytes` at p (the same in every lane): loads behind its end give 0, stores there are dropped.  (What may lie
+// behind the end is told by the lane's offset alone: the check subtracts the scalar offset from the size, unsigned.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
+}
+
+// A request's chunks for 16 NC value columns of a head.  Waves 0-3 carry the state: wave w holds key dims 32 w .. + 31 of it
+// and token tile w of X and U.  Waves 4-7, one beside each of them on its SIMD, convolve the next chunk's values and form the
+// outputs of token tile w - 4, from the same parts in LDS; so the chain from state to state has only its own work in it.
+//
+// State, X and U pass through LDS as fp16 parts.  They are brought into fp16's range by a power of two for each column, from a
+// bound on the column's norm that holds whatever the values: |s_j| <= |s_{j-1}| + |v_j| (the step shrinks s), so |S|, |X|, |U| <=
+// |S before the chunk| + 65 max |v|.
 template <int NC>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void prompt_scan_kernel(PromptDev d) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_scan_kernel(PromptDev d) {
   constexpr int COLS = 16 * NC, BLOCKS = PV / COLS, SS = PK + 8, XS = PC + 8;
   __shared__ __attribute__((aligned(16))) _Float16 sp[2][COLS][SS];  // the state's parts
   __shared__ __attribute__((aligned(16))) _Float16 xp[2][COLS][XS];  // X's
-  __shared__ __attribute__((aligned(16))) _Float16 up[4][COLS][XS];  // U's parts; the decayed U's
+  __shared__ __attribute__((aligned(16))) _Float16 up[4][COLS][XS];  // U's; the decayed U's
+  __shared__ __attribute__((aligned(16))) float vp[2][COLS][PC + 4];  // values of a chunk and the next
   __shared__ float most[4][COLS];
-  // the 2 BLOCKS workgroups of a (request, key head) on one XCD, which the chunks' operands came from
+  // the 2 BLOCKS workgroups of a (request, key head) on one XCD, where the chunks' operands came from
   const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
   const int grp = (at / (2 * BLOCKS)) * 8 + xcd, in = at % (2 * BLOCKS);
   const int r = grp / PHK, hk = grp % PHK, hh = in / BLOCKS, hv = 2 * hk + hh, col0 = (in % BLOCKS) * COLS;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
   int t0, n;
   int64_t slot;
   bool old;
   request_of(d, r, t0, n, slot, old);
+  t0 = __builtin_amdgcn_readfirstlane(t0), n = __builtin_amdgcn_readfirstlane(n);
   if (n <= kShort || slot < 0) return;
   const int chunks = (n + PC - 1) / PC;
   const uint8_t* u = d.units + ((int64_t)first_unit(d, r, t0) * PHK + hk) * kUnit;  // a chunk's operands, then the next's
   constexpr int64_t kNext = (int64_t)PHK * kUnit;
-
-  // ---- the state: dims 32 wave + 16 i + 4 g + q of column 16 j + c
-  float* const hp = d.h0 + ((slot * PHV + hv) * PV + col0 + c) * PK + 32 * wave + 4 * g;
-  v4f S[2][NC];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < NC; ++j) S[i][j] = old ? *reinterpret_cast<const v4f*>(hp + 16 * j * PK + 16 * i) : v4f{0.f, 0.f, 0.f, 0.f};
-  // ---- values: tokens 16 wave + 4 g + q of a chunk
-  const int vch = 2 * PHK * PK + hv * PV + col0 + c;
-  float cw[NC][4];
-  uint32_t raw[NC][7];
-  float v[NC][4];
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    const v2i w = *reinterpret_cast<const v2i*>(d.conv_w + (int64_t)(vch + 16 * j) * 4);
-    cw[j][0] = bf_lo((uint32_t)w[0]), cw[j][1] = bf_hi((uint32_t)w[0]), cw[j][2] = bf_lo((uint32_t)w[1]), cw[j][3] = bf_hi((uint32_t)w[1]);
-  }
-  auto load_v = [&](int ch) {
-#pragma unroll
-    for (int i = 0; i < 7; ++i) {
-      const int t = ch * PC + 16 * wave + 4 * g + i - 3;
-#pragma unroll
-      for (int j = 0; j < NC; ++j) raw[j][i] = d.mixed[(int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + vch + 16 * j];
-    }
+  const int head = kUHead + hh * kHeadBytes, nks = w < 2 ? 1 : 2;
+  float before[NC], vmost[NC];
+  int fe[NC];  // the columns' exponents
+  auto columns = [&](int j) {
+    return fmaxf(fmaxf(most[0][16 * j + c], most[1][16 * j + c]), fmaxf(most[2][16 * j + c], most[3][16 * j + c]));
   };
-  auto conv_v = [&](int ch) {
+  auto next_factor = [&](float e) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float y = __builtin_fmaf(bf2f(raw[j][q + 3]), cw[j][3],
-                                       __builtin_fmaf(bf2f(raw[j][q + 2]), cw[j][2],
-                                                      __builtin_fmaf(bf2f(raw[j][q + 1]), cw[j][1], bf2f(raw[j][q]) * cw[j][0])));
-        v[j][q] = ch * PC + 16 * wave + 4 * g + q < n ? fast_silu(y) : 0.f;
-      }
-      float m = fmaxf(fmaxf(fabsf(v[j][0]), fabsf(v[j][1])), fmaxf(fabsf(v[j][2]), fabsf(v[j][3])));
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      if (g == 0) most[wave][16 * j + c] = m;
-    }
-  };
-  auto store_s = [&](const float* f) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        v4h hi, lo;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          _Float16 a, b;
-          split(S[i][j][q] * f[j], a, b);
-          hi[q] = a, lo[q] = b;
-        }
-        *reinterpret_cast<v4h*>(&sp[0][16 * j + c][32 * wave + 16 * i + 4 * g]) = hi;
-        *reinterpret_cast<v4h*>(&sp[1][16 * j + c][32 * wave + 16 * i + 4 * g]) = lo;
-      }
-  };
-  load_v(0);
-  if (wave == 0 && g == 0) {  // the inputs before the request's first
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) raw[j][i] = old ? d.conv_state[slot * d.cs_slot + (int64_t)(vch + 16 * j) * 3 + i] : 0;
-  }
-  // ---- operands of a chunk
-  v8h K[2][4], Kt[2][2][2], Q[2][4], T[2][2], P[2][2];
-  v4f eb, rest, bt;
-  float eend;
-  auto piece = [&](const uint8_t* p, int off) { return *reinterpret_cast<const v8h*>(p + off + 16 * lane); };
-  auto load_kq = [&](const uint8_t* p) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      K[0][s] = piece(p, kUK + (wave * 4 + s) * kPiece);
-      K[1][s] = piece(p, kUK + (16 + wave * 4 + s) * kPiece);
-      Q[0][s] = piece(p, kUQ + (wave * 4 + s) * kPiece);
-      Q[1][s] = piece(p, kUQ + (16 + wave * 4 + s) * kPiece);
-    }
-  };
-  auto load_t = [&](const uint8_t* p) {
-    const uint8_t* h = p + kUHead + hh * kHeadBytes;
-    const int last = wave < 2 ? 0 : 1;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      T[0][s] = piece(h, kHT + tri_piece(wave, min(s, last)) * kPiece);
-      T[1][s] = piece(h, kHT + (6 + tri_piece(wave, min(s, last))) * kPiece);
-    }
-  };
-  auto load_kt = [&](const uint8_t* p) {
-    const uint8_t* h = p + kUHead + hh * kHeadBytes;
-    const int last = wave < 2 ? 0 : 1;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        Kt[0][i][s] = piece(p, kUKt + ((2 * wave + i) * 2 + s) * kPiece);
-        Kt[1][i][s] = piece(p, kUKt + (16 + (2 * wave + i) * 2 + s) * kPiece);
-      }
-      P[0][s] = piece(h, kHP + tri_piece(wave, min(s, last)) * kPiece);
-      P[1][s] = piece(h, kHP + (6 + tri_piece(wave, min(s, last))) * kPiece);
-    }
-  };
-  auto load_gates = [&](const uint8_t* p) {
-    const float* gt = reinterpret_cast<const float*>(p + kUHead + hh * kHeadBytes + kHGate);
-    eb = *reinterpret_cast<const v4f*>(gt + 16 * wave + 4 * g);
-    rest = *reinterpret_cast<const v4f*>(gt + 64 + 16 * wave + 4 * g);
-    bt = *reinterpret_cast<const v4f*>(gt + 128 + 16 * wave + 4 * g);
-    eend = gt[192];
-  };
-  load_kq(u), load_t(u), load_kt(u), load_gates(u);
-  // ---- the columns' bounds: the state's norms, then the first chunk's values
-  float before[NC], vmost[NC], fac[NC];
-#pragma unroll
-  for (int j = 0; j < NC; ++j) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) ss = fmaxf(ss, fabsf(S[i][j][q]));
-    ss = fmaxf(ss, __shfl_xor(ss, 16));
-    ss = fmaxf(ss, __shfl_xor(ss, 32));
-    if (g == 0) most[wave][16 * j + c] = ss;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < NC; ++j)  // a norm is at most sqrt(128) times the largest value
-    before[j] = 11.32f * fmaxf(fmaxf(most[0][16 * j + c], most[1][16 * j + c]), fmaxf(most[2][16 * j + c], most[3][16 * j + c]));
-#pragma unroll
-  for (int j = 0; j < NC; ++j) vmost[j] = 0.f;
-  __syncthreads();
-  conv_v(0);
-  __syncthreads();
-  auto next_factor = [&](float e) {  // (behind a barrier since conv_v)
-#pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const float m = fmaxf(fmaxf(most[0][16 * j + c], most[1][16 * j + c]), fmaxf(most[2][16 * j + c], most[3][16 * j + c]));
+      const float m = columns(j);
       before[j] = __builtin_fmaf(64.f, vmost[j], before[j] * e);  // (what the chunk adds is not decayed by all of e)
       vmost[j] = m;
-      fac[j] = factor_of(__builtin_fmaf(65.f, m, before[j]) * 1.01f);
+      fe[j] = factor_of(__builtin_fmaf(65.f, m, before[j]) * 1.01f);
     }
   };
-  next_factor(1.f);
-  store_s(fac);
-  if (chunks > 1) load_v(1);
-  __syncthreads();
-  const int nks = wave < 2 ? 1 : 2;
-  uint16_t* const outp = d.out + (int64_t)(t0 + 16 * wave + 4 * g) * PZ + hv * PV + col0 + c;
-  int8_t* const expp = d.exps + (int64_t)(t0 + 16 * wave) * 256 + hv * 8 + col0 / 16;
+  auto load = [&](__amdgpu_buffer_rsrc_t b, int off) {
+    return __builtin_bit_cast(v8h, __builtin_amdgcn_raw_buffer_load_b128(b, 16 * lane, off, 0));
+  };
+  auto load_gate = [&](__amdgpu_buffer_rsrc_t b, int k) {  // of the wave's tokens
+    return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(b, 16 * g, head + kHGate + 256 * k + 64 * w, 0));
+  };
+  auto load_end = [&](__amdgpu_buffer_rsrc_t b) {  // e^{b_end}
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, 0, head + kHGate + 4 * (PC - 1), 0));
+  };
 
-  for (int ch = 0; ch < chunks; ++ch) {
-    const bool more = ch + 1 < chunks;
-    const uint8_t* const un = u + kNext;
-    v4f o[NC];
-    float inv[NC];
-    // ---- K S and Q S
+  if (wave < 4) {
+    // ---- dims 32 w + 16 i + 4 g + q of column 16 j + c
+    float* const hp = d.h0 + ((slot * PHV + hv) * PV + col0 + c) * PK + 32 * w + 4 * g;
+    v4f S[2][NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1, q1 = a1, q2 = a1;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const v8h bh = *reinterpret_cast<const v8h*>(&sp[0][16 * j + c][32 * s + 8 * g]);
-        const v8h bl = *reinterpret_cast<const v8h*>(&sp[1][16 * j + c][32 * s + 8 * g]);
-        a1 = mma(K[0][s], bh, a1);
-        a2 = mma(K[1][s], bh, a2);
-        q1 = mma(Q[0][s], bh, q1);
-        q2 = mma(Q[1][s], bh, q2);
-        a2 = mma(K[0][s], bl, a2);
-        q2 = mma(Q[0][s], bl, q2);
-      }
-      inv[j] = 0x1p-8f / fac[j];
-      v4h hi, lo;
+      for (int j = 0; j < NC; ++j) S[i][j] = old ? *reinterpret_cast<const v4f*>(hp + 16 * j * PK + 16 * i) : v4f{0.f, 0.f, 0.f, 0.f};
+    auto store_s = [&]() {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float ks = __builtin_fmaf(a2[q], kUnlow, a1[q]) * 0x1p-8f;
-        _Float16 a, b;
-        split(bt[q] * __builtin_fmaf(-eb[q], ks, v[j][q] * fac[j]), a, b);
-        hi[q] = a, lo[q] = b;
-        o[j][q] = eb[q] * __builtin_fmaf(q2[q], kUnlow, q1[q]);
-      }
-      *reinterpret_cast<v4h*>(&xp[0][16 * j + c][16 * wave + 4 * g]) = hi;
-      *reinterpret_cast<v4h*>(&xp[1][16 * j + c][16 * wave + 4 * g]) = lo;
-    }
-    const v4f fade = rest;
-    const float e = eend;
-    if (more) {
-      load_kq(un);
-      load_gates(un);
-      conv_v(ch + 1);
-      if (ch + 2 < chunks) load_v(ch + 2);
-    }
-    __syncthreads();
-    // ---- U = T X
+      for (int j = 0; j < NC; ++j) {
+        const float f = __builtin_ldexpf(1.f, fe[j]);
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+        for (int i = 0; i < 2; ++i) {
+          v4h hi, lo;
+          v4f x;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s < nks) {
-          const v8h bh = *reinterpret_cast<const v8h*>(&xp[0][16 * j + c][32 * s + 8 * g]);
-          const v8h bl = *reinterpret_cast<const v8h*>(&xp[1][16 * j + c][32 * s + 8 * g]);
-          a1 = mma(T[0][s], bh, a1);
-          a2 = mma(T[1][s], bh, a2);
-          a2 = mma(T[0][s], bl, a2);
+          for (int q = 0; q < 4; ++q) x[q] = S[i][j][q] * f;
+          split4(x, hi, lo);
+          *reinterpret_cast<v4h*>(&sp[0][16 * j + c][32 * w + 16 * i + 4 * g]) = hi;
+          *reinterpret_cast<v4h*>(&sp[1][16 * j + c][32 * w + 16 * i + 4 * g]) = lo;
         }
       }
-      v4h uh, ul, dh, dl;
+    };
+    v8h K[2][4], Kt[2][2][2], T[2][2];
+    v4f rest, bt, beb;
+    float e, e_next;  // e^{b_end}; asked for with the first loads of its chunk, so that no wait for it is a wait for later ones
+    auto load_k = [&](__amdgpu_buffer_rsrc_t b) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float x = __builtin_fmaf(a2[q], kUnlow, a1[q]) * 0x1p-8f;
-        _Float16 a, b;
-        split(x, a, b);
-        uh[q] = a, ul[q] = b;
-        split(x * fade[q], a, b);
-        dh[q] = a, dl[q] = b;
+      for (int s = 0; s < 4; ++s) K[0][s] = load(b, kUK + (w * 4 + s) * kPiece), K[1][s] = load(b, kUK + (16 + w * 4 + s) * kPiece);
+      bt = load_gate(b, 2), beb = load_gate(b, 3), e_next = load_end(b);
+    };
+    auto load_t = [&](__amdgpu_buffer_rsrc_t b) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int k = tri_piece(w, min(s, nks - 1)) * kPiece;
+        T[0][s] = load(b, head + kHT + k), T[1][s] = load(b, head + kHT + 6 * kPiece + k);
       }
-      *reinterpret_cast<v4h*>(&up[0][16 * j + c][16 * wave + 4 * g]) = uh;
-      *reinterpret_cast<v4h*>(&up[1][16 * j + c][16 * wave + 4 * g]) = ul;
-      *reinterpret_cast<v4h*>(&up[2][16 * j + c][16 * wave + 4 * g]) = dh;
-      *reinterpret_cast<v4h*>(&up[3][16 * j + c][16 * wave + 4 * g]) = dl;
-    }
-    if (more) {
-      load_t(un);
-      next_factor(e);
-    }
-    __syncthreads();
-    // ---- S' = e^{b_end} S + K^T U, and its parts for the next chunk
+      rest = load_gate(b, 1);
+    };
+    auto load_kt = [&](__amdgpu_buffer_rsrc_t b) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int k = kUKt + ((2 * w + i) * 2 + s) * kPiece;
+          Kt[0][i][s] = load(b, k), Kt[1][i][s] = load(b, k + 16 * kPiece);
+        }
+    };
+    __amdgpu_buffer_rsrc_t ub = buffer(u, kUnit);
+    load_k(ub), load_t(ub), load_kt(ub);
+    e = e_next;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
+      float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(S[i][j][q]));
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      if (g == 0) most[w][16 * j + c] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NC; ++j) before[j] = 11.32f * columns(j), vmost[j] = 0.f;  // a norm: at most sqrt(128) times the largest
+    __syncthreads();
+    __syncthreads();
+    next_factor(1.f);
+    store_s();
+    __syncthreads();
+    for (int ch = 0; ch < chunks; ++ch) {
+      const uint8_t* const un = ch + 1 < chunks ? u + kNext : u;  // (the last chunk's operands twice)
+      const __amdgpu_buffer_rsrc_t nb = buffer(un, kUnit);
+      // ---- X = beta (V - e^b K S)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const v4f v = *reinterpret_cast<const v4f*>(&vp[ch & 1][16 * j + c][16 * w + 4 * g]);
+        const float f = __builtin_ldexpf(1.f, fe[j]);
         v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const v8h bh = *reinterpret_cast<const v8h*>(&sp[0][16 * j + c][32 * s + 8 * g]);
+          const v8h bl = *reinterpret_cast<const v8h*>(&sp[1][16 * j + c][32 * s + 8 * g]);
+          a1 = mma(K[0][s], bh, a1);
+          a2 = mma(K[1][s], bh, a2);
+          (s & 1 ? a1 : a2) = mma(K[0][s], bl, s & 1 ? a1 : a2);
+        }
+        v4h hi, lo;
+        v4f x;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(-beb[q], a1[q] + a2[q], bt[q] * f * v[q]);
+        split4(x, hi, lo);
+        *reinterpret_cast<v4h*>(&xp[0][16 * j + c][16 * w + 4 * g]) = hi;
+        *reinterpret_cast<v4h*>(&xp[1][16 * j + c][16 * w + 4 * g]) = lo;
+      }
+      load_k(nb);
+      __syncthreads();
+      // ---- U = T X
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s < nks) {
+            const v8h bh = *reinterpret_cast<const v8h*>(&xp[0][16 * j + c][32 * s + 8 * g]);
+            const v8h bl = *reinterpret_cast<const v8h*>(&xp[1][16 * j + c][32 * s + 8 * g]);
+            a1 = mma(T[0][s], bh, a1);
+            a2 = mma(T[1][s], bh, a2);
+            a2 = mma(T[0][s], bl, a2);
+          }
+        }
+        v4h uh, ul, dh, dl;
+        v4f x, y;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] = a1[q] + a2[q], y[q] = x[q] * rest[q], x[q] *= 0x1p-8f;
+        split4(y, dh, dl);
+        split4(x, uh, ul);
+        *reinterpret_cast<v4h*>(&up[2][16 * j + c][16 * w + 4 * g]) = dh;
+        *reinterpret_cast<v4h*>(&up[3][16 * j + c][16 * w + 4 * g]) = dl;
+        *reinterpret_cast<v4h*>(&up[0][16 * j + c][16 * w + 4 * g]) = uh;
+        *reinterpret_cast<v4h*>(&up[1][16 * j + c][16 * w + 4 * g]) = ul;
+      }
+      load_t(nb);
+      __syncthreads();
+      // ---- S' = e^{b_end} S + K^T U, and its parts for the next chunk
+      v4f a[2][NC][2];
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const v8h bh = *reinterpret_cast<const v8h*>(&up[2][16 * j + c][32 * s + 8 * g]);
           const v8h bl = *reinterpret_cast<const v8h*>(&up[3][16 * j + c][32 * s + 8 * g]);
-          a1 = mma(Kt[0][i][s], bh, a1);
-          a2 = mma(Kt[1][i][s], bh, a2);
-          a2 = mma(Kt[0][i][s], bl, a2);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (s == 0) a[i][j][0] = a[i][j][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            a[i][j][0] = mma(Kt[0][i][s], bh, a[i][j][0]);
+            a[i][j][1] = mma(Kt[1][i][s], bh, a[i][j][1]);
+            a[i][j][s] = mma(Kt[0][i][s], bl, a[i][j][s]);
+          }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          S[i][j][q] = __builtin_fmaf(__builtin_fmaf(a2[q], kUnlow, a1[q]), inv[j], e * S[i][j][q]);
+      for (int j = 0; j < NC; ++j) {
+        const float inv = __builtin_ldexpf(0x1p-8f, -fe[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) S[i][j][q] = __builtin_fmaf(a[i][j][0][q] + a[i][j][1][q], inv, e * S[i][j][q]);
       }
+      load_kt(nb);
+      next_factor(e);  // (behind the last chunk: of values that nothing reads)
+      store_s();
+      u = un, e = e_next;
+      __syncthreads();
     }
-    if (more) store_s(fac);
-    // ---- O = e^b Q S + P U
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) *reinterpret_cast<v4f*>(hp + 16 * j * PK + 16 * i) = S[i][j];
+  } else {
+    // ---- values: tokens 16 w + 4 g + q of a chunk, of the channel of column 16 j + c
+    const int vch = 2 * PHK * PK + hv * PV + col0 + c;
+    float cw[NC][4];
+    uint32_t raw[NC][7];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+      const v2i k = *reinterpret_cast<const v2i*>(d.conv_w + (int64_t)(vch + 16 * j) * 4);
+      cw[j][0] = bf_lo((uint32_t)k[0]), cw[j][1] = bf_hi((uint32_t)k[0]), cw[j][2] = bf_lo((uint32_t)k[1]), cw[j][3] = bf_hi((uint32_t)k[1]);
+#pragma unroll
+      for (int i = 0; i < 7; ++i) {
+        const int t = 16 * w + 4 * g + i - 3;
+        raw[j][i] = d.mixed[(int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + vch + 16 * j];
+        if (t < 0) raw[j][i] = old ? d.conv_state[slot * d.cs_slot + (int64_t)(vch + 16 * j) * 3 + i] : 0;
+      }
+    }
+    const int vat = ((16 * w + 4 * g) * PQKV + vch) * 2;
+    auto load_v = [&](int ch) {  // a later chunk's: its rows and the three before them
+      const int row = t0 + ch * PC - 3;
+      const __amdgpu_buffer_rsrc_t b = buffer(d.mixed + (int64_t)row * PQKV,
+                                              __builtin_amdgcn_readfirstlane(max(min(d.rows - row, PC + 3), 0)) * PQKV * 2);
+#pragma unroll
+      for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int i = 0; i < 7; ++i) raw[j][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, vat + i * PQKV * 2 + 32 * j, 0, 0);
+    };
+    auto conv_v = [&](int ch) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        v4f v;
+        float m = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float y = bf2f(raw[j][q]) * cw[j][0];
+          y = __builtin_fmaf(bf2f(raw[j][q + 1]), cw[j][1], y);
+          y = __builtin_fmaf(bf2f(raw[j][q + 2]), cw[j][2], y);
+          y = fast_silu(__builtin_fmaf(bf2f(raw[j][q + 3]), cw[j][3], y));
+          v[q] = ch * PC + 16 * w + 4 * g + q < n ? y : 0.f;
+          m = fmaxf(m, fabsf(v[q]));
+        }
+        *reinterpret_cast<v4f*>(&vp[ch & 1][16 * j + c][16 * w + 4 * g]) = v;
+        const auto p16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        m = fmaxf(__uint_as_float(p16[0]), __uint_as_float(p16[1]));
+        const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        m = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
+        if (g == 0) most[w][16 * j + c] = m;
+      }
+    };
+    v8h Q[2][4], P[2][2];
+    v4f eb;
+    float e, e_next;
+    auto load_q = [&](__amdgpu_buffer_rsrc_t b) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) Q[0][s] = load(b, kUQ + (w * 4 + s) * kPiece), Q[1][s] = load(b, kUQ + (16 + w * 4 + s) * kPiece);
+      eb = load_gate(b, 0), e_next = load_end(b);
+    };
+    auto load_p = [&](__amdgpu_buffer_rsrc_t b) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if (s < nks) {
-          const v8h bh = *reinterpret_cast<const v8h*>(&up[0][16 * j + c][32 * s + 8 * g]);
-          const v8h bl = *reinterpret_cast<const v8h*>(&up[1][16 * j + c][32 * s + 8 * g]);
-          a1 = mma(P[0][s], bh, a1);
-          a2 = mma(P[1][s], bh, a2);
-          a2 = mma(P[0][s], bl, a2);
-        }
+        const int k = tri_piece(w, min(s, nks - 1)) * kPiece;
+        P[0][s] = load(b, head + kHP + k), P[1][s] = load(b, head + kHP + 6 * kPiece + k);
       }
-      float y[4], m = 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        y[q] = (o[j][q] + __builtin_fmaf(a2[q], kUnlow, a1[q])) * (inv[j] * d.scale);
-        m = fmaxf(m, fabsf(y[q]));
-      }
-      // the tile's outputs as fp16 times a power of two, in out's place until the norm
-      m = __uint_as_float(wave_max_u32(__float_as_uint(m)));
-      int ex = 0;
-      (void)__builtin_frexpf(m, &ex);
-      ex = min(max(ex, -110), 127);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int t = ch * PC + 16 * wave + 4 * g + q;
-        if (t < n) {
-          outp[((int64_t)ch * PC + q) * PZ + 16 * j] = __builtin_bit_cast(uint16_t, (_Float16)__builtin_ldexpf(y[q], 14 - ex));
-        }
-      }
-      if (g == 0 && ch * PC + 16 * wave + c < n) expp[((int64_t)ch * PC + c) * 256 + j] = (int8_t)ex;
-    }
-    if (more) load_kt(un);
-    u = un;
+    };
+    __amdgpu_buffer_rsrc_t ub = buffer(u, kUnit);
+    load_q(ub), load_p(ub);
+    e = e_next;
     __syncthreads();
-  }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < NC; ++j) before[j] = 11.32f * columns(j), vmost[j] = 0.f;
+    __syncthreads();
+    conv_v(0);
+    load_v(1);
+    __syncthreads();
+    next_factor(1.f);
+    __syncthreads();
+    // where a lane's outputs go, from the chunk's first row: rows of the wave's tile; four rows' exponent by four lanes
+    const int oat = (16 * w + 4 * g) * PZ * 2 + (hv * PV + col0 + c) * 2;
+    const int eat = c < 4 ? (16 * w + 4 * g + c) * 256 + hv * 8 + col0 / 16 : 0x7fffff00;
+    for (int ch = 0; ch < chunks; ++ch) {
+      const uint8_t* const un = ch + 1 < chunks ? u + kNext : u;
+      const __amdgpu_buffer_rsrc_t nb = buffer(un, kUnit);
+      // ---- e^b Q S
+      v4f o[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) *reinterpret_cast<v4f*>(hp + 16 * j * PK + 16 * i) = S[i][j];
-  // ---- the conv state: the request's last three inputs (longer than three).  This workgroup's value channels; q and k by the
-  // first workgroup of the key head, behind the kernel that read them
-  for (int i = tid; i < COLS * 3; i += 256) {
-    const int cc = 2 * PHK * PK + hv * PV + col0 + i / 3;
-    d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
-  }
-  if (in == 0)
-    for (int i = tid; i < 2 * PK * 3; i += 256) {
-      const int cc = (i / (3 * PK)) * (PHK * PK) + hk * PK + i / 3 % PK;
+      for (int j = 0; j < NC; ++j) {
+        v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const v8h bh = *reinterpret_cast<const v8h*>(&sp[0][16 * j + c][32 * s + 8 * g]);
+          const v8h bl = *reinterpret_cast<const v8h*>(&sp[1][16 * j + c][32 * s + 8 * g]);
+          a1 = mma(Q[0][s], bh, a1);
+          a2 = mma(Q[1][s], bh, a2);
+          (s & 1 ? a1 : a2) = mma(Q[0][s], bl, s & 1 ? a1 : a2);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[j][q] = eb[q] * (a1[q] + a2[q]);
+      }
+      load_q(nb);
+      __syncthreads();
+      conv_v(ch + 1);
+      load_v(ch + 2);
+      __syncthreads();
+      // ---- + P U: as fp16 times a power of two for four rows, in out's place until the norm
+      const int rows = min(n - ch * PC, PC);
+      const __amdgpu_buffer_rsrc_t ob = buffer(d.out + (int64_t)(t0 + ch * PC) * PZ, rows * PZ * 2);
+      const __amdgpu_buffer_rsrc_t xb = buffer(d.exps + (int64_t)(t0 + ch * PC) * 256, rows * 256);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        v4f a1 = o[j], a2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (s < nks) {
+            const v8h bh = *reinterpret_cast<const v8h*>(&up[0][16 * j + c][32 * s + 8 * g]);
+            const v8h bl = *reinterpret_cast<const v8h*>(&up[1][16 * j + c][32 * s + 8 * g]);
+            a1 = mma(P[0][s], bh, a1);
+            a2 = mma(P[1][s], bh, a2);
+            a2 = mma(P[0][s], bl, a2);
+          }
+        }
+        const float f = __builtin_ldexpf(0x1p-8f, -fe[j]) * d.scale;
+        float y[4], m = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          y[q] = (a1[q] + a2[q]) * f;
+          m = fmaxf(m, fabsf(y[q]));
+        }
+        int ex = 0;
+        (void)__builtin_frexpf(__uint_as_float(row16_max_u32(__float_as_uint(m))), &ex);
+        ex = min(max(ex, -110), 127);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (_Float16)__builtin_ldexpf(y[q], 14 - ex)), ob,
+                                                oat + q * PZ * 2 + 32 * j, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)ex, xb, eat + j, 0, 0);
+      }
+      load_p(nb);
+      next_factor(e);
+      u = un, e = e_next;
+      __syncthreads();
+    }
+    // ---- the conv state: the request's last three inputs (it has more).  This workgroup's value channels; q and k by the first
+    // workgroup of the key head, behind the kernel that read them
+    const int ot = tid - 256;
+    for (int i = ot; i < COLS * 3; i += 256) {
+      const int cc = 2 * PHK * PK + hv * PV + col0 + i / 3;
       d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
     }
+    if (in == 0)
+      for (int i = ot; i < 2 * PK * 3; i += 256) {
+        const int cc = (i / (3 * PK)) * (PHK * PK) + hk * PK + i / 3 % PK;
+        d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
+      }
+  }
 }
 
 // The gated norm of the chunks' rows: a wave a row, 16 lanes a head.
@@ -970,8 +1021,9 @@ extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream)
   const hipStream_t st = static_cast<hipStream_t>(stream);
   prompt_steps_kernel<<<(unsigned)a->B * PHK, 512, 0, st>>>(d);
   if (units) {
-    prompt_chunks_kernel<<<(unsigned)units * PHK, 256, 0, st>>>(d);
-    prompt_scan_kernel<1><<<(unsigned)a->B * PHK * 16, 256, 0, st>>>(d);
+    prompt_chunks_kernel<<<(unsigned)units * PHK, 512, 0, st>>>(d);
+    if (a->B >= 8) prompt_scan_kernel<4><<<(unsigned)a->B * PHK * 4, 512, 0, st>>>(d);
+    else prompt_scan_kernel<1><<<(unsigned)a->B * PHK * 16, 512, 0, st>>>(d);
     prompt_norm_kernel<<<(unsigned)(a->rows + 3) / 4, 256, 0, st>>>(d);
   }
   return check_launch("q36_gdn_prompt");
