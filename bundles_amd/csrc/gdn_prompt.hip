@@ -18,9 +18,11 @@ constexpr int kGroup = 8;  // tokens whose conv, norms and gates are formed at o
 constexpr int kShort = 8;  // requests of up to so many new tokens go token by token, longer ones by chunks
 constexpr int PC = 64;     // tokens of a chunk
 
-// A chunk's operands for one key head, as the scan's lanes load them: pieces of 1 KB, lane l's 16 bytes at 16 l, element (row
-// r, depth k) of a 16 x 32 operand piece in lane r + 16 (k / 8).  fp16 times 2^8, in a plane of high and one of low parts.
-// (The factor keeps small entries exact: T's are of the size of beta, and what they multiply can be large.)
+// A chunk's operands for one key head, as the scan's lanes load them: pieces of 1 KB, 16 rows by a depth of 32, lane l's 16
+// bytes at 16 l: row l % 16, depths 4 g .. + 3 and 16 + 4 g .. + 3 (g = l / 16), in which order two results' registers are
+// the other operand of the next product.  fp16 in a plane of high and one of low parts, times 2^8 but for K^T.  (The factor
+// keeps small entries exact: T's are of the size of beta, and what they multiply can be large.  K^T goes without, so that its
+// products add up to the state in the state's own scale.)
 constexpr int kPiece = 1024;
 constexpr int kUK = 0;                        // K: [plane][token tile 4][depth 4] (depth: key dims by 32)
 constexpr int kUKt = kUK + 32 * kPiece;       // K^T: [plane][dim tile 8][depth 2] (depth: tokens by 32)
@@ -58,6 +60,7 @@ struct PromptDev {
   uint8_t* units;
   int8_t* exps;
   int by_row;
+  int both;  // more than one scan kernel is launched: which one works is told by the requests' lengths
 };
 
 // Request r's rows, inside the batch whatever qsl holds, and its slot (-1: none).
@@ -104,8 +107,12 @@ __device__ __forceinline__ void split4(v4f x, v4h& hi, v4h& lo) {
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
     const v2h h = __builtin_convertvector((q36_v2f){x[i], x[i + 1]}, v2h);
-    const v2h l = __builtin_convertvector(
-        (q36_v2f){__builtin_fmaf((float)h[0], -1.f, x[i]), __builtin_fmaf((float)h[1], -1.f, x[i + 1])}, v2h);
+    // x - hi, exact: one instruction on the packed halves where the compiler takes two.  (Where x is a matrix instruction's
+    // result, the conversion that made h has waited for it.)
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(x[i]));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(x[i + 1]));
+    const v2h l = __builtin_convertvector((q36_v2f){r0, r1}, v2h);
     hi[i] = h[0], hi[i + 1] = h[1], lo[i] = l[0], lo[i + 1] = l[1];
   }
 }
@@ -234,7 +241,7 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
       const float rstd = 1.f / sqrtf(wave_sum_bfly(o0 * o0 + o1 * o1) / (float)PV + d.eps);
       const float y0 = o0 * rstd * bf2f(d.norm_w[lane]) * silu(bf2f(d.z[o + lane]));
       const float y1 = o1 * rstd * bf2f(d.norm_w[lane + 64]) * silu(bf2f(d.z[o + lane + 64]));
-      const uint32_t y = pack_bf2(y0, y1);
+      const uint32_t y = pack_bf2_hw(y0, y1);
       d.out[o + lane] = (uint16_t)y;
       d.out[o + lane + 64] = (uint16_t)(y >> 16);
       if (d.oq) {
@@ -262,7 +269,8 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
 //   A_ij = beta_i e^{b_i - b_j} k_i . k_j (j < i), T = (I + A)^-1
 //   U = T (beta (V - e^b K S)),  O = e^b Q S + (e^{b_i - b_j} q_i . k_j, j <= i) U,  S' = e^{b_end} S + K^T (e^{b_end - b} U)
 // A first kernel forms what does not depend on S, for all chunks at once; a second walks a request's chunks with S in
-// registers, a workgroup for every 16 or 32 value columns of a head; a third applies the gated norm to whole heads.
+// registers, by whole heads, whose gated norm is in it, or, where requests are few, by 16 value columns of a head, and another
+// applies the norm.
 //
 // Products are of fp16 operands in two parts (x = hi + lo / 2^11, three products: 22 bits), in fp32 sums, so the state keeps
 // fp32's accuracy at a third of the fp16 rate, where the fp32 matrix instruction has a sixteenth.  The output, though bf16,
@@ -375,6 +383,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
   // ---- K K^T (waves 0-3) and Q K^T (4-7) on and below the diagonal: rows 16 (w & 3) .. + 15.  The operands' pieces go to the
   // workspace as read; then K^T's, gathered eight tokens a lane
   const int w = wave & 3, what = wave < 4 ? 1 : 0;
+  auto depth = [&](const _Float16* row, int s) {  // a piece's share of a row
+    const v4h x = *reinterpret_cast<const v4h*>(row + 32 * s + 4 * g), y = *reinterpret_cast<const v4h*>(row + 32 * s + 16 + 4 * g);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
   v4f qk[4];
   {
     v8h a[2][4];
@@ -382,7 +394,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        a[p][s] = *reinterpret_cast<const v8h*>(&planes[what][p][16 * w + c][32 * s + 8 * g]);
+        a[p][s] = depth(planes[what][p][16 * w + c], s);
         *reinterpret_cast<v8h*>(u + (what ? kUK : kUQ) + (p * 16 + w * 4 + s) * kPiece + 16 * lane) = a[p][s];
       }
 #pragma unroll
@@ -392,8 +404,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
         v4f q2 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const v8h bh = *reinterpret_cast<const v8h*>(&planes[1][0][16 * j + c][32 * s + 8 * g]);
-          const v8h bl = *reinterpret_cast<const v8h*>(&planes[1][1][16 * j + c][32 * s + 8 * g]);
+          const v8h bh = depth(planes[1][0][16 * j + c], s), bl = depth(planes[1][1][16 * j + c], s);
           qk[j] = mma(a[0][s], bh, qk[j]);
           q2 = mma(a[1][s], bh, q2);
           q2 = mma(a[0][s], bl, q2);
@@ -407,8 +418,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
       const int k = wave * 4 + i, p = k >> 4, tile = (k >> 1) & 7, s = k & 1;
       v8h x;
 #pragma unroll
-      for (int t = 0; t < 8; ++t) x[t] = planes[1][p][32 * s + 8 * g + t][16 * tile + c];
-      *reinterpret_cast<v8h*>(u + kUKt + k * kPiece + 16 * lane) = x;
+      for (int t = 0; t < 8; ++t) x[t] = planes[1][p][32 * s + (t >> 2) * 16 + 4 * g + (t & 3)][16 * tile + c];
+      *reinterpret_cast<v8h*>(u + kUKt + k * kPiece + 16 * lane) = x * (_Float16)0x1p-8f;
     }
   }
   __syncthreads();
@@ -448,7 +459,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         v4h a, b;
-        v4f x = *reinterpret_cast<const v4f*>(&m[h][16 * pw + c][32 * s + 8 * g + 4 * j]);
+        v4f x = *reinterpret_cast<const v4f*>(&m[h][16 * pw + c][32 * s + 16 * j + 4 * g]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[q] *= f;
         split4(x, a, b);
@@ -529,11 +540,38 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
   pieces(am, wave, 8, kHT, 256.f);
 }
 
-// The exponent of the largest power of two that keeps bound times it within 2^15.
-__device__ __forceinline__ int factor_of(float bound) {
-  int e = 0;
-  (void)__builtin_frexpf(bound, &e);  // bound < 2^e
-  return bound > 0.f ? min(max(15 - e, -100), 100) : 0;
+// The gated norm of one row of a head, 8 of its values a lane of 16: out, and its e4m3 codes where asked for.
+__device__ __forceinline__ void norm_store(const PromptDev& d, int64_t row, int hv, int c, const float (&x)[8], v4i z, v4i wn) {
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) ss = __builtin_fmaf(x[k], x[k], ss);
+  const float rstd = 1.f / sqrtf(row16_sum(ss) * (1.f / PV) + d.eps);
+  float y[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float zz = (k & 1) ? bf_hi((uint32_t)z[k >> 1]) : bf_lo((uint32_t)z[k >> 1]);
+    const float ww = (k & 1) ? bf_hi((uint32_t)wn[k >> 1]) : bf_lo((uint32_t)wn[k >> 1]);
+    y[k] = x[k] * rstd * ww * fast_silu(zz);
+  }
+  v4i w;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = (int)pack_bf2_hw(y[2 * k], y[2 * k + 1]);
+  const int64_t at = row * PZ + hv * PV + 8 * c;
+  *reinterpret_cast<v4i*>(d.out + at) = w;
+  if (d.oq) {
+    float f[8], m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      f[k] = (k & 1) ? bf_hi((uint32_t)w[k >> 1]) : bf_lo((uint32_t)w[k >> 1]);
+      m = fmaxf(m, fabsf(f[k]));
+    }
+    m = fmaxf(m, lane_xor<1>(m));
+    m = fmaxf(m, lane_xor<2>(m));
+    m = fmaxf(m, lane_xor<4>(m));
+    m = fmaxf(m, lane_xor<8>(m));
+    *reinterpret_cast<uint2*>(d.oq + at) = e4m3_run8(f, m > 0.f ? 448.f / m : 0.f);
+    if (c == 0) d.oqs[row * PHV + hv] = m / 448.f;
+  }
 }
 
 // A buffer of `bytes` at p (the same in every lane): loads behind its end give 0, stores there are dropped.  (What may lie
@@ -542,25 +580,48 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int byte
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
 }
 
-// A request's chunks for 16 NC value columns of a head.  Waves 0-3 carry the state: wave w holds key dims 32 w .. + 31 of it
+// Whether the batch's longest request has at most a quarter of its chunks: whole heads then fill the chip.  One request's
+// chunks follow each other, 2.0 us each where a workgroup has 16 columns of a head and 4.9 where it has all, which then costs
+// 2.1 times less in all: 16 prompts of 1000 tokens 588 us by columns and 344 by heads, one of 8192 424 and 800.
+__device__ __forceinline__ bool many_chunks(const PromptDev& d) {
+  if (!d.both) return false;
+  int sum = 0, most = 0;
+  for (int i = threadIdx.x & 63; i < d.B; i += 64) {
+    const int n = min(max(d.qsl[i + 1], 0), d.rows) - min(max(d.qsl[i], 0), d.rows);
+    const int ch = n > kShort ? (n + PC - 1) / PC : 0;
+    sum += ch, most = max(most, ch);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o), most = max(most, __shfl_xor(most, o));
+  return __builtin_amdgcn_readfirstlane(sum) >= 4 * __builtin_amdgcn_readfirstlane(most);
+}
+
+// The power of two, 2^exponent, that brings a column into fp16's range: |S|, |X|, |U| <= bound, which holds whatever the values,
+// since |s_j| <= |s_{j-1}| + |v_j| (the step shrinks s): |S before the chunk| + 65 max |v|.  It stays while the bound is
+// between 2^13 and 2^15 of it.  (All lanes the same.)
+__device__ __forceinline__ int next_exponent(int fe, float bound) {
+  int e = 0;
+  (void)__builtin_frexpf(bound * 1.01f, &e);  // bound < 2^e
+  const int top = min(max(15 - __builtin_amdgcn_readfirstlane(e), -100), 100);
+  return __builtin_amdgcn_readfirstlane(!(bound > 0.f) || (fe <= top && fe >= top - 1) ? fe : top);
+}
+__device__ __forceinline__ float all_max(float m) { return __uint_as_float(wave_max_u32(__float_as_uint(m))); }
+
+// A request's chunks for 16 value columns of a head.  Waves 0-3 carry the state: wave w holds key dims 32 w .. + 31 of it
 // and token tile w of X and U.  Waves 4-7, one beside each of them on its SIMD, convolve the next chunk's values and form the
 // outputs of token tile w - 4, from the same parts in LDS; so the chain from state to state has only its own work in it.
-//
-// State, X and U pass through LDS as fp16 parts.  They are brought into fp16's range by a power of two for each column, from a
-// bound on the column's norm that holds whatever the values: |s_j| <= |s_{j-1}| + |v_j| (the step shrinks s), so |S|, |X|, |U| <=
-// |S before the chunk| + 65 max |v|.
-template <int NC>
+// State, X and U pass through LDS as fp16 parts, in the order of an operand's depth.
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_scan_kernel(PromptDev d) {
-  constexpr int COLS = 16 * NC, BLOCKS = PV / COLS, SS = PK + 8, XS = PC + 8;
-  __shared__ __attribute__((aligned(16))) _Float16 sp[2][COLS][SS];  // the state's parts
-  __shared__ __attribute__((aligned(16))) _Float16 xp[2][COLS][XS];  // X's
-  __shared__ __attribute__((aligned(16))) _Float16 up[4][COLS][XS];  // U's; the decayed U's
-  __shared__ __attribute__((aligned(16))) float vp[2][COLS][PC + 4];  // values of a chunk and the next
-  __shared__ float most[4][COLS];
+  constexpr int BLOCKS = PV / 16, SS = PK + 8, XS = PC + 8;
+  __shared__ __attribute__((aligned(16))) _Float16 sp[2][16][SS];   // the state's parts
+  __shared__ __attribute__((aligned(16))) _Float16 xp[2][16][XS];   // X's
+  __shared__ __attribute__((aligned(16))) _Float16 up[4][16][XS];   // U's; the decayed U's
+  __shared__ __attribute__((aligned(16))) float vp[2][16][PC + 4];  // values of a chunk and the next
+  __shared__ float most[4];
   // the 2 BLOCKS workgroups of a (request, key head) on one XCD, where the chunks' operands came from
   const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
   const int grp = (at / (2 * BLOCKS)) * 8 + xcd, in = at % (2 * BLOCKS);
-  const int r = grp / PHK, hk = grp % PHK, hh = in / BLOCKS, hv = 2 * hk + hh, col0 = (in % BLOCKS) * COLS;
+  const int r = grp / PHK, hk = grp % PHK, hh = in / BLOCKS, hv = 2 * hk + hh, col0 = (in % BLOCKS) * 16;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
   int t0, n;
@@ -568,24 +629,19 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   bool old;
   request_of(d, r, t0, n, slot, old);
   t0 = __builtin_amdgcn_readfirstlane(t0), n = __builtin_amdgcn_readfirstlane(n);
-  if (n <= kShort || slot < 0) return;
+  if (n <= kShort || slot < 0 || many_chunks(d)) return;
   const int chunks = (n + PC - 1) / PC;
   const uint8_t* u = d.units + ((int64_t)first_unit(d, r, t0) * PHK + hk) * kUnit;  // a chunk's operands, then the next's
   constexpr int64_t kNext = (int64_t)PHK * kUnit;
   const int head = kUHead + hh * kHeadBytes, nks = w < 2 ? 1 : 2;
-  float before[NC], vmost[NC];
-  int fe[NC];  // the columns' exponents
-  auto columns = [&](int j) {
-    return fmaxf(fmaxf(most[0][16 * j + c], most[1][16 * j + c]), fmaxf(most[2][16 * j + c], most[3][16 * j + c]));
-  };
+  const int mine = 32 * (w >> 1) + 8 * g + 4 * (w & 1);  // of tokens 16 w + 4 g .. in a depth's order
+  float before, vmost = 0.f;
+  int fe = 0;  // the columns' exponent
+  auto columns = [&]() { return fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])); };
   auto next_factor = [&](float e) {
-#pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const float m = columns(j);
-      before[j] = __builtin_fmaf(64.f, vmost[j], before[j] * e);  // (what the chunk adds is not decayed by all of e)
-      vmost[j] = m;
-      fe[j] = factor_of(__builtin_fmaf(65.f, m, before[j]) * 1.01f);
-    }
+    before = __builtin_fmaf(64.f, vmost, before * e);  // (what the chunk adds is not decayed by all of e)
+    vmost = columns();
+    return next_exponent(fe, __builtin_fmaf(65.f, vmost, before));
   };
   auto load = [&](__amdgpu_buffer_rsrc_t b, int off) {
     return __builtin_bit_cast(v8h, __builtin_amdgcn_raw_buffer_load_b128(b, 16 * lane, off, 0));
@@ -596,30 +652,28 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   auto load_end = [&](__amdgpu_buffer_rsrc_t b) {  // e^{b_end}
     return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, 0, head + kHGate + 4 * (PC - 1), 0));
   };
+  auto part = [&](const _Float16* row, int s) { return *reinterpret_cast<const v8h*>(row + 32 * s + 8 * g); };
 
   if (wave < 4) {
-    // ---- dims 32 w + 16 i + 4 g + q of column 16 j + c
+    // ---- dims 32 w + 16 i + 4 g + q of column c, times 2^fe
     float* const hp = d.h0 + ((slot * PHV + hv) * PV + col0 + c) * PK + 32 * w + 4 * g;
-    v4f S[2][NC];
+    v4f S[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) S[i] = old ? *reinterpret_cast<const v4f*>(hp + 16 * i) : v4f{0.f, 0.f, 0.f, 0.f};
+    auto store_s = [&](int to) {
+      if (to != fe) {
+        const float f = __builtin_ldexpf(1.f, to - fe);
 #pragma unroll
-      for (int j = 0; j < NC; ++j) S[i][j] = old ? *reinterpret_cast<const v4f*>(hp + 16 * j * PK + 16 * i) : v4f{0.f, 0.f, 0.f, 0.f};
-    auto store_s = [&]() {
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const float f = __builtin_ldexpf(1.f, fe[j]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v4h hi, lo;
-          v4f x;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) x[q] = S[i][j][q] * f;
-          split4(x, hi, lo);
-          *reinterpret_cast<v4h*>(&sp[0][16 * j + c][32 * w + 16 * i + 4 * g]) = hi;
-          *reinterpret_cast<v4h*>(&sp[1][16 * j + c][32 * w + 16 * i + 4 * g]) = lo;
-        }
+          for (int q = 0; q < 4; ++q) S[i][q] *= f;
+        fe = to;
       }
+      v4h h[2], l[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) split4(S[i], h[i], l[i]);
+      *reinterpret_cast<v8h*>(&sp[0][c][32 * w + 8 * g]) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      *reinterpret_cast<v8h*>(&sp[1][c][32 * w + 8 * g]) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
     };
     v8h K[2][4], Kt[2][2][2], T[2][2];
     v4f rest, bt, beb;
@@ -649,38 +703,32 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
     __amdgpu_buffer_rsrc_t ub = buffer(u, kUnit);
     load_k(ub), load_t(ub), load_kt(ub);
     e = e_next;
-#pragma unroll
-    for (int j = 0; j < NC; ++j) {
+    {
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(S[i][j][q]));
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      if (g == 0) most[w][16 * j + c] = m;
+        for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(S[i][q]));
+      m = all_max(m);
+      if (lane == 0) most[w] = m;
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NC; ++j) before[j] = 11.32f * columns(j), vmost[j] = 0.f;  // a norm: at most sqrt(128) times the largest
+    before = 11.32f * columns();  // a norm: at most sqrt(128) times the largest
     __syncthreads();
     __syncthreads();
-    next_factor(1.f);
-    store_s();
+    store_s(next_factor(1.f));
     __syncthreads();
     for (int ch = 0; ch < chunks; ++ch) {
       const uint8_t* const un = ch + 1 < chunks ? u + kNext : u;  // (the last chunk's operands twice)
       const __amdgpu_buffer_rsrc_t nb = buffer(un, kUnit);
       // ---- X = beta (V - e^b K S)
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const v4f v = *reinterpret_cast<const v4f*>(&vp[ch & 1][16 * j + c][16 * w + 4 * g]);
-        const float f = __builtin_ldexpf(1.f, fe[j]);
+      {
+        const v4f v = *reinterpret_cast<const v4f*>(&vp[ch & 1][c][16 * w + 4 * g]);
+        const float f = __builtin_ldexpf(1.f, fe);
         v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const v8h bh = *reinterpret_cast<const v8h*>(&sp[0][16 * j + c][32 * s + 8 * g]);
-          const v8h bl = *reinterpret_cast<const v8h*>(&sp[1][16 * j + c][32 * s + 8 * g]);
+          const v8h bh = part(sp[0][c], s), bl = part(sp[1][c], s);
           a1 = mma(K[0][s], bh, a1);
           a2 = mma(K[1][s], bh, a2);
           (s & 1 ? a1 : a2) = mma(K[0][s], bl, s & 1 ? a1 : a2);
@@ -690,20 +738,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(-beb[q], a1[q] + a2[q], bt[q] * f * v[q]);
         split4(x, hi, lo);
-        *reinterpret_cast<v4h*>(&xp[0][16 * j + c][16 * w + 4 * g]) = hi;
-        *reinterpret_cast<v4h*>(&xp[1][16 * j + c][16 * w + 4 * g]) = lo;
+        *reinterpret_cast<v4h*>(&xp[0][c][mine]) = hi;
+        *reinterpret_cast<v4h*>(&xp[1][c][mine]) = lo;
       }
       load_k(nb);
       __syncthreads();
       // ---- U = T X
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
+      {
         v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (s < nks) {
-            const v8h bh = *reinterpret_cast<const v8h*>(&xp[0][16 * j + c][32 * s + 8 * g]);
-            const v8h bl = *reinterpret_cast<const v8h*>(&xp[1][16 * j + c][32 * s + 8 * g]);
+            const v8h bh = part(xp[0][c], s), bl = part(xp[1][c], s);
             a1 = mma(T[0][s], bh, a1);
             a2 = mma(T[1][s], bh, a2);
             a2 = mma(T[0][s], bl, a2);
@@ -715,62 +761,58 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
         for (int q = 0; q < 4; ++q) x[q] = a1[q] + a2[q], y[q] = x[q] * rest[q], x[q] *= 0x1p-8f;
         split4(y, dh, dl);
         split4(x, uh, ul);
-        *reinterpret_cast<v4h*>(&up[2][16 * j + c][16 * w + 4 * g]) = dh;
-        *reinterpret_cast<v4h*>(&up[3][16 * j + c][16 * w + 4 * g]) = dl;
-        *reinterpret_cast<v4h*>(&up[0][16 * j + c][16 * w + 4 * g]) = uh;
-        *reinterpret_cast<v4h*>(&up[1][16 * j + c][16 * w + 4 * g]) = ul;
+        *reinterpret_cast<v4h*>(&up[2][c][mine]) = dh;
+        *reinterpret_cast<v4h*>(&up[3][c][mine]) = dl;
+        *reinterpret_cast<v4h*>(&up[0][c][mine]) = uh;
+        *reinterpret_cast<v4h*>(&up[1][c][mine]) = ul;
       }
       load_t(nb);
       __syncthreads();
       // ---- S' = e^{b_end} S + K^T U, and its parts for the next chunk
-      v4f a[2][NC][2];
+      v4f a[2][2];
 #pragma unroll
-      for (int j = 0; j < NC; ++j)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const v8h bh = *reinterpret_cast<const v8h*>(&up[2][16 * j + c][32 * s + 8 * g]);
-          const v8h bl = *reinterpret_cast<const v8h*>(&up[3][16 * j + c][32 * s + 8 * g]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (s == 0) a[i][j][0] = a[i][j][1] = v4f{0.f, 0.f, 0.f, 0.f};
-            a[i][j][0] = mma(Kt[0][i][s], bh, a[i][j][0]);
-            a[i][j][1] = mma(Kt[1][i][s], bh, a[i][j][1]);
-            a[i][j][s] = mma(Kt[0][i][s], bl, a[i][j][s]);
-          }
-        }
-#pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const float inv = __builtin_ldexpf(0x1p-8f, -fe[j]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) S[i][j][q] = __builtin_fmaf(a[i][j][0][q] + a[i][j][1][q], inv, e * S[i][j][q]);
+        for (int q = 0; q < 4; ++q) a[i][0][q] = e * S[i][q];
+        a[i][1] = v4f{0.f, 0.f, 0.f, 0.f};
       }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const v8h bh = part(up[2][c], s), bl = part(up[3][c], s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          a[i][0] = mma(Kt[0][i][s], bh, a[i][0]);
+          a[i][1] = mma(Kt[1][i][s], bh, a[i][1]);
+          a[i][s] = mma(Kt[0][i][s], bl, a[i][s]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) S[i][q] = a[i][0][q] + a[i][1][q];
       load_kt(nb);
-      next_factor(e);  // (behind the last chunk: of values that nothing reads)
-      store_s();
+      store_s(next_factor(e));  // (behind the last chunk: by values that nothing reads)
       u = un, e = e_next;
       __syncthreads();
     }
+    const float f = __builtin_ldexpf(1.f, -fe);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int j = 0; j < NC; ++j) *reinterpret_cast<v4f*>(hp + 16 * j * PK + 16 * i) = S[i][j];
+      for (int q = 0; q < 4; ++q) S[i][q] *= f;
+      *reinterpret_cast<v4f*>(hp + 16 * i) = S[i];
+    }
   } else {
-    // ---- values: tokens 16 w + 4 g + q of a chunk, of the channel of column 16 j + c
+    // ---- values: tokens 16 w + 4 g + q of a chunk, of the channel of column c
     const int vch = 2 * PHK * PK + hv * PV + col0 + c;
-    float cw[NC][4];
-    uint32_t raw[NC][7];
+    const v2i k = *reinterpret_cast<const v2i*>(d.conv_w + (int64_t)vch * 4);
+    const float w0 = bf_lo((uint32_t)k[0]), w1 = bf_hi((uint32_t)k[0]), w2 = bf_lo((uint32_t)k[1]), w3 = bf_hi((uint32_t)k[1]);
+    uint32_t raw[7];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const v2i k = *reinterpret_cast<const v2i*>(d.conv_w + (int64_t)(vch + 16 * j) * 4);
-      cw[j][0] = bf_lo((uint32_t)k[0]), cw[j][1] = bf_hi((uint32_t)k[0]), cw[j][2] = bf_lo((uint32_t)k[1]), cw[j][3] = bf_hi((uint32_t)k[1]);
-#pragma unroll
-      for (int i = 0; i < 7; ++i) {
-        const int t = 16 * w + 4 * g + i - 3;
-        raw[j][i] = d.mixed[(int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + vch + 16 * j];
-        if (t < 0) raw[j][i] = old ? d.conv_state[slot * d.cs_slot + (int64_t)(vch + 16 * j) * 3 + i] : 0;
-      }
+    for (int i = 0; i < 7; ++i) {
+      const int t = 16 * w + 4 * g + i - 3;
+      raw[i] = d.mixed[(int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + vch];
+      if (t < 0) raw[i] = old ? d.conv_state[slot * d.cs_slot + (int64_t)vch * 3 + i] : 0;
     }
     const int vat = ((16 * w + 4 * g) * PQKV + vch) * 2;
     auto load_v = [&](int ch) {  // a later chunk's: its rows and the three before them
@@ -778,31 +820,23 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       const __amdgpu_buffer_rsrc_t b = buffer(d.mixed + (int64_t)row * PQKV,
                                               __builtin_amdgcn_readfirstlane(max(min(d.rows - row, PC + 3), 0)) * PQKV * 2);
 #pragma unroll
-      for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int i = 0; i < 7; ++i) raw[j][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, vat + i * PQKV * 2 + 32 * j, 0, 0);
+      for (int i = 0; i < 7; ++i) raw[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, vat + i * PQKV * 2, 0, 0);
     };
     auto conv_v = [&](int ch) {
+      v4f v;
+      float m = 0.f;
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        v4f v;
-        float m = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float y = bf2f(raw[j][q]) * cw[j][0];
-          y = __builtin_fmaf(bf2f(raw[j][q + 1]), cw[j][1], y);
-          y = __builtin_fmaf(bf2f(raw[j][q + 2]), cw[j][2], y);
-          y = fast_silu(__builtin_fmaf(bf2f(raw[j][q + 3]), cw[j][3], y));
-          v[q] = ch * PC + 16 * w + 4 * g + q < n ? y : 0.f;
-          m = fmaxf(m, fabsf(v[q]));
-        }
-        *reinterpret_cast<v4f*>(&vp[ch & 1][16 * j + c][16 * w + 4 * g]) = v;
-        const auto p16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-        m = fmaxf(__uint_as_float(p16[0]), __uint_as_float(p16[1]));
-        const auto p32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-        m = fmaxf(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
-        if (g == 0) most[w][16 * j + c] = m;
+      for (int q = 0; q < 4; ++q) {
+        float y = bf2f(raw[q]) * w0;
+        y = __builtin_fmaf(bf2f(raw[q + 1]), w1, y);
+        y = __builtin_fmaf(bf2f(raw[q + 2]), w2, y);
+        y = fast_silu(__builtin_fmaf(bf2f(raw[q + 3]), w3, y));
+        v[q] = ch * PC + 16 * w + 4 * g + q < n ? y : 0.f;
+        m = fmaxf(m, fabsf(v[q]));
       }
+      *reinterpret_cast<v4f*>(&vp[ch & 1][c][16 * w + 4 * g]) = v;
+      m = all_max(m);
+      if (lane == 0) most[w] = m;
     };
     v8h Q[2][4], P[2][2];
     v4f eb;
@@ -823,13 +857,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
     load_q(ub), load_p(ub);
     e = e_next;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NC; ++j) before[j] = 11.32f * columns(j), vmost[j] = 0.f;
+    before = 11.32f * columns();
     __syncthreads();
     conv_v(0);
     load_v(1);
     __syncthreads();
-    next_factor(1.f);
+    fe = next_factor(1.f);
     __syncthreads();
     // where a lane's outputs go, from the chunk's first row: rows of the wave's tile; four rows' exponent by four lanes
     const int oat = (16 * w + 4 * g) * PZ * 2 + (hv * PV + col0 + c) * 2;
@@ -838,21 +871,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       const uint8_t* const un = ch + 1 < chunks ? u + kNext : u;
       const __amdgpu_buffer_rsrc_t nb = buffer(un, kUnit);
       // ---- e^b Q S
-      v4f o[NC];
+      v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const v8h bh = *reinterpret_cast<const v8h*>(&sp[0][16 * j + c][32 * s + 8 * g]);
-          const v8h bl = *reinterpret_cast<const v8h*>(&sp[1][16 * j + c][32 * s + 8 * g]);
-          a1 = mma(Q[0][s], bh, a1);
-          a2 = mma(Q[1][s], bh, a2);
-          (s & 1 ? a1 : a2) = mma(Q[0][s], bl, s & 1 ? a1 : a2);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[j][q] = eb[q] * (a1[q] + a2[q]);
+      for (int s = 0; s < 4; ++s) {
+        const v8h bh = part(sp[0][c], s), bl = part(sp[1][c], s);
+        a1 = mma(Q[0][s], bh, a1);
+        a2 = mma(Q[1][s], bh, a2);
+        (s & 1 ? a1 : a2) = mma(Q[0][s], bl, s & 1 ? a1 : a2);
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) a1[q] = eb[q] * (a1[q] + a2[q]);
       load_q(nb);
       __syncthreads();
       conv_v(ch + 1);
@@ -862,46 +890,42 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       const int rows = min(n - ch * PC, PC);
       const __amdgpu_buffer_rsrc_t ob = buffer(d.out + (int64_t)(t0 + ch * PC) * PZ, rows * PZ * 2);
       const __amdgpu_buffer_rsrc_t xb = buffer(d.exps + (int64_t)(t0 + ch * PC) * 256, rows * 256);
+      a2 = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        v4f a1 = o[j], a2 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (s < nks) {
-            const v8h bh = *reinterpret_cast<const v8h*>(&up[0][16 * j + c][32 * s + 8 * g]);
-            const v8h bl = *reinterpret_cast<const v8h*>(&up[1][16 * j + c][32 * s + 8 * g]);
-            a1 = mma(P[0][s], bh, a1);
-            a2 = mma(P[1][s], bh, a2);
-            a2 = mma(P[0][s], bl, a2);
-          }
+      for (int s = 0; s < 2; ++s) {
+        if (s < nks) {
+          const v8h bh = part(up[0][c], s), bl = part(up[1][c], s);
+          a1 = mma(P[0][s], bh, a1);
+          a2 = mma(P[1][s], bh, a2);
+          a2 = mma(P[0][s], bl, a2);
         }
-        const float f = __builtin_ldexpf(0x1p-8f, -fe[j]) * d.scale;
-        float y[4], m = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          y[q] = (a1[q] + a2[q]) * f;
-          m = fmaxf(m, fabsf(y[q]));
-        }
-        int ex = 0;
-        (void)__builtin_frexpf(__uint_as_float(row16_max_u32(__float_as_uint(m))), &ex);
-        ex = min(max(ex, -110), 127);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (_Float16)__builtin_ldexpf(y[q], 14 - ex)), ob,
-                                                oat + q * PZ * 2 + 32 * j, 0, 0);
-        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)ex, xb, eat + j, 0, 0);
       }
+      const float f = __builtin_ldexpf(0x1p-8f, -fe) * d.scale;
+      float y[4], m = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        y[q] = (a1[q] + a2[q]) * f;
+        m = fmaxf(m, fabsf(y[q]));
+      }
+      int ex = 0;
+      (void)__builtin_frexpf(__uint_as_float(row16_max_u32(__float_as_uint(m))), &ex);
+      ex = min(max(ex, -110), 127);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (_Float16)__builtin_ldexpf(y[q], 14 - ex)), ob,
+                                              oat + q * PZ * 2, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b8((uint8_t)ex, xb, eat, 0, 0);
       load_p(nb);
-      next_factor(e);
+      fe = next_factor(e);
       u = un, e = e_next;
       __syncthreads();
     }
-    // ---- the conv state: the request's last three inputs (it has more).  This workgroup's value channels; q and k by the first
-    // workgroup of the key head, behind the kernel that read them
+    // ---- the conv state: the request's last three inputs (it has more).  This workgroup's value channels; q and k by the key
+    // head's first workgroup, behind the kernel that read them
     const int ot = tid - 256;
-    for (int i = ot; i < COLS * 3; i += 256) {
-      const int cc = 2 * PHK * PK + hv * PV + col0 + i / 3;
-      d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
+    if (ot < 48) {
+      const int cc = 2 * PHK * PK + hv * PV + col0 + ot / 3;
+      d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + ot % 3] = d.mixed[(int64_t)(t0 + n - 3 + ot % 3) * PQKV + cc];
     }
     if (in == 0)
       for (int i = ot; i < 2 * PK * 3; i += 256) {
@@ -909,6 +933,315 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
         d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
       }
   }
+}
+
+// 16 bytes a lane from memory into LDS at byte `at` + 16 lane of the workgroup's, past the registers.  In asm, so that the
+// compiler does not hold reads of LDS back until every copy in flight has landed; the caller waits (wait_vm0).
+__device__ __forceinline__ void copy16(const uint8_t* src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+}
+__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8)); }
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// A whole head's LDS: a chunk's operands (K and Q; K^T, T and P), the gates of two chunks, the outputs
+constexpr int kLQ = 32 * kPiece, kLKt = 64 * kPiece, kLT = 96 * kPiece, kLP = 108 * kPiece, kLGate = 120 * kPiece,
+              kLOut = 122 * kPiece, kOutRow = PV + 4;
+constexpr int kHeadsLds = kLOut + PC * kOutRow * 4;
+
+// A request's chunks for a whole value head, 16 columns a wave.  A wave's columns need nothing of another's: it holds their
+// state (lane (c, g): column c, dims 16 t + 4 g + q), and each product's registers, rounded to two parts, are the next one's
+// operand.  What the waves share are the chunk's other operands, in LDS: K and Q of the next chunk arrive while T, P and K^T
+// are used, and the other way round, with a barrier at either change.
+//
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_heads_kernel(PromptDev d) {
+  constexpr int W = 8;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  // the two workgroups of a (request, key head) on one XCD, where the chunks' operands came from
+  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  const int grp = (at / 2) * 8 + xcd, hh = at % 2, r = grp / PHK, hk = grp % PHK, hv = 2 * hk + hh;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), col0 = 16 * wave;
+  int t0, n;
+  int64_t slot;
+  bool old;
+  request_of(d, r, t0, n, slot, old);
+  t0 = __builtin_amdgcn_readfirstlane(t0), n = __builtin_amdgcn_readfirstlane(n);
+  if (n <= kShort || slot < 0 || !many_chunks(d)) return;
+  const int chunks = (n + PC - 1) / PC;
+  const uint8_t* u = d.units + ((int64_t)first_unit(d, r, t0) * PHK + hk) * kUnit + 16 * lane;
+  constexpr int64_t kNext = (int64_t)PHK * kUnit;
+  const int head = kUHead + hh * kHeadBytes;
+  const uint32_t base = (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) uint8_t*)lds);
+  auto copy_kq = [&](const uint8_t* p, int half) {
+#pragma unroll
+    for (int i = 0; i < 64 / W; ++i) {
+      const int k = wave + W * i;
+      copy16(p + (k < 32 ? kUK : kUQ - 32 * kPiece) + k * kPiece, base + k * kPiece);
+    }
+    if (wave == 0) copy16(p + head + kHGate, base + kLGate + half * kPiece);
+  };
+  auto copy_tp = [&](const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < 56 / W; ++i) {
+      const int k = wave + W * i;
+      copy16(p + (k < 32 ? kUKt : head - 32 * kPiece) + k * kPiece, base + kLKt + k * kPiece);
+    }
+  };
+  const uint8_t *const kq = lds + 16 * lane, *const tp = lds + kLKt + 16 * lane;  // (an instruction's offset has 16 bits)
+  auto piece = [&](int off) { return *reinterpret_cast<const v8h*>(off < kLKt ? kq + off : tp + (off - kLKt)); };
+  auto gate = [&](int half, int k, int m) {  // of tokens 16 m + 4 g ..
+    return *reinterpret_cast<const v4f*>(lds + kLGate + half * kPiece + 256 * k + 64 * m + 16 * g);
+  };
+  copy_kq(u, 0);
+  copy_tp(u);
+
+  // ---- the state, times 2^fe
+  float* const hp = d.h0 + ((slot * PHV + hv) * PV + col0 + c) * PK + 4 * g;
+  v4f S[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) S[t] = old ? *reinterpret_cast<const v4f*>(hp + 16 * t) : v4f{0.f, 0.f, 0.f, 0.f};
+  // ---- values: tokens 16 m + 4 g + q of a chunk
+  const int vch = 2 * PHK * PK + hv * PV + col0 + c;
+  const v2i wr = *reinterpret_cast<const v2i*>(d.conv_w + (int64_t)vch * 4);
+  const float w0 = bf_lo((uint32_t)wr[0]), w1 = bf_hi((uint32_t)wr[0]), w2 = bf_lo((uint32_t)wr[1]), w3 = bf_hi((uint32_t)wr[1]);
+  uint32_t raw[4][7];
+#pragma unroll
+  for (int m = 0; m < 4; ++m)
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+      const int t = 16 * m + 4 * g + i - 3;
+      raw[m][i] = d.mixed[(int64_t)(t0 + min(max(t, 0), n - 1)) * PQKV + vch];
+      if (t < 0) raw[m][i] = old ? d.conv_state[slot * d.cs_slot + (int64_t)vch * 3 + i] : 0;
+    }
+  const int vat = (4 * g * PQKV + vch) * 2;
+  auto load_v = [&](int ch) {  // a later chunk's: its rows and the three before them
+    const int row = t0 + ch * PC - 3;
+    const __amdgpu_buffer_rsrc_t b = buffer(d.mixed + (int64_t)row * PQKV,
+                                            __builtin_amdgcn_readfirstlane(max(min(d.rows - row, PC + 3), 0)) * PQKV * 2);
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        raw[m][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(b, vat + (16 * m + i) * PQKV * 2, 0, 0);
+  };
+  v4f v[4];
+  float before, vmost = 0.f;
+  int fe = 0;  // the columns' exponent
+  auto conv_v = [&](int ch) {
+    float most = 0.f;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y = bf2f(raw[m][q]) * w0;
+        y = __builtin_fmaf(bf2f(raw[m][q + 1]), w1, y);
+        y = __builtin_fmaf(bf2f(raw[m][q + 2]), w2, y);
+        y = fast_silu(__builtin_fmaf(bf2f(raw[m][q + 3]), w3, y));
+        v[m][q] = ch * PC + 16 * m + 4 * g + q < n ? y : 0.f;
+        most = fmaxf(most, fabsf(v[m][q]));
+      }
+    return all_max(most);
+  };
+  auto next_factor = [&](float e, float most) {
+    before = __builtin_fmaf(64.f, vmost, before * e);  // (what the chunk adds is not decayed by all of e)
+    vmost = most;
+    const int to = next_exponent(fe, __builtin_fmaf(65.f, most, before));
+    if (to != fe) {
+      const float f = __builtin_ldexpf(1.f, to - fe);
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) S[t][q] *= f;
+      fe = to;
+    }
+  };
+  {
+    float m = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m = fmaxf(m, fabsf(S[t][q]));
+    before = 11.32f * all_max(m);  // a norm: at most sqrt(128) times the largest
+    next_factor(1.f, conv_v(0));
+  }
+  wait_vm0();
+  barrier();
+
+  for (int ch = 0; ch < chunks; ++ch) {
+    const uint8_t* const un = ch + 1 < chunks ? u + kNext : u;  // (the last chunk's operands twice)
+    const int half = ch & 1, rows = min(n - ch * PC, PC);
+    load_v(ch + 1);
+    v4i z[2];  // of the rows that the wave will norm
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      z[i] = *reinterpret_cast<const v4i*>(d.z + (int64_t)(t0 + ch * PC + min(8 * wave + 4 * i + g, rows - 1)) * PZ + hv * PV + 8 * c);
+    // ---- X = beta (V - e^b K S), Q S
+    v4f o[4];
+    v8h xh[2], xl[2];
+    {
+      v8h bh[4], bl[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        v4h h[2], l[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          split4(S[2 * s + i], h[i], l[i]);
+        }
+        bh[s] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        bl[s] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+      v4f a[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (s == 0) a[m] = v4f{0.f, 0.f, 0.f, 0.f};
+          const v8h kh = piece((4 * m + s) * kPiece), kl = piece((16 + 4 * m + s) * kPiece);
+          a[m] = mma(kh, bh[s], a[m]);
+          a[m] = mma(kl, bh[s], a[m]);
+          a[m] = mma(kh, bl[s], a[m]);
+        }
+      const float fv = __builtin_ldexpf(1.f, fe);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v4h h[2], l[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int m = 2 * i + k;
+          const v4f bt = gate(half, 2, m), beb = gate(half, 3, m);
+          v4f x;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(-beb[q], a[m][q], bt[q] * fv * v[m][q]);
+          split4(x, h[k], l[k]);
+        }
+        xh[i] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        xl[i] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          if (s == 0) o[m] = v4f{0.f, 0.f, 0.f, 0.f};
+          const v8h qh = piece(kLQ + (4 * m + s) * kPiece), ql = piece(kLQ + (16 + 4 * m + s) * kPiece);
+          o[m] = mma(qh, bh[s], o[m]);
+          o[m] = mma(ql, bh[s], o[m]);
+          o[m] = mma(qh, bl[s], o[m]);
+        }
+    }
+    wait_vm0();
+    barrier();  // every wave is done with K and Q; T, P and K^T are there
+    copy_kq(un, half ^ 1);
+    // ---- U = T X
+    v8h uh[2], ul[2], dh[2], dl[2];
+    {
+      v4f a[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        a[m] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s <= m / 2; ++s) {
+          const v8h th = piece(kLT + tri_piece(m, s) * kPiece), tl = piece(kLT + (6 + tri_piece(m, s)) * kPiece);
+          a[m] = mma(th, xh[s], a[m]);
+          a[m] = mma(tl, xh[s], a[m]);
+          a[m] = mma(th, xl[s], a[m]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v4h h[2], l[2], hd[2], ld[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int m = 2 * i + k;
+          const v4f rest = gate(half, 1, m);
+          v4f x, y;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] = a[m][q] * rest[q], x[q] = a[m][q] * 0x1p-8f;
+          split4(y, hd[k], ld[k]);
+          split4(x, h[k], l[k]);
+        }
+        dh[i] = __builtin_shufflevector(hd[0], hd[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        dl[i] = __builtin_shufflevector(ld[0], ld[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        uh[i] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        ul[i] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+    // ---- S' = e^{b_end} S + K^T U
+    const float e = *reinterpret_cast<const float*>(lds + kLGate + half * kPiece + 4 * (PC - 1));
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) S[t][q] *= e;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const v8h kh = piece(kLKt + (2 * t + s) * kPiece), kl = piece(kLKt + (16 + 2 * t + s) * kPiece);
+        S[t] = mma(kh, dh[s], S[t]);
+        S[t] = mma(kl, dh[s], S[t]);
+        S[t] = mma(kh, dl[s], S[t]);
+      }
+    }
+    // ---- O = e^b Q S + P U
+    const float fo = __builtin_ldexpf(0x1p-8f, -fe) * d.scale;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const v4f eb = gate(half, 0, m);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[m][q] *= eb[q];
+#pragma unroll
+      for (int s = 0; s <= m / 2; ++s) {
+        const v8h ph = piece(kLP + tri_piece(m, s) * kPiece), pl = piece(kLP + (6 + tri_piece(m, s)) * kPiece);
+        o[m] = mma(ph, uh[s], o[m]);
+        o[m] = mma(pl, uh[s], o[m]);
+        o[m] = mma(ph, ul[s], o[m]);
+      }
+    }
+    next_factor(e, conv_v(ch + 1));  // (behind the last chunk: of values that nothing reads)
+    {
+      float* const os = reinterpret_cast<float*>(lds + kLOut);
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) os[(16 * m + 4 * g + q) * kOutRow + col0 + c] = o[m][q] * fo;
+    }
+    wait_vm0();
+    barrier();  // every wave is done with T, P and K^T; the next K and Q are there
+    copy_tp(un);
+    u = un;
+    {  // the gated norm: eight rows a wave, 16 lanes a row
+      const float* const os = reinterpret_cast<const float*>(lds + kLOut);
+      const v4i wn = *reinterpret_cast<const v4i*>(d.norm_w + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = 8 * wave + 4 * i + g;
+        if (t < rows) {
+          const v4f x0 = *reinterpret_cast<const v4f*>(os + t * kOutRow + 8 * c), x1 = *reinterpret_cast<const v4f*>(os + t * kOutRow + 8 * c + 4);
+          const float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+          norm_store(d, t0 + ch * PC + t, hv, c, x, z[i], wn);
+        }
+      }
+    }
+  }
+  const float fs = __builtin_ldexpf(1.f, -fe);
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) S[t][q] *= fs;
+    *reinterpret_cast<v4f*>(hp + 16 * t) = S[t];
+  }
+  // ---- the conv state: the request's last three inputs (it has more).  This workgroup's value channels; q and k by the key
+  // head's first workgroup, behind the kernel that read them
+  for (int i = lane; i < 48; i += 64) {
+    const int cc = 2 * PHK * PK + hv * PV + col0 + i / 3;
+    d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
+  }
+  if (hh == 0)
+    for (int i = tid; i < 2 * PK * 3; i += 64 * W) {
+      const int cc = (i / (3 * PK)) * (PHK * PK) + hk * PK + i / 3 % PK;
+      d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
+    }
+  wait_vm0();  // (copies of the last chunk's operands again may be on their way into this workgroup's LDS)
 }
 
 // The gated norm of the chunks' rows: a wave a row, 16 lanes a head.
@@ -921,7 +1254,7 @@ __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptDev d) {
   int64_t slot;
   bool old;
   request_of(d, r, t0, n, slot, old);
-  if (n <= kShort || slot < 0 || row < t0 || row >= t0 + n) return;
+  if (n <= kShort || slot < 0 || row < t0 || row >= t0 + n || many_chunks(d)) return;
   const int c = lane & 15;
   const v4i wr = *reinterpret_cast<const v4i*>(d.norm_w + 8 * c);
   v4i o[8], z[8];
@@ -935,41 +1268,11 @@ __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptDev d) {
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t at = (int64_t)row * PZ + i * 512 + lane * 8;
     const v8h h = __builtin_bit_cast(v8h, o[i]);
-    float x[8], ss = 0.f;
+    float x[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      x[k] = __builtin_ldexpf((float)h[k], ex[i] - 14);
-      ss = __builtin_fmaf(x[k], x[k], ss);
-    }
-    const float rstd = 1.f / sqrtf(row16_sum(ss) * (1.f / PV) + d.eps);
-    float y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float zz = (k & 1) ? bf_hi((uint32_t)z[i][k >> 1]) : bf_lo((uint32_t)z[i][k >> 1]);
-      const float ww = (k & 1) ? bf_hi((uint32_t)wr[k >> 1]) : bf_lo((uint32_t)wr[k >> 1]);
-      y[k] = x[k] * rstd * ww * fast_silu(zz);
-    }
-    v4i w;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = (int)pack_bf2(y[2 * k], y[2 * k + 1]);
-    *reinterpret_cast<v4i*>(d.out + at) = w;
-    if (d.oq) {
-      float f[8], m = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        f[k] = (k & 1) ? bf_hi((uint32_t)w[k >> 1]) : bf_lo((uint32_t)w[k >> 1]);
-        m = fmaxf(m, fabsf(f[k]));
-      }
-      m = fmaxf(m, lane_xor<1>(m));
-      m = fmaxf(m, lane_xor<2>(m));
-      m = fmaxf(m, lane_xor<4>(m));
-      m = fmaxf(m, lane_xor<8>(m));
-      const uint2 q = e4m3_run8(f, m > 0.f ? 448.f / m : 0.f);
-      *reinterpret_cast<uint2*>(d.oq + at) = q;
-      if (c == 0) d.oqs[(int64_t)row * PHV + 4 * i + (lane >> 4)] = m / 448.f;
-    }
+    for (int k = 0; k < 8; ++k) x[k] = __builtin_ldexpf((float)h[k], ex[i] - 14);
+    norm_store(d, row, 4 * i + (lane >> 4), c, x, z[i], wr);
   }
 }
 
@@ -1015,15 +1318,19 @@ extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream)
               static_cast<const uint16_t*>(a->b), static_cast<uint16_t*>(a->conv_state), a->cs_slot,
               static_cast<const uint16_t*>(a->conv_w), a->A_log, a->dt_bias, a->h0, a->qsl, a->state_idx, a->prefix,
               static_cast<const uint16_t*>(a->norm_w), static_cast<uint16_t*>(a->out), static_cast<uint8_t*>(a->oq), a->oqs,
-              static_cast<uint8_t*>(a->workspace), nullptr, a->B > a->rows / (kShort + 1)};
+              static_cast<uint8_t*>(a->workspace), nullptr, a->B > a->rows / (kShort + 1), a->B >= 4};
   const int64_t units = chunk_units(a->rows, a->B);
   d.exps = reinterpret_cast<int8_t*>(d.units + units * PHK * kUnit);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   prompt_steps_kernel<<<(unsigned)a->B * PHK, 512, 0, st>>>(d);
   if (units) {
     prompt_chunks_kernel<<<(unsigned)units * PHK, 512, 0, st>>>(d);
-    if (a->B >= 8) prompt_scan_kernel<4><<<(unsigned)a->B * PHK * 4, 512, 0, st>>>(d);
-    else prompt_scan_kernel<1><<<(unsigned)a->B * PHK * 16, 512, 0, st>>>(d);
+    if (d.both) {
+      const int rc = ensure_lds(reinterpret_cast<const void*>(prompt_heads_kernel), kHeadsLds, "q36_gdn_prompt");
+      if (rc != Q36_OK) return rc;
+      prompt_heads_kernel<<<(unsigned)a->B * PHK * 2, 512, kHeadsLds, st>>>(d);
+    }
+    prompt_scan_kernel<<<(unsigned)a->B * PHK * 16, 512, 0, st>>>(d);
     prompt_norm_kernel<<<(unsigned)(a->rows + 3) / 4, 256, 0, st>>>(d);
   }
   return check_launch("q36_gdn_prompt");
