@@ -867,7 +867,13 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
     // where a lane's outputs go, from the chunk's first row: rows of the wave's tile; four rows' exponent by four lanes
     const int oat = (16 * w + 4 * g) * PZ * 2 + (hv * PV + col0 + c) * 2;
     const int eat = c < 4 ? (16 * w + 4 * g + c) * 256 + hv * 8 + col0 / 16 : 0x7fffff00;
+    // The key head's 16 workgroups touch a sixteenth each of the operands two chunks on, a lane a line, so that every load of
+    // them finds its line in L2: those that miss take longer than a chunk.
+    const int touch = min((in * 4 + w) * (kUnit / 64) + lane * 128, kUnit - 4);
+    uint32_t seen = 0;
     for (int ch = 0; ch < chunks; ++ch) {
+      asm volatile("" ::"v"(seen));  // (touched a chunk ago)
+      if (lane * 128 < kUnit / 64) seen = *reinterpret_cast<const volatile uint32_t*>(u + (ch + 2 < chunks ? 2 * kNext : 0) + touch);
       const uint8_t* const un = ch + 1 < chunks ? u + kNext : u;
       const __amdgpu_buffer_rsrc_t nb = buffer(un, kUnit);
       // ---- e^b Q S
