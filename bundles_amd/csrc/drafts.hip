@@ -7,9 +7,10 @@
 // not, the token is drawn from max(p - q, 0); behind the last draft from p: the first index whose running sum passes
 // u_last times the total.  Temperature 0 (or NaN): p is 1 at the first largest logit.
 //
-// The draw compares running sums over the whole vocabulary with one number, so weights and sums are fp64 (a weight is good
-// to 7e-12): with fp32 weights one draw in a few hundred would land on a neighbour.  fp64 costs no more than fp32 here, the
-// vector unit issues both at one rate.
+// The draw compares running sums over the whole vocabulary with one number, so its weights and sums are fp64 (a weight is
+// good to 7e-12): with fp32 weights one draw in a few hundred would land on a neighbour.  That is so of the row drawn from
+// alone.  In a large call the other rows' sums are fp32, good to 2^-19, which the drafts' tests can do with: a test as close to
+// its border as 2^-17 sums its row again in fp64.
 #include <type_traits>
 
 #include "q36_device.h"
@@ -20,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256, kPer = 16, kSeg = kThreads * kPer;  // logits a thread, a segment
 constexpr int kMaxT = 8;
+constexpr double kClose = 0x1p-17;  // of fp32 sums: 4096 terms by 16, 64, 4 and the segments, rounded 2^-24 each time, weights 2^-22
 
 struct DraftsDev {
   int B, T, V, segs;
@@ -29,10 +31,12 @@ struct DraftsDev {
   const int32_t* drafts;
   const float* uniforms;
   const float* probs;  // [B, T - 1, V] or null
+  int narrow;          // the rows' sums are fp32's
   double* psum;        // [rows, segs] sum of a segment's weights, relative to its largest logit
   float* pmax;         // [rows, segs] that logit
   int32_t* pidx;       // [rows, segs] its first index
-  double* rsum;        // [B, segs] a segment's residual
+  double* esum;        // [B, segs] the drawn row's sums in fp64, where psum is not
+  double* rsum;        // [B, segs] its residual
   int32_t* tokens;
   int32_t* counts;
 };
@@ -114,7 +118,7 @@ __device__ __forceinline__ double wave_sum_d(double v) {
 }
 
 // A segment of a row: its largest logit, the first index of it, the sum of its weights.
-template <bool F32, bool VEC>
+template <bool F32, bool VEC, bool WIDE>
 __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
   __shared__ float wm[4];
   __shared__ int wi[4];
@@ -137,9 +141,17 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
   for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o));
   double sum = 0.0;
   if (s > 0.0 && m > -__builtin_inff()) {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
-    sum = wave_sum_d(sum);
+      for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
+      sum = wave_sum_d(sum);
+    } else {
+      const float sf = (float)fmin(s, 1e30);  // (weights of a temperature below 1e-30: 1 at the largest, else 0)
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) t += x[i] == m ? 1.f : __builtin_amdgcn_exp2f(fmaxf((x[i] - m) * sf, -200.f));
+      sum = (double)wave_sum_bfly(t);
+    }
   }
   if (lane == 0) wm[wave] = m, wi[wave] = first, ws[wave] = sum;
   __syncthreads();
@@ -158,96 +170,165 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
 
 // What a request's rows say: the accepted drafts, and the row the next token is drawn from.
 struct Chain {
-  float m[kMaxT];     // a row's largest logit
-  int idx[kMaxT];     // its first index
-  double norm[kMaxT]; // sum of the row's weights
-  float xd[kMaxT];    // the draft's logit
-  double q[kMaxT];    // its draft probability
-  int j, refused, ended;
+  float m[kMaxT];      // a row's largest logit
+  int idx[kMaxT];      // its first index
+  double norm[kMaxT];  // sum of the row's weights
+  bool wide[kMaxT];    // in fp64
+  double p[kMaxT];     // the draft's weight (its probability, where greedy)
+  double q[kMaxT];     // its draft probability
+  double u[kMaxT];
+  int tok[kMaxT];      // the draft, -1 without one
+  double part[4];
+  int j, refused, ended, close;
 };
 
-// Every wave takes rows wave, wave + waves, ..; then thread 0 walks the drafts.  (Callers synchronise behind it.)
-template <bool F32>
+__device__ __forceinline__ int min64(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
+  return v;
+}
+
+// Sum of a row's weights in fp64, by the whole workgroup.
+template <bool F32, bool VEC>
+__device__ double wide_sum(const DraftsDev& d, int64_t row, float m, double s, double* part) {
+  double sum = 0.0;
+  for (int base = threadIdx.x * kPer; base < d.V; base += kSeg) {
+    float x[kPer];
+    load_logits<F32, VEC>(d, row, base, x);
+    for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
+  }
+  sum = wave_sum_d(sum);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = (part[0] + part[1]) + (part[2] + part[3]);
+  __syncthreads();
+  return sum;
+}
+
+// Waves take rows wave, wave + 4; then thread 0 walks the drafts.  Behind a synchronisation.
+template <bool F32, bool VEC>
 __device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  for (int t = wave; t < d.T; t += waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int t = wave; t < d.T; t += 4) {
     const int64_t row = (int64_t)b * d.T + t, o = row * d.segs;
-    float m = -__builtin_inff();
-    for (int i = lane; i < d.segs; i += 64) m = fmaxf(m, d.pmax[o + i]);
+    const float u = d.uniforms[row];
+    int tok = t + 1 < d.T ? d.drafts[(int64_t)b * (d.T - 1) + t] : -1;
+    if (tok >= d.V) tok = -1;
+    const bool on = lane < d.segs;
+    const float pm = on ? d.pmax[o + lane] : -__builtin_inff();
+    const double ps = on ? d.psum[o + lane] : 0.0;
+    const int pi = on ? d.pidx[o + lane] : 0x7fffffff;
+    const float xd = tok >= 0 ? logit_at<F32>(d, row, tok) : -__builtin_inff();
+    const double q = tok >= 0 && d.probs ? (double)d.probs[((int64_t)b * (d.T - 1) + t) * d.V + tok] : 1.0;
+    float m = pm;
+    for (int i = lane + 64; i < d.segs; i += 64) m = fmaxf(m, d.pmax[o + i]);
     m = wave_max(m);
-    double n = 0.0;
-    int first = 0x7fffffff;
-    for (int i = lane; i < d.segs; i += 64) {
-      const float pm = d.pmax[o + i];
-      if (pm > -__builtin_inff()) {
-        if (pm == m) first = min(first, d.pidx[o + i]);
-        if (s > 0.0) n += d.psum[o + i] * weight(pm, m, s);
+    int first = pm == m ? pi : 0x7fffffff;
+    double n = s > 0.0 && pm > -__builtin_inff() ? ps * weight(pm, m, s) : 0.0;
+    for (int i = lane + 64; i < d.segs; i += 64) {
+      const float v = d.pmax[o + i];
+      if (v > -__builtin_inff()) {
+        if (v == m) first = min(first, d.pidx[o + i]);
+        if (s > 0.0) n += d.psum[o + i] * weight(v, m, s);
       }
     }
     n = wave_sum_d(n);
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) first = min(first, __shfl_xor(first, k));
+    first = min64(first);
     if (lane == 0) {
-      c->m[t] = m, c->idx[t] = first, c->norm[t] = n;
-      if (t + 1 < d.T) {
-        const int tok = d.drafts[(int64_t)b * (d.T - 1) + t];
-        const bool in = tok >= 0 && tok < d.V;
-        c->xd[t] = in ? logit_at<F32>(d, row, tok) : -__builtin_inff();
-        c->q[t] = in && d.probs ? (double)d.probs[((int64_t)b * (d.T - 1) + t) * d.V + tok] : 1.0;
-      }
+      c->m[t] = m, c->idx[t] = first, c->norm[t] = n, c->wide[t] = !d.narrow;
+      c->p[t] = s > 0.0 ? (xd > -__builtin_inff() ? weight(xd, m, s) : 0.0) : (first == tok ? 1.0 : 0.0);
+      c->q[t] = q, c->u[t] = (double)u, c->tok[t] = tok;
     }
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int j = 0, refused = 0, ended = 0;
-    for (; j < d.T; ++j) {
-      const float m = c->m[j];
-      if (!(m > -__builtin_inff())) {  // a row that leaves no token
-        ended = 1;
-        break;
+  for (;;) {
+    if (threadIdx.x == 0) {
+      int j = 0, refused = 0, ended = 0, close = 0;
+      for (; j < d.T; ++j) {
+        if (!(c->m[j] > -__builtin_inff())) {  // a row that leaves no token
+          ended = 1;
+          break;
+        }
+        if (j == d.T - 1 || c->tok[j] < 0) break;  // no draft: the token is drawn from p
+        const double need = c->u[j] * c->q[j], p = s > 0.0 ? c->p[j] / c->norm[j] : c->p[j];
+        if (s > 0.0 && !c->wide[j] && fabs(need - p) <= kClose * p) {
+          close = 1;
+          break;
+        }
+        if (!(need < p)) {
+          refused = 1;
+          break;
+        }
       }
-      if (j == d.T - 1) break;
-      const int tok = d.drafts[(int64_t)b * (d.T - 1) + j];
-      if (tok < 0 || tok >= d.V) break;  // no draft: the token is drawn from p
-      const double p = s > 0.0 ? weight(c->xd[j], m, s) / c->norm[j] : (c->idx[j] == tok ? 1.0 : 0.0);
-      if (!((double)d.uniforms[(int64_t)b * d.T + j] * c->q[j] < p)) {
-        refused = 1;
-        break;
-      }
+      c->j = j, c->refused = refused, c->ended = ended, c->close = close;
     }
-    c->j = j, c->refused = refused, c->ended = ended;
+    __syncthreads();
+    if (!c->close) return;
+    const int j = c->j;
+    const double n = wide_sum<F32, VEC>(d, (int64_t)b * d.T + j, c->m[j], s, c->part);
+    if (threadIdx.x == 0) c->norm[j] = n, c->wide[j] = true;
+    __syncthreads();
   }
+}
+
+// The drawn row's sum in fp64 from its segments', where it is not: by every wave, the same bits.
+__device__ void widen(const DraftsDev& d, int b, double s, Chain* c) {
+  if (!d.narrow || s <= 0.0 || c->ended) return;
+  double n = 0.0;
+  for (int i = threadIdx.x & 63; i < d.segs; i += 64) n += d.esum[(int64_t)b * d.segs + i];
+  n = wave_sum_d(n);
+  __syncthreads();
+  if (threadIdx.x == 0) c->norm[c->j] = n;
+  __syncthreads();
+}
+
+// The drawn row's weights in fp64, relative to the row's largest logit.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void drafts_exact_kernel(DraftsDev d) {
+  __shared__ Chain c;
+  const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
+  const double s = heat_of(d, b);
+  if (!(s > 0.0)) return;
+  walk<F32, VEC>(d, b, s, &c);
+  if (c.ended) return;
+  float x[kPer];
+  load_logits<F32, VEC>(d, (int64_t)b * d.T + c.j, seg * kSeg + tid * kPer, x);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += weight(x[i], c.m[c.j], s);
+  sum = wave_sum_d(sum);
+  if ((tid & 63) == 0) c.part[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) d.esum[(int64_t)b * d.segs + seg] = (c.part[0] + c.part[1]) + (c.part[2] + c.part[3]);
 }
 
 // Residual sums of the row that a request's token is drawn from, where draft probabilities were given.
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) {
   __shared__ Chain c;
-  __shared__ double ws[4];
   const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
   const double s = heat_of(d, b);
-  walk<F32>(d, b, s, &c);
-  __syncthreads();
+  walk<F32, VEC>(d, b, s, &c);
+  if (!c.refused) return;
+  widen(d, b, s, &c);
+  const int j = c.j, base = seg * kSeg + tid * kPer;
+  const int64_t row = (int64_t)b * d.T + j;
+  const float* q = d.probs + ((int64_t)b * (d.T - 1) + j) * d.V;
+  float x[kPer];
+  load_logits<F32, VEC>(d, row, base, x);
+  const double inv = 1.0 / c.norm[j];
   double sum = 0.0;
-  if (c.refused) {
-    const int j = c.j;
-    const int64_t row = (int64_t)b * d.T + j;
-    const float* q = d.probs + ((int64_t)b * (d.T - 1) + j) * d.V;
-    const int base = seg * kSeg + tid * kPer;
-    float x[kPer];
-    load_logits<F32, VEC>(d, row, base, x);
-    const double inv = 1.0 / c.norm[j];
-    for (int i = 0; i < kPer; ++i) {
-      if (base + i >= d.V) break;
-      const double p = s > 0.0 ? weight(x[i], c.m[j], s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
-      const double r = p - (double)q[base + i];
-      sum += r > 0.0 ? r : 0.0;
-    }
-    sum = wave_sum_d(sum);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool in = base + i < d.V;
+    const double p = s > 0.0 ? weight(x[i], c.m[j], s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
+    const double r = p - (double)q[in ? base + i : 0];
+    sum += in && r > 0.0 ? r : 0.0;
   }
-  if ((tid & 63) == 0) ws[tid >> 6] = sum;
+  sum = wave_sum_d(sum);
+  if ((tid & 63) == 0) c.part[tid >> 6] = sum;
   __syncthreads();
-  if (tid == 0) d.rsum[(int64_t)b * d.segs + seg] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+  if (tid == 0) d.rsum[(int64_t)b * d.segs + seg] = (c.part[0] + c.part[1]) + (c.part[2] + c.part[3]);
 }
 
 // One workgroup a request: the drafts' walk, the segment in which the running sum passes the threshold, the index in it.
@@ -259,17 +340,16 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   __shared__ int found, last;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double s = heat_of(d, b);
-  walk<F32>(d, b, s, &c);
-  __syncthreads();
+  walk<F32, VEC>(d, b, s, &c);
+  widen(d, b, s, &c);
   const int j = c.j;
   int32_t* const out = d.tokens + (int64_t)b * d.T;
-  const int32_t* const tok = d.drafts + (int64_t)b * (d.T - 1);
-  if (tid < d.T) out[tid] = tid < j ? tok[tid] : -1;
+  if (tid < d.T) out[tid] = tid < j ? c.tok[tid] : -1;
   if (tid == 0) d.counts[b] = c.ended ? j : j + 1;
   if (c.ended) return;
   const int64_t row = (int64_t)b * d.T + j;
-  const int dt = c.refused ? tok[j] : -1;  // the refused draft
-  const double u = (double)d.uniforms[(int64_t)b * d.T + d.T - 1];
+  const int dt = c.refused ? c.tok[j] : -1;  // the refused draft
+  const double u = c.u[d.T - 1];
   // ---- the segment.  Wave 0 walks 64 at a time; the refused draft's own weight leaves its segment's sum.
   if (wave == 0) {
     const int64_t o = row * d.segs;
@@ -279,31 +359,36 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
       if (md == 2) return d.rsum[(int64_t)b * d.segs + i];
       double w;
       if (s > 0.0) {
-        const float pm = d.pmax[o + i];
-        w = pm > -__builtin_inff() ? d.psum[o + i] * weight(pm, c.m[j], s) * inv : 0.0;
+        if (d.narrow) {
+          w = d.esum[(int64_t)b * d.segs + i] * inv;
+        } else {
+          const float pm = d.pmax[o + i];
+          w = pm > -__builtin_inff() ? d.psum[o + i] * weight(pm, c.m[j], s) * inv : 0.0;
+        }
       } else {
         w = c.idx[j] / kSeg == i ? 1.0 : 0.0;
       }
       if (md == 1 && dt / kSeg == i) {
-        w -= s > 0.0 ? weight(c.xd[j], c.m[j], s) * inv : (c.idx[j] == dt ? 1.0 : 0.0);
+        w -= c.p[j] * inv;
         w = w > 0.0 ? w : 0.0;
       }
       return w;
     };
     int md = c.refused ? (d.probs ? 2 : 1) : 0;
-    double all = 0.0;
+    double mine = part(lane, md), all = 0.0;
     for (int pass = 0; pass < 2; ++pass) {
-      all = 0.0;
-      for (int i0 = 0; i0 < d.segs; i0 += 64) all += wave_sum_d(part(i0 + lane, md));
+      all = wave_sum_d(mine);
+      for (int i0 = 64; i0 < d.segs; i0 += 64) all += wave_sum_d(part(i0 + lane, md));
       if (all > 0.0 || md == 0) break;
       md = 0;  // nothing is left of the row beside the draft: p itself
+      mine = part(lane, md);
     }
     const double goal = u * all;
     double before = 0.0, base = 0.0;
     int at = -1, tail = -1;
     double tail_base = 0.0;
     for (int i0 = 0; i0 < d.segs && at < 0; i0 += 64) {
-      const double w = part(i0 + lane, md);
+      const double w = i0 ? part(i0 + lane, md) : mine;
       double run = w;
 #pragma unroll
       for (int k = 1; k < 64; k <<= 1) {
@@ -372,6 +457,11 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   if (tid == 0) out[j] = found != 0x7fffffff ? found : last;
 }
 
+#ifndef NFROM
+#define NFROM (12 << 20)
+#endif
+constexpr int64_t kNarrowFrom = NFROM;
+
 int64_t segments(int64_t V) { return (V + kSeg - 1) / kSeg; }
 
 }  // namespace
@@ -382,7 +472,7 @@ using namespace q36;
 extern "C" size_t q36_verify_drafts_workspace_bytes(int32_t B, int32_t T, int32_t V) {
   if (B < 1 || T < 1 || T > kMaxT || V < 1) return 0;
   const size_t s = (size_t)segments(V);
-  return align_up((size_t)B * T * s * 8, 256) + 2 * align_up((size_t)B * T * s * 4, 256) + align_up((size_t)B * s * 8, 256);
+  return align_up((size_t)B * T * s * 8, 256) + 2 * align_up((size_t)B * T * s * 4, 256) + 2 * align_up((size_t)B * s * 8, 256);
 }
 
 extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t stream) {
@@ -402,18 +492,25 @@ extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t s
   Q36_REQUIRE((int64_t)a->B * a->T * segs < (1ll << 32) / kThreads, "q36_verify_drafts: B x T x V too large");  // a launch's threads
   const size_t n = (size_t)a->B * a->T * segs;
   char* w = static_cast<char*>(a->workspace);
+  const int narrow = kNarrowFrom >= 0 && a->T > 1 && (int64_t)a->B * (a->T - 1) * a->V >= kNarrowFrom;
   DraftsDev d{a->B, a->T, a->V, (int)segs, a->ld, a->logits, a->temperature, a->drafts, a->uniforms,
-              a->T > 1 ? a->draft_probs : nullptr, nullptr, nullptr, nullptr, nullptr, a->tokens, a->counts};
+              a->T > 1 ? a->draft_probs : nullptr, narrow, nullptr, nullptr, nullptr, nullptr, nullptr, a->tokens, a->counts};
   d.psum = reinterpret_cast<double*>(w), w += align_up(n * 8, 256);
   d.pmax = reinterpret_cast<float*>(w), w += align_up(n * 4, 256);
   d.pidx = reinterpret_cast<int32_t*>(w), w += align_up(n * 4, 256);
+  d.esum = reinterpret_cast<double*>(w), w += align_up((size_t)a->B * segs * 8, 256);
   d.rsum = reinterpret_cast<double*>(w);
   // 16 bytes a lane where every row starts at such a boundary
   const bool vec = aligned16(a->logits) && a->ld % (a->logits_f32 ? 4 : 8) == 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto f32, auto v) {
     constexpr bool F = decltype(f32)::value, W = decltype(v)::value;
-    drafts_sums_kernel<F, W><<<(unsigned)n, kThreads, 0, st>>>(d);
+    if (narrow) {
+      drafts_sums_kernel<F, W, false><<<(unsigned)n, kThreads, 0, st>>>(d);
+      drafts_exact_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
+    } else {
+      drafts_sums_kernel<F, W, true><<<(unsigned)n, kThreads, 0, st>>>(d);
+    }
     if (d.probs) drafts_residual_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
     drafts_pick_kernel<F, W><<<a->B, kThreads, 0, st>>>(d);
   };

@@ -199,3 +199,30 @@ def test_drafts_graph_replays(lm, dev):
         got = tok.clone(), n.clone()
         want = lm.verify_drafts(x2, d2, u2, ws, h2, q2)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype,probs,V", [(torch.bfloat16, False, 50001), (torch.float32, True, 50008), (torch.bfloat16, True, 131071)])
+def test_drafts_large_calls(lm, dev, dtype, probs, V):
+    """Calls large enough that the rows' sums are fp32 and the drawn row alone is summed in fp64; some requests greedy."""
+    B, T = 12600000 // (3 * V) + 1, 4
+    print(f"drafts B={B} T={T} V={V} probs={probs} {dtype}", flush=True)
+    x, d, u, heat, q = inputs(B, T, V, dev, V, dtype, probs)
+    heat[::5] = 0.0
+    n = compare(lm, x, d, u, heat, q)
+    assert n.min() < n.max()
+
+
+def test_drafts_numbers_at_the_border(lm, dev):
+    """Numbers within an fp32 step of the drafts' probabilities, on either side, in a call whose sums are fp32: the tests
+    come out as with sums in 64 bits."""
+    B, T, V = 64, 4, 65544
+    x, d, u, heat, _ = inputs(B, T, V, dev, 77)
+    y = x.cpu().double().view(B, T, V) / heat.cpu().double()[:, None, None]
+    p = torch.softmax(y, -1)[:, :-1].gather(-1, d.cpu().long()[..., None])[..., 0]
+    near = p.float()
+    near[::3] = torch.nextafter(near[::3], torch.zeros(()))
+    near[1::3] = torch.nextafter(near[1::3], torch.ones(()))
+    assert float(((near.double() - p).abs() / p).max()) < 2.0 ** -22
+    u[:, :-1] = near.to(dev)
+    n = compare(lm, x, d, u, heat)
+    assert {1, 2} <= set(n.tolist())
