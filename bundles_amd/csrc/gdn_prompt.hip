@@ -7,6 +7,8 @@
 //
 // Everything is formed in fp32 and rounded once.  (The verify kernels round the conv's tap products, its output and o to
 // bf16, as the reference's does.)
+#include <algorithm>
+
 #include "q36_device.h"
 #include "q36_host.h"
 
@@ -14,7 +16,7 @@ namespace q36 {
 namespace {
 
 constexpr int PK = 128, PV = 128, PHK = 16, PHV = 32, PQKV = 8192, PZ = PHV * PV;
-constexpr int kGroup = 8;  // tokens whose conv, norms and gates are formed at once
+constexpr int kGroup = 8;  // tokens whose conv, norms and gates are formed at once, a wave's norm each
 constexpr int kShort = 8;  // requests of up to so many new tokens go token by token, longer ones by chunks
 constexpr int PC = 64;     // tokens of a chunk
 
@@ -172,17 +174,27 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
   for (int i = 0; i < 4; ++i) cw[i] = bf2f(d.conv_w[(int64_t)ch * 4 + i]);
   for (int g0 = 0; g0 < n; g0 += kGroup) {
     const int G = min(kGroup, n - g0);
-    for (int t = 0; t < G; ++t) {
-      const float x = bf2f(d.mixed[(int64_t)(t0 + g0 + t) * PQKV + ch]);
-      float y = w0 * cw[0];
-      y = __builtin_fmaf(w1, cw[1], y);
-      y = __builtin_fmaf(w2, cw[2], y);
-      y = __builtin_fmaf(x, cw[3], y);
-      w0 = w1, w1 = w2, w2 = x;
-      y = silu(y);
-      if (tid < 128) qs[t][tid] = y;
-      else if (tid < 256) ks[t][tid - 128] = y;
-      else vs[t][tid - 256] = y;
+    uint16_t x[kGroup];
+    uint32_t zr[2];  // of the outputs that the wave will norm: token wave of head i, two columns a lane
+#pragma unroll
+    for (int t = 0; t < kGroup; ++t) x[t] = d.mixed[(int64_t)(t0 + g0 + min(t, G - 1)) * PQKV + ch];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      zr[i] = *reinterpret_cast<const uint32_t*>(d.z + (int64_t)(t0 + g0 + min(wave, G - 1)) * PZ + (2 * hk + i) * PV + 2 * lane);
+#pragma unroll
+    for (int t = 0; t < kGroup; ++t) {
+      if (t < G) {
+        const float xt = bf2f(x[t]);
+        float y = w0 * cw[0];
+        y = __builtin_fmaf(w1, cw[1], y);
+        y = __builtin_fmaf(w2, cw[2], y);
+        y = __builtin_fmaf(xt, cw[3], y);
+        w0 = w1, w1 = w2, w2 = xt;
+        y = silu(y);
+        if (tid < 128) qs[t][tid] = y;
+        else if (tid < 256) ks[t][tid - 128] = y;
+        else vs[t][tid - 256] = y;
+      }
     }
     if (tid < 2 * G) {
       const int t = tid >> 1, h = 2 * hk + (tid & 1);
@@ -234,24 +246,22 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
       }
     }
     __syncthreads();
-    for (int p = wave; p < 2 * G; p += 8) {
-      const int t = p >> 1, h = p & 1;
-      const int64_t row = t0 + g0 + t, o = row * PZ + (2 * hk + h) * PV;
-      const float o0 = os[t][h * PV + lane], o1 = os[t][h * PV + lane + 64];
-      const float rstd = 1.f / sqrtf(wave_sum_bfly(o0 * o0 + o1 * o1) / (float)PV + d.eps);
-      const float y0 = o0 * rstd * bf2f(d.norm_w[lane]) * silu(bf2f(d.z[o + lane]));
-      const float y1 = o1 * rstd * bf2f(d.norm_w[lane + 64]) * silu(bf2f(d.z[o + lane + 64]));
-      const uint32_t y = pack_bf2_hw(y0, y1);
-      d.out[o + lane] = (uint16_t)y;
-      d.out[o + lane + 64] = (uint16_t)(y >> 16);
-      if (d.oq) {
-        const float f0 = bf_lo(y), f1 = bf_hi(y);
-        const float m = wave_max(fmaxf(fabsf(f0), fabsf(f1)));
-        const float inv = m > 0.f ? 448.f / m : 0.f;
-        const uint32_t cd = f2e4m3x2_hw(f0 * inv, f1 * inv);
-        d.oq[o + lane] = (uint8_t)(cd & 0xffu);
-        d.oq[o + lane + 64] = (uint8_t)((cd >> 8) & 0xffu);
-        if (lane == 0) d.oqs[row * PHV + 2 * hk + h] = m / 448.f;
+    if (wave < G) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t row = t0 + g0 + wave, o = row * PZ + (2 * hk + h) * PV + 2 * lane;
+        const float o0 = os[wave][h * PV + 2 * lane], o1 = os[wave][h * PV + 2 * lane + 1];
+        const float rstd = 1.f / sqrtf(wave_sum_bfly(o0 * o0 + o1 * o1) / (float)PV + d.eps);
+        const uint32_t nw = reinterpret_cast<const uint32_t*>(d.norm_w)[lane];
+        const uint32_t y = pack_bf2_hw(o0 * rstd * bf_lo(nw) * silu(bf_lo(zr[h])), o1 * rstd * bf_hi(nw) * silu(bf_hi(zr[h])));
+        *reinterpret_cast<uint32_t*>(d.out + o) = y;
+        if (d.oq) {
+          const float f0 = bf_lo(y), f1 = bf_hi(y);
+          const float m = wave_max(fmaxf(fabsf(f0), fabsf(f1)));
+          const float inv = m > 0.f ? 448.f / m : 0.f;
+          *reinterpret_cast<uint16_t*>(d.oq + o) = (uint16_t)f2e4m3x2_hw(f0 * inv, f1 * inv);
+          if (lane == 0) d.oqs[row * PHV + 2 * hk + h] = m / 448.f;
+        }
       }
     }
   }
@@ -618,8 +628,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   __shared__ __attribute__((aligned(16))) _Float16 up[4][16][XS];   // U's; the decayed U's
   __shared__ __attribute__((aligned(16))) float vp[2][16][PC + 4];  // values of a chunk and the next
   __shared__ float most[4];
+  if (many_chunks(d)) return;
   // the 2 BLOCKS workgroups of a (request, key head) on one XCD, where the chunks' operands came from
-  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  for (int item = blockIdx.x; item < d.B * PHK * 2 * BLOCKS; item += gridDim.x) {
+  const int xcd = item & 7, at = item >> 3;
   const int grp = (at / (2 * BLOCKS)) * 8 + xcd, in = at % (2 * BLOCKS);
   const int r = grp / PHK, hk = grp % PHK, hh = in / BLOCKS, hv = 2 * hk + hh, col0 = (in % BLOCKS) * 16;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
@@ -629,7 +641,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   bool old;
   request_of(d, r, t0, n, slot, old);
   t0 = __builtin_amdgcn_readfirstlane(t0), n = __builtin_amdgcn_readfirstlane(n);
-  if (n <= kShort || slot < 0 || many_chunks(d)) return;
+  if (n <= kShort || slot < 0) continue;
+  if (item != (int)blockIdx.x) __syncthreads();  // (another item's last reads of LDS)
   const int chunks = (n + PC - 1) / PC;
   const uint8_t* u = d.units + ((int64_t)first_unit(d, r, t0) * PHK + hk) * kUnit;  // a chunk's operands, then the next's
   constexpr int64_t kNext = (int64_t)PHK * kUnit;
@@ -938,6 +951,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
         const int cc = (i / (3 * PK)) * (PHK * PK) + hk * PK + i / 3 % PK;
         d.conv_state[slot * d.cs_slot + (int64_t)cc * 3 + i % 3] = d.mixed[(int64_t)(t0 + n - 3 + i % 3) * PQKV + cc];
       }
+  }
   }
 }
 
@@ -1253,14 +1267,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
 // The gated norm of the chunks' rows: a wave a row, 16 lanes a head.
 __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptDev d) {
   const int lane = threadIdx.x & 63;
-  const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  if (row >= d.rows) return;
+  if (many_chunks(d)) return;
+  for (int row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); row < d.rows; row += gridDim.x * 4) {
   const int r = last_at_most(d.B, row, [&](int i) { return d.qsl[i]; });
   int t0, n;
   int64_t slot;
   bool old;
   request_of(d, r, t0, n, slot, old);
-  if (n <= kShort || slot < 0 || row < t0 || row >= t0 + n || many_chunks(d)) return;
+  if (n <= kShort || slot < 0 || row < t0 || row >= t0 + n) continue;
   const int c = lane & 15;
   const v4i wr = *reinterpret_cast<const v4i*>(d.norm_w + 8 * c);
   v4i o[8], z[8];
@@ -1279,6 +1293,7 @@ __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptDev d) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = __builtin_ldexpf((float)h[k], ex[i] - 14);
     norm_store(d, row, 4 * i + (lane >> 4), c, x, z[i], wr);
+  }
   }
 }
 
@@ -1336,8 +1351,10 @@ extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream)
       if (rc != Q36_OK) return rc;
       prompt_heads_kernel<<<(unsigned)a->B * PHK * 2, 512, kHeadsLds, st>>>(d);
     }
-    prompt_scan_kernel<<<(unsigned)a->B * PHK * 16, 512, 0, st>>>(d);
-    prompt_norm_kernel<<<(unsigned)(a->rows + 3) / 4, 256, 0, st>>>(d);
+    // (beside the other scan, one of the two finds nothing to do: few workgroups, that it may end soon)
+    const unsigned items = (unsigned)a->B * PHK * 16, quads = (unsigned)(a->rows + 3) / 4;
+    prompt_scan_kernel<<<d.both ? std::min(items, 1024u) : items, 512, 0, st>>>(d);
+    prompt_norm_kernel<<<d.both ? std::min(quads, 2048u) : quads, 256, 0, st>>>(d);
   }
   return check_launch("q36_gdn_prompt");
 }
