@@ -23,6 +23,20 @@ constexpr int kThreads = 256, kPer = 16, kSeg = kThreads * kPer;  // logits a th
 constexpr int kMaxT = 8;
 constexpr double kClose = 0x1p-17;  // of fp32 sums: 4096 terms by 16, 64, 4 and the segments, rounded 2^-24 each time, weights 2^-22
 
+// What a request's rows say: the accepted drafts, and the row the next token is drawn from.
+struct Chain {
+  float m[kMaxT];      // a row's largest logit
+  int idx[kMaxT];      // its first index
+  double norm[kMaxT];  // sum of the row's weights
+  bool wide[kMaxT];    // in fp64
+  double p[kMaxT];     // the draft's weight (its probability, where greedy)
+  double q[kMaxT];     // its draft probability
+  double u[kMaxT];
+  int tok[kMaxT];      // the draft, -1 without one
+  double part[4];
+  int j, refused, ended, close;
+};
+
 struct DraftsDev {
   int B, T, V, segs;
   int64_t ld;
@@ -37,6 +51,7 @@ struct DraftsDev {
   int32_t* pidx;       // [rows, segs] its first index
   double* esum;        // [B, segs] the drawn row's sums in fp64, where psum is not
   double* rsum;        // [B, segs] its residual
+  Chain* chains;  // [B] what a kernel of its own found of the drafts, or null: the pick finds it
   int32_t* tokens;
   int32_t* counts;
 };
@@ -48,7 +63,8 @@ __device__ __forceinline__ double heat_of(const DraftsDev& d, int b) {
 }
 
 // 2^((x - m) s) for x <= m, 1 at x == m whatever m is (an infinite largest logit leaves weight to its equals alone): the
-// fraction's power by its series up to f^9, off by at most (ln 2 / 2)^10 / 10! = 7e-12.
+// fraction's power by its series up to f^9, off by at most (ln 2 / 2)^10 / 10! = 7e-12.  (The whole part by an addition of
+// 1.5 2^52 and on the exponent's bits, in place of rounding, conversion and ldexp: 8 % slower.)
 __device__ __forceinline__ double weight(float x, float m, double s) {
   double y = ((double)x - (double)m) * s;
   y = y > -1100.0 ? y : -1100.0;  // (also NaN: minus infinity below itself, or beside an infinite largest)
@@ -117,6 +133,12 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   return v;
 }
 
+__device__ __forceinline__ int min64(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
+  return v;
+}
+
 // A segment of a row: its largest logit, the first index of it, the sum of its weights.
 template <bool F32, bool VEC, bool WIDE>
 __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
@@ -134,11 +156,13 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
 #pragma unroll
   for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
   m = wave_max(m);
-  int first = 0x7fffffff;
+  int first = 0;
+  if (!(s > 0.0)) {  // (the index says something in greedy requests alone)
+    first = 0x7fffffff;
 #pragma unroll
-  for (int i = kPer - 1; i >= 0; --i) first = x[i] == m ? base + i : first;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o));
+    for (int i = kPer - 1; i >= 0; --i) first = x[i] == m ? base + i : first;
+    first = min64(first);
+  }
   double sum = 0.0;
   if (s > 0.0 && m > -__builtin_inff()) {
     if constexpr (WIDE) {
@@ -148,8 +172,13 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
     } else {
       const float sf = (float)fmin(s, 1e30);  // (weights of a temperature below 1e-30: 1 at the largest, else 0)
       float t = 0.f;
+      if (m < __builtin_inff()) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) t += x[i] == m ? 1.f : __builtin_amdgcn_exp2f(fmaxf((x[i] - m) * sf, -200.f));
+        for (int i = 0; i < kPer; ++i) t += __builtin_amdgcn_exp2f((x[i] - m) * sf);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) t += x[i] == m ? 1.f : 0.f;
+      }
       sum = (double)wave_sum_bfly(t);
     }
   }
@@ -166,26 +195,6 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
     const int64_t o = row * d.segs + seg;
     d.pmax[o] = M, d.psum[o] = S, d.pidx[o] = I;
   }
-}
-
-// What a request's rows say: the accepted drafts, and the row the next token is drawn from.
-struct Chain {
-  float m[kMaxT];      // a row's largest logit
-  int idx[kMaxT];      // its first index
-  double norm[kMaxT];  // sum of the row's weights
-  bool wide[kMaxT];    // in fp64
-  double p[kMaxT];     // the draft's weight (its probability, where greedy)
-  double q[kMaxT];     // its draft probability
-  double u[kMaxT];
-  int tok[kMaxT];      // the draft, -1 without one
-  double part[4];
-  int j, refused, ended, close;
-};
-
-__device__ __forceinline__ int min64(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
-  return v;
 }
 
 // Sum of a row's weights in fp64, by the whole workgroup.
@@ -271,6 +280,22 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
   }
 }
 
+// Large calls, whose segments each need it, have the walk in a kernel of its own (256 requests of 8 rows: 244 -> 190 us with the
+// walk in each of 9728 workgroups taken out).
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void drafts_walk_kernel(DraftsDev d) {
+  __shared__ Chain c;
+  walk<F32, VEC>(d, blockIdx.x, heat_of(d, blockIdx.x), &c);
+  static_assert(sizeof(Chain) % 8 == 0 && sizeof(Chain) / 4 <= kThreads, "a word a thread");
+  if (threadIdx.x < sizeof(Chain) / 4)
+    reinterpret_cast<uint32_t*>(d.chains + blockIdx.x)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&c)[threadIdx.x];
+}
+__device__ __forceinline__ void read_chain(const DraftsDev& d, int b, Chain* c) {
+  if (threadIdx.x < sizeof(Chain) / 4)
+    reinterpret_cast<uint32_t*>(c)[threadIdx.x] = reinterpret_cast<const uint32_t*>(d.chains + b)[threadIdx.x];
+  __syncthreads();
+}
+
 // The drawn row's sum in fp64 from its segments', where it is not: by every wave, the same bits.
 __device__ void widen(const DraftsDev& d, int b, double s, Chain* c) {
   if (!d.narrow || s <= 0.0 || c->ended) return;
@@ -289,7 +314,7 @@ __global__ __launch_bounds__(kThreads) void drafts_exact_kernel(DraftsDev d) {
   const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
   const double s = heat_of(d, b);
   if (!(s > 0.0)) return;
-  walk<F32, VEC>(d, b, s, &c);
+  read_chain(d, b, &c);
   if (c.ended) return;
   float x[kPer];
   load_logits<F32, VEC>(d, (int64_t)b * d.T + c.j, seg * kSeg + tid * kPer, x);
@@ -308,7 +333,7 @@ __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) 
   __shared__ Chain c;
   const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
   const double s = heat_of(d, b);
-  walk<F32, VEC>(d, b, s, &c);
+  read_chain(d, b, &c);
   if (!c.refused) return;
   widen(d, b, s, &c);
   const int j = c.j, base = seg * kSeg + tid * kPer;
@@ -340,7 +365,8 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   __shared__ int found, last;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double s = heat_of(d, b);
-  walk<F32, VEC>(d, b, s, &c);
+  if (d.chains) read_chain(d, b, &c);
+  else walk<F32, VEC>(d, b, s, &c);
   widen(d, b, s, &c);
   const int j = c.j;
   int32_t* const out = d.tokens + (int64_t)b * d.T;
@@ -457,10 +483,9 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   if (tid == 0) out[j] = found != 0x7fffffff ? found : last;
 }
 
-#ifndef NFROM
-#define NFROM (12 << 20)
-#endif
-constexpr int64_t kNarrowFrom = NFROM;
+// Logits behind which fp32 sums pay for two launches more and the drawn row's second reading.  us with fp32 / fp64 sums: 32
+// requests of 4 rows of 151936 (15 M) 39.7 / 35.8, 64 of 5 (39 M) 82 / 98, 256 of 8 (272 M) 187 / 305.
+constexpr int64_t kNarrowFrom = 24 << 20;
 
 int64_t segments(int64_t V) { return (V + kSeg - 1) / kSeg; }
 
@@ -472,7 +497,8 @@ using namespace q36;
 extern "C" size_t q36_verify_drafts_workspace_bytes(int32_t B, int32_t T, int32_t V) {
   if (B < 1 || T < 1 || T > kMaxT || V < 1) return 0;
   const size_t s = (size_t)segments(V);
-  return align_up((size_t)B * T * s * 8, 256) + 2 * align_up((size_t)B * T * s * 4, 256) + 2 * align_up((size_t)B * s * 8, 256);
+  return align_up((size_t)B * T * s * 8, 256) + 2 * align_up((size_t)B * T * s * 4, 256) + 2 * align_up((size_t)B * s * 8, 256) +
+         align_up((size_t)B * sizeof(Chain), 256);
 }
 
 extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t stream) {
@@ -492,14 +518,15 @@ extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t s
   Q36_REQUIRE((int64_t)a->B * a->T * segs < (1ll << 32) / kThreads, "q36_verify_drafts: B x T x V too large");  // a launch's threads
   const size_t n = (size_t)a->B * a->T * segs;
   char* w = static_cast<char*>(a->workspace);
-  const int narrow = kNarrowFrom >= 0 && a->T > 1 && (int64_t)a->B * (a->T - 1) * a->V >= kNarrowFrom;
+  const int narrow = a->T > 1 && (int64_t)a->B * (a->T - 1) * a->V >= kNarrowFrom;
   DraftsDev d{a->B, a->T, a->V, (int)segs, a->ld, a->logits, a->temperature, a->drafts, a->uniforms,
-              a->T > 1 ? a->draft_probs : nullptr, narrow, nullptr, nullptr, nullptr, nullptr, nullptr, a->tokens, a->counts};
+              a->T > 1 ? a->draft_probs : nullptr, narrow, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, a->tokens, a->counts};
   d.psum = reinterpret_cast<double*>(w), w += align_up(n * 8, 256);
   d.pmax = reinterpret_cast<float*>(w), w += align_up(n * 4, 256);
   d.pidx = reinterpret_cast<int32_t*>(w), w += align_up(n * 4, 256);
   d.esum = reinterpret_cast<double*>(w), w += align_up((size_t)a->B * segs * 8, 256);
-  d.rsum = reinterpret_cast<double*>(w);
+  d.rsum = reinterpret_cast<double*>(w), w += align_up((size_t)a->B * segs * 8, 256);
+  if (narrow || d.probs) d.chains = reinterpret_cast<Chain*>(w);
   // 16 bytes a lane where every row starts at such a boundary
   const bool vec = aligned16(a->logits) && a->ld % (a->logits_f32 ? 4 : 8) == 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -507,10 +534,11 @@ extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t s
     constexpr bool F = decltype(f32)::value, W = decltype(v)::value;
     if (narrow) {
       drafts_sums_kernel<F, W, false><<<(unsigned)n, kThreads, 0, st>>>(d);
-      drafts_exact_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
     } else {
       drafts_sums_kernel<F, W, true><<<(unsigned)n, kThreads, 0, st>>>(d);
     }
+    if (d.chains) drafts_walk_kernel<F, W><<<a->B, kThreads, 0, st>>>(d);
+    if (narrow) drafts_exact_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
     if (d.probs) drafts_residual_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
     drafts_pick_kernel<F, W><<<a->B, kThreads, 0, st>>>(d);
   };

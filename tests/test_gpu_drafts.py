@@ -204,7 +204,7 @@ def test_drafts_graph_replays(lm, dev):
 @pytest.mark.parametrize("dtype,probs,V", [(torch.bfloat16, False, 50001), (torch.float32, True, 50008), (torch.bfloat16, True, 131071)])
 def test_drafts_large_calls(lm, dev, dtype, probs, V):
     """Calls large enough that the rows' sums are fp32 and the drawn row alone is summed in fp64; some requests greedy."""
-    B, T = 12600000 // (3 * V) + 1, 4
+    B, T = 25200000 // (3 * V) + 1, 4
     print(f"drafts B={B} T={T} V={V} probs={probs} {dtype}", flush=True)
     x, d, u, heat, q = inputs(B, T, V, dev, V, dtype, probs)
     heat[::5] = 0.0
@@ -215,7 +215,7 @@ def test_drafts_large_calls(lm, dev, dtype, probs, V):
 def test_drafts_numbers_at_the_border(lm, dev):
     """Numbers within an fp32 step of the drafts' probabilities, on either side, in a call whose sums are fp32: the tests
     come out as with sums in 64 bits."""
-    B, T, V = 64, 4, 65544
+    B, T, V = 130, 4, 65544
     x, d, u, heat, _ = inputs(B, T, V, dev, 77)
     y = x.cpu().double().view(B, T, V) / heat.cpu().double()[:, None, None]
     p = torch.softmax(y, -1)[:, :-1].gather(-1, d.cpu().long()[..., None])[..., 0]
