@@ -41,6 +41,16 @@ class GdnPools:
 
 
 @dataclass
+class GdnPrompt:
+    """One recurrent layer's pools for a batch of prompt chunks (q36_gdn_prompt), any number of new tokens a request."""
+    conv_state: torch.Tensor          # bf16 [slots, 8192, 3], updated in place
+    h0: torch.Tensor                  # fp32 [slots, 32, 128, 128], updated in place
+    qsl: torch.Tensor                 # int32 [B + 1] first row of each request
+    state_idx: torch.Tensor           # int32 or int64 [B]: its slot (outside the pools: a padded request)
+    prefix: torch.Tensor | None = None  # int32 [B]: tokens before these (0: from zero states); None: all continue
+
+
+@dataclass
 class KvView:
     """The attention layer's e4m3 KV cache (one-token pages) for one verify batch (q36_attn_decode)."""
     k_cache: torch.Tensor      # uint8 (e4m3 codes) [slots, 2, 256]
@@ -68,6 +78,11 @@ class EngineView:
     """The engine lookups the layer node makes; every method may return None (run stock)."""
 
     def gdn_pools(self, layer_id: int, forward_batch) -> GdnPools | None:
+        return None
+
+    def gdn_prompt(self, layer_id: int, forward_batch) -> GdnPrompt | None:
+        """A batch that gdn_pools does not serve, as prompt chunks (an engine that wants its prompts here says so).  The rings
+        of its requests are empty afterwards: the engine sets their cursors to 0."""
         return None
 
     def kv_view(self, layer_id: int, forward_batch) -> KvView | None:

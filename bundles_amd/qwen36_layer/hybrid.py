@@ -212,10 +212,25 @@ def lm_mode(rows: int, vocab: int) -> str:
     return lm_node.row_mode(rows, vocab)
 
 
+def accept(logits, drafts, uniforms, st: HybridState, ws: lmhead8.VerifyWorkspace, temperature=None, draft_probs=None,
+           stream=None):
+    """What follows a verify step over the rings (forward(..., logits=...)): the drafts against its logits, and what stands
+    committed to every recurrent layer's state.  Returns lmhead8.verify_drafts' (tokens, counts)."""
+    if st.gdn_form != "ring":
+        raise ValueError("hybrid.accept: the recurrent layers' state must be in the ring form")
+    tokens, counts = lmhead8.verify_drafts(logits, drafts, uniforms, ws, temperature=temperature, draft_probs=draft_probs,
+                                           stream=stream)
+    for conv, S, R in zip(st.conv_state, st.S, st.ring):
+        gdn_fused.gdn_ring_commit(conv, R["window"], S, R["d"], R["dlo"], R["k"], R["klo"], R["g"], R["idx"], R["idx"], R["idx"],
+                                  R["wp"], R["cb"], counts, T=st.T, stream=stream)
+    return tokens, counts
+
+
 def forward(x: torch.Tensor, w: HybridWeights, st: HybridState, ws: HybridWorkspace, trace: dict | None = None,
-            stream=None) -> torch.Tensor:
+            stream=None, logits=None) -> torch.Tensor:
     """x bf16 [B*T, 2048] (the embedded tokens) -> greedy ids int32 [B*T].  With trace (a dict), the
-    inputs and outputs of every stage are kept there (copies) for stage-by-stage checks."""
+    inputs and outputs of every stage are kept there (copies) for stage-by-stage checks.  logits (bf16 or fp32 [B*T, V]):
+    receives the lm_head's, as accept reads them."""
     b = ws.bufs
     M = st.B * st.T
     if x.shape != (M, HIDDEN):
@@ -297,7 +312,7 @@ def forward(x: torch.Tensor, w: HybridWeights, st: HybridState, ws: HybridWorksp
     keep("final", h)
     mode = lm_mode(M, w.lm_q.shape[0])
     lmhead8.w8a8_lmhead_argmax(h, w.lm_q if w.lm_qt is None else None, w.lm_s, ws.lmhead, norm_w=None, eps=w.eps,
-                               ids=b["ids"], q_t=w.lm_qt, stream=stream,
+                               ids=b["ids"], q_t=w.lm_qt, stream=stream, logits=logits,
                                two_term=mode == "two_term", w8a16=mode == "w8a16")
     keep("ids", b["ids"])
     return b["ids"]

@@ -9,7 +9,8 @@ served module and its submodule dict untouched.  This node does the same with li
                     batches and deferred finalize run the stock block.
   GDN mixer      <- _replace_gdn_prefill's target-verify branch (L/layer.py:289-309) with
                     gdn_verify_fused (L/gdn_fused.py:37-57): in_proj, the verify over the ReplaySSM ring
-                    with its gated norm, and out_proj, on a verify batch; stock otherwise.  A batch of at
+                    with its gated norm, and out_proj, on a verify batch; where the engine hands a prompt
+                    batch over (gdn_prompt), the same steps over prompt chunks; stock otherwise.  A batch of at
                     most DENSE8_ROWS rows projects through DENSE8 int8 copies of the served weights
                     (W8A16, L/layer.py:13-17, L/dense8_store.py:8-13), wider ones through the e4m3 copies.
   attention      <- attn_fused.install (L/attn_fused.py:213-273): the q/gate/k/v projection with the q/k
@@ -113,6 +114,28 @@ class _ChunkScratch(_Scratch):
         self.attn = attn_fused.Workspace(rows, device)
 
 
+class _PromptScratch(_Scratch):
+    """The same for the recurrent layers' prompt chunks, whose workspace grows with the requests too."""
+
+    _by_device: dict = {}
+
+    @classmethod
+    def get(cls, device, rows: int, B: int = 64):
+        sets = cls._by_device.setdefault(device, [])
+        if not sets or sets[-1].rows < rows or sets[-1].B < B:
+            more, many = (sets[-1].rows, sets[-1].B) if sets else (MAX_TOKENS, 64)
+            if rows > more:
+                more = max(rows, min(2 * more, MAX_ROWS) if sets else more)
+            sets.append(cls(device, more, many if B <= many else max(B, 2 * many)))
+        return sets[-1]
+
+    def __init__(self, device, rows: int, B: int):
+        self.rows, self.B = rows, B
+        self.lin2048 = LinearWorkspace(rows, HIDDEN, device)
+        self.lin4096 = LinearWorkspace(rows, PROJ_IN, device)
+        self.prompt = gdn_fused.PromptWorkspace(rows, B, device)
+
+
 # ---- MoE ---------------------------------------------------------------------------------------------
 class _MoeNode:
     """The replica's private MoE block: row batches on libq36, the rest on stock."""
@@ -186,6 +209,12 @@ def _tiled_dense8(w: torch.Tensor):
     return tile_w16(q), s
 
 
+def _gives_prompts(engine) -> bool:
+    """Whether an engine has a gdn_prompt of its own (EngineView's takes no batch)."""
+    view = getattr(engine, "gdn_prompt", None)
+    return view is not None and getattr(view, "__func__", None) is not EngineView.gdn_prompt
+
+
 def gdn_layer_refusal(core, norm) -> str | None:
     """Why the ring verify cannot serve this recurrent layer (None: it can): the layer half of the
     reference's served-layout check (L/gdn_fused.py:30-34), a bias-free SiLU conv and the swish-gated
@@ -202,7 +231,8 @@ def gdn_layer_refusal(core, norm) -> str | None:
 
 class _GdnMixer:
     """The recurrent mixer's target-verify step: in_proj (e4m3 blocks, columns split q|k|v, z, b, a),
-    q36_gdn_verify_ring over the engine's pools (conv, delta rule, ring appends, gated norm), out_proj."""
+    q36_gdn_verify_ring over the engine's pools (conv, delta rule, ring appends, gated norm), out_proj.  Prompt chunks, where
+    the engine hands them over (gdn_prompt): q36_gdn_prompt in its place."""
 
     def __init__(self, lin, replica_lin, engine: EngineView, max_tokens: int, dense8_rows: int = DENSE8_ROWS):
         w_qkvz, w_ba, w_out = lin.in_proj_qkvz.weight, lin.in_proj_ba.weight, lin.out_proj.weight
@@ -234,6 +264,43 @@ class _GdnMixer:
             # in the W8A16 kernel's tile order (1 KB contiguous loads; the same results)
             self.in8 = _tiled_dense8(w_in) if self.dense8_rows > 0 else None
             self.out8 = _tiled_dense8(w_out.contiguous()) if self.dense8_rows > 0 else None
+        # prompt batches may be captured first of all: their workspaces are there before
+        if self.refusal is None and _gives_prompts(engine):
+            _PromptScratch.get(w_in.device, MAX_TOKENS)
+
+    def _prompt(self, hidden_states, forward_batch):
+        """Prompt chunks, where the engine hands them over (gdn_prompt): in_proj, q36_gdn_prompt, out_proj."""
+        x = hidden_states
+        rows = x.shape[0] if isinstance(x, torch.Tensor) and x.dim() == 2 else 0
+        view = getattr(self.engine, "gdn_prompt", None)
+        p = (view(self.layer_id, forward_batch)
+             if view is not None and self.refusal is None and 0 < rows <= MAX_ROWS and x.dtype == torch.bfloat16 else None)
+        if p is None:
+            return self.stock(self.replica, hidden_states, forward_batch)
+        sc = _PromptScratch.get(x.device, rows, p.qsl.numel() - 1)
+        x = x.contiguous()
+        e = dict(dtype=torch.bfloat16, device=x.device)
+        mixed, z = torch.empty((rows, GDN_QKV), **e), torch.empty((rows, GDN_Z), **e)
+        b, a = torch.empty((rows, GDN_HV), **e), torch.empty((rows, GDN_HV), **e)
+        segs = [(0, mixed), (GDN_QKV, z), (GDN_QKV + GDN_Z, b), (GDN_QKV + GDN_Z + GDN_HV, a)]
+        dense8 = rows <= self.dense8_rows
+        if dense8:
+            dense8_linear(x, *self.in8, segments=segs, tiled=True)
+        else:
+            fp8_linear(x, self.in_proj, sc.lin2048, segments=segs)
+        # (rows of no request stay zero)
+        core, oq = torch.zeros((rows, GDN_Z), **e), None
+        if not dense8:
+            oq = linear_rows(rows, PROJ_IN, x.device)
+            oq.codes.zero_(), oq.scales.zero_()
+        gdn_fused.gdn_prompt(mixed, z, a, b, p.conv_state, self.conv_w, self.A_log, self.dt_bias, p.h0, p.qsl, p.state_idx,
+                             self.norm_w, sc.prompt, self.eps, self.scale, prefix=p.prefix, out=core, oq=oq)
+        out = torch.empty((rows, HIDDEN), **e)
+        if dense8:
+            dense8_linear(core, *self.out8, segments=[(0, out)], tiled=True)
+        else:
+            fp8_linear(core, self.out_proj, sc.lin4096, segments=[(0, out)], xq=oq)
+        return out
 
     def __call__(self, hidden_states, forward_batch):
         x = hidden_states
@@ -242,7 +309,7 @@ class _GdnMixer:
                  if self.refusal is None and verify_batch(forward_batch) and 0 < rows <= self.max_tokens
                  and x.dtype == torch.bfloat16 else None)
         if pools is None or rows % pools.draft:
-            return self.stock(self.replica, hidden_states, forward_batch)
+            return self._prompt(hidden_states, forward_batch)
         sc = _Scratch.get(x.device, rows)
         x = x.contiguous()
         e = dict(dtype=torch.bfloat16, device=x.device)
