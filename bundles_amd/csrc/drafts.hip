@@ -11,6 +11,10 @@
 // good to 7e-12): with fp32 weights one draw in a few hundred would land on a neighbour.  That is so of the row drawn from
 // alone.  In a large call the other rows' sums are fp32, good to 2^-19, which the drafts' tests can do with: a test as close to
 // its border as 2^-17 sums its row again in fp64.
+//
+// Reading the logits once bounds a large call: 256 requests of 8 rows of 151936 (622 MB) 180 us, of them 131 in the sums (4.75
+// TB/s), 38 in the drawn rows' second reading, 12 and 7 in the pick and the walk.  A small one is bound by its two launches
+// and the latencies in them: one row 19 us.
 #include <type_traits>
 
 #include "q36_device.h"
@@ -280,8 +284,8 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
   }
 }
 
-// Large calls, whose segments each need it, have the walk in a kernel of its own (256 requests of 8 rows: 244 -> 190 us with the
-// walk in each of 9728 workgroups taken out).
+// Large calls, whose segments each need it, have the walk in a kernel of its own (256 requests of 8 rows: 180 us,
+// 244 with the walk in each of 9728 workgroups).
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void drafts_walk_kernel(DraftsDev d) {
   __shared__ Chain c;
@@ -484,7 +488,7 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
 }
 
 // Logits behind which fp32 sums pay for two launches more and the drawn row's second reading.  us with fp32 / fp64 sums: 32
-// requests of 4 rows of 151936 (15 M) 39.7 / 35.8, 64 of 5 (39 M) 82 / 98, 256 of 8 (272 M) 187 / 305.
+// requests of 4 rows of 151936 (15 M) 39.7 / 35.8, 64 of 5 (39 M) 80 / 98, 256 of 8 (272 M) 180 / 305.
 constexpr int64_t kNarrowFrom = 24 << 20;
 
 int64_t segments(int64_t V) { return (V + kSeg - 1) / kSeg; }

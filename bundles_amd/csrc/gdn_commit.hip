@@ -5,7 +5,8 @@
 //   n = write_pos + accepted; conv_state = window[:, accepted - 1 .. accepted + 1]
 //   n + room > 16:  h0 <- e^{G_n} h0 + sum_{c < n} e^{G_n - G_c} (d + dlo)_c (k + klo)_c^T,  G_c = g_0 + .. + g_c
 //
-// Bytes bound it: a folded request moves 4 MB of checkpoint and up to 0.4 MB of ring, the others 0.15 MB.
+// Bytes bound it: a folded request moves 4 MB of checkpoint and up to 0.4 MB of ring, the others 0.15 MB.  256 requests of 8
+// drafts (597 MB): 133 us, 4.5 TB/s (a copy moves 4.75).
 #include "q36_device.h"
 #include "q36_host.h"
 

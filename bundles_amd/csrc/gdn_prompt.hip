@@ -133,6 +133,8 @@ __device__ __forceinline__ float silu(float x) { return x / (1.f + expf_q(-x)); 
 // log(1 + e^x)
 __device__ __forceinline__ float softplus(float x) { return x > 20.f ? x : log1pf(expf_q(x)); }
 
+// Requests of few tokens, and padded ones.  The state's way in and out bounds it (4 MB a request; five requests of one token 4.6
+// us), and behind it about 1.5 us a token.
 // One 512-thread workgroup a (request, key head): both value heads' states in registers, rows (tid / 8) + 64 j (head j / 2),
 // columns 32 jj + 4 (tid % 8) .. + 3; a row's dot is 16 local fma and three steps over its 8 threads.
 __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
@@ -282,12 +284,13 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
 // registers, by whole heads, whose gated norm is in it, or, where requests are few, by 16 value columns of a head, and another
 // applies the norm.
 //
-// Products are of fp16 operands in two parts (x = hi + lo / 2^11, three products: 22 bits), in fp32 sums, so the state keeps
+// Products are of fp16 operands in two parts (x = hi + lo, three products: 22 bits), in fp32 sums, so the state keeps
 // fp32's accuracy at a third of the fp16 rate, where the fp32 matrix instruction has a sixteenth.  The output, though bf16,
 // needs them too: where the state is of nearly one key, a row hangs on one q . k that may be small beside |q| |k|, or on a sum
 // of U that nearly cancels, and the norm brings the row back to size (high parts alone: rows 8 % off, 0.1 % elsewhere).
 
-// q, k of a chunk for one key head; T, P and gates of its two value heads.
+// q, k of a chunk for one key head; T, P and gates of its two value heads.  Its writes bound it: 147 KB a chunk and key head, 600
+// MB for 16 prompts of 1000 tokens in 165 us (3.7 TB/s; a copy moves 4.75).
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void prompt_chunks_kernel(PromptDev d) {
   constexpr int RS = PK + 8, MS = PC + 4;  // padded rows, in elements
   __shared__ __attribute__((aligned(16))) _Float16 planes[2][2][PC][RS];  // [q, k][hi, lo]; later A and P
@@ -591,8 +594,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int byte
 }
 
 // Whether the batch's longest request has at most a quarter of its chunks: whole heads then fill the chip.  One request's
-// chunks follow each other, 2.0 us each where a workgroup has 16 columns of a head and 4.9 where it has all, which then costs
-// 2.1 times less in all: 16 prompts of 1000 tokens 588 us by columns and 344 by heads, one of 8192 424 and 800.
+// chunks follow each other, 2.2 us each where a workgroup has 16 columns of a head and 10 where it has all eight times as many.
+// A call by columns / by heads, us: 16 prompts of 1000 tokens 926 / 484, 24 of 1 to 900 279 / 248, one of
+// 8192 407 / 1120.
 __device__ __forceinline__ bool many_chunks(const PromptDev& d) {
   if (!d.both) return false;
   int sum = 0, most = 0;
@@ -620,7 +624,9 @@ __device__ __forceinline__ float all_max(float m) { return __uint_as_float(wave_
 // A request's chunks for 16 value columns of a head.  Waves 0-3 carry the state: wave w holds key dims 32 w .. + 31 of it
 // and token tile w of X and U.  Waves 4-7, one beside each of them on its SIMD, convolve the next chunk's values and form the
 // outputs of token tile w - 4, from the same parts in LDS; so the chain from state to state has only its own work in it.
-// State, X and U pass through LDS as fp16 parts, in the order of an operand's depth.
+// State, X and U pass through LDS as fp16 parts, in the order of an operand's depth.  The chain bounds it, 2.2 us a chunk (280 us
+// for one prompt of 8192 tokens): four dependent products and what lies between them through LDS 1.25 us, the rest loads that
+// arrive later than that.
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_scan_kernel(PromptDev d) {
   constexpr int BLOCKS = PV / 16, SS = PK + 8, XS = PC + 8;
   __shared__ __attribute__((aligned(16))) _Float16 sp[2][16][SS];   // the state's parts
@@ -974,8 +980,10 @@ constexpr int kHeadsLds = kLOut + PC * kOutRow * 4;
 // A request's chunks for a whole value head, 16 columns a wave.  A wave's columns need nothing of another's: it holds their
 // state (lane (c, g): column c, dims 16 t + 4 g + q), and each product's registers, rounded to two parts, are the next one's
 // operand.  What the waves share are the chunk's other operands, in LDS: K and Q of the next chunk arrive while T, P and K^T
-// are used, and the other way round, with a barrier at either change.
-//
+// are used, and the other way round, with a barrier at either change.  16 prompts of 1000 tokens: 340 us, 10 a chunk.  A chunk
+// of a head reads 1.12 MB of LDS (8700 clk at 128 bytes), has 10000 clk of vector instructions a SIMD (the splitting into parts
+// most of it) and 5800 of matrix instructions, at two waves a SIMD little of it beside each other; 72 us are the operands' way
+// into LDS.  (32 columns a wave read half of LDS but do not fit the registers: 570 for 484 us a call.)
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_heads_kernel(PromptDev d) {
   constexpr int W = 8;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -1264,7 +1272,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   wait_vm0();  // (copies of the last chunk's operands again may be on their way into this workgroup's LDS)
 }
 
-// The gated norm of the chunks' rows: a wave a row, 16 lanes a head.
+// The gated norm of the chunks' rows: a wave a row, 16 lanes a head.  8192 rows in 35 us, 24 KB each: 5.7 TB/s, some of it from
+// the cache.
 __global__ __launch_bounds__(256) void prompt_norm_kernel(PromptDev d) {
   const int lane = threadIdx.x & 63;
   if (many_chunks(d)) return;

@@ -218,6 +218,8 @@ def accept(logits, drafts, uniforms, st: HybridState, ws: lmhead8.VerifyWorkspac
     committed to every recurrent layer's state.  Returns lmhead8.verify_drafts' (tokens, counts)."""
     if st.gdn_form != "ring":
         raise ValueError("hybrid.accept: the recurrent layers' state must be in the ring form")
+    if tuple(uniforms.shape) != (st.B, st.T):
+        raise ValueError(f"hybrid.accept: uniforms {tuple(uniforms.shape)} are not [{st.B}, {st.T}]")
     tokens, counts = lmhead8.verify_drafts(logits, drafts, uniforms, ws, temperature=temperature, draft_probs=draft_probs,
                                            stream=stream)
     for conv, S, R in zip(st.conv_state, st.S, st.ring):

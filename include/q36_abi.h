@@ -31,6 +31,8 @@
  *                         format the configuration asks for)
  *   q36_pack_frag8     <- (no reference counterpart: a prepare-time reordering of the 8-bit
  *                         weights into the operand order of the gfx950 MFMA)
+ *   q36_gdn_prompt, q36_verify_drafts, q36_gdn_ring_commit <- (no reference counterpart: its serving engine runs the recurrent
+ *                         layers' prompts, samples behind a verify step and commits what stands)
  */
 #ifndef Q36_ABI_H
 #define Q36_ABI_H
@@ -324,6 +326,8 @@ int q36_gdn_ring_commit(const q36_gdn_commit_args* a, q36_stream_t stream);
  * beta = sigmoid(b), S <- e^g S, u = beta (v - S k), S <- S + u k^T, o = S q, out = bf16(o rsqrt(mean o^2 + eps) norm_w
  * silu(z)), formed in fp32 and rounded once.  (The verify entries round the conv's tap products, its output and o
  * to bf16.)  oq / oqs (optional): out's e4m3 codes and scales as q36_gdn_ring_args'.
+ * Values and states up to 2^50 (their outputs are squared in fp32); beyond, and with infinities or NaN, what comes out of that head of that request says nothing
+ * (other heads and requests keep theirs).
  * A request without rows is left as it is; a slot outside [0, slots) marks a padded request: zero rows, nothing else
  * written.  Rows of no request are left as they were.  Requests with rows must name distinct slots.  Whatever the device data
  * hold, every access stays inside the buffers.
@@ -712,7 +716,9 @@ int q36_lmhead_argmax(const q36_lmhead_args* a, q36_stream_t stream);
  * p where that leaves nothing; where no draft is refused, of p.  T = 1: a token is drawn.  tokens int32 [B, T]: the drafts that stand,
  * that token, -1 behind; counts int32 [B]: how many.
  * NaN logits count as minus infinity; logits of plus infinity share the row.  A row of minus infinity alone leaves no token:
- * it ends its request, count without one more.  Weights and sums in fp64 (a weight within 7e-12 of itself).
+ * it ends its request, count without one more.  The drawn row's weights and sums in fp64 (a
+ * weight within 7e-12 of itself), the others' in fp64 or, in large calls, fp32, their tests within 2^-17 of the border again
+ * in fp64.
  * 1 <= T <= 8, B <= 65535, V <= 2^24, B T ceil(V / 4096) < 2^24.  Workspace: q36_verify_drafts_workspace_bytes(B, T, V), 256-byte aligned, any contents. */
 typedef struct q36_verify_drafts_args {
   int32_t B, T, V, logits_f32;

@@ -226,3 +226,34 @@ def test_drafts_numbers_at_the_border(lm, dev):
     u[:, :-1] = near.to(dev)
     n = compare(lm, x, d, u, heat)
     assert {1, 2} <= set(n.tolist())
+
+
+def test_drafts_large_graph_and_two_streams(lm, dev):
+    """The large form replayed with new values, and beside another call on a stream and workspace of its own."""
+    B, T, V = 130, 4, 65544
+    x, d, u, heat, _ = inputs(B, T, V, dev, 78)
+    ws = lm.VerifyWorkspace(B, T, V, dev)
+    tok, n = torch.empty((B, T), dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.int32, device=dev)
+    lm.verify_drafts(x, d, u, ws, heat, None, tok, n)
+    first = tok.clone(), n.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        lm.verify_drafts(x, d, u, ws, heat, None, tok, n)
+    seen = []
+    for k in range(3):
+        u.copy_(torch.rand((B, T), generator=torch.Generator().manual_seed(k)))
+        ws.buf.fill_(0xFF)
+        g.replay()
+        torch.cuda.synchronize()
+        seen.append((u.clone(), tok.clone(), n.clone()))
+        want = lm.verify_drafts(x, d, u, lm.VerifyWorkspace(B, T, V, dev), heat)
+        assert torch.equal(tok, want[0]) and torch.equal(n, want[1])
+    assert not torch.equal(seen[0][1], first[0])
+    spaces, streams, got = [lm.VerifyWorkspace(B, T, V, dev) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        got.append(lm.verify_drafts(x, d, seen[i][0], spaces[i], heat, stream=streams[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(got[i][0], seen[i][1]) and torch.equal(got[i][1], seen[i][2])

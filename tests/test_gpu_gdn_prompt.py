@@ -285,3 +285,72 @@ def test_prompt_hostile_row_starts(gdn, dev):
     f["qsl"] = torch.tensor([-(1 << 31), 60, 10], dtype=torch.int32, device=dev)
     out = call(gdn, f, out=torch.zeros_like(out))
     assert torch.equal(out[:60], good[:60]) and not bool(out[60:].any())
+
+
+def codes_of(out):
+    """The e4m3 codes and scales of an output's rows, by head (exact divisions, on the CPU)."""
+    y = out.float().view(-1, HV, D).cpu()
+    m = y.abs().amax(-1)
+    inv = torch.where(m > 0, torch.full_like(m, 448) / m, torch.zeros_like(m))
+    return (y * inv[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8), m / 448
+
+
+# from four requests on, batches of even lengths go by whole heads, a long request among short ones by columns
+@pytest.mark.parametrize("lens", [[100] * 4, [65, 64, 66, 80, 9], [9] * 6, [63, 129, 128, 127, 64, 1, 0, 8, 192, 200], [700, 1, 9, 20, 3, 64],
+                                  [17] * 300])
+@pytest.mark.parametrize("size", [1.0, 3e4])
+def test_prompt_four_requests_and_more(gdn, dev, lens, size):
+    from bundles_amd.qwen36_layer.glue import linear_rows
+    n, B = sum(lens), len(lens)
+    print(f"prompt of {B} requests {lens[:10]} size={size}", flush=True)
+    f = inputs(lens, dev, 50 + n + B, tuple(range(0, B, 3)), rows=n + 5, pad=16)
+    f["mixed"][:, 2 * HK * D:] = (f["mixed"][:, 2 * HK * D:].float() * size).to(torch.bfloat16)
+    f["mixed"][n:], f["z"][n:], f["a"][n:], f["b"][n:] = (float("nan") for _ in range(4))  # rows of no request
+    f["state_idx"][1] = B + 3  # padded
+    out = torch.full((n + 5, HV * D), 7.0, dtype=torch.bfloat16, device=dev)
+    oq = linear_rows(n + 5, 4096, dev)
+    want = plain(f, out)
+    call(gdn, f, out=out, oq=oq)
+    check(out, f, want)
+    assert bool((out[n:] == 7.0).all())
+    codes, scales = codes_of(out[:n])
+    assert torch.equal(oq.codes.view(torch.uint8).view(-1, HV, D)[:n].cpu(), codes)
+    assert torch.equal(oq.scales.view(-1, HV)[:n].cpu(), scales)
+
+
+def test_prompt_replays_from_one_rule_to_the_other(gdn, dev):
+    """One captured call whose lengths change between batches that go by heads and by columns."""
+    f = inputs([60] * 5, dev, 61, (1,), rows=320)
+    ws = gdn.PromptWorkspace(320, 5, dev)
+    out = torch.zeros((320, HV * D), dtype=torch.bfloat16, device=dev)
+    call(gdn, f, ws, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(gdn, f, ws, out=out)
+    for step, lens in enumerate([[60] * 5, [300, 1, 1, 1, 9], [64] * 5, [0, 0, 320, 0, 0], [1] * 5, [8, 9, 100, 70, 65]]):
+        n = inputs(lens, dev, 70 + step, (step % 5,), rows=320)
+        for k, t in n.items():
+            f[k].copy_(t)
+        out.zero_()
+        ws.buf.fill_(0x7F)
+        g.replay()
+        torch.cuda.synchronize()
+        eager = call(gdn, n, out=torch.zeros_like(out))
+        assert torch.equal(out, eager) and torch.equal(f["h0"], n["h0"]) and torch.equal(f["conv_state"], n["conv_state"])
+
+
+def test_prompt_two_streams(gdn, dev):
+    """Two calls at once, on streams and workspaces of their own, beside each other's results."""
+    fs = [inputs(lens, dev, 80 + i, (0,)) for i, lens in enumerate(([900, 30], [70] * 8))]
+    alone = [{k: v.clone() for k, v in f.items()} for f in fs]
+    wants = [call(gdn, f) for f in alone]
+    spaces = [gdn.PromptWorkspace(f["mixed"].shape[0], len(f["state_idx"]), dev) for f in fs]
+    outs = [torch.empty_like(w) for w in wants]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in fs]
+    for f, ws, o, s in zip(fs, spaces, outs, streams):
+        call(gdn, f, ws, out=o, stream=s)
+    torch.cuda.synchronize()
+    for f, a, o, w in zip(fs, alone, outs, wants):
+        assert torch.equal(o, w) and torch.equal(f["h0"], a["h0"]) and torch.equal(f["conv_state"], a["conv_state"])
