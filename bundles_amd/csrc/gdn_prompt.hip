@@ -16,7 +16,6 @@ namespace q36 {
 namespace {
 
 constexpr int PK = 128, PV = 128, PHK = 16, PHV = 32, PQKV = 8192, PZ = PHV * PV;
-constexpr int kGroup = 8;  // tokens whose conv, norms and gates are formed at once, a wave's norm each
 constexpr int kShort = 8;  // requests of up to so many new tokens go token by token, longer ones by chunks
 constexpr int PC = 64;     // tokens of a chunk
 
@@ -119,6 +118,12 @@ __device__ __forceinline__ void split4(v4f x, v4h& hi, v4h& lo) {
   }
 }
 
+// A buffer of `bytes` at p (the same in every lane): loads behind its end give 0, stores there are dropped.  (What may lie
+// behind the end is told by the lane's offset alone: the check subtracts the scalar offset from the size, unsigned.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
+}
+
 __device__ __forceinline__ float fast_silu(float x) {
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
@@ -137,12 +142,17 @@ __device__ __forceinline__ float softplus(float x) { return x > 20.f ? x : log1p
 // us), and behind it about 1.5 us a token.
 // One 512-thread workgroup a (request, key head): both value heads' states in registers, rows (tid / 8) + 64 j (head j / 2),
 // columns 32 jj + 4 (tid % 8) .. + 3; a row's dot is 16 local fma and three steps over its 8 threads.
-__global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
-  __shared__ __attribute__((aligned(16))) float qs[kGroup][PK], ks[kGroup][PK];
-  __shared__ float vs[kGroup][2 * PV], os[kGroup][2 * PV];
-  __shared__ float eg[kGroup][2], beta[kGroup][2];
-  const int r = blockIdx.x / PHK, hk = blockIdx.x % PHK;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+struct StepsLds {
+  float qs[kShort][PK], ks[kShort][PK];
+  float vs[kShort][2 * PV], os[kShort][2 * PV];
+  float eg[kShort][2], beta[kShort][2];
+};
+__device__ __forceinline__ void steps(const PromptDev& d, int block, StepsLds& lds) {
+  auto &qs = lds.qs, &ks = lds.ks;
+  auto &vs = lds.vs, &os = lds.os;
+  auto &eg = lds.eg, &beta = lds.beta;
+  const int r = block / PHK, hk = block % PHK;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int t0, n;
   int64_t slot;
   bool old;
@@ -160,13 +170,21 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
     return;
   }
   const int r0 = tid >> 3, c8 = tid & 7;
-  float* const hp = d.h0 + (slot * PHV + 2 * hk) * (int64_t)(PV * PK);
+  const __amdgpu_buffer_rsrc_t hb = buffer(d.h0 + (slot * PHV + 2 * hk) * (int64_t)(PV * PK), 2 * PV * PK * 4);
+  const int hat = (r0 * PK + 4 * c8) * 4;
   v4f st[4][4];
+  if (old) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj)
-      st[j][jj] = old ? *reinterpret_cast<const v4f*>(hp + (r0 + 64 * j) * PK + 32 * jj + 4 * c8) : v4f{0.f, 0.f, 0.f, 0.f};
+      for (int jj = 0; jj < 4; ++jj)
+        st[j][jj] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(hb, hat + 128 * jj, 64 * j * PK * 4, 0));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) st[j][jj] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
   // one conv channel a thread: q and k of the key head, v of its value heads
   const int ch = tid < 256 ? (tid >> 7) * (PHK * PK) + hk * PK + (tid & 127) : 2 * PHK * PK + hk * 2 * PV + (tid - 256);
   uint16_t* const cs = d.conv_state + slot * d.cs_slot + (int64_t)ch * 3;
@@ -174,106 +192,118 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
   float cw[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) cw[i] = bf2f(d.conv_w[(int64_t)ch * 4 + i]);
-  for (int g0 = 0; g0 < n; g0 += kGroup) {
-    const int G = min(kGroup, n - g0);
-    uint16_t x[kGroup];
-    uint32_t zr[2];  // of the outputs that the wave will norm: token wave of head i, two columns a lane
+  const __amdgpu_buffer_rsrc_t mb = buffer(d.mixed + (int64_t)t0 * PQKV, n * PQKV * 2);  // (rows behind it: 0)
+  uint16_t x[kShort];
 #pragma unroll
-    for (int t = 0; t < kGroup; ++t) x[t] = d.mixed[(int64_t)(t0 + g0 + min(t, G - 1)) * PQKV + ch];
+  for (int t = 0; t < kShort; ++t) x[t] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(mb, ch * 2 + t * PQKV * 2, 0, 0);
+  uint32_t zr[2];  // of the outputs that the wave will norm: token wave of head i, two columns a lane
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      zr[i] = *reinterpret_cast<const uint32_t*>(d.z + (int64_t)(t0 + g0 + min(wave, G - 1)) * PZ + (2 * hk + i) * PV + 2 * lane);
+  for (int i = 0; i < 2; ++i)
+    zr[i] = *reinterpret_cast<const uint32_t*>(d.z + (int64_t)(t0 + min(wave, n - 1)) * PZ + (2 * hk + i) * PV + 2 * lane);
 #pragma unroll
-    for (int t = 0; t < kGroup; ++t) {
-      if (t < G) {
-        const float xt = bf2f(x[t]);
-        float y = w0 * cw[0];
-        y = __builtin_fmaf(w1, cw[1], y);
-        y = __builtin_fmaf(w2, cw[2], y);
-        y = __builtin_fmaf(xt, cw[3], y);
-        w0 = w1, w1 = w2, w2 = xt;
-        y = silu(y);
-        if (tid < 128) qs[t][tid] = y;
-        else if (tid < 256) ks[t][tid - 128] = y;
-        else vs[t][tid - 256] = y;
-      }
+  for (int t = 0; t < kShort; ++t) {
+    if (t < n) {
+      const float xt = bf2f(x[t]);
+      float y = w0 * cw[0];
+      y = __builtin_fmaf(w1, cw[1], y);
+      y = __builtin_fmaf(w2, cw[2], y);
+      y = __builtin_fmaf(xt, cw[3], y);
+      w0 = w1, w1 = w2, w2 = xt;
+      y = silu(y);
+      if (tid < 128) qs[t][tid] = y;
+      else if (tid < 256) ks[t][tid - 128] = y;
+      else vs[t][tid - 256] = y;
     }
-    if (tid < 2 * G) {
-      const int t = tid >> 1, h = 2 * hk + (tid & 1);
-      const int64_t o = (int64_t)(t0 + g0 + t) * PHV + h;
-      const float dt = d.dt_f32 ? static_cast<const float*>(d.dt_bias)[h] : bf2f(static_cast<const uint16_t*>(d.dt_bias)[h]);
-      eg[t][tid & 1] = expf_q(-expf_q(d.A_log[h]) * softplus(bf2f(d.a[o]) + dt));
-      beta[t][tid & 1] = sigmoid_q(bf2f(d.b[o]));
-    }
-    __syncthreads();
-    for (int p = wave; p < 2 * G; p += 8) {
-      float* x = (p & 1) ? ks[p >> 1] : qs[p >> 1];
-      const float a0 = x[lane], a1 = x[lane + 64];
-      float rr = 1.f / sqrtf(wave_sum_bfly(a0 * a0 + a1 * a1) + 1e-6f);
-      if (!(p & 1)) rr = rr * d.scale;
-      x[lane] = a0 * rr;
-      x[lane + 64] = a1 * rr;
-    }
-    __syncthreads();
-    for (int t = 0; t < G; ++t) {
-      v4f kk[4], qq[4];
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
-        kk[jj] = *reinterpret_cast<const v4f*>(&ks[t][32 * jj + 4 * c8]);
-        qq[jj] = *reinterpret_cast<const v4f*>(&qs[t][32 * jj + 4 * c8]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = eg[t][j >> 1];
-        float kv = 0.f, ov = 0.f;
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) kv = __builtin_fmaf(st[j][jj][i], kk[jj][i], kv);
-        kv = kv + lane_xor<1>(kv);
-        kv = kv + lane_xor<2>(kv);
-        kv = kv + lane_xor<4>(kv);
-        const float u = beta[t][j >> 1] * (vs[t][r0 + 64 * j] - e * kv);
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            st[j][jj][i] = __builtin_fmaf(e, st[j][jj][i], u * kk[jj][i]);
-            ov = __builtin_fmaf(st[j][jj][i], qq[jj][i], ov);
-          }
-        ov = ov + lane_xor<1>(ov);
-        ov = ov + lane_xor<2>(ov);
-        ov = ov + lane_xor<4>(ov);
-        if (c8 == 0) os[t][r0 + 64 * j] = ov;
-      }
-    }
-    __syncthreads();
-    if (wave < G) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t row = t0 + g0 + wave, o = row * PZ + (2 * hk + h) * PV + 2 * lane;
-        const float o0 = os[wave][h * PV + 2 * lane], o1 = os[wave][h * PV + 2 * lane + 1];
-        const float rstd = 1.f / sqrtf(wave_sum_bfly(o0 * o0 + o1 * o1) / (float)PV + d.eps);
-        const uint32_t nw = reinterpret_cast<const uint32_t*>(d.norm_w)[lane];
-        const uint32_t y = pack_bf2_hw(o0 * rstd * bf_lo(nw) * silu(bf_lo(zr[h])), o1 * rstd * bf_hi(nw) * silu(bf_hi(zr[h])));
-        *reinterpret_cast<uint32_t*>(d.out + o) = y;
-        if (d.oq) {
-          const float f0 = bf_lo(y), f1 = bf_hi(y);
-          const float m = wave_max(fmaxf(fabsf(f0), fabsf(f1)));
-          const float inv = m > 0.f ? 448.f / m : 0.f;
-          *reinterpret_cast<uint16_t*>(d.oq + o) = (uint16_t)f2e4m3x2_hw(f0 * inv, f1 * inv);
-          if (lane == 0) d.oqs[row * PHV + 2 * hk + h] = m / 448.f;
-        }
-      }
-    }
+  }
+  if (tid < 2 * n) {
+    const int t = tid >> 1, h = 2 * hk + (tid & 1);
+    const int64_t o = (int64_t)(t0 + t) * PHV + h;
+    const float dt = d.dt_f32 ? static_cast<const float*>(d.dt_bias)[h] : bf2f(static_cast<const uint16_t*>(d.dt_bias)[h]);
+    eg[t][tid & 1] = expf_q(-expf_q(d.A_log[h]) * softplus(bf2f(d.a[o]) + dt));
+    beta[t][tid & 1] = sigmoid_q(bf2f(d.b[o]));
   }
   cs[0] = (uint16_t)(__float_as_uint(w0) >> 16);
   cs[1] = (uint16_t)(__float_as_uint(w1) >> 16);
   cs[2] = (uint16_t)(__float_as_uint(w2) >> 16);
+  __syncthreads();
+  for (int p = wave; p < 2 * n; p += 8) {
+    float* v = (p & 1) ? ks[p >> 1] : qs[p >> 1];
+    const float a0 = v[lane], a1 = v[lane + 64];
+    float rr = 1.f / sqrtf(wave_sum_bfly(a0 * a0 + a1 * a1) + 1e-6f);
+    if (!(p & 1)) rr = rr * d.scale;
+    v[lane] = a0 * rr;
+    v[lane + 64] = a1 * rr;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int t = 0; t < n; ++t) {
+    v4f kk[4];
+    float u[4];
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) kk[jj] = *reinterpret_cast<const v4f*>(&ks[t][32 * jj + 4 * c8]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float kv = 0.f;
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kv = __builtin_fmaf(st[j][jj][i], kk[jj][i], kv);
+      u[j] = kv;
+    }
+    const float e[2] = {eg[t][0], eg[t][1]}, bt[2] = {beta[t][0], beta[t][1]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float kv = u[j];
+      kv = kv + lane_xor<1>(kv);
+      kv = kv + lane_xor<2>(kv);
+      kv = kv + lane_xor<4>(kv);
+      u[j] = bt[j >> 1] * (vs[t][r0 + 64 * j] - e[j >> 1] * kv);
+    }
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      const v4f qq = *reinterpret_cast<const v4f*>(&qs[t][32 * jj + 4 * c8]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          st[j][jj][i] = __builtin_fmaf(e[j >> 1], st[j][jj][i], u[j] * kk[jj][i]);
+          o[j] = __builtin_fmaf(st[j][jj][i], qq[i], o[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float ov = o[j];
+      ov = ov + lane_xor<1>(ov);
+      ov = ov + lane_xor<2>(ov);
+      ov = ov + lane_xor<4>(ov);
+      if (c8 == 0) os[t][r0 + 64 * j] = ov;
+    }
+  }
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) *reinterpret_cast<v4f*>(hp + (r0 + 64 * j) * PK + 32 * jj + 4 * c8) = st[j][jj];
+    for (int jj = 0; jj < 4; ++jj)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, st[j][jj]), hb, hat + 128 * jj, 64 * j * PK * 4, 0);
+  if (wave < n) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t row = t0 + wave, o = row * PZ + (2 * hk + h) * PV + 2 * lane;
+      const float o0 = os[wave][h * PV + 2 * lane], o1 = os[wave][h * PV + 2 * lane + 1];
+      const float rstd = 1.f / sqrtf(wave_sum_bfly(o0 * o0 + o1 * o1) / (float)PV + d.eps);
+      const uint32_t nw = reinterpret_cast<const uint32_t*>(d.norm_w)[lane];
+      const uint32_t y = pack_bf2_hw(o0 * rstd * bf_lo(nw) * silu(bf_lo(zr[h])), o1 * rstd * bf_hi(nw) * silu(bf_hi(zr[h])));
+      *reinterpret_cast<uint32_t*>(d.out + o) = y;
+      if (d.oq) {
+        const float f0 = bf_lo(y), f1 = bf_hi(y);
+        const float m = wave_max(fmaxf(fabsf(f0), fabsf(f1)));
+        const float inv = m > 0.f ? 448.f / m : 0.f;
+        *reinterpret_cast<uint16_t*>(d.oq + o) = (uint16_t)f2e4m3x2_hw(f0 * inv, f1 * inv);
+        if (lane == 0) d.oqs[row * PHV + 2 * hk + h] = m / 448.f;
+      }
+    }
+  }
 }
 
 
@@ -291,15 +321,20 @@ __global__ __launch_bounds__(512) void prompt_steps_kernel(PromptDev d) {
 
 // q, k of a chunk for one key head; T, P and gates of its two value heads.  Its writes bound it: 147 KB a chunk and key head, 600
 // MB for 16 prompts of 1000 tokens in 165 us (3.7 TB/s; a copy moves 4.75).
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void prompt_chunks_kernel(PromptDev d) {
-  constexpr int RS = PK + 8, MS = PC + 4;  // padded rows, in elements
-  __shared__ __attribute__((aligned(16))) _Float16 planes[2][2][PC][RS];  // [q, k][hi, lo]; later A and P
-  __shared__ double run[2][PC];  // log2 of the decay up to a token
-  __shared__ float beta[2][PC];
+constexpr int RS = PK + 8, MS = PC + 4;  // padded rows, in elements
+struct ChunkLds {
+  _Float16 planes[2][2][PC][RS];  // [q, k][hi, lo]; later A and P
+  double run[2][PC];  // log2 of the decay up to a token
+  float beta[2][PC];
+};
+__device__ __forceinline__ void chunk(const PromptDev& d, int block, ChunkLds& lds) {
+  auto& planes = lds.planes;
+  auto& run = lds.run;
+  auto& beta = lds.beta;
   float(*const am)[PC][MS] = reinterpret_cast<float(*)[PC][MS]>(&planes[0][0][0][0]);
   float(*const pm)[PC][MS] = am + 2;
   static_assert(sizeof(planes) >= 4 * PC * MS * 4, "A and P in the planes' place");
-  const int unit = blockIdx.x / PHK, hk = blockIdx.x % PHK;
+  const int unit = block / PHK, hk = block % PHK;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = last_at_most(d.B, unit, [&](int i) { return first_unit(d, i, min(max(d.qsl[i], 0), d.rows)); });
   int t0, n;
@@ -308,7 +343,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
   request_of(d, r, t0, n, slot, old);
   const int chunk = unit - first_unit(d, r, t0), c0 = chunk * PC;  // (of the request; first token in it)
   if (n <= kShort || slot < 0 || chunk < 0 || c0 >= n) return;
-  uint8_t* const u = d.units + (int64_t)blockIdx.x * kUnit;
+  uint8_t* const u = d.units + (int64_t)block * kUnit;
   const int g = lane >> 4, c = lane & 15;
 
   // ---- conv, SiLU, unit vectors: thread (run of 4 tokens, 8 channels of q or k)
@@ -553,6 +588,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void p
   pieces(am, wave, 8, kHT, 256.f);
 }
 
+// Short requests and chunks in one launch: neither waits for the other (24 prompts of 1 to 900 tokens: a call 248 -> 236 us, one
+// of 517 47 -> 45).
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void prompt_front_kernel(PromptDev d) {
+  __shared__ __attribute__((aligned(16))) union Lds {
+    StepsLds steps;
+    ChunkLds chunk;
+  } lds;
+  const int first = d.B * PHK;
+  if ((int)blockIdx.x < first) steps(d, blockIdx.x, lds.steps);
+  else chunk(d, blockIdx.x - first, lds.chunk);
+}
+
 // The gated norm of one row of a head, 8 of its values a lane of 16: out, and its e4m3 codes where asked for.
 __device__ __forceinline__ void norm_store(const PromptDev& d, int64_t row, int hv, int c, const float (&x)[8], v4i z, v4i wn) {
   float ss = 0.f;
@@ -587,15 +634,9 @@ __device__ __forceinline__ void norm_store(const PromptDev& d, int64_t row, int 
   }
 }
 
-// A buffer of `bytes` at p (the same in every lane): loads behind its end give 0, stores there are dropped.  (What may lie
-// behind the end is told by the lane's offset alone: the check subtracts the scalar offset from the size, unsigned.)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
-}
-
 // Whether the batch's longest request has at most a quarter of its chunks: whole heads then fill the chip.  One request's
 // chunks follow each other, 2.2 us each where a workgroup has 16 columns of a head and 10 where it has all eight times as many.
-// A call by columns / by heads, us: 16 prompts of 1000 tokens 926 / 484, 24 of 1 to 900 279 / 248, one of
+// A call by columns / by heads, us: 16 prompts of 1000 tokens 926 / 484, 24 of 1 to 900 279 / 248 (both before short requests went beside them), one of
 // 8192 407 / 1120.
 __device__ __forceinline__ bool many_chunks(const PromptDev& d) {
   if (!d.both) return false;
@@ -1352,9 +1393,8 @@ extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream)
   const int64_t units = chunk_units(a->rows, a->B);
   d.exps = reinterpret_cast<int8_t*>(d.units + units * PHK * kUnit);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  prompt_steps_kernel<<<(unsigned)a->B * PHK, 512, 0, st>>>(d);
+  prompt_front_kernel<<<(unsigned)(a->B + units) * PHK, 512, 0, st>>>(d);
   if (units) {
-    prompt_chunks_kernel<<<(unsigned)units * PHK, 512, 0, st>>>(d);
     if (d.both) {
       const int rc = ensure_lds(reinterpret_cast<const void*>(prompt_heads_kernel), kHeadsLds, "q36_gdn_prompt");
       if (rc != Q36_OK) return rc;
