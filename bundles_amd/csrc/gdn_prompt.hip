@@ -669,11 +669,12 @@ __device__ __forceinline__ float all_max(float m) { return __uint_as_float(wave_
 // for one prompt of 8192 tokens): four dependent products and what lies between them through LDS 1.25 us, the rest loads that
 // arrive later than that.
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_scan_kernel(PromptDev d) {
-  constexpr int BLOCKS = PV / 16, SS = PK + 8, XS = PC + 8;
-  __shared__ __attribute__((aligned(16))) _Float16 sp[2][16][SS];   // the state's parts
-  __shared__ __attribute__((aligned(16))) _Float16 xp[2][16][XS];   // X's
-  __shared__ __attribute__((aligned(16))) _Float16 up[4][16][XS];   // U's; the decayed U's
-  __shared__ __attribute__((aligned(16))) float vp[2][16][PC + 4];  // values of a chunk and the next
+  constexpr int BLOCKS = PV / 16;
+  // parts in pieces of 1 KB as a chunk's operands', so that lanes read side by side
+  __shared__ v8h sp[2][4][64];   // the state's
+  __shared__ v8h xp[2][2][64];   // X's
+  __shared__ v8h up[4][2][64];   // U's; the decayed U's
+  __shared__ v4f vp[2][4][64];   // values of a chunk and the next, by token tile
   __shared__ float most[4];
   if (many_chunks(d)) return;
   // the 2 BLOCKS workgroups of a (request, key head) on one XCD, where the chunks' operands came from
@@ -694,7 +695,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   const uint8_t* u = d.units + ((int64_t)first_unit(d, r, t0) * PHK + hk) * kUnit;  // a chunk's operands, then the next's
   constexpr int64_t kNext = (int64_t)PHK * kUnit;
   const int head = kUHead + hh * kHeadBytes, nks = w < 2 ? 1 : 2;
-  const int mine = 32 * (w >> 1) + 8 * g + 4 * (w & 1);  // of tokens 16 w + 4 g .. in a depth's order
+  auto tile = [&](v8h(&p)[2][64]) -> v4h& {  // of tokens 16 w + 4 g .. in a depth's order
+    return reinterpret_cast<v4h*>(p[w >> 1])[2 * lane + (w & 1)];
+  };
   float before, vmost = 0.f;
   int fe = 0;  // the columns' exponent
   auto columns = [&]() { return fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])); };
@@ -712,7 +715,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
   auto load_end = [&](__amdgpu_buffer_rsrc_t b) {  // e^{b_end}
     return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, 0, head + kHGate + 4 * (PC - 1), 0));
   };
-  auto part = [&](const _Float16* row, int s) { return *reinterpret_cast<const v8h*>(row + 32 * s + 8 * g); };
 
   if (wave < 4) {
     // ---- dims 32 w + 16 i + 4 g + q of column c, times 2^fe
@@ -732,8 +734,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       v4h h[2], l[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) split4(S[i], h[i], l[i]);
-      *reinterpret_cast<v8h*>(&sp[0][c][32 * w + 8 * g]) = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      *reinterpret_cast<v8h*>(&sp[1][c][32 * w + 8 * g]) = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      sp[0][w][lane] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      sp[1][w][lane] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
     };
     v8h K[2][4], Kt[2][2][2], T[2][2];
     v4f rest, bt, beb;
@@ -783,12 +785,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       const __amdgpu_buffer_rsrc_t nb = buffer(un, kUnit);
       // ---- X = beta (V - e^b K S)
       {
-        const v4f v = *reinterpret_cast<const v4f*>(&vp[ch & 1][c][16 * w + 4 * g]);
+        const v4f v = vp[ch & 1][w][lane];
         const float f = __builtin_ldexpf(1.f, fe);
         v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const v8h bh = part(sp[0][c], s), bl = part(sp[1][c], s);
+          const v8h bh = sp[0][s][lane], bl = sp[1][s][lane];
           a1 = mma(K[0][s], bh, a1);
           a2 = mma(K[1][s], bh, a2);
           (s & 1 ? a1 : a2) = mma(K[0][s], bl, s & 1 ? a1 : a2);
@@ -798,8 +800,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[q] = __builtin_fmaf(-beb[q], a1[q] + a2[q], bt[q] * f * v[q]);
         split4(x, hi, lo);
-        *reinterpret_cast<v4h*>(&xp[0][c][mine]) = hi;
-        *reinterpret_cast<v4h*>(&xp[1][c][mine]) = lo;
+        tile(xp[0]) = hi;
+        tile(xp[1]) = lo;
       }
       load_k(nb);
       __syncthreads();
@@ -809,7 +811,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           if (s < nks) {
-            const v8h bh = part(xp[0][c], s), bl = part(xp[1][c], s);
+            const v8h bh = xp[0][s][lane], bl = xp[1][s][lane];
             a1 = mma(T[0][s], bh, a1);
             a2 = mma(T[1][s], bh, a2);
             a2 = mma(T[0][s], bl, a2);
@@ -821,10 +823,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
         for (int q = 0; q < 4; ++q) x[q] = a1[q] + a2[q], y[q] = x[q] * rest[q], x[q] *= 0x1p-8f;
         split4(y, dh, dl);
         split4(x, uh, ul);
-        *reinterpret_cast<v4h*>(&up[2][c][mine]) = dh;
-        *reinterpret_cast<v4h*>(&up[3][c][mine]) = dl;
-        *reinterpret_cast<v4h*>(&up[0][c][mine]) = uh;
-        *reinterpret_cast<v4h*>(&up[1][c][mine]) = ul;
+        tile(up[2]) = dh;
+        tile(up[3]) = dl;
+        tile(up[0]) = uh;
+        tile(up[1]) = ul;
       }
       load_t(nb);
       __syncthreads();
@@ -838,7 +840,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const v8h bh = part(up[2][c], s), bl = part(up[3][c], s);
+        const v8h bh = up[2][s][lane], bl = up[3][s][lane];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           a[i][0] = mma(Kt[0][i][s], bh, a[i][0]);
@@ -894,7 +896,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
         v[q] = ch * PC + 16 * w + 4 * g + q < n ? y : 0.f;
         m = fmaxf(m, fabsf(v[q]));
       }
-      *reinterpret_cast<v4f*>(&vp[ch & 1][c][16 * w + 4 * g]) = v;
+      vp[ch & 1][w][lane] = v;
       m = all_max(m);
       if (lane == 0) most[w] = m;
     };
@@ -940,7 +942,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       v4f a1 = {0.f, 0.f, 0.f, 0.f}, a2 = a1;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const v8h bh = part(sp[0][c], s), bl = part(sp[1][c], s);
+        const v8h bh = sp[0][s][lane], bl = sp[1][s][lane];
         a1 = mma(Q[0][s], bh, a1);
         a2 = mma(Q[1][s], bh, a2);
         (s & 1 ? a1 : a2) = mma(Q[0][s], bl, s & 1 ? a1 : a2);
@@ -960,7 +962,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s < nks) {
-          const v8h bh = part(up[0][c], s), bl = part(up[1][c], s);
+          const v8h bh = up[0][s][lane], bl = up[1][s][lane];
           a1 = mma(P[0][s], bh, a1);
           a2 = mma(P[1][s], bh, a2);
           a2 = mma(P[0][s], bl, a2);
