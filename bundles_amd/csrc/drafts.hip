@@ -130,18 +130,41 @@ __device__ __forceinline__ float logit_at(const DraftsDev& d, int64_t row, int i
   return x == x ? x : -__builtin_inff();
 }
 
-// Sum over the wave, the same in every lane.
+// Lanes' values moved within rows of 16 (CTRL), lanes without a source and rows outside ROWS get 0.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t b = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, ROWS == 0xf);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, ROWS == 0xf);
+  return __longlong_as_double(((uint64_t)hi << 32) | lo);
+}
+// Sum over the wave, the same in every lane.  (By register moves: through LDS each of the six steps waits for it twice.)
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  v += moved<0xB1>(v);   // xor 1, xor 2, the half rows, the rows
+  v += moved<0x4E>(v);
+  v += moved<0x141>(v);
+  v += moved<0x140>(v);
+  auto pair = [](double x, auto swap) {
+    const uint64_t b = __double_as_longlong(x);
+    const auto lo = swap((uint32_t)b), hi = swap((uint32_t)(b >> 32));
+    return __longlong_as_double(((uint64_t)(uint32_t)hi[0] << 32) | (uint32_t)lo[0]) +
+           __longlong_as_double(((uint64_t)(uint32_t)hi[1] << 32) | (uint32_t)lo[1]);
+  };
+  v = pair(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  return pair(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ double wave_prefix_d(double v) {
+  v += moved<0x111>(v);  // by 1, 2, 4, 8 lanes in a row
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<0x142, 0xa>(v);  // a row's last lane to the odd row behind it, then the lower half's to the upper
+  v += moved<0x143, 0xc>(v);
   return v;
 }
 
-__device__ __forceinline__ int min64(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
-  return v;
-}
+__device__ __forceinline__ int min64(int v) { return (int)~wave_max_u32(~(uint32_t)v); }  // (v >= 0)
 
 // A segment of a row: its largest logit, the first index of it, the sum of its weights.
 template <bool F32, bool VEC, bool WIDE>
@@ -218,9 +241,10 @@ __device__ double wide_sum(const DraftsDev& d, int64_t row, float m, double s, d
   return sum;
 }
 
-// Waves take rows wave, wave + 4; then thread 0 walks the drafts.  Behind a synchronisation.
+// Waves take rows wave, wave + 4; then thread 0 walks the drafts.  Behind a synchronisation.  segw (or null): the weights of the
+// rows' first 64 segments.
 template <bool F32, bool VEC>
-__device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
+__device__ void walk(const DraftsDev& d, int b, double s, Chain* c, double (*segw)[64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int t = wave; t < d.T; t += 4) {
     const int64_t row = (int64_t)b * d.T + t, o = row * d.segs;
@@ -238,6 +262,7 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
     m = wave_max(m);
     int first = pm == m ? pi : 0x7fffffff;
     double n = s > 0.0 && pm > -__builtin_inff() ? ps * weight(pm, m, s) : 0.0;
+    if (segw) segw[t][lane] = n;
     for (int i = lane + 64; i < d.segs; i += 64) {
       const float v = d.pmax[o + i];
       if (v > -__builtin_inff()) {
@@ -289,7 +314,7 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c) {
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void drafts_walk_kernel(DraftsDev d) {
   __shared__ Chain c;
-  walk<F32, VEC>(d, blockIdx.x, heat_of(d, blockIdx.x), &c);
+  walk<F32, VEC>(d, blockIdx.x, heat_of(d, blockIdx.x), &c, nullptr);
   static_assert(sizeof(Chain) % 8 == 0 && sizeof(Chain) / 4 <= kThreads, "a word a thread");
   if (threadIdx.x < sizeof(Chain) / 4)
     reinterpret_cast<uint32_t*>(d.chains + blockIdx.x)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&c)[threadIdx.x];
@@ -300,11 +325,16 @@ __device__ __forceinline__ void read_chain(const DraftsDev& d, int b, Chain* c) 
   __syncthreads();
 }
 
+// A lane's segment's sum, asked for before anything else.
+__device__ __forceinline__ double first_of(const DraftsDev& d, bool on, const double* sums, int b) {
+  const int lane = threadIdx.x & 63;
+  return on && lane < d.segs ? sums[(int64_t)b * d.segs + lane] : 0.0;
+}
 // The drawn row's sum in fp64 from its segments', where it is not: by every wave, the same bits.
-__device__ void widen(const DraftsDev& d, int b, double s, Chain* c) {
+__device__ void widen(const DraftsDev& d, int b, double s, Chain* c, double e0) {
   if (!d.narrow || s <= 0.0 || c->ended) return;
-  double n = 0.0;
-  for (int i = threadIdx.x & 63; i < d.segs; i += 64) n += d.esum[(int64_t)b * d.segs + i];
+  double n = e0;
+  for (int i = (threadIdx.x & 63) + 64; i < d.segs; i += 64) n += d.esum[(int64_t)b * d.segs + i];
   n = wave_sum_d(n);
   __syncthreads();
   if (threadIdx.x == 0) c->norm[c->j] = n;
@@ -336,10 +366,10 @@ template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) {
   __shared__ Chain c;
   const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
-  const double s = heat_of(d, b);
+  const double s = heat_of(d, b), e0 = first_of(d, d.narrow, d.esum, b);
   read_chain(d, b, &c);
   if (!c.refused) return;
-  widen(d, b, s, &c);
+  widen(d, b, s, &c, e0);
   const int j = c.j, base = seg * kSeg + tid * kPer;
   const int64_t row = (int64_t)b * d.T + j;
   const float* q = d.probs + ((int64_t)b * (d.T - 1) + j) * d.V;
@@ -367,11 +397,12 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   __shared__ double total[4], rest;
   __shared__ int pick_seg, mode;  // mode: 0 the weights p, 1 p without the draft, 2 max(p - q, 0)
   __shared__ int found, last;
+  __shared__ double segw[kMaxT][64];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const double s = heat_of(d, b);
+  const double s = heat_of(d, b), e0 = first_of(d, d.narrow, d.esum, b), r0 = first_of(d, d.probs, d.rsum, b);
   if (d.chains) read_chain(d, b, &c);
-  else walk<F32, VEC>(d, b, s, &c);
-  widen(d, b, s, &c);
+  else walk<F32, VEC>(d, b, s, &c, segw);
+  widen(d, b, s, &c, e0);
   const int j = c.j;
   int32_t* const out = d.tokens + (int64_t)b * d.T;
   if (tid < d.T) out[tid] = tid < j ? c.tok[tid] : -1;
@@ -386,11 +417,13 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
     const double inv = s > 0.0 ? 1.0 / c.norm[j] : 1.0;
     auto part = [&](int i, int md) -> double {
       if (i >= d.segs) return 0.0;
-      if (md == 2) return d.rsum[(int64_t)b * d.segs + i];
+      if (md == 2) return i < 64 ? r0 : d.rsum[(int64_t)b * d.segs + i];
       double w;
       if (s > 0.0) {
         if (d.narrow) {
-          w = d.esum[(int64_t)b * d.segs + i] * inv;
+          w = (i < 64 ? e0 : d.esum[(int64_t)b * d.segs + i]) * inv;
+        } else if (i < 64 && !d.chains) {
+          w = segw[j][i] * inv;
         } else {
           const float pm = d.pmax[o + i];
           w = pm > -__builtin_inff() ? d.psum[o + i] * weight(pm, c.m[j], s) * inv : 0.0;
@@ -419,12 +452,7 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
     double tail_base = 0.0;
     for (int i0 = 0; i0 < d.segs && at < 0; i0 += 64) {
       const double w = i0 ? part(i0 + lane, md) : mine;
-      double run = w;
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) {
-        const double v = __shfl_up(run, k);
-        if (lane >= k) run += v;
-      }
+      const double run = wave_prefix_d(w);
       const uint64_t over = __ballot(before + run > goal && w > 0.0), some = __ballot(w > 0.0);
       if (over) {
         const int l = __builtin_ctzll(over);
@@ -461,12 +489,7 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
     w[i] = p;
     sum += p;
   }
-  double run = sum;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    const double v = __shfl_up(run, k);
-    if (lane >= k) run += v;
-  }
+  double run = wave_prefix_d(sum);
   if (lane == 63) total[wave] = run;
   __syncthreads();
   run -= sum;
