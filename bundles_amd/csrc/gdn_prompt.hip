@@ -1138,6 +1138,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
     before = 11.32f * all_max(m);  // a norm: at most sqrt(128) times the largest
     next_factor(1.f, conv_v(0));
   }
+  const v4i wn = *reinterpret_cast<const v4i*>(d.norm_w + 8 * c);
   wait_vm0();
   barrier();
 
@@ -1282,7 +1283,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
     u = un;
     {  // the gated norm: eight rows a wave, 16 lanes a row
       const float* const os = reinterpret_cast<const float*>(lds + kLOut);
-      const v4i wn = *reinterpret_cast<const v4i*>(d.norm_w + 8 * c);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int t = 8 * wave + 4 * i + g;
