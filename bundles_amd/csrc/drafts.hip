@@ -14,7 +14,7 @@
 //
 // Reading the logits once bounds a large call: 256 requests of 8 rows of 151936 (622 MB) 180 us, of them 131 in the sums (4.75
 // TB/s), 38 in the drawn rows' second reading, 12 and 7 in the pick and the walk.  A small one is bound by its two launches
-// and the latencies in them: one row 19 us.
+// and the latencies in them: one row 18 us.
 #include <type_traits>
 
 #include "q36_device.h"

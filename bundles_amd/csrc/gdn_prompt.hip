@@ -635,9 +635,9 @@ __device__ __forceinline__ void norm_store(const PromptDev& d, int64_t row, int 
 }
 
 // Whether the batch's longest request has at most a quarter of its chunks: whole heads then fill the chip.  One request's
-// chunks follow each other, 2.2 us each where a workgroup has 16 columns of a head and 10 where it has all eight times as many.
-// A call by columns / by heads, us: 16 prompts of 1000 tokens 926 / 484, 24 of 1 to 900 279 / 248 (both before short requests went beside them), one of
-// 8192 407 / 1120.
+// chunks follow each other, 2.3 us each where a workgroup has 16 columns of a head and 10 where it has all eight times as many;
+// four requests of one length by columns take the chip in turns, 9 us a chunk of each.  A call by columns / by heads, us: 16 prompts
+// of 1000 tokens 839 / 473, 24 of 1 to 900 277 / 229, one of 8192 407 / 1120.
 __device__ __forceinline__ bool many_chunks(const PromptDev& d) {
   if (!d.both) return false;
   int sum = 0, most = 0;
@@ -665,9 +665,9 @@ __device__ __forceinline__ float all_max(float m) { return __uint_as_float(wave_
 // A request's chunks for 16 value columns of a head.  Waves 0-3 carry the state: wave w holds key dims 32 w .. + 31 of it
 // and token tile w of X and U.  Waves 4-7, one beside each of them on its SIMD, convolve the next chunk's values and form the
 // outputs of token tile w - 4, from the same parts in LDS; so the chain from state to state has only its own work in it.
-// State, X and U pass through LDS as fp16 parts, in the order of an operand's depth.  The chain bounds it, 2.2 us a chunk (280 us
-// for one prompt of 8192 tokens): four dependent products and what lies between them through LDS 1.25 us, the rest loads that
-// arrive later than that.
+// State, X and U pass through LDS as fp16 parts, in the order of an operand's depth.  The chain bounds it, 2.3 us a chunk (297
+// us for one prompt of 8192 tokens): three dependent products and what lies between them through LDS 1.25 us, the rest loads that
+// arrive later than that (128 KB a chunk from L2).
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_scan_kernel(PromptDev d) {
   constexpr int BLOCKS = PV / 16;
   // parts in pieces of 1 KB as a chunk's operands', so that lanes read side by side
@@ -954,7 +954,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void p
       conv_v(ch + 1);
       load_v(ch + 2);
       __syncthreads();
-      // ---- + P U: as fp16 times a power of two for four rows, in out's place until the norm
+      // ---- + P U: as fp16 times a power of two for 16 columns of four rows, in out's place until the norm.  (Half a step of
+      // 2^-12 of the largest of the 64, beside the bf16 output's 2^-9; in fp32 this pass moved twice the bytes.)
       const int rows = min(n - ch * PC, PC);
       const __amdgpu_buffer_rsrc_t ob = buffer(d.out + (int64_t)(t0 + ch * PC) * PZ, rows * PZ * 2);
       const __amdgpu_buffer_rsrc_t xb = buffer(d.exps + (int64_t)(t0 + ch * PC) * 256, rows * 256);
@@ -1023,10 +1024,10 @@ constexpr int kHeadsLds = kLOut + PC * kOutRow * 4;
 // A request's chunks for a whole value head, 16 columns a wave.  A wave's columns need nothing of another's: it holds their
 // state (lane (c, g): column c, dims 16 t + 4 g + q), and each product's registers, rounded to two parts, are the next one's
 // operand.  What the waves share are the chunk's other operands, in LDS: K and Q of the next chunk arrive while T, P and K^T
-// are used, and the other way round, with a barrier at either change.  16 prompts of 1000 tokens: 340 us, 10 a chunk.  A chunk
-// of a head reads 1.12 MB of LDS (8700 clk at 128 bytes), has 10000 clk of vector instructions a SIMD (the splitting into parts
-// most of it) and 5800 of matrix instructions, at two waves a SIMD little of it beside each other; 72 us are the operands' way
-// into LDS.  (32 columns a wave read half of LDS but do not fit the registers: 570 for 484 us a call.)
+// are used, and the other way round, with a barrier at either change.  16 prompts of 1000 tokens: 313 us, 10 a chunk
+// and CU, of which the vector units have 42 % (the splitting into parts, conv and norm most of it), the matrix units 28 %, LDS 23 % (a
+// chunk reads 1 MB of it), little of it beside each other at two waves a SIMD.  (32 columns a wave read half of LDS but do not fit
+// the registers: 570 for 484 us a call; the norm and the conv at other times in a SIMD's two waves: 3 % slower.)
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void prompt_heads_kernel(PromptDev d) {
   constexpr int W = 8;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
