@@ -1378,8 +1378,8 @@ extern "C" int q36_gdn_prompt(const q36_gdn_prompt_args* a, q36_stream_t stream)
   Q36_REQUIRE(a->slots >= 1, "q36_gdn_prompt: slots=%d", a->slots);
   Q36_REQUIRE(a->cs_slot >= PQKV * 3 && a->cs_slot % 8 == 0, "q36_gdn_prompt: conv_state slot stride %lld", (long long)a->cs_slot);
   Q36_REQUIRE(aligned16(a->mixed) && aligned16(a->z) && aligned16(a->conv_state) && aligned16(a->conv_w) && aligned16(a->h0) &&
-                  aligned16(a->out),
-              "q36_gdn_prompt: mixed, z, conv_state, conv_w, h0 and out must be 16-byte aligned");
+                  aligned16(a->norm_w) && aligned16(a->out),
+              "q36_gdn_prompt: mixed, z, conv_state, conv_w, h0, norm_w and out must be 16-byte aligned");
   Q36_REQUIRE((reinterpret_cast<uintptr_t>(a->dt_bias) & 3u) == 0, "q36_gdn_prompt: dt_bias must be 4-byte aligned");
   Q36_REQUIRE((a->oq == nullptr) == (a->oqs == nullptr), "q36_gdn_prompt: oq and oqs go together");
   Q36_REQUIRE(!a->oq || (aligned16(a->oq) && (reinterpret_cast<uintptr_t>(a->oqs) & 3u) == 0),

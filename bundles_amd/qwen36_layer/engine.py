@@ -81,8 +81,8 @@ class EngineView:
         return None
 
     def gdn_prompt(self, layer_id: int, forward_batch) -> GdnPrompt | None:
-        """A batch that gdn_pools does not serve, as prompt chunks (an engine that wants its prompts here says so).  The rings
-        of its requests are empty afterwards: the engine sets their cursors to 0."""
+        """A batch that gdn_pools does not serve, as prompt chunks (an engine that wants its prompts here says so).  Its
+        requests' rings hold nothing: new ones' cursors are 0, others were committed with room for 16."""
         return None
 
     def kv_view(self, layer_id: int, forward_batch) -> KvView | None:

@@ -153,7 +153,8 @@ def gdn_ring_commit(conv_state, window, h0, d_ring, dlo_ring, k_ring, klo_ring, 
 
     accepted int32/int64 [B]: how many of each request's T window tokens stand, the first included
     (lmhead8.verify_drafts' counts).  The conv state goes to the last accepted token; where the ring then has no room
-    for another `room` tokens (None: T), its entries are folded into the checkpoint h0.  advance: the cursors write_pos and
+    for another `room` tokens (None: T; 16: in any case, as before a prompt that continues the request or a copy of its state), its
+    entries are folded into the checkpoint h0.  advance: the cursors write_pos and
     cache_base move too; recurrent layers that share them commit one after another, the last one with advance.
     A request with accepted < 1 or an index outside its pool is left as it is."""
     what = "gdn_ring_commit"
@@ -214,7 +215,8 @@ def gdn_prompt(mixed, z, a, b, conv_state, conv_w, A_log, dt_bias, h0, qsl, stat
     and of the recurrent state h0 fp32 [slots, 32, 128, 128], both updated in place.  prefix int32 [B] (optional): requests
     with 0 tokens before these begin from zero states, whatever their slots hold.  oq (glue.linear_rows(rows, 4096)): out's
     e4m3 codes also go there.  Rows of no request are left as they were; a slot outside the pool marks a padded request, whose
-    rows are zeroed.  Requests with rows name distinct slots."""
+    rows are zeroed.  Requests with rows name distinct slots; the ring of one that continues from verify steps is empty
+    (gdn_ring_commit(..., room=16))."""
     what, rows = "gdn_prompt", mixed.shape[0]
     for t, n, w in ((mixed, "mixed", QKV_DIM), (z, "z", N_V_HEADS * HEAD_V), (a, "a", N_V_HEADS), (b, "b", N_V_HEADS)):
         if t.dtype != torch.bfloat16 or t.dim() < 2 or t.shape[0] != rows or t.numel() != rows * w or not t.is_contiguous():

@@ -284,7 +284,7 @@ int q36_gdn_verify_ring(const q36_gdn_ring_args* a, q36_stream_t stream);
  * accepted[r] (int32, or int64 with idx_i64 bit 3): how many of the window's T tokens stand, the first one included, as
  * q36_verify_drafts counts them; more than T counts as T.  With n = min(write_pos + accepted, 16):
  *   conv_state <- the window record's rows for draft accepted - 1 (the three inputs up to the last accepted token);
- *   n + room > 16 (room: the next window's tokens): the ring is folded into the checkpoint,
+ *   n + room > 16 (room: the next window's tokens; 16 empties the ring in any case): the ring is folded into the checkpoint,
  *     h0 <- e^{G_n} h0 + sum_{c < n} e^{G_n - G_c} (d + dlo)_c (k + klo)_c^T, G_c = g_0 + .. + g_c, in fp32;
  *   with advance: write_pos <- n, or 0 where folded, and cache_base <- (cache_base + n) & 15 there.
  * Recurrent layers that share their cursors commit one after another, the last with advance.  A request with an index outside
@@ -331,7 +331,9 @@ int q36_gdn_ring_commit(const q36_gdn_commit_args* a, q36_stream_t stream);
  * A request without rows is left as it is; a slot outside [0, slots) marks a padded request: zero rows, nothing else
  * written.  Rows of no request are left as they were.  Requests with rows must name distinct slots.  Whatever the device data
  * hold, every access stays inside the buffers.
- * B <= 65535, rows <= 2^20; mixed, z, conv_state, conv_w, h0, out, oq 16-byte, workspace 256-byte aligned, cs_slot a multiple
+ * The ring of a request that continues from verify steps must be empty (q36_gdn_ring_commit with room = 16); out overlaps no
+ * input.
+ * B <= 65535, rows <= 2^20; mixed, z, conv_state, conv_w, h0, norm_w, out, oq 16-byte, workspace 256-byte aligned, cs_slot a multiple
  * of 8.  Workspace: q36_gdn_prompt_workspace_bytes(rows, B), any contents, one for calls that follow one another. */
 typedef struct q36_gdn_prompt_args {
   int32_t B, rows, slots, idx_i64, dt_f32;

@@ -47,7 +47,7 @@ def ring_pools(B, T, dev, seed):
 
 @pytest.mark.parametrize("T", [1, 4, 5])
 def test_prompts_then_drafts(ops, dev, T):
-    """Three requests: prompts of 70, 9 and 1 tokens, then ten verify steps, each continued from what was accepted."""
+    """Three requests: prompts of 70, 9 and 1 tokens, ten verify steps, each continued from what was accepted, prompts again."""
     gdn, lm = ops
     print(f"run T={T}", flush=True)
     lens, B, L, V = [70, 9, 1], 3, 150, 999
@@ -71,7 +71,7 @@ def test_prompts_then_drafts(ops, dev, T):
         x, d, u, heat, _ = drafts_test.inputs(B, T, V, dev, 100 * T + step)
         tokens, counts = lm.verify_drafts(x, d if T > 1 else None, u, ws, temperature=heat)
         before = p["write_pos"].clone()
-        gdn.gdn_ring_commit(*(p[n] for n in commit_test.NAMES[:-1]), counts, T=T)
+        gdn.gdn_ring_commit(*(p[n] for n in commit_test.NAMES[:-1]), counts, T=T, room=16 if step == 9 else None)
         folds += int((p["write_pos"] < before).sum())
         n = counts.tolist()
         assert all(1 <= c <= T for c in n) and ((tokens >= 0).sum(1) == counts).all()
@@ -81,18 +81,20 @@ def test_prompts_then_drafts(ops, dev, T):
             last = torch.cat([last.new_zeros((3 - last.shape[0], QKV)), last])  # (zeros before a request's first token)
             assert torch.equal(p["conv_state"][p["state_idx"][b]], last.t()), (step, b)
     assert folds > 0 or T == 1
-    # what is left in the rings goes into the checkpoints: the state of the accepted tokens
-    p["accepted"] = torch.ones(B, dtype=torch.int64, device=dev)
-    p["write_pos"] -= 1
-    gdn.gdn_ring_commit(*(p[n] for n in commit_test.NAMES), T=T, room=16, advance=False)
-    for b in range(B):
-        if int(p["write_pos"][p["replay_idx"][b]]) < 0:  # (nothing was in the ring)
-            p["write_pos"][p["replay_idx"][b]] += 1
+    # the last commit left the rings empty, so a prompt can follow: four tokens of one request, sixteen of the others
+    assert not p["write_pos"][p["replay_idx"]].any()
+    more = [4, 16, 16]
+    cut = {n: torch.cat([rows(n, b, at[b], at[b] + more[b]) for b in range(B)]) for n in ("mixed", "z", "a", "b")}
+    gdn.gdn_prompt(cut["mixed"], cut["z"], cut["a"], cut["b"], p["conv_state"], f["conv_w"], f["A_log"], f["dt_bias"], p["h0"],
+                   torch.tensor([0, 4, 20, 36], dtype=torch.int32, device=dev), p["state_idx"], f["norm_w"],
+                   gdn.PromptWorkspace(36, B, dev))
+    at = [n + m for n, m in zip(at, more)]
     whole = dict(f, **{n: torch.cat([rows(n, b, 0, at[b]) for b in range(B)]) for n in ("mixed", "z", "a", "b")})
     whole["qsl"] = torch.tensor(np.concatenate([[0], np.cumsum(at)]), dtype=torch.int32, device=dev)
-    _, _, h0 = prompt_test.plain(whole)
+    _, conv, h0 = prompt_test.plain(whole)
     for b in range(B):
         want, got = h0[whole["state_idx"][b]], p["h0"][p["state_idx"][b]].double()
+        assert torch.equal(p["conv_state"][p["state_idx"][b]].double(), conv[whole["state_idx"][b]])
         off = float((got - want).norm() / want.norm())
         print(f"request {b}: {at[b]} tokens, state off by {off:.2e}", flush=True)
         assert off < 2.0 ** -5

@@ -78,7 +78,7 @@ DRAFTS = dict(B=2, T=4, V=1000, ld=1000, workspace_bytes=1 << 30)
         (dict(B=-1), "B="), (dict(B=65536), "B="), (dict(rows=-1), "rows"), (dict(rows=(1 << 20) + 1), "rows"),
         (dict(slots=0), "slots"), (dict(cs_slot=24575), "stride"), (dict(cs_slot=24577), "stride"), (dict(mixed=None), "null"),
         (dict(qsl=None), "null"), (dict(state_idx=None), "null"), (dict(workspace=None), "null"), (dict(out=None), "null"),
-        (dict(mixed=P + 2), "aligned"), (dict(h0=P + 4), "aligned"), (dict(out=P + 8), "aligned"), (dict(dt_bias=P + 2), "aligned"),
+        (dict(mixed=P + 2), "aligned"), (dict(h0=P + 4), "aligned"), (dict(out=P + 8), "aligned"), (dict(norm_w=P + 2), "aligned"), (dict(dt_bias=P + 2), "aligned"),
         (dict(oq=P), "together"), (dict(oqs=P), "together"), (dict(oq=P + 4, oqs=P), "aligned"), (dict(workspace_bytes=0), "workspace"),
         (dict(workspace=P + 128), "workspace")]
 ] + [
