@@ -100,6 +100,55 @@ def test_prompts_then_drafts(ops, dev, T):
         assert off < 2.0 ** -5
 
 
+def test_captured_steps(ops, dev):
+    """Verify step, verification and commit in one captured graph, replayed over changing inputs: every replay leaves the pools
+    as eager calls leave theirs."""
+    gdn, lm = ops
+    B, T, V = 5, 4, 700
+    print("captured steps", flush=True)
+    pools = [ring_pools(B, T, dev, 7) for _ in range(2)]
+    for p in pools:
+        for t in p.values():
+            if t.is_floating_point():
+                t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(8)) * 0.1)
+        p["g_ring"].copy_(-p["g_ring"].abs())
+    ws = [lm.VerifyWorkspace(B, T, V, dev) for _ in range(2)]
+    qsl = torch.arange(0, (B + 1) * T, T, dtype=torch.int32, device=dev)
+
+    def inputs(seed):
+        f = prompt_test.inputs([T] * B, dev, seed)
+        x, d, u, heat, _ = drafts_test.inputs(B, T, V, dev, seed)
+        return dict({k: f[k] for k in ("mixed", "z", "a", "b", "conv_w", "A_log", "dt_bias", "norm_w")}, x=x, d=d, u=u, heat=heat)
+
+    def step(i, p, w):
+        out = gdn.gdn_verify_ring(i["mixed"], i["z"], i["a"], i["b"], p["conv_state"], i["conv_w"], p["window"], i["A_log"],
+                                  i["dt_bias"], p["h0"], p["d_ring"], p["dlo_ring"], p["k_ring"], p["klo_ring"], p["g_ring"], qsl,
+                                  p["state_idx"], p["replay_idx"], p["win_idx"], p["write_pos"], p["cache_base"], i["norm_w"], T=T)
+        tokens, counts = lm.verify_drafts(i["x"], i["d"], i["u"], w, temperature=i["heat"])
+        gdn.gdn_ring_commit(*(p[k] for k in commit_test.NAMES[:-1]), counts, T=T)
+        return out, tokens, counts
+    held = inputs(100)
+    saved = {k: t.clone() for k, t in pools[0].items()}
+    step(held, pools[0], ws[0])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = step(held, pools[0], ws[0])
+    for k, t in saved.items():
+        pools[0][k].copy_(t)
+    for n in range(24):
+        new = inputs(100 + n)
+        for k, t in new.items():
+            held[k].copy_(t)
+        g.replay()
+        torch.cuda.synchronize()
+        want = step(new, pools[1], ws[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want)), n
+        assert all(torch.equal(pools[0][k], pools[1][k]) for k in pools[0]), n
+    assert int(pools[1]["cache_base"][pools[1]["replay_idx"]].ne(13).sum()) > 0  # rings were folded
+
+
 @pytest.mark.parametrize("lens", [[5, 20], [100, 1, 60, 9]])
 def test_layer_node_gdn_prompt(ops, dev, lens):
     """The recurrent mixer over an engine's prompt batch (25 rows project through the DENSE8 copies, more through the e4m3
