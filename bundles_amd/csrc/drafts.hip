@@ -66,12 +66,11 @@ __device__ __forceinline__ double heat_of(const DraftsDev& d, int b) {
   return t > 0.f ? 1.4426950408889634074 / (double)fminf(t, 1e30f) : 0.0;
 }
 
-// 2^((x - m) s) for x <= m, 1 at x == m whatever m is (an infinite largest logit leaves weight to its equals alone): the
-// fraction's power by its series up to f^9, off by at most (ln 2 / 2)^10 / 10! = 7e-12.  (The whole part by an addition of
-// 1.5 2^52 and on the exponent's bits, in place of rounding, conversion and ldexp: 8 % slower.)
+// 2^((x - m) s) for x <= m, m finite; 0 for NaN: the fraction's power by its series up to f^9, off by at most (ln 2 / 2)^10 / 10! =
+// 7e-12.  (The whole part by an addition of 1.5 2^52 and on the exponent's bits, in place of rounding, conversion and ldexp: 8 %
+// slower.)
 __device__ __forceinline__ double weight(float x, float m, double s) {
-  double y = ((double)x - (double)m) * s;
-  y = y > -1100.0 ? y : -1100.0;  // (also NaN: minus infinity below itself, or beside an infinite largest)
+  const double y = __builtin_fmax(((double)x - (double)m) * s, -1100.0);  // (of NaN and a number: the number)
   const double n = __builtin_rint(y), f = y - n;
   double p = 1.0178086009239699e-07;
   p = __builtin_fma(p, f, 1.3215486790144307e-06);
@@ -83,11 +82,12 @@ __device__ __forceinline__ double weight(float x, float m, double s) {
   p = __builtin_fma(p, f, 2.4022650695910071e-01);
   p = __builtin_fma(p, f, 6.9314718055994531e-01);
   p = __builtin_fma(p, f, 1.0);
-  p = __builtin_ldexp(p, (int)n);
-  return x == m ? 1.0 : p;
+  return __builtin_ldexp(p, (int)n);
 }
+// The same for any m: an infinite largest logit leaves weight to its equals alone.
+__device__ __forceinline__ double weight_any(float x, float m, double s) { return x == m ? 1.0 : weight(x, m, s); }
 
-// Logits base .. base + kPer - 1 of a row; past V and NaN: minus infinity.
+// Logits base .. base + kPer - 1 of a row; past V: minus infinity.
 template <bool F32, bool VEC>
 __device__ __forceinline__ void load_logits(const DraftsDev& d, int64_t row, int base, float (&x)[kPer]) {
   const float none = -__builtin_inff();
@@ -119,8 +119,17 @@ __device__ __forceinline__ void load_logits(const DraftsDev& d, int64_t row, int
                    : bf2f(static_cast<const uint16_t*>(d.logits)[row * d.ld + base + i]);
     }
   }
+}
+// The same for weights against the row's (or segment's) largest, m: where that is infinite, its equals become 0, the others minus
+// infinity, m 0.
+template <bool F32, bool VEC>
+__device__ __forceinline__ void load_against(const DraftsDev& d, int64_t row, int base, float& m, float (&x)[kPer]) {
+  load_logits<F32, VEC>(d, row, base, x);
+  if (m == __builtin_inff()) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = x[i] == x[i] ? x[i] : none;
+    for (int i = 0; i < kPer; ++i) x[i] = x[i] == m ? 0.f : -__builtin_inff();
+    m = 0.f;
+  }
 }
 
 template <bool F32>
@@ -179,9 +188,9 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
   const int base = seg * kSeg + tid * kPer;
   load_logits<F32, VEC>(d, row, base, x);
   const double s = heat_of(d, (int)(row / d.T));
-  float m = x[0];
+  float m = -__builtin_inff();
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
+  for (int i = 0; i < kPer; ++i) m = fmaxf(m, x[i]);  // (NaN drop out)
   m = wave_max(m);
   int first = 0;
   if (!(s > 0.0)) {  // (the index says something in greedy requests alone)
@@ -193,15 +202,20 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
   double sum = 0.0;
   if (s > 0.0 && m > -__builtin_inff()) {
     if constexpr (WIDE) {
+      if (m < __builtin_inff()) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
+        for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += x[i] == m ? 1.0 : 0.0;
+      }
       sum = wave_sum_d(sum);
     } else {
       const float sf = (float)fmin(s, 1e30);  // (weights of a temperature below 1e-30: 1 at the largest, else 0)
       float t = 0.f;
       if (m < __builtin_inff()) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) t += __builtin_amdgcn_exp2f((x[i] - m) * sf);
+        for (int i = 0; i < kPer; ++i) t += __builtin_amdgcn_exp2f(fmaxf((x[i] - m) * sf, -200.f));  // (NaN: 0)
       } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) t += x[i] == m ? 1.f : 0.f;
@@ -217,7 +231,7 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
     int I = 0x7fffffff;
     for (int w = 3; w >= 0; --w) {
       if (wm[w] == M) I = wi[w];
-      if (s > 0.0 && wm[w] > -__builtin_inff()) S += ws[w] * weight(wm[w], M, s);
+      if (s > 0.0 && wm[w] > -__builtin_inff()) S += ws[w] * weight_any(wm[w], M, s);
     }
     const int64_t o = row * d.segs + seg;
     d.pmax[o] = M, d.psum[o] = S, d.pidx[o] = I;
@@ -229,9 +243,10 @@ template <bool F32, bool VEC>
 __device__ double wide_sum(const DraftsDev& d, int64_t row, float m, double s, double* part) {
   double sum = 0.0;
   for (int base = threadIdx.x * kPer; base < d.V; base += kSeg) {
-    float x[kPer];
-    load_logits<F32, VEC>(d, row, base, x);
-    for (int i = 0; i < kPer; ++i) sum += weight(x[i], m, s);
+    float x[kPer], top = m;
+    load_against<F32, VEC>(d, row, base, top, x);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, s);
   }
   sum = wave_sum_d(sum);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
@@ -261,20 +276,20 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c, double (*seg
     for (int i = lane + 64; i < d.segs; i += 64) m = fmaxf(m, d.pmax[o + i]);
     m = wave_max(m);
     int first = pm == m ? pi : 0x7fffffff;
-    double n = s > 0.0 && pm > -__builtin_inff() ? ps * weight(pm, m, s) : 0.0;
+    double n = s > 0.0 && pm > -__builtin_inff() ? ps * weight_any(pm, m, s) : 0.0;
     if (segw) segw[t][lane] = n;
     for (int i = lane + 64; i < d.segs; i += 64) {
       const float v = d.pmax[o + i];
       if (v > -__builtin_inff()) {
         if (v == m) first = min(first, d.pidx[o + i]);
-        if (s > 0.0) n += d.psum[o + i] * weight(v, m, s);
+        if (s > 0.0) n += d.psum[o + i] * weight_any(v, m, s);
       }
     }
     n = wave_sum_d(n);
     first = min64(first);
     if (lane == 0) {
       c->m[t] = m, c->idx[t] = first, c->norm[t] = n, c->wide[t] = !d.narrow;
-      c->p[t] = s > 0.0 ? (xd > -__builtin_inff() ? weight(xd, m, s) : 0.0) : (first == tok ? 1.0 : 0.0);
+      c->p[t] = s > 0.0 ? (xd > -__builtin_inff() ? weight_any(xd, m, s) : 0.0) : (first == tok ? 1.0 : 0.0);
       c->q[t] = q, c->u[t] = (double)u, c->tok[t] = tok;
     }
   }
@@ -350,11 +365,11 @@ __global__ __launch_bounds__(kThreads) void drafts_exact_kernel(DraftsDev d) {
   if (!(s > 0.0)) return;
   read_chain(d, b, &c);
   if (c.ended) return;
-  float x[kPer];
-  load_logits<F32, VEC>(d, (int64_t)b * d.T + c.j, seg * kSeg + tid * kPer, x);
+  float x[kPer], top = c.m[c.j];
+  load_against<F32, VEC>(d, (int64_t)b * d.T + c.j, seg * kSeg + tid * kPer, top, x);
   double sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) sum += weight(x[i], c.m[c.j], s);
+  for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, s);
   sum = wave_sum_d(sum);
   if ((tid & 63) == 0) c.part[tid >> 6] = sum;
   __syncthreads();
@@ -373,14 +388,14 @@ __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) 
   const int j = c.j, base = seg * kSeg + tid * kPer;
   const int64_t row = (int64_t)b * d.T + j;
   const float* q = d.probs + ((int64_t)b * (d.T - 1) + j) * d.V;
-  float x[kPer];
-  load_logits<F32, VEC>(d, row, base, x);
+  float x[kPer], top = c.m[j];
+  load_against<F32, VEC>(d, row, base, top, x);
   const double inv = 1.0 / c.norm[j];
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const bool in = base + i < d.V;
-    const double p = s > 0.0 ? weight(x[i], c.m[j], s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
+    const double p = s > 0.0 ? weight(x[i], top, s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
     const double r = p - (double)q[in ? base + i : 0];
     sum += in && r > 0.0 ? r : 0.0;
   }
@@ -426,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
           w = segw[j][i] * inv;
         } else {
           const float pm = d.pmax[o + i];
-          w = pm > -__builtin_inff() ? d.psum[o + i] * weight(pm, c.m[j], s) * inv : 0.0;
+          w = pm > -__builtin_inff() ? d.psum[o + i] * weight_any(pm, c.m[j], s) * inv : 0.0;
         }
       } else {
         w = c.idx[j] / kSeg == i ? 1.0 : 0.0;
@@ -473,14 +488,14 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   // ---- the index: every thread's 16 weights, their running sums over the workgroup
   const int md = mode, base = pick_seg * kSeg + tid * kPer;
   if (pick_seg < 0) return;  // (cannot be: the row has weight)
-  float x[kPer];
-  load_logits<F32, VEC>(d, row, base, x);
+  float x[kPer], top = c.m[j];
+  load_against<F32, VEC>(d, row, base, top, x);
   double w[kPer], sum = 0.0;
   const double inv = s > 0.0 ? 1.0 / c.norm[j] : 1.0;
   const float* q = md == 2 ? d.probs + ((int64_t)b * (d.T - 1) + j) * d.V : nullptr;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    double p = s > 0.0 ? weight(x[i], c.m[j], s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
+    double p = s > 0.0 ? weight(x[i], top, s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
     if (base + i >= d.V || (md == 1 && base + i == dt)) p = 0.0;
     if (md == 2 && base + i < d.V) {
       p -= (double)q[base + i];
