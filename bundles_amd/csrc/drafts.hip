@@ -12,9 +12,9 @@
 // alone.  In a large call the other rows' sums are fp32, good to 2^-19, which the drafts' tests can do with: a test as close to
 // its border as 2^-17 sums its row again in fp64.
 //
-// Reading the logits once bounds a large call: 256 requests of 8 rows of 151936 (622 MB) 180 us, of them 131 in the sums (4.75
-// TB/s), 38 in the drawn rows' second reading, 12 and 7 in the pick and the walk.  A small one is bound by its two launches
-// and the latencies in them: one row 18 us.
+// Reading the logits once bounds a large call: 256 requests of 8 rows of 151936 (622 MB) 169 us, of them 125 in the sums (5.0
+// TB/s), 34 in the drawn rows' second reading (fp64 arithmetic), 11 and 7 in the pick and the walk.  A small one is bound by its
+// two launches and the latencies in them: one row 18 us.
 #include <type_traits>
 
 #include "q36_device.h"
@@ -324,8 +324,8 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c, double (*seg
   }
 }
 
-// Large calls, whose segments each need it, have the walk in a kernel of its own (256 requests of 8 rows: 180 us,
-// 244 with the walk in each of 9728 workgroups).
+// Large calls, whose segments each need it, have the walk in a kernel of its own (256 requests of 8 rows: 244 us
+// with the walk in each of 9728 workgroups, 180 without).
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void drafts_walk_kernel(DraftsDev d) {
   __shared__ Chain c;
@@ -525,8 +525,9 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   if (tid == 0) out[j] = found != 0x7fffffff ? found : last;
 }
 
-// Logits behind which fp32 sums pay for two launches more and the drawn row's second reading.  us with fp32 / fp64 sums: 32
-// requests of 4 rows of 151936 (15 M) 39.7 / 35.8, 64 of 5 (39 M) 80 / 98, 256 of 8 (272 M) 180 / 305.
+// Logits (of the rows with drafts) from which fp32 sums pay for two launches more and the drawn row's second reading.  us with fp32 /
+// fp64 sums, rows of 151936: 32 requests of 4 (15 M) 31.2 / 30.7, 48 of 4 (22 M) 35.3 / 35.9, 64 of 4 (29 M) 40.6 / 42.1, 64 of 5 (39
+// M) 44.2 / 49.3, 256 of 8 (272 M) 167 / 255.
 constexpr int64_t kNarrowFrom = 24 << 20;
 
 int64_t segments(int64_t V) { return (V + kSeg - 1) / kSeg; }
