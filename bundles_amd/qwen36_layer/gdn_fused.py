@@ -58,15 +58,19 @@ def gdn_verify_fused(mixed, z, a, b, conv_state, conv_w, A_log, dt_bias, S0, nor
 
 
 RING = 16
+D_RING, D_INNER = (N_V_HEADS, RING, HEAD_V), (RING * HEAD_V, HEAD_V, 1)  # a ring pool's slot, and its strides
+K_RING, K_INNER = (N_K_HEADS, RING, HEAD_K), (RING * HEAD_K, HEAD_K, 1)
 
 
 def _pool(t, name, dtype, tail, inner_strides, what="gdn_verify_ring"):
     """A slot pool [slots, *tail] with the given innermost strides (the slot stride is free but a
-    multiple of 8 elements), as the reference's host checks require (L/qk_gdn_verify.cu:872-904)."""
-    st = t.stride()
-    if t.dtype != dtype or t.shape[1:] != tail or st[1:] != inner_strides or st[0] % 8 != 0:
+    multiple of 8 elements), as the reference's host checks require (L/qk_gdn_verify.cu:872-904): its slots
+    and the slot stride.  (Each look at a tensor's shape or strides costs 0.2 us.)"""
+    st, sh = t.stride(), t.shape
+    if t.dtype != dtype or sh[1:] != tail or st[1:] != inner_strides or st[0] % 8 != 0:
         raise ValueError(f"{what}: {name} must be a {dtype} [slots, {', '.join(map(str, tail))}] pool with "
                          f"contiguous heads, got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
+    return sh[0], st[0]
 
 
 def _idx(t, name, n, what="gdn_verify_ring"):
@@ -161,25 +165,26 @@ def gdn_ring_commit(conv_state, window, h0, d_ring, dlo_ring, k_ring, klo_ring, 
     if not 1 <= T <= 8 or accepted.dim() != 1:
         raise ValueError(f"{what}: accepted must be [B] and the draft window 1..8, got {tuple(accepted.shape)}, {T}")
     B, room = accepted.shape[0], T if room is None else room
-    _pool(conv_state, "conv_state", torch.bfloat16, (QKV_DIM, 3), (3, 1), what)
+    slots, cs_slot = _pool(conv_state, "conv_state", torch.bfloat16, (QKV_DIM, 3), (3, 1), what)
     if window.dim() == 4:  # the deduplicated [wslots, T, 8192, 3] view of [wslots, 8192, T + 2]
-        if window.dtype != torch.bfloat16 or window.shape[1:] != (T, QKV_DIM, 3) or window.stride()[1:] != (1, T + 2, 1) or \
-                window.stride(0) % 8:
+        (wslots, *tail), (win_slot, *inner) = window.shape, window.stride()
+        if window.dtype != torch.bfloat16 or tail != [T, QKV_DIM, 3] or inner != [1, T + 2, 1] or win_slot % 8:
             raise ValueError(f"{what}: conv windows must be the deduplicated [slots, T, 8192, 3] view of [slots, 8192, T + 2]")
     else:
-        _pool(window, "window", torch.bfloat16, (QKV_DIM, T + 2), (T + 2, 1), what)
-    if h0.dtype != torch.float32 or h0.shape[1:] != (N_V_HEADS, HEAD_V, HEAD_K) or not h0.is_contiguous():
+        wslots, win_slot = _pool(window, "window", torch.bfloat16, (QKV_DIM, T + 2), (T + 2, 1), what)
+    sh = h0.shape
+    if h0.dtype != torch.float32 or sh[1:] != (N_V_HEADS, HEAD_V, HEAD_K) or not h0.is_contiguous():
         raise ValueError(f"{what}: the checkpoint must be a contiguous fp32 [slots, 32, 128, 128] pool")
-    for t, n in ((d_ring, "d ring"), (dlo_ring, "d ring (low parts)")):
-        _pool(t, n, torch.bfloat16, (N_V_HEADS, RING, HEAD_V), (RING * HEAD_V, HEAD_V, 1), what)
-    for t, n in ((k_ring, "k ring"), (klo_ring, "k ring (low parts)")):
-        _pool(t, n, torch.bfloat16, (N_K_HEADS, RING, HEAD_K), (RING * HEAD_K, HEAD_K, 1), what)
-    if g_ring.dtype != torch.float32 or g_ring.shape[1:] != (N_V_HEADS, RING) or g_ring.stride()[1:] != (RING, 1) or \
-            g_ring.stride(0) % 4:
+    dn, d_slot = _pool(d_ring, "d ring", torch.bfloat16, D_RING, D_INNER, what)
+    en, dlo_slot = _pool(dlo_ring, "d ring (low parts)", torch.bfloat16, D_RING, D_INNER, what)
+    kn, k_slot = _pool(k_ring, "k ring", torch.bfloat16, K_RING, K_INNER, what)
+    ln, klo_slot = _pool(klo_ring, "k ring (low parts)", torch.bfloat16, K_RING, K_INNER, what)
+    gs, gn = g_ring.stride(), g_ring.shape
+    if g_ring.dtype != torch.float32 or gn[1:] != (N_V_HEADS, RING) or gs[1:] != (RING, 1) or gs[0] % 4:
         raise ValueError(f"{what}: g ring must be an fp32 [slots, 32, 16] pool")
     flags = (_idx(state_idx, "state_idx", B, what) | _idx(replay_idx, "replay_idx", B, what) << 1 |
              _idx(win_idx, "win_idx", B, what) << 2 | _idx(accepted, "accepted", B, what) << 3)
-    rslots = min(d_ring.shape[0], dlo_ring.shape[0], k_ring.shape[0], klo_ring.shape[0], g_ring.shape[0])
+    rslots = min(dn, en, kn, ln, gn[0])
     for t, n in ((write_pos, "write_pos"), (cache_base, "cache_base")):
         if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < rslots:
             raise ValueError(f"{what}: ring cursor {n} must be contiguous int32 [ring slots]")
@@ -187,10 +192,10 @@ def gdn_ring_commit(conv_state, window, h0, d_ring, dlo_ring, k_ring, klo_ring, 
                   "cache_base accepted", conv_state, window, h0, d_ring, dlo_ring, k_ring, klo_ring, g_ring, state_idx,
                   replay_idx, win_idx, write_pos, cache_base, accepted)
     args = pack_commit(
-        B, T, room, int(advance), min(conv_state.shape[0], h0.shape[0]), rslots, window.shape[0], flags,
-        ptr(conv_state), conv_state.stride(0), ptr(window), window.stride(0), ptr(h0), ptr(d_ring), ptr(dlo_ring),
-        d_ring.stride(0), dlo_ring.stride(0), ptr(k_ring), ptr(klo_ring), k_ring.stride(0), klo_ring.stride(0), ptr(g_ring),
-        g_ring.stride(0), ptr(state_idx), ptr(replay_idx), ptr(win_idx), ptr(accepted), ptr(write_pos), ptr(cache_base))
+        B, T, room, int(advance), min(slots, sh[0]), rslots, wslots, flags, conv_state.data_ptr(), cs_slot, window.data_ptr(),
+        win_slot, h0.data_ptr(), d_ring.data_ptr(), dlo_ring.data_ptr(), d_slot, dlo_slot, k_ring.data_ptr(), klo_ring.data_ptr(),
+        k_slot, klo_slot, g_ring.data_ptr(), gs[0], state_idx.data_ptr(), replay_idx.data_ptr(), win_idx.data_ptr(),
+        accepted.data_ptr(), write_pos.data_ptr(), cache_base.data_ptr())
     check(_lib.packed().q36_gdn_ring_commit(args, _lib.stream_handle(stream)), "q36_gdn_ring_commit")
 
 
@@ -219,23 +224,26 @@ def gdn_prompt(mixed, z, a, b, conv_state, conv_w, A_log, dt_bias, h0, qsl, stat
     (gdn_ring_commit(..., room=16))."""
     what, rows = "gdn_prompt", mixed.shape[0]
     for t, n, w in ((mixed, "mixed", QKV_DIM), (z, "z", N_V_HEADS * HEAD_V), (a, "a", N_V_HEADS), (b, "b", N_V_HEADS)):
-        if t.dtype != torch.bfloat16 or t.dim() < 2 or t.shape[0] != rows or t.numel() != rows * w or not t.is_contiguous():
-            raise ValueError(f"{what}: {n} must be contiguous bf16 [{rows}, {w}], got {t.dtype} {tuple(t.shape)}")
+        sh = t.shape
+        if t.dtype != torch.bfloat16 or len(sh) < 2 or sh[0] != rows or t.numel() != rows * w or not t.is_contiguous():
+            raise ValueError(f"{what}: {n} must be contiguous bf16 [{rows}, {w}], got {t.dtype} {tuple(sh)}")
     if qsl.dtype != torch.int32 or qsl.dim() != 1 or qsl.numel() < 1 or not qsl.is_contiguous():
         raise ValueError(f"{what}: qsl must hold B + 1 int32 row starts")
     B = qsl.numel() - 1
-    _pool(conv_state, "conv_state", torch.bfloat16, (QKV_DIM, 3), (3, 1), what)
+    slots, cs_slot = _pool(conv_state, "conv_state", torch.bfloat16, (QKV_DIM, 3), (3, 1), what)
     for t, n, dt, shape in ((conv_w, "conv_w", torch.bfloat16, (QKV_DIM, 4)), (A_log, "A_log", torch.float32, (N_V_HEADS,)),
                             (norm_w, "norm_w", torch.bfloat16, (HEAD_V,)), (prefix, "prefix", torch.int32, (B,))):
         if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
             raise ValueError(f"{what}: {n} must be contiguous {dt} {list(shape)}")
     if dt_bias.dtype not in (torch.float32, torch.bfloat16) or dt_bias.numel() != N_V_HEADS or not dt_bias.is_contiguous():
         raise ValueError(f"{what}: dt_bias must hold 32 fp32 or bf16 values")
-    if h0.dtype != torch.float32 or h0.shape[1:] != (N_V_HEADS, HEAD_V, HEAD_K) or not h0.is_contiguous():
+    sh = h0.shape
+    if h0.dtype != torch.float32 or sh[1:] != (N_V_HEADS, HEAD_V, HEAD_K) or not h0.is_contiguous():
         raise ValueError(f"{what}: the state must be a contiguous fp32 [slots, 32, 128, 128] pool")
     flag = _idx(state_idx, "state_idx", B, what)
-    out = torch.empty((rows, N_V_HEADS * HEAD_V), dtype=torch.bfloat16, device=mixed.device) if out is None else out
-    if out.dtype != torch.bfloat16 or out.shape != (rows, N_V_HEADS * HEAD_V) or not out.is_contiguous():
+    if out is None:
+        out = torch.empty((rows, N_V_HEADS * HEAD_V), dtype=torch.bfloat16, device=mixed.device)
+    elif out.dtype != torch.bfloat16 or out.shape != (rows, N_V_HEADS * HEAD_V) or not out.is_contiguous():
         raise ValueError(f"{what}: out must be contiguous bf16 [{rows}, 4096]")
     if oq is not None and (oq.T != rows or oq.frag or oq.codes.shape[1] != N_V_HEADS * HEAD_V):
         raise ValueError(f"{what}: oq must be row-major rows of this batch (glue.linear_rows)")
@@ -245,9 +253,9 @@ def gdn_prompt(mixed, z, a, b, conv_state, conv_w, A_log, dt_bias, h0, qsl, stat
                   conv_state, conv_w, A_log, dt_bias, h0, qsl, state_idx, norm_w, ws.buf, prefix, out,
                   None if oq is None else oq.codes)
     args = pack_prompt(
-        B, rows, min(conv_state.shape[0], h0.shape[0]), flag, int(dt_bias.dtype == torch.float32), eps, scale, ptr(mixed), ptr(z),
-        ptr(a), ptr(b), ptr(conv_state), conv_state.stride(0), ptr(conv_w), ptr(A_log), ptr(dt_bias), ptr(h0), ptr(qsl),
-        ptr(state_idx), ptr(prefix), ptr(norm_w), ptr(out), ptr(None if oq is None else oq.codes),
-        ptr(None if oq is None else oq.scales), ptr(ws.buf), ws.buf.numel())
+        B, rows, min(slots, sh[0]), flag, int(dt_bias.dtype == torch.float32), eps, scale, mixed.data_ptr(), z.data_ptr(),
+        a.data_ptr(), b.data_ptr(), conv_state.data_ptr(), cs_slot, conv_w.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(),
+        h0.data_ptr(), qsl.data_ptr(), state_idx.data_ptr(), ptr(prefix), norm_w.data_ptr(), out.data_ptr(),
+        ptr(None if oq is None else oq.codes), ptr(None if oq is None else oq.scales), ws.buf.data_ptr(), ws.buf.numel())
     check(_lib.packed().q36_gdn_prompt(args, _lib.stream_handle(stream)), "q36_gdn_prompt")
     return out
