@@ -87,20 +87,25 @@ __device__ __forceinline__ double weight(float x, float m, double s) {
 // The same for any m: an infinite largest logit leaves weight to its equals alone.
 __device__ __forceinline__ double weight_any(float x, float m, double s) { return x == m ? 1.0 : weight(x, m, s); }
 
+// 16 bytes of a row that begins at any element: loads of 16 bytes need no alignment here, and 16 loads of an element each made calls
+// over rows of odd length (64 requests of 5 rows of 151935, 256 of 8) 142 and 706 us, for 49 and 171.
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(2)));
+
 // Logits base .. base + kPer - 1 of a row; past V: minus infinity.
-template <bool F32, bool VEC>
+template <bool F32>
 __device__ __forceinline__ void load_logits(const DraftsDev& d, int64_t row, int base, float (&x)[kPer]) {
   const float none = -__builtin_inff();
-  if (VEC && base + kPer <= d.V) {
+  if (base + kPer <= d.V) {
     if constexpr (F32) {
-      const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(d.logits) + row * d.ld + base);
+      const v4f_any* p = reinterpret_cast<const v4f_any*>(static_cast<const float*>(d.logits) + row * d.ld + base);
       v4f r[kPer / 4];
 #pragma unroll
       for (int i = 0; i < kPer / 4; ++i) r[i] = p[i];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) x[i] = r[i >> 2][i & 3];
     } else {
-      const v4i* p = reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(d.logits) + row * d.ld + base);
+      const v4i_any* p = reinterpret_cast<const v4i_any*>(static_cast<const uint16_t*>(d.logits) + row * d.ld + base);
       v4i r[kPer / 8];
 #pragma unroll
       for (int i = 0; i < kPer / 8; ++i) r[i] = p[i];
@@ -122,13 +127,29 @@ __device__ __forceinline__ void load_logits(const DraftsDev& d, int64_t row, int
 }
 // The same for weights against the row's (or segment's) largest, m: where that is infinite, its equals become 0, the others minus
 // infinity, m 0.
-template <bool F32, bool VEC>
+template <bool F32>
 __device__ __forceinline__ void load_against(const DraftsDev& d, int64_t row, int base, float& m, float (&x)[kPer]) {
-  load_logits<F32, VEC>(d, row, base, x);
+  load_logits<F32>(d, row, base, x);
   if (m == __builtin_inff()) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = x[i] == m ? 0.f : -__builtin_inff();
     m = 0.f;
+  }
+}
+
+// Draft probabilities base .. base + kPer - 1 of a row; past V: 0.
+__device__ __forceinline__ void load_probs(const float* q, int base, int V, float (&y)[kPer]) {
+  if (base + kPer <= V) {
+    const v4f_any* p = reinterpret_cast<const v4f_any*>(q + base);
+#pragma unroll
+    for (int i = 0; i < kPer / 4; ++i) {
+      const v4f_any r = p[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[4 * i + k] = r[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) y[i] = base + i < V ? q[base + i] : 0.f;
   }
 }
 
@@ -176,7 +197,7 @@ __device__ __forceinline__ double wave_prefix_d(double v) {
 __device__ __forceinline__ int min64(int v) { return (int)~wave_max_u32(~(uint32_t)v); }  // (v >= 0)
 
 // A segment of a row: its largest logit, the first index of it, the sum of its weights.
-template <bool F32, bool VEC, bool WIDE>
+template <bool F32, bool WIDE>
 __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
   __shared__ float wm[4];
   __shared__ int wi[4];
@@ -186,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   float x[kPer];
   const int base = seg * kSeg + tid * kPer;
-  load_logits<F32, VEC>(d, row, base, x);
+  load_logits<F32>(d, row, base, x);
   const double s = heat_of(d, (int)(row / d.T));
   float m = -__builtin_inff();
 #pragma unroll
@@ -239,12 +260,12 @@ __global__ __launch_bounds__(kThreads) void drafts_sums_kernel(DraftsDev d) {
 }
 
 // Sum of a row's weights in fp64, by the whole workgroup.
-template <bool F32, bool VEC>
+template <bool F32>
 __device__ double wide_sum(const DraftsDev& d, int64_t row, float m, double s, double* part) {
   double sum = 0.0;
   for (int base = threadIdx.x * kPer; base < d.V; base += kSeg) {
     float x[kPer], top = m;
-    load_against<F32, VEC>(d, row, base, top, x);
+    load_against<F32>(d, row, base, top, x);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, s);
   }
@@ -258,7 +279,7 @@ __device__ double wide_sum(const DraftsDev& d, int64_t row, float m, double s, d
 
 // Waves take rows wave, wave + 4; then thread 0 walks the drafts.  Behind a synchronisation.  segw (or null): the weights of the
 // rows' first 64 segments.
-template <bool F32, bool VEC>
+template <bool F32>
 __device__ void walk(const DraftsDev& d, int b, double s, Chain* c, double (*segw)[64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int t = wave; t < d.T; t += 4) {
@@ -318,7 +339,7 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c, double (*seg
     __syncthreads();
     if (!c->close) return;
     const int j = c->j;
-    const double n = wide_sum<F32, VEC>(d, (int64_t)b * d.T + j, c->m[j], s, c->part);
+    const double n = wide_sum<F32>(d, (int64_t)b * d.T + j, c->m[j], s, c->part);
     if (threadIdx.x == 0) c->norm[j] = n, c->wide[j] = true;
     __syncthreads();
   }
@@ -326,10 +347,10 @@ __device__ void walk(const DraftsDev& d, int b, double s, Chain* c, double (*seg
 
 // Large calls, whose segments each need it, have the walk in a kernel of its own (256 requests of 8 rows: 244 us
 // with the walk in each of 9728 workgroups, 180 without).
-template <bool F32, bool VEC>
+template <bool F32>
 __global__ __launch_bounds__(kThreads) void drafts_walk_kernel(DraftsDev d) {
   __shared__ Chain c;
-  walk<F32, VEC>(d, blockIdx.x, heat_of(d, blockIdx.x), &c, nullptr);
+  walk<F32>(d, blockIdx.x, heat_of(d, blockIdx.x), &c, nullptr);
   static_assert(sizeof(Chain) % 8 == 0 && sizeof(Chain) / 4 <= kThreads, "a word a thread");
   if (threadIdx.x < sizeof(Chain) / 4)
     reinterpret_cast<uint32_t*>(d.chains + blockIdx.x)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&c)[threadIdx.x];
@@ -357,7 +378,7 @@ __device__ void widen(const DraftsDev& d, int b, double s, Chain* c, double e0) 
 }
 
 // The drawn row's weights in fp64, relative to the row's largest logit.
-template <bool F32, bool VEC>
+template <bool F32>
 __global__ __launch_bounds__(kThreads) void drafts_exact_kernel(DraftsDev d) {
   __shared__ Chain c;
   const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
@@ -366,7 +387,7 @@ __global__ __launch_bounds__(kThreads) void drafts_exact_kernel(DraftsDev d) {
   read_chain(d, b, &c);
   if (c.ended) return;
   float x[kPer], top = c.m[c.j];
-  load_against<F32, VEC>(d, (int64_t)b * d.T + c.j, seg * kSeg + tid * kPer, top, x);
+  load_against<F32>(d, (int64_t)b * d.T + c.j, seg * kSeg + tid * kPer, top, x);
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, s);
@@ -377,7 +398,7 @@ __global__ __launch_bounds__(kThreads) void drafts_exact_kernel(DraftsDev d) {
 }
 
 // Residual sums of the row that a request's token is drawn from, where draft probabilities were given.
-template <bool F32, bool VEC>
+template <bool F32>
 __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) {
   __shared__ Chain c;
   const int b = blockIdx.x / (unsigned)d.segs, seg = blockIdx.x % (unsigned)d.segs, tid = threadIdx.x;
@@ -388,15 +409,16 @@ __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) 
   const int j = c.j, base = seg * kSeg + tid * kPer;
   const int64_t row = (int64_t)b * d.T + j;
   const float* q = d.probs + ((int64_t)b * (d.T - 1) + j) * d.V;
-  float x[kPer], top = c.m[j];
-  load_against<F32, VEC>(d, row, base, top, x);
+  float x[kPer], y[kPer], top = c.m[j];
+  load_probs(q, base, d.V, y);
+  load_against<F32>(d, row, base, top, x);
   const double inv = 1.0 / c.norm[j];
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const bool in = base + i < d.V;
     const double p = s > 0.0 ? weight(x[i], top, s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
-    const double r = p - (double)q[in ? base + i : 0];
+    const double r = p - (double)y[i];
     sum += in && r > 0.0 ? r : 0.0;
   }
   sum = wave_sum_d(sum);
@@ -406,7 +428,7 @@ __global__ __launch_bounds__(kThreads) void drafts_residual_kernel(DraftsDev d) 
 }
 
 // One workgroup a request: the drafts' walk, the segment in which the running sum passes the threshold, the index in it.
-template <bool F32, bool VEC>
+template <bool F32>
 __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   __shared__ Chain c;
   __shared__ double total[4], rest;
@@ -416,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const double s = heat_of(d, b), e0 = first_of(d, d.narrow, d.esum, b), r0 = first_of(d, d.probs, d.rsum, b);
   if (d.chains) read_chain(d, b, &c);
-  else walk<F32, VEC>(d, b, s, &c, segw);
+  else walk<F32>(d, b, s, &c, segw);
   widen(d, b, s, &c, e0);
   const int j = c.j;
   int32_t* const out = d.tokens + (int64_t)b * d.T;
@@ -489,16 +511,17 @@ __global__ __launch_bounds__(kThreads) void drafts_pick_kernel(DraftsDev d) {
   const int md = mode, base = pick_seg * kSeg + tid * kPer;
   if (pick_seg < 0) return;  // (cannot be: the row has weight)
   float x[kPer], top = c.m[j];
-  load_against<F32, VEC>(d, row, base, top, x);
+  load_against<F32>(d, row, base, top, x);
   double w[kPer], sum = 0.0;
   const double inv = s > 0.0 ? 1.0 / c.norm[j] : 1.0;
-  const float* q = md == 2 ? d.probs + ((int64_t)b * (d.T - 1) + j) * d.V : nullptr;
+  float y[kPer] = {};
+  if (md == 2) load_probs(d.probs + ((int64_t)b * (d.T - 1) + j) * d.V, base, d.V, y);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     double p = s > 0.0 ? weight(x[i], top, s) * inv : (base + i == c.idx[j] ? 1.0 : 0.0);
     if (base + i >= d.V || (md == 1 && base + i == dt)) p = 0.0;
     if (md == 2 && base + i < d.V) {
-      p -= (double)q[base + i];
+      p -= (double)y[i];
       p = p > 0.0 ? p : 0.0;
     }
     w[i] = p;
@@ -570,24 +593,20 @@ extern "C" int q36_verify_drafts(const q36_verify_drafts_args* a, q36_stream_t s
   d.esum = reinterpret_cast<double*>(w), w += align_up((size_t)a->B * segs * 8, 256);
   d.rsum = reinterpret_cast<double*>(w), w += align_up((size_t)a->B * segs * 8, 256);
   if (narrow || d.probs) d.chains = reinterpret_cast<Chain*>(w);
-  // 16 bytes a lane where every row starts at such a boundary
-  const bool vec = aligned16(a->logits) && a->ld % (a->logits_f32 ? 4 : 8) == 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  auto go = [&](auto f32, auto v) {
-    constexpr bool F = decltype(f32)::value, W = decltype(v)::value;
+  auto go = [&](auto f32) {
+    constexpr bool F = decltype(f32)::value;
     if (narrow) {
-      drafts_sums_kernel<F, W, false><<<(unsigned)n, kThreads, 0, st>>>(d);
+      drafts_sums_kernel<F, false><<<(unsigned)n, kThreads, 0, st>>>(d);
     } else {
-      drafts_sums_kernel<F, W, true><<<(unsigned)n, kThreads, 0, st>>>(d);
+      drafts_sums_kernel<F, true><<<(unsigned)n, kThreads, 0, st>>>(d);
     }
-    if (d.chains) drafts_walk_kernel<F, W><<<a->B, kThreads, 0, st>>>(d);
-    if (narrow) drafts_exact_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
-    if (d.probs) drafts_residual_kernel<F, W><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
-    drafts_pick_kernel<F, W><<<a->B, kThreads, 0, st>>>(d);
+    if (d.chains) drafts_walk_kernel<F><<<a->B, kThreads, 0, st>>>(d);
+    if (narrow) drafts_exact_kernel<F><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
+    if (d.probs) drafts_residual_kernel<F><<<(unsigned)(a->B * segs), kThreads, 0, st>>>(d);
+    drafts_pick_kernel<F><<<a->B, kThreads, 0, st>>>(d);
   };
-  constexpr std::true_type yes;
-  constexpr std::false_type no;
-  if (a->logits_f32) vec ? go(yes, yes) : go(yes, no);
-  else vec ? go(no, yes) : go(no, no);
+  if (a->logits_f32) go(std::true_type{});
+  else go(std::false_type{});
   return check_launch("q36_verify_drafts");
 }
